@@ -1,0 +1,298 @@
+/* k_norm, k_clip: the global L2 norm of many gradients, and the gradients
+ * scaled to it (gfx950, wave64; include/d3s_train.h).
+ *
+ * The tensors' addresses and lengths travel as kernel arguments (up to
+ * CLIP_TENSORS a launch), so the call keeps nothing and may be captured.  A
+ * launch's elements are cut into chunks of one size; chunk i belongs to the
+ * tensor whose range of chunk numbers holds it (a search in the arguments).
+ * k_norm: workgroups take chunks in turn, square in 64 bits (a bf16's square is
+ * exact and an fp32's keeps its range: nothing overflows, and the order costs no
+ * accuracy; the conversions hide behind the loads) and leave one partial sum
+ * each.  k_clip: every workgroup adds all partial sums in one order (they are a
+ * few kilobytes of L2; a launch of its own for it would cost more), and scales
+ * its chunks, from the last to the first: the end of the norm's pass is what
+ * the cache still holds.
+ * Bound: HBM; the second pass over the gradients is the operation's own. */
+#include "d3s_device.h"
+#include "d3s_train_internal.h"
+
+namespace d3s {
+namespace {
+
+constexpr int CT = 256;
+constexpr int CW = CT / WAVE;
+constexpr int CLIP_TENSORS = 128;  /* tensors a launch */
+constexpr int CLIP_GROUPS = 1024;  /* workgroups a launch of k_norm: its partial sums */
+constexpr int CU = 4;              /* 16-byte loads a lane has in flight */
+
+struct ClipArgs {
+  const void *src[CLIP_TENSORS];
+  uint32_t first[CLIP_TENSORS]; /* the tensor's first chunk */
+  uint64_t numel[CLIP_TENSORS]; /* elements << 1 | bf16 */
+  int n;
+  uint32_t chunks;
+  uint32_t chunk; /* 16-byte units a chunk */
+};
+struct ClipOut {
+  void *dst[CLIP_TENSORS];
+};
+
+/* a chunk of a tensor: elements [j0, j1) from an aligned start, or cut by the tensor's ends */
+struct Chunk {
+  int t;
+  bool bf16;
+  int64_t j0, j1;
+};
+
+__device__ __forceinline__ Chunk find_chunk(const ClipArgs &a, uint32_t i) {
+  int lo = 0, hi = a.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.first[mid] <= i)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  Chunk c;
+  c.t = lo;
+  c.bf16 = (a.numel[lo] & 1u) != 0u;
+  const int64_t n = (int64_t)(a.numel[lo] >> 1), per = (int64_t)a.chunk * (c.bf16 ? 8 : 4);
+  const int64_t lead = (int64_t)((uintptr_t)a.src[lo] & 15u) / (c.bf16 ? 2 : 4);
+  c.j0 = (int64_t)(i - a.first[lo]) * per - lead;
+  c.j1 = c.j0 + per < n ? c.j0 + per : n;
+  return c;
+}
+
+__device__ __forceinline__ double square(float g) { return (double)g * (double)g; }
+
+template <bool BF16>
+__device__ __forceinline__ double squares(uint4 q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (BF16) {
+      const double x = d3s_u2f(w[i] << 16), y = d3s_u2f(w[i] & 0xffff0000u);
+      s = fma(y, y, fma(x, x, s));
+    } else {
+      const double x = d3s_u2f(w[i]);
+      s = fma(x, x, s);
+    }
+  }
+  return s;
+}
+
+template <bool BF16>
+__device__ __forceinline__ float element(const void *p, int64_t j) {
+  if constexpr (BF16) return d3s_u2f((uint32_t)((const uint16_t *)p)[j] << 16);
+  return ((const float *)p)[j];
+}
+
+/* the whole 16-byte units of [j0, j1) (j0 at an aligned address, or before the
+ * tensor's start), and the elements before and after them */
+template <bool BF16>
+struct Span {
+  static constexpr int EPC = BF16 ? 8 : 4;
+  int64_t head0, head1, tail0, tail1; /* single elements */
+  int64_t body;                       /* the first whole unit's element */
+  int units;
+  __device__ __forceinline__ Span(const Chunk &c) {
+    body = c.j0 < 0 ? c.j0 + EPC : c.j0;
+    if (body > c.j1) body = c.j1;
+    head0 = c.j0 < 0 ? 0 : c.j0;
+    head1 = body;
+    units = (int)((c.j1 - body) / EPC);
+    tail0 = body + (int64_t)units * EPC;
+    tail1 = c.j1;
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ double chunk_squares(const void *p, const Chunk &c) {
+  const Span<BF16> s(c);
+  const uint4 *b = (const uint4 *)((const char *)p + s.body * (BF16 ? 2 : 4));
+  double sum[2] = {0.0, 0.0};
+  int i = (int)threadIdx.x;
+  for (; i + (CU - 1) * CT < s.units; i += CU * CT) {
+    uint4 q[CU];
+#pragma unroll
+    for (int u = 0; u < CU; u++) q[u] = b[i + u * CT];
+#pragma unroll
+    for (int u = 0; u < CU; u++) sum[u & 1] += squares<BF16>(q[u]);
+  }
+  for (; i < s.units; i += CT) sum[0] += squares<BF16>(b[i]);
+  const int64_t h = s.head0 + threadIdx.x, e = s.tail0 + threadIdx.x;
+  if (h < s.head1) sum[1] += square(element<BF16>(p, h));
+  if (e < s.tail1) sum[1] += square(element<BF16>(p, e));
+  return sum[0] + sum[1];
+}
+
+/* the workgroup's sum, in thread order by a fixed tree, in every thread */
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[CW];
+#pragma unroll
+  for (int o = WAVE / 2; o > 0; o /= 2) v += __shfl_xor(v, o);
+  __syncthreads();
+  if (lane_id() == 0) part[threadIdx.x / WAVE] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int w = 1; w < CW; w++) v += part[w];
+  return v;
+}
+
+__global__ __launch_bounds__(CT) void k_norm(ClipArgs a, double *parts) {
+  double sum = 0.0;
+  for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
+    const Chunk c = find_chunk(a, i);
+    sum += c.bf16 ? chunk_squares<true>(a.src[c.t], c) : chunk_squares<false>(a.src[c.t], c);
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+}
+
+/* the norm from its partial sums, in every thread */
+__device__ __forceinline__ float norm_of(const double *parts, int n_parts) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n_parts; i += CT) s += parts[i];
+  return (float)sqrt(block_sum(s));
+}
+
+__global__ __launch_bounds__(CT) void k_norm_write(const double *parts, int n_parts, float *norm) {
+  const float v = norm_of(parts, n_parts);
+  if (threadIdx.x == 0) *norm = v;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint4 scaled(uint4 q, float scale) {
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (BF16) {
+      const float x = d3s_u2f(w[i] << 16) * scale, y = d3s_u2f(w[i] & 0xffff0000u) * scale;
+      w[i] = (uint32_t)d3s_f32_to_bf16_rn(x) | (uint32_t)d3s_f32_to_bf16_rn(y) << 16;
+    } else {
+      w[i] = d3s_f2u(d3s_u2f(w[i]) * scale);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool BF16>
+__device__ __forceinline__ void scale_one(const void *p, void *d, int64_t j, float scale, bool keep) {
+  if constexpr (BF16) {
+    const uint16_t g = ((const uint16_t *)p)[j];
+    ((uint16_t *)d)[j] = keep ? g : d3s_f32_to_bf16_rn(d3s_u2f((uint32_t)g << 16) * scale);
+  } else {
+    const float g = ((const float *)p)[j];
+    ((float *)d)[j] = keep ? g : g * scale;
+  }
+}
+
+/* keep: the bits as they are (no clipping) */
+template <bool BF16>
+__device__ __forceinline__ void chunk_scale(const void *p, void *d, const Chunk &c, float scale, bool keep) {
+  const Span<BF16> s(c);
+  constexpr int ES = BF16 ? 2 : 4;
+  const uint4 *b = (const uint4 *)((const char *)p + s.body * ES);
+  char *o = (char *)d + s.body * ES; /* (at any element: the stores may be unaligned) */
+  int i = (int)threadIdx.x;
+  for (; i + (CU - 1) * CT < s.units; i += CU * CT) {
+    uint4 q[CU];
+#pragma unroll
+    for (int u = 0; u < CU; u++) q[u] = b[i + u * CT];
+#pragma unroll
+    for (int u = 0; u < CU; u++) {
+      if (!keep) q[u] = scaled<BF16>(q[u], scale);
+      __builtin_memcpy(o + (int64_t)(i + u * CT) * 16, &q[u], 16);
+    }
+  }
+  for (; i < s.units; i += CT) {
+    uint4 q = b[i];
+    if (!keep) q = scaled<BF16>(q, scale);
+    __builtin_memcpy(o + (int64_t)i * 16, &q, 16);
+  }
+  const int64_t h = s.head0 + threadIdx.x, e = s.tail0 + threadIdx.x;
+  if (h < s.head1) scale_one<BF16>(p, d, h, scale, keep);
+  if (e < s.tail1) scale_one<BF16>(p, d, e, scale, keep);
+}
+
+__global__ __launch_bounds__(CT) void k_clip(ClipArgs a, ClipOut out, const double *parts, int n_parts,
+                                             float max_norm, float *norm) {
+  const float v = norm_of(parts, n_parts);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
+  const bool keep = !(v > max_norm && v < __builtin_inff());
+  const float scale = max_norm / v;
+  for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
+    const Chunk c = find_chunk(a, a.chunks - 1 - i);
+    if (keep && out.dst[c.t] == a.src[c.t]) continue;
+    if (c.bf16)
+      chunk_scale<true>(a.src[c.t], out.dst[c.t], c, scale, keep);
+    else
+      chunk_scale<false>(a.src[c.t], out.dst[c.t], c, scale, keep);
+  }
+}
+
+int launches(int n_tensors) { return (n_tensors + CLIP_TENSORS - 1) / CLIP_TENSORS; }
+
+/* tensors [t0, t0 + n) and their chunks */
+void fill(ClipArgs &a, const void *const *src, const int64_t *numel, const int32_t *dtypes, int t0, int n) {
+  /* chunks of 4 KiB (a 16-byte unit a lane) up to 64 KiB, by what fills the workgroups */
+  auto units = [&](int i) {
+    const int size = dtypes[i] == D3S_DTYPE_BF16 ? 2 : 4;
+    return numel[i] == 0 ? (int64_t)0 : (numel[i] * size + (int64_t)((uintptr_t)src[i] & 15u) + 15) / 16;
+  };
+  int64_t total = 0;
+  for (int i = t0; i < t0 + n; i++) total += units(i);
+  int64_t chunk = CT;
+  while (chunk < 16 * CT && total > chunk * CLIP_GROUPS) chunk *= 2;
+  for (;;) { /* (chunk numbers are 32 bits) */
+    int64_t at = 0;
+    for (int i = 0; i < n; i++) {
+      a.src[i] = src[t0 + i];
+      a.first[i] = (uint32_t)at;
+      a.numel[i] = (uint64_t)numel[t0 + i] << 1 | (dtypes[t0 + i] == D3S_DTYPE_BF16 ? 1u : 0u);
+      at += (units(t0 + i) + chunk - 1) / chunk;
+    }
+    a.n = n;
+    a.chunks = (uint32_t)at;
+    a.chunk = (uint32_t)chunk;
+    if (at <= 0x7fffffff || chunk >= (int64_t)1 << 30) return;
+    chunk *= 2;
+  }
+}
+
+}  // namespace
+
+size_t clip_workspace_bytes(int n_tensors) {
+  const size_t parts = (size_t)launches(n_tensors > 0 ? n_tensors : 1) * CLIP_GROUPS;
+  return split_counter_bytes() + parts * sizeof(double);
+}
+
+void launch_clip(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int n_tensors,
+                 float max_norm, float *norm, void *ws, hipStream_t s) {
+  double *parts = (double *)((char *)ws + split_counter_bytes());
+  ClipArgs a;
+  int n_parts = 0;
+  for (int t0 = 0; t0 < n_tensors; t0 += CLIP_TENSORS) {
+    fill(a, src, numel, dtypes, t0, min(n_tensors - t0, CLIP_TENSORS));
+    if (a.chunks == 0) continue;
+    const int groups = min((int)min(a.chunks, 0x7fffffffu), CLIP_GROUPS);
+    k_norm<<<groups, CT, 0, s>>>(a, parts + n_parts);
+    n_parts += groups;
+  }
+  bool written = false;
+  for (int t0 = 0; dst && n_parts > 0 && t0 < n_tensors; t0 += CLIP_TENSORS) {
+    const int n = min(n_tensors - t0, CLIP_TENSORS);
+    fill(a, src, numel, dtypes, t0, n);
+    if (a.chunks == 0) continue;
+    ClipOut o;
+    for (int i = 0; i < n; i++) o.dst[i] = dst[t0 + i];
+    const int groups = min((int)min(a.chunks, 0x7fffffffu), 2 * CLIP_GROUPS);
+    k_clip<<<groups, CT, 0, s>>>(a, o, parts, n_parts, max_norm, written ? nullptr : norm);
+    written = true;
+  }
+  if (!written) k_norm_write<<<1, CT, 0, s>>>(parts, n_parts, norm);
+}
+
+}  // namespace d3s

@@ -28,6 +28,9 @@ ERR_SCRATCH = -6
 ERR_WORKSPACE = -7
 SCRATCH_BYTES = 4 << 20
 MAX_VOCAB = (1 << 24) - 1
+MAX_TOKENS = 64
+MAX_TOP = 64
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # D3S_ACT_*
 
 _lib = None
 
@@ -39,6 +42,16 @@ class RasParams(ctypes.Structure):
                 ("retry_top_k", ctypes.c_int), ("eos_id", ctypes.c_int32),
                 ("semantic_start", ctypes.c_int32), ("semantic_end", ctypes.c_int32),
                 ("code_vocab", ctypes.c_int32)]
+
+
+class DenseParams(ctypes.Structure):
+    """d3s_dense_params (include/d3s_train.h)"""
+    _fields_ = [("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_transposed", ctypes.c_int),
+                ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64), ("w_transposed", ctypes.c_int),
+                ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("bias", ctypes.c_void_p),
+                ("activation", ctypes.c_int), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+                ("z", ctypes.c_void_p), ("z_stride", ctypes.c_int64), ("y", ctypes.c_void_p),
+                ("y_stride", ctypes.c_int64), ("y_dtype", ctypes.c_int)]
 
 
 def ras_params(**kw):
@@ -106,6 +119,31 @@ def lib():
         L.d3s_exp2_selftest.restype = i32
         L.d3s_log2_selftest.argtypes = [vp, vp, i64, vp]
         L.d3s_log2_selftest.restype = i32
+        rows = [vp, i32, i64, i64, i64, vp, f32, vp, vp, i32]
+        scores = rows + [vp, vp, vp, i32, vp, vp, vp]
+        L.d3s_logprob.argtypes = scores + [vp]
+        L.d3s_logprob_ws.argtypes = scores + [vp, i64, vp]
+        L.d3s_logprob_workspace_bytes.argtypes = [i32, i64, i64, i32]
+        L.d3s_logprob_backward.argtypes = rows + [vp, vp, vp, vp, vp, i64, vp]
+        dense = ctypes.POINTER(DenseParams)
+        L.d3s_dense_bf16.argtypes = [dense, vp]
+        L.d3s_dense_bf16_ws.argtypes = [dense, vp, i64, vp]
+        L.d3s_dense_workspace_bytes.argtypes = [dense]
+        slopes = [vp, i64, vp, i64, i64, i64, i32, vp, i64, vp]
+        L.d3s_dense_activation_backward_bf16.argtypes = slopes + [vp]
+        L.d3s_dense_activation_backward_bf16_ws.argtypes = slopes + [vp, i64, vp]
+        L.d3s_dense_activation_backward_workspace_bytes.argtypes = [i64, i64, i32]
+        clip = [vp, vp, vp, vp, i32, f32, vp]
+        L.d3s_clip_grads.argtypes = clip + [vp]
+        L.d3s_clip_grads_ws.argtypes = clip + [vp, i64, vp]
+        L.d3s_clip_grads_workspace_bytes.argtypes = [i32]
+        for f in (L.d3s_logprob, L.d3s_logprob_ws, L.d3s_logprob_backward, L.d3s_dense_bf16, L.d3s_dense_bf16_ws,
+                  L.d3s_dense_activation_backward_bf16, L.d3s_dense_activation_backward_bf16_ws, L.d3s_clip_grads,
+                  L.d3s_clip_grads_ws):
+            f.restype = i32
+        for f in (L.d3s_logprob_workspace_bytes, L.d3s_dense_workspace_bytes,
+                  L.d3s_dense_activation_backward_workspace_bytes, L.d3s_clip_grads_workspace_bytes):
+            f.restype = i64
         L.d3s_version.argtypes = []
         L.d3s_version.restype = ctypes.c_char_p
         L.d3_sample.argtypes = [vp, i32, i32, f32, i32, f32, ctypes.c_ulonglong, vp]
@@ -411,3 +449,68 @@ def linear_sample_bf16(x, w, u, temperature, top_p, flags=0, want_probs=True, ke
     for b in bufs.values():
         b.free()
     return out
+
+
+# ---- scoring and training (include/d3s_train.h), on device pointers (ints) ----
+def _temperature(temperature):
+    return (temperature[1], 0.0) if isinstance(temperature, tuple) else (None, temperature)
+
+
+def logprob_raw(logits, dtype, n_rows, vocab, row_stride, temperature, banned, tokens, n_tokens, logprobs,
+                entropy=None, row_stats=None, n_top=0, top_ids=None, top_logprobs=None, counters=None, stream=None,
+                workspace=None):
+    """d3s_logprob, or d3s_logprob_ws with workspace = (address, bytes).
+    temperature: a float, or a device pointer as ("ptr", address)."""
+    t_ptr, t_s = _temperature(temperature)
+    args = (logits, dtype, n_rows, vocab, row_stride, t_ptr, t_s, banned, tokens, n_tokens, logprobs, entropy,
+            row_stats, n_top, top_ids, top_logprobs, counters)
+    if workspace is not None:
+        return lib().d3s_logprob_ws(*args, workspace[0], workspace[1], stream)
+    return lib().d3s_logprob(*args, stream)
+
+
+def logprob_backward_raw(logits, dtype, n_rows, vocab, row_stride, temperature, banned, tokens, n_tokens, row_stats,
+                         entropy, grad_logprobs, grad_entropy, grad_logits, grad_row_stride, stream=None):
+    """d3s_logprob_backward; temperature as in logprob_raw."""
+    t_ptr, t_s = _temperature(temperature)
+    return lib().d3s_logprob_backward(logits, dtype, n_rows, vocab, row_stride, t_ptr, t_s, banned, tokens, n_tokens,
+                                      row_stats, entropy, grad_logprobs, grad_entropy, grad_logits, grad_row_stride,
+                                      stream)
+
+
+def dense_params(x, x_stride, w, w_stride, m, n, k, y, y_stride, y_dtype, x_transposed=False, w_transposed=False,
+                 bias=None, activation=0, residual=None, residual_stride=0, z=None, z_stride=0):
+    return DenseParams(x, x_stride, x_transposed, w, w_stride, w_transposed, m, n, k, bias, activation, residual,
+                       residual_stride, z, z_stride, y, y_stride, y_dtype)
+
+
+def dense_raw(x, x_stride, w, w_stride, m, n, k, y, y_stride, y_dtype, x_transposed=False, w_transposed=False,
+              bias=None, activation=0, residual=None, residual_stride=0, z=None, z_stride=0, stream=None,
+              workspace=None):
+    """d3s_dense_bf16: y [m, n] = residual + act(x w^T + bias), or
+    d3s_dense_bf16_ws with workspace = (address, bytes)."""
+    p = DenseParams(x, x_stride, x_transposed, w, w_stride, w_transposed, m, n, k, bias, activation, residual,
+                    residual_stride, z, z_stride, y, y_stride, y_dtype)
+    if workspace is not None:
+        return lib().d3s_dense_bf16_ws(ctypes.byref(p), workspace[0], workspace[1], stream)
+    return lib().d3s_dense_bf16(ctypes.byref(p), stream)
+
+
+def dense_activation_backward_raw(dy, dy_stride, z, z_stride, m, n, activation, dz, dz_stride, dbias, stream=None,
+                                  workspace=None):
+    """d3s_dense_activation_backward_bf16, or its _ws form with workspace =
+    (address, bytes)."""
+    args = (dy, dy_stride, z, z_stride, m, n, activation, dz, dz_stride, dbias)
+    if workspace is not None:
+        return lib().d3s_dense_activation_backward_bf16_ws(*args, workspace[0], workspace[1], stream)
+    return lib().d3s_dense_activation_backward_bf16(*args, stream)
+
+
+def clip_grads_raw(src, dst, numel, dtypes, n_tensors, max_norm, norm, stream=None, workspace=None):
+    """d3s_clip_grads, or its _ws form with workspace = (address, bytes).  src,
+    dst, numel, dtypes: host arrays' addresses (uint64, uint64 or None, int64,
+    int32 per tensor)."""
+    args = (src, dst, numel, dtypes, n_tensors, max_norm, norm)
+    if workspace is not None:
+        return lib().d3s_clip_grads_ws(*args, workspace[0], workspace[1], stream)
+    return lib().d3s_clip_grads(*args, stream)
