@@ -88,10 +88,10 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
 }
 
 /* 16 columns a workgroup, 16 threads a column, each a sixteenth of the runs */
-__global__ __launch_bounds__(AT) void k_column_sums(const float *parts, int runs, int n, float *dbias) {
+__global__ __launch_bounds__(AT) void k_column_sums(const float *parts, int runs, int n, int group0, float *dbias) {
   __shared__ float sum[16][17];
   const int c = (int)threadIdx.x % 16, q = (int)threadIdx.x / 16;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  const int64_t col = ((int64_t)group0 + blockIdx.x) * 16 + c;
   const int per = (runs + 15) / 16, r1 = min(runs, (q + 1) * per);
   float v = 0.0f;
   if (col < n) {
@@ -130,7 +130,7 @@ void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s) {
   /* (at most 2^27 workgroups: 2^35 threads would pass the launch's count) */
   for (int64_t g = 0; g < groups; g += GRID_MOST)
     k_column_sums<<<dim3((unsigned)min((int64_t)GRID_MOST, groups - g)), AT, 0, s>>>(
-        parts + g * 16, sp.runs, a.n, a.dbias + g * 16);
+        parts, sp.runs, a.n, (int)g, a.dbias);
 }
 
 }  // namespace d3s

@@ -158,9 +158,9 @@ __device__ __forceinline__ void add_batch(Sums &s, const float *v, float c) {
 }
 
 struct ScoreLds {
-  uint64_t list[LIST + 2];
+  alignas(16) uint64_t list[LIST + 2]; /* (read in pairs, the next in fours) */
   uint64_t ranked[D3S_MAX_TOP];
-  uint32_t lane_max[ST];
+  alignas(16) uint32_t lane_max[ST];
   float wm[SW], wS[SW], wA[SW];
   uint64_t bound;
   uint32_t count, last;
