@@ -70,7 +70,7 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
         if (e < left) {
           const float v = one(bf(a.dy[i * a.dy_stride + j + e]), a.z ? bf(a.z[i * a.z_stride + j + e]) : 0.0f);
           acc[e] += v;
-          if (a.dz) a.dz[i * a.dz_stride + j + e] = d3s_f32_to_bf16_rn(v);
+          if (a.dz) a.dz[i * a.dz_stride + j + e] = pack1(v);
         }
   }
   if constexpr (SUM) {

@@ -1,0 +1,428 @@
+/* k_tile: a tile of y = residual + act(x w^T + bias) on the matrix cores, bf16
+ * operands in either order, fp32 sums (gfx950, wave64; include/d3s_train.h).
+ * Device code and its launch; each order of the operands is a translation unit.
+ *
+ * A workgroup of four waves owns TM x TN outputs; the inner length runs in
+ * stages of 64, each operand's stage in LDS as [row][64]: rows of eight 16-byte
+ * chunks, chunk c of row r at place c ^ (r ^ r / 8) % 8, so that a wave's reads
+ * (one chunk of 32 rows) and its writes touch every bank alike.
+ * Two stages lie in LDS.  Fragments are read one step of 16 ahead of the matrix
+ * instructions; the last step of a stage runs after the barrier that frees it,
+ * so the next stage's first reads, and the filling of the freed one, hide
+ * behind its products.
+ * A stage reaches LDS directly (operands stored by rows, at 16 bytes), through
+ * registers as it is (the same at any other element), or through registers and
+ * turned (operands stored by the inner index: a thread holds 8 rows of R / 32
+ * inner indices and writes each row's together). */
+#ifndef D3S_DENSE_TILE_H
+#define D3S_DENSE_TILE_H
+
+#include <type_traits>
+
+#include "d3s_dense.h"
+#include "d3s_epilogue.h"
+
+namespace d3s {
+namespace {
+
+constexpr int TT = 256;        /* threads of a workgroup */
+constexpr int TK = TILE_K;     /* the inner length of a stage */
+constexpr int STEP = 16;       /* ... of a matrix instruction */
+constexpr unsigned TILE_GRID = 1 << 22; /* workgroups a launch: their threads are counted in 32 bits */
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+#define D3S_LDS __attribute__((address_space(3)))
+#define D3S_GLOBAL __attribute__((address_space(1)))
+
+/* elements [at, at + 8) of a stored row of `len`, zeros past its end (at < len) */
+__device__ __forceinline__ uint4 row_chunk(const uint16_t *row, int64_t at, int64_t len) {
+  uint64_t v[2] = {0u, 0u};
+  if (len >= 8) { /* near its end the row's last eight, moved down */
+    const int64_t from = at < len - 8 ? at : len - 8;
+    __builtin_memcpy(v, row + from, 16);
+    const int s = (int)(at - from) * 16; /* 0 .. 112 */
+    const uint64_t hi = v[1];
+    v[1] = s < 64 ? hi >> s : 0u;
+    v[0] = s == 0 ? v[0] : s < 64 ? v[0] >> s | hi << (64 - s) : hi >> (s - 64);
+  } else {
+#pragma nounroll
+    for (int64_t e = len - 1; e >= at; e--) {
+      v[1] = v[1] << 16 | v[0] >> 48;
+      v[0] = v[0] << 16 | row[e];
+    }
+  }
+  return make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
+}
+
+/* how an operand's stages reach LDS */
+enum Way { DIRECT, ROWS, TURNED };
+
+/* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED: stored [k, rows]). */
+template <int R, Way WAY>
+struct Part {
+  static constexpr int BYTES = R * TK * 2;
+  static constexpr int PER = R * TK / 8 / TT;                      /* 16-byte loads a thread */
+  static constexpr int DIRECTS = WAY == DIRECT ? PER : 0;          /* of them into LDS */
+  static constexpr int LOADS = WAY == DIRECT ? 0 : PER;            /* ... into registers */
+  static constexpr int WRITES = WAY == DIRECT ? 0 : WAY == ROWS ? PER : 8; /* and from them */
+  const uint16_t *p;
+  int64_t stride;
+  int rows, r0;
+  uint32_t off[WAY == DIRECT ? PER : 1]; /* bytes from the tile's first row, and where that is */
+  __amdgpu_buffer_rsrc_t from;
+  const uint16_t *mine;                  /* ROWS, TURNED: the thread's first chunk of stage 0 */
+  int to;                                /* TURNED: its first row in LDS (below 0: not the tile's) */
+  uint4 q[PER];
+
+  static __device__ __forceinline__ int tid() { return (int)threadIdx.x; }
+  static __device__ __forceinline__ int turn(int r) { return (r ^ r >> 3) & 7; }
+  /* DIRECT, ROWS: the u-th place's row and chunk (eight places a row, in order) */
+  static __device__ __forceinline__ int row(int u) { return (u * TT + tid()) / 8; }
+  static __device__ __forceinline__ int chunk(int u) { return tid() % 8 ^ turn(row(u)); }
+  /* TURNED: the thread's inner indices inside a stage, PER of them from here */
+  static __device__ __forceinline__ int inner() { return tid() / (R / 8) * PER; }
+
+  __device__ __forceinline__ Part(const uint16_t *base, int64_t st, int n, int first)
+      : p(base), stride(st), rows(n), r0(first) {
+    /* rows past the end are the last one again: their outputs are not written */
+    if constexpr (WAY == DIRECT) {
+      from = __builtin_amdgcn_make_buffer_rsrc((void *)(p + (int64_t)r0 * stride), 0, -1, 0x00020000);
+#pragma unroll
+      for (int u = 0; u < PER; u++) off[u] = (uint32_t)(min(row(u), rows - 1 - r0) * stride + chunk(u) * 8) * 2u;
+    } else if constexpr (WAY == TURNED) {
+      /* eight rows that end with the last (written twice, the same), where there are eight */
+      to = tid() % (R / 8) * 8;
+      if (rows >= 8) to = min(to, rows - 8 - r0);
+      mine = p + (int64_t)inner() * stride + (r0 + to);
+    }
+  }
+  /* the u-th 16 bytes of stage k0, straight into LDS (a buffer load: one 32-bit
+   * register of address a lane; the sum of its offsets stays below 2^32) */
+  __device__ __forceinline__ void direct(int u, int k0, char *lds) const {
+    const int wid = __builtin_amdgcn_readfirstlane(tid() / WAVE);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (D3S_LDS void *)(lds + (u * TT + wid * WAVE) * 16), 16, (int)off[u],
+                                             k0 * 2, 0, 0);
+  }
+  /* the same into registers, from start(k0): a whole stage, at least eight rows if TURNED */
+  __device__ __forceinline__ const uint16_t *start(int k0) const {
+    return WAY == TURNED ? mine + (int64_t)k0 * stride : p + k0;
+  }
+  __device__ __forceinline__ void load(int u, const uint16_t *at) {
+    if constexpr (WAY == ROWS)
+      q[u] = load16(at + ((int64_t)min(r0 + row(u), rows - 1) * stride + chunk(u) * 8));
+    else
+      q[u] = load16(at + u * stride);
+  }
+  /* the same of any stage: something finite or not from k1 on */
+  __device__ __forceinline__ void load_some(int k0, int k1) {
+#pragma unroll
+    for (int u = 0; u < PER; u++) {
+      if constexpr (WAY == TURNED) {
+        const uint16_t *at = p + (int64_t)min(k0 + inner() + u, k1 - 1) * stride;
+        if (rows >= 8)
+          q[u] = load16(at + (r0 + to));
+        else
+          q[u] = r0 + to < rows ? row_chunk(at, r0 + to, rows) : make_uint4(0u, 0u, 0u, 0u);
+      } else {
+        const int k = k0 + chunk(u) * 8;
+        const uint16_t *at = p + (int64_t)min(r0 + row(u), rows - 1) * stride;
+        q[u] = k >= k1 ? make_uint4(0u, 0u, 0u, 0u) : WAY == DIRECT ? load16(at + k) : row_chunk(at, k, k1);
+      }
+    }
+  }
+  /* the v-th write of the registers into a stage (rows that are not the tile's: to `spare`) */
+  __device__ __forceinline__ void write(int v, char *lds, char *spare) const {
+    if constexpr (WAY != TURNED) {
+      *(uint4 *)(lds + (v * TT + tid()) * 16) = q[v];
+    } else if constexpr (WAY == TURNED) {
+      uint32_t w[PER > 1 ? PER / 2 : 1];
+      auto word = [&](int u) { return v < 2 ? q[u].x : v < 4 ? q[u].y : v < 6 ? q[u].z : q[u].w; };
+#pragma unroll
+      for (int u = 0; u + 1 < PER; u += 2)
+        w[u / 2] = __builtin_amdgcn_perm(word(u + 1), word(u), v & 1 ? 0x07060302u : 0x05040100u);
+      const int r = to + v, k = inner();
+      char *at = r < 0 ? spare : lds + (r * (TK * 2) + (k / 8 ^ turn(r)) * 16 + k % 8 * 2);
+      if constexpr (PER == 8)
+        *(uint4 *)at = make_uint4(w[0], w[1], w[2], w[3]);
+      else if constexpr (PER == 4)
+        *(uint2 *)at = make_uint2(w[0], w[1]);
+      else if constexpr (PER == 2)
+        *(uint32_t *)at = w[0];
+      else
+        *(uint16_t *)at = (uint16_t)(word(0) >> (16 * (v & 1)));
+    }
+  }
+  __device__ __forceinline__ void write_all(char *lds, char *spare) const {
+#pragma unroll
+    for (int v = 0; v < (WAY == TURNED ? 8 : PER); v++) write(v, lds, spare);
+  }
+  /* the fragment of rows r .. r + 31 (r a multiple of 32), inner indices 16 step .. + 15 */
+  static __device__ __forceinline__ bf16x8 fragment(const char *lds, int r, int step) {
+    const int at = r + (lane_id() & 31), c = (step * 2 + (lane_id() >> 5)) ^ turn(at);
+    return *(const bf16x8 *)(lds + at * (TK * 2) + c * 16);
+  }
+};
+
+/* all but the last N loads of the wave are there, and its reads of LDS; then every wave's */
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 7 << 4 | (N >> 4) << 14); /* vmcnt N, lgkmcnt 0 */
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int TM, int TN, int WAVES_M, Way WX, Way WW>
+__global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operands a, Out o, TilePlan pl) {
+  constexpr int WAVES_N = 4 / WAVES_M;
+  constexpr int WM = TM / WAVES_M, WN = TN / WAVES_N, FM = WM / 32, FN = WN / 32;
+  constexpr int STEPS = TK / STEP;
+  using PX = Part<TM, WX>;
+  using PW = Part<TN, WW>;
+  constexpr int STAGE = PX::BYTES + PW::BYTES;
+  constexpr int OUT_ROW = WN + 4; /* a row of outputs in LDS, fp32 */
+  constexpr int OUT_BYTES = 4 * 32 * OUT_ROW * 4;
+  constexpr int ROOM = 2 * STAGE > OUT_BYTES ? 2 * STAGE : OUT_BYTES;
+  __shared__ __attribute__((aligned(1024))) char lds[ROOM + 16];
+  char *spare = lds + ROOM;
+
+  /* workgroups go to the eight XCDs in turn: each takes a run of neighbouring
+   * tiles, in columns of eight, whose operands its L2 then holds */
+  const unsigned turn = blockIdx.x % 8, each = gridDim.x / 8;
+  const unsigned t = pl.first + turn * each + min(turn, gridDim.x % 8) + blockIdx.x / 8;
+  const unsigned split = t / pl.tiles, tile = t % pl.tiles;
+  const unsigned wide = pl.group * pl.n_tiles, band = tile / wide, in = tile % wide;
+  const unsigned high = min(pl.group, pl.m_tiles - band * pl.group); /* tiles in a column of the band */
+  const int i0 = pl.i0 + (int)(band * pl.group + in % high) * TM, j0 = pl.j0 + (int)(in / high) * TN;
+
+  const int lane = lane_id(), wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
+  const int wi = wid / WAVES_N * WM, wj = wid % WAVES_N * WN; /* the wave's rows and outputs */
+  PX px(a.x, a.x_stride, o.m, i0);
+  PW pw(a.w, a.w_stride, o.n, j0);
+
+  f32x16 acc[FM][FN];
+#pragma unroll
+  for (int p = 0; p < FM; p++)
+#pragma unroll
+    for (int q = 0; q < FN; q++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[p][q][i] = 0.0f;
+
+  const int whole = a.k / TK;
+  const int s0 = min(whole, (int)split * pl.stages);
+  const int s1 = split == pl.splits - 1 ? whole : min(whole, s0 + pl.stages);
+  bf16x8 fx[2][FM], fw[2][FN];
+  auto read = [&](int to, const char *stage, int step, int f) {
+    if (f < FM)
+      fx[to][f] = PX::fragment(stage, wi + f * 32, step);
+    else
+      fw[to][f - FM] = PW::fragment(stage + PX::BYTES, wj + (f - FM) * 32, step);
+  };
+  auto read_all = [&](int to, const char *stage, int step) {
+#pragma unroll
+    for (int f = 0; f < FM + FN; f++) read(to, stage, step, f);
+  };
+  constexpr int DIRECTS = PX::DIRECTS + PW::DIRECTS, LOADS = PX::LOADS + PW::LOADS, WRITES = PX::WRITES + PW::WRITES;
+  auto direct = [&](int u, int k0, char *to) {
+    if (u < PX::DIRECTS)
+      px.direct(u, k0, to);
+    else
+      pw.direct(u - PX::DIRECTS, k0, to + PX::BYTES);
+  };
+  struct Start {
+    const uint16_t *x, *w;
+  };
+  auto start = [&](int k0) { return Start{px.start(k0), pw.start(k0)}; };
+  auto load = [&](int u, const Start &at) {
+    if (u < PX::LOADS)
+      px.load(u, at.x);
+    else
+      pw.load(u - PX::LOADS, at.w);
+  };
+  auto write = [&](int v, char *to) {
+    if (v < PX::WRITES)
+      px.write(v, to, spare);
+    else
+      pw.write(v - PX::WRITES, to + PX::BYTES, spare);
+  };
+  /* the products of fragments `from`; after the n-th of them, and pinned there,
+   * beside(n): its share of what goes on meanwhile */
+  constexpr int PRODUCTS = FM * FN;
+  auto multiply = [&](int from, auto beside) {
+#pragma unroll
+    for (int n = 0; n < PRODUCTS; n++) {
+      const int p = n / FN, q = n % FN;
+      acc[p][q] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[from][q], fx[from][p], acc[p][q], 0, 0, 0);
+      beside(n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  /* product n's share of `of` things spread over the products from `from` to `to` */
+  auto share = [](int n, int from, int to, int of, auto each) {
+    const int size = (of + to - from - 1) / (to - from), i0 = (n - from) * size;
+#pragma unroll
+    for (int i = i0; i < i0 + size; i++)
+      if (n >= from && n < to && i < of) each(i);
+  };
+  /* Direct loads: the issue of one takes longer than a product hides beside an
+   * LDS read, so they follow the reads, half of them in the next stage's first
+   * step.  With operands through registers they come last (an LDS write behind
+   * them would wait for them), all at once. */
+  constexpr int LATE = LOADS == 0 ? DIRECTS / 2 : 0, SOON = DIRECTS - LATE, HALF = PRODUCTS / 2;
+  constexpr int WRITTEN = DIRECTS > 0 ? HALF : PRODUCTS;
+
+  /* TURNED operands of fewer than eight rows have no whole loads */
+  const int full = (WX == TURNED && o.m < 8) || (WW == TURNED && o.n < 8) ? s0 : s1;
+  if (s0 < full) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const int k0 = min(s0 + b, s1 - 1) * TK;
+      const Start at = start(k0);
+#pragma unroll
+      for (int u = 0; u < LOADS; u++) load(u, at);
+#pragma unroll
+      for (int u = 0; u < (b == 0 ? DIRECTS : SOON); u++) direct(u, k0, lds + b * STAGE);
+#pragma unroll
+      for (int v = 0; v < WRITES; v++) write(v, lds + b * STAGE);
+    }
+    stage_barrier<SOON>();
+    read_all(0, lds, 0);
+    char *here = lds;
+    for (int s = s0; s < s1; s++) { /* (the last two stages fill buffers that nothing reads) */
+      char *next = here == lds ? lds + STAGE : lds;
+      const int near = min(s + 1, s1 - 1) * TK, far = min(s + 2, s1 - 1) * TK;
+      const Start at = start(far);
+#pragma unroll
+      for (int j = 0; j < STEPS - 1; j++)
+        multiply(j & 1, [&](int n) {
+          share(n, 0, PRODUCTS, FM + FN, [&](int f) { read((j + 1) & 1, here, j + 1, f); });
+          if (j == 0) share(n, HALF, PRODUCTS, LATE, [&](int u) { direct(SOON + u, near, next); });
+          if (j == 0) share(n, 0, PRODUCTS, LOADS, [&](int u) { load(u, at); });
+        });
+      stage_barrier<LOADS>();
+      multiply(1, [&](int n) {
+        share(n, 0, PRODUCTS, FM + FN, [&](int f) { read(0, next, 0, f); });
+        share(n, 0, WRITTEN, WRITES, [&](int v) { write(v, here); });
+        share(n, HALF, PRODUCTS, SOON, [&](int u) { direct(u, far, here); });
+      });
+      here = next;
+    }
+  }
+  /* the rest of the inner length, what whole loads do not reach: zeros from its end on */
+  const int end = split == pl.splits - 1 ? a.k : s1 * TK;
+  for (int k0 = full * TK; k0 < end; k0 += TK) {
+    px.load_some(k0, end);
+    pw.load_some(k0, end);
+    stage_barrier<0>();
+    px.write_all(lds, spare);
+    pw.write_all(lds + PX::BYTES, spare);
+    stage_barrier<0>();
+#pragma nounroll
+    for (int j = 0; j < STEPS && k0 + j * STEP < end; j++) {
+      read_all(0, lds, j);
+      const int n = end - (k0 + j * STEP + (lane >> 5) * 8); /* of the lane's eight */
+      uint4 mask;
+      auto some = [&](int d) { return n >= 2 * d + 2 ? ~0u : n == 2 * d + 1 ? 0xffffu : 0u; };
+      mask = make_uint4(some(0), some(1), some(2), some(3));
+      auto cut = [&](bf16x8 &f) {
+        uint4 v = __builtin_bit_cast(uint4, f);
+        f = __builtin_bit_cast(bf16x8, make_uint4(v.x & mask.x, v.y & mask.y, v.z & mask.z, v.w & mask.w));
+      };
+#pragma unroll
+      for (int p = 0; p < FM; p++) cut(fx[0][p]);
+#pragma unroll
+      for (int q = 0; q < FN; q++) cut(fw[0][q]);
+      multiply(0, [](int) {});
+    }
+  }
+
+  /* Each wave's outputs, 32 rows at a time, through its part of LDS, so that
+   * a row leaves in whole lines.  Lane l holds row l % 32, and four neighbouring
+   * outputs from 8 i + 4 (l / 32) in registers 4 i .. 4 i + 3.  One copy of the
+   * code that writes rows (unrolled four times it does not fit the instruction
+   * cache); the residual's rows are loaded 32 ahead. */
+  stage_barrier<0>();
+  constexpr int ACROSS = WN / 8, DOWN = WAVE / ACROSS, ROUNDS = 32 / DOWN;
+  float *mine = (float *)lds + wid * 32 * OUT_ROW;
+  const int i_at = i0 + wi + lane / ACROSS, j_at = j0 + wj + lane % ACROSS * 8;
+  const uint4 bias = bias_eight(o, j_at);
+  const bool works = o.bias || o.z || o.act != D3S_ACT_NONE;
+  Eight ahead[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; r++) get_eight(o, i_at + r * DOWN, j_at, ahead[r]);
+#pragma nounroll
+  for (int p = 0; p < FM; p++) {
+    wave_lds_sync();
+#pragma unroll
+    for (int c = 0; c < FM; c++)
+      if (c == p) {
+#pragma unroll
+        for (int q = 0; q < FN; q++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            *(f32x4 *)(mine + (lane & 31) * OUT_ROW + q * 32 + i * 8 + (lane >> 5) * 4) =
+                f32x4{acc[c][q][4 * i], acc[c][q][4 * i + 1], acc[c][q][4 * i + 2], acc[c][q][4 * i + 3]};
+      }
+    wave_lds_sync();
+    Eight now[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) now[r] = ahead[r];
+    if (p + 1 < FM) {
+#pragma unroll
+      for (int r = 0; r < ROUNDS; r++) get_eight(o, i_at + (p + 1) * 32 + r * DOWN, j_at, ahead[r]);
+    }
+    float *row = mine + lane / ACROSS * OUT_ROW + lane % ACROSS * 8;
+    if (works) {
+#pragma nounroll
+      for (int r = 0; r < ROUNDS; r++)
+        activate_eight(o, i_at + p * 32 + r * DOWN, j_at, row + r * DOWN * OUT_ROW, bias);
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++)
+      put_eight(o, i_at + p * 32 + r * DOWN, j_at, row + r * DOWN * OUT_ROW, now[r]);
+    if (j_at < o.n && j_at + 8 > o.n) {
+#pragma nounroll
+      for (int r = 0; r < 32; r += DOWN)
+        for (int e = 0; e < o.n - j_at && i_at + p * 32 + r < o.m; e++)
+          put_one(o, i_at + p * 32 + r, j_at + e, row[r * OUT_ROW + e]);
+    }
+  }
+}
+
+template <int TM, int TN, int WAVES_M, Way WX, Way WW>
+void launch_ways(const Operands &a, const Out &o, TilePlan pl, hipStream_t s) {
+  const unsigned all = pl.tiles * pl.splits;
+  for (pl.first = 0; pl.first < all; pl.first += TILE_GRID)
+    k_tile<TM, TN, WAVES_M, WX, WW><<<dim3(min(TILE_GRID, all - pl.first)), TT, 0, s>>>(a, o, pl);
+}
+
+template <int TM, int TN, int WAVES_M, bool XT, bool WT>
+void launch_shape(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
+  constexpr Way X = XT ? TURNED : DIRECT, W = WT ? TURNED : DIRECT, XR = XT ? TURNED : ROWS, WR = WT ? TURNED : ROWS;
+  if (!XT && !pl.x_direct) {
+    if (!WT && !pl.w_direct)
+      launch_ways<TM, TN, WAVES_M, XR, WR>(a, o, pl, s);
+    else
+      launch_ways<TM, TN, WAVES_M, XR, W>(a, o, pl, s);
+  } else {
+    if (!WT && !pl.w_direct)
+      launch_ways<TM, TN, WAVES_M, X, WR>(a, o, pl, s);
+    else
+      launch_ways<TM, TN, WAVES_M, X, W>(a, o, pl, s);
+  }
+}
+
+}  // namespace
+
+template <bool XT, bool WT>
+void launch_tiles(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
+  if (pl.tm == 256)
+    launch_shape<256, 256, 2, XT, WT>(a, o, pl, s);
+  else
+    launch_shape<128, 128, 2, XT, WT>(a, o, pl, s);
+}
+
+}  // namespace d3s
+
+#endif

@@ -3,8 +3,8 @@
 #ifndef D3S_EPILOGUE_H
 #define D3S_EPILOGUE_H
 
+#include "d3s_dense.h"
 #include "d3s_device.h"
-#include "d3s_train_internal.h"
 
 namespace d3s {
 namespace {
@@ -20,16 +20,32 @@ constexpr float GELU_A = 0.044715f;
 
 __device__ __forceinline__ float tanh_of(float u) { return 1.0f - 2.0f / (1.0f + __expf(2.0f * u)); }
 
-__device__ __forceinline__ float activate(float z, int act) {
+template <int ACT>
+__device__ __forceinline__ float activated(float z) {
   /* far below, z times a probability that is 0 in fp32 (-inf times it would be NaN) */
-  if (act > D3S_ACT_RELU && z < -100.0f) return 0.0f;
-  switch (act) {
+  if (ACT > D3S_ACT_RELU && z < -100.0f) return 0.0f;
+  switch (ACT) {
     case D3S_ACT_RELU: return z < 0.0f ? 0.0f : z; /* (a NaN stays one) */
     case D3S_ACT_SILU: return z * logistic(z);
     case D3S_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
     case D3S_ACT_GELU_TANH: return 0.5f * z * (1.0f + tanh_of(GELU_C * z * fmaf(GELU_A * z, z, 1.0f)));
   }
   return z;
+}
+template <int ACT, int N>
+__device__ __forceinline__ void activate_each(float *z) {
+#pragma unroll
+  for (int e = 0; e < N; e++) z[e] = activated<ACT>(z[e]);
+}
+/* (one branch for all N) */
+template <int N>
+__device__ __forceinline__ void activate(float *z, int act) {
+  switch (act) {
+    case D3S_ACT_RELU: activate_each<D3S_ACT_RELU, N>(z); break;
+    case D3S_ACT_SILU: activate_each<D3S_ACT_SILU, N>(z); break;
+    case D3S_ACT_GELU: activate_each<D3S_ACT_GELU, N>(z); break;
+    case D3S_ACT_GELU_TANH: activate_each<D3S_ACT_GELU_TANH, N>(z); break;
+  }
 }
 
 __device__ __forceinline__ float slope(float z, int act) {
@@ -53,76 +69,102 @@ __device__ __forceinline__ float slope(float z, int act) {
 
 __device__ __forceinline__ float bf(uint16_t b) { return d3s_u2f((uint32_t)b << 16); }
 
-/* what a product's kernel needs to write its outputs */
-struct Out {
-  const uint16_t *bias;
-  const void *residual;
-  uint16_t *z;
-  void *y;
-  int64_t residual_stride, z_stride, y_stride;
-  int m, n, act;
-  bool f32;
-};
+/* two rounded to bf16, to nearest even */
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+__device__ __forceinline__ uint16_t pack1(float a) { return (uint16_t)pack2(a, 0.0f); }
+
+/* 16 bytes at any element */
+__device__ __forceinline__ uint4 load16(const void *p) {
+  uint4 q;
+  __builtin_memcpy(&q, p, 16);
+  return q;
+}
+__device__ __forceinline__ void store16(void *p, uint4 q) { __builtin_memcpy(p, &q, 16); }
 
 /* output (i, j), its sum s */
 __device__ __forceinline__ void put_one(const Out &o, int i, int j, float s) {
   if (o.bias) s += bf(o.bias[j]);
-  if (o.z) o.z[(int64_t)i * o.z_stride + j] = d3s_f32_to_bf16_rn(s);
-  s = activate(s, o.act);
+  if (o.z) o.z[(int64_t)i * o.z_stride + j] = pack1(s);
+  activate<1>(&s, o.act);
   if (o.f32) {
     if (o.residual) s += ((const float *)o.residual)[(int64_t)i * o.residual_stride + j];
     ((float *)o.y)[(int64_t)i * o.y_stride + j] = s;
   } else {
     if (o.residual) s += bf(((const uint16_t *)o.residual)[(int64_t)i * o.residual_stride + j]);
-    ((uint16_t *)o.y)[(int64_t)i * o.y_stride + j] = d3s_f32_to_bf16_rn(s);
+    ((uint16_t *)o.y)[(int64_t)i * o.y_stride + j] = pack1(s);
   }
 }
 
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  return (uint32_t)d3s_f32_to_bf16_rn(a) | (uint32_t)d3s_f32_to_bf16_rn(b) << 16;
-}
+/* elements of y's type: eight neighbouring ones of a residual */
+struct Eight {
+  uint4 lo, hi; /* (bf16: lo alone) */
+};
 
-/* outputs (i, j .. j + 3), all inside; the addresses may lie at any element */
-__device__ __forceinline__ void put_four(const Out &o, int i, int j, f32x4 s) {
-  if (o.bias) {
-    uint16_t b[4];
-    __builtin_memcpy(b, o.bias + j, 8);
-#pragma unroll
-    for (int e = 0; e < 4; e++) s[e] += bf(b[e]);
-  }
-  if (o.z) {
-    const uint32_t w[2] = {pack2(s[0], s[1]), pack2(s[2], s[3])};
-    __builtin_memcpy(o.z + (int64_t)i * o.z_stride + j, w, 8);
-  }
-#pragma unroll
-  for (int e = 0; e < 4; e++) s[e] = activate(s[e], o.act);
+/* residual (i, j .. j + 7); nothing where the eight are not all there */
+__device__ __forceinline__ void get_eight(const Out &o, int i, int j, Eight &r) {
+  r.lo = r.hi = make_uint4(0u, 0u, 0u, 0u);
+  if (!o.residual || i >= o.m || j + 8 > o.n) return;
+  const int64_t at = (int64_t)i * o.residual_stride + j;
   if (o.f32) {
-    if (o.residual) {
-      f32x4 r;
-      __builtin_memcpy(&r, (const float *)o.residual + (int64_t)i * o.residual_stride + j, 16);
-      s += r;
-    }
-    __builtin_memcpy((float *)o.y + (int64_t)i * o.y_stride + j, &s, 16);
+    r.lo = load16((const float *)o.residual + at);
+    r.hi = load16((const float *)o.residual + at + 4);
   } else {
-    if (o.residual) {
-      uint16_t r[4];
-      __builtin_memcpy(r, (const uint16_t *)o.residual + (int64_t)i * o.residual_stride + j, 8);
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[e] += bf(r[e]);
-    }
-    const uint32_t w[2] = {pack2(s[0], s[1]), pack2(s[2], s[3])};
-    __builtin_memcpy((uint16_t *)o.y + (int64_t)i * o.y_stride + j, w, 8);
+    r.lo = load16((const uint16_t *)o.residual + at);
   }
 }
 
-__device__ __forceinline__ void put_edge(const Out &o, int i, int j, f32x4 s) {
-  if (i >= o.m) return;
-  if (j + 4 <= o.n) {
-    put_four(o, i, j, s);
-  } else {
+__device__ __forceinline__ void bf_eight(uint4 q, float *v) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (j + e < o.n) put_one(o, i, j + e, s[e]);
+  for (int e = 0; e < 4; e++) {
+    v[2 * e] = d3s_u2f(w[e] << 16);
+    v[2 * e + 1] = d3s_u2f(w[e] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack_eight(const float *s) {
+  return make_uint4(pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7]));
+}
+
+/* the bias of outputs j .. j + 7, zeros where the eight are not all there */
+__device__ __forceinline__ uint4 bias_eight(const Out &o, int j) {
+  return o.bias && j + 8 <= o.n ? load16(o.bias + j) : make_uint4(0u, 0u, 0u, 0u);
+}
+
+/* Outputs (i, j .. j + 7), in two steps, so that the second, light, can be
+ * unrolled over rows whose residuals are in flight: first the sums at `sum` (16-byte
+ * aligned) become activations, with the bias as bias_eight gave it ... */
+__device__ __forceinline__ void activate_eight(const Out &o, int i, int j, float *sum, uint4 bias) {
+  if (i >= o.m || j + 8 > o.n) return;
+  float s[8], v[8];
+  const f32x4 a = *(const f32x4 *)sum, b = *(const f32x4 *)(sum + 4);
+  bf_eight(bias, v);
+#pragma unroll
+  for (int e = 0; e < 4; e++) s[e] = a[e] + v[e], s[e + 4] = b[e] + v[e + 4];
+  if (o.z) store16(o.z + (int64_t)i * o.z_stride + j, pack_eight(s));
+  activate<8>(s, o.act);
+  *(f32x4 *)sum = f32x4{s[0], s[1], s[2], s[3]};
+  *(f32x4 *)(sum + 4) = f32x4{s[4], s[5], s[6], s[7]};
+}
+/* ... then they are written, with the residual as get_eight gave it.  Where the
+ * eight are not all there, `sum` still holds sums. */
+__device__ __forceinline__ void put_eight(const Out &o, int i, int j, const float *sum, const Eight &r) {
+  if (i >= o.m || j + 8 > o.n) return;
+  f32x4 a = *(const f32x4 *)sum, b = *(const f32x4 *)(sum + 4);
+  if (o.f32) {
+    if (o.residual) a += __builtin_bit_cast(f32x4, r.lo), b += __builtin_bit_cast(f32x4, r.hi);
+    float *y = (float *)o.y + (int64_t)i * o.y_stride + j;
+    store16(y, __builtin_bit_cast(uint4, a));
+    store16(y + 4, __builtin_bit_cast(uint4, b));
+  } else {
+    float s[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, v[8];
+    bf_eight(r.lo, v);
+#pragma unroll
+    for (int e = 0; e < 8; e++) s[e] = o.residual ? s[e] + v[e] : s[e];
+    store16((uint16_t *)o.y + (int64_t)i * o.y_stride + j, pack_eight(s));
   }
 }
 
