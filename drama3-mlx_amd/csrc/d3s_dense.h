@@ -25,15 +25,31 @@ struct Out {
   bool f32;
 };
 
-/* m_tiles by n_tiles tiles of tm x tn from output (i0, j0), walked in columns
- * of `group`; each cut into `splits` of `stages` stages.  (An output takes two
+/* m_tiles by n_tiles tiles of tm x tn, walked in columns of `group`; each cut into `splits` of `stages` stages.  (An output takes two
  * bytes: the tiles of what fits the memory are counted in 32 bits.) */
 struct TilePlan {
   unsigned tiles, first, m_tiles, n_tiles, group, splits;
-  int i0, j0, stages;
+  int stages;
   int tm, tn;
+  float *parts;       /* the splits' sums, and their arrivals (a 128-byte line a tile) */
+  uint32_t *arrivals;
   bool x_direct, w_direct; /* operands by rows at 16 bytes: see Way */
 };
+
+/* k_few's: rows from i0 on (at most FEW_ROWS), the inner length cut into
+ * `splits` of `batches` batches */
+constexpr int FEW_ROWS = 64;
+struct FewPlan {
+  unsigned tiles, splits;
+  int i0, batches;
+  uint64_t *parts;
+  uint32_t *arrivals;
+};
+int few_outputs(bool w_transposed); /* a workgroup's */
+int few_batch(bool w_transposed);
+int few_waves(bool w_transposed); /* batches at a time */
+size_t few_part_bytes(bool w_transposed, int rows); /* a split's sums of one workgroup */
+void launch_few(const Operands &a, const Out &o, bool x_transposed, bool w_transposed, const FewPlan &pl, hipStream_t s);
 
 template <bool XT, bool WT>
 void launch_tiles(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s);

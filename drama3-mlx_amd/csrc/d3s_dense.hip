@@ -1,45 +1,165 @@
-/* Dense layers (include/d3s_train.h): which tiles a product is cut into
- * (gfx950; the kernel is in d3s_dense_tile.h). */
+/* Dense layers (include/d3s_train.h): which kernel takes a product, in which
+ * tiles (gfx950; the kernels are in d3s_dense_tile.h and d3s_dense_few.hip). */
 #include "d3s_dense.h"
 
 namespace d3s {
 namespace {
 
+constexpr int CUS = 256;
+
 /* operands whose chunks go to LDS directly: rows at 16 bytes, a tile's 256 of
  * them within 32-bit offsets */
-bool at_16(const uint16_t *p, int64_t stride) {
-  return ((uintptr_t)p & 15u) == 0u && stride % 8 == 0 && stride < ((int64_t)1 << 22);
+bool direct_at(uintptr_t p, int64_t stride) { return p % 16 == 0 && stride % 8 == 0 && stride < ((int64_t)1 << 22); }
+
+/* A product: its sizes, and how its operands lie. */
+struct Product {
+  int64_t m, n, k;
+  bool x_turned, w_turned, x_direct, w_direct;
+};
+
+Product product_of(const d3s_dense_params &p, uintptr_t x, uintptr_t w) {
+  Product r{p.m, p.n, p.k, p.x_transposed != 0, p.w_transposed != 0, false, false};
+  r.x_direct = !r.x_turned && direct_at(x, p.x_stride);
+  r.w_direct = !r.w_turned && direct_at(w, p.w_stride);
+  return r;
 }
 
-TilePlan plan(const d3s_dense_params &p, int tm, int tn) {
-  TilePlan pl{};
-  pl.tm = tm;
-  pl.tn = tn;
-  pl.m_tiles = (unsigned)((p.m + tm - 1) / tm);
-  pl.n_tiles = (unsigned)((p.n + tn - 1) / tn);
-  pl.tiles = pl.m_tiles * pl.n_tiles;
-  pl.group = 8;
-  pl.x_direct = at_16(p.x, p.x_stride);
-  pl.w_direct = at_16(p.w, p.w_stride);
-  pl.splits = 1;
-  pl.stages = (int)(p.k / TILE_K);
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+/* Microseconds of m rows in tiles of tm x tn, one workgroup a CU: rounds of
+ * workgroups, each its stages and what it spends before and after them.
+ * Measured, by how many operands go to LDS directly: a stage of 256 x 256 1.45
+ * (both), 1.55 (one, the other turned) and 1.72; of 256 x 128 0.93 and 1.27; of
+ * 128 x 128 0.52 and 0.80, with half of the CUs idle 0.38 and 0.72.  Around them
+ * 14, 10 and 6, and for split sums 3 and 1 a split.
+ * (8192 x 2048 x 2048, both direct: 63, 78 and 87 us in the three tiles;
+ * 2048 x 2048 x 2048: 50, 29 and 22; 4096 x 2048 x 8192, both turned: 217, 163
+ * and 210; 256 x 2048 x 8192: 128 x 128 with 1, 2, 4 and 8 splits 49, 31, 22
+ * and 24.) */
+double tile_us(const Product &p, int64_t m, int tm, int tn, int splits) {
+  const int direct = p.x_direct + p.w_direct;
+  const double wgs = (double)up(m, tm) * (double)up(p.n, tn) * splits;
+  const double rounds = (double)(int64_t)((wgs + CUS - 1) / CUS), stages = (double)up(p.k, (int64_t)TILE_K * splits);
+  if (tn == 256) {
+    const bool mixed = direct == 1 && p.x_turned != p.w_turned;
+    return rounds * (stages * (direct == 2 ? 1.45 : mixed ? 1.55 : 1.72) + 14);
+  }
+  if (tm == 256) return rounds * (stages * (direct == 2 ? 0.93 : 1.27) + 10);
+  const bool few = wgs <= CUS * 3 / 4;
+  const double stage = direct == 2 ? (few ? 0.38 : 0.52) : few ? 0.72 : 0.80;
+  return rounds * (stages * stage + 6) + (splits > 1 ? 3 + splits : 0);
+}
+
+/* ... and of k_few: the weights at 4 TB/s */
+double few_us(const Product &p) { return 6 + (double)p.n * (double)p.k * 2 / 4e6; }
+
+struct Plan {
+  TilePlan tile; /* no tiles: no such launch */
+  FewPlan few;
+  int64_t tile_rows;
+};
+
+size_t tile_bytes(const TilePlan &t) { return t.splits > 1 ? (size_t)t.tiles * t.splits * t.tm * t.tn * sizeof(float) : 0; }
+size_t few_bytes(const Plan &pl, const Product &p) {
+  return pl.few.splits > 1 ? (size_t)pl.few.tiles * pl.few.splits * few_part_bytes(p.w_turned, (int)(p.m - pl.few.i0)) : 0;
+}
+
+Plan plan(const Product &p) {
+  Plan pl{};
+  /* Few rows: k_few, which turns weights eight outputs at a time.  33 to 64 rows
+   * (64 x 2048 x 2048: 9.3 us, in tiles 14.2; 64 x 4097 x 2048: 19.8, in tiles 15.8) while
+   * its workgroups of 16 outputs, each of which reads all of x, run at once. */
+  const bool can = !p.w_turned || p.n >= 8;
+  int64_t few = 0;
+  if (can && (p.m <= 32 || (p.m <= FEW_ROWS && !p.w_turned && p.n <= 16 * CUS))) few = p.m;
+
+  double best = 1e300;
+  auto choose = [&](int64_t m, double also) {
+    auto offer = [&](int tm, int tn, int splits) {
+      const double us = tile_us(p, m, tm, tn, splits) + also;
+      if (us >= best) return;
+      best = us;
+      pl.tile_rows = m;
+      pl.tile.tm = tm, pl.tile.tn = tn, pl.tile.splits = (unsigned)splits;
+    };
+    offer(256, 256, 1);
+    offer(256, 128, 1);
+    /* (every split has its stages, and fewer workgroups than twice the CUs) */
+    for (int s = 1; s <= 8; s++)
+      if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(p.n, 128) * s <= 2 * CUS)) offer(128, 128, s);
+  };
+  if (few == 0) {
+    choose(p.m, 0);
+    /* a last row of tiles that is nearly empty may cost a round of its own */
+    const int64_t rest = p.m % 128;
+    if (can && rest > 0 && rest <= 32 && p.m > 256) {
+      const double with = best;
+      choose(p.m - rest, few_us(p));
+      if (best < with) few = rest;
+    }
+    TilePlan &t = pl.tile;
+    t.m_tiles = (unsigned)up(pl.tile_rows, t.tm);
+    t.n_tiles = (unsigned)up(p.n, t.tn);
+    t.tiles = t.m_tiles * t.n_tiles;
+    t.group = 8;
+    t.stages = (int)up(p.k / TILE_K, t.splits);
+    t.x_direct = p.x_direct;
+    t.w_direct = p.w_direct;
+  }
+  if (few > 0) {
+    FewPlan &f = pl.few;
+    f.i0 = (int)(p.m - few);
+    f.tiles = (unsigned)up(p.n, few_outputs(p.w_turned));
+    /* the inner length over more workgroups while there are fewer than CUs, at
+     * least two batches a wave (one with four fragments of rows) */
+    const int64_t batches = up(p.k, few_batch(p.w_turned));
+    int64_t most = batches / (few_waves(p.w_turned) * (few > 32 ? 1 : 2)), want = CUS / (int64_t)f.tiles;
+    if (want < most) most = want;
+    if (most > 16) most = 16;
+    f.splits = most > 1 ? (unsigned)most : 1u;
+    f.batches = (int)up(batches, f.splits);
+  }
   return pl;
+}
+
+size_t bytes_of(const Product &p) {
+  const Plan pl = plan(p);
+  const size_t a = tile_bytes(pl.tile), b = pl.few.tiles ? few_bytes(pl, p) : 0;
+  return a > b ? a : b; /* (one launch after the other) */
 }
 
 }  // namespace
 
-size_t dense_workspace_bytes(const d3s_dense_params &p) { return 0; }
+/* for whatever alignment the operands come at */
+size_t dense_workspace_bytes(const d3s_dense_params &p) {
+  size_t most = 0;
+  for (int at = 0; at < 4; at++) {
+    const size_t b = bytes_of(product_of(p, (uintptr_t)(at & 1) * 2, (uintptr_t)(at >> 1) * 2));
+    most = b > most ? b : most;
+  }
+  return most ? split_counter_bytes() + most : 0;
+}
 
 void launch_dense(const d3s_dense_params &p, void *ws, hipStream_t s) {
   const Operands a{p.x, p.w, p.x_stride, p.w_stride, (int)p.k};
-  const Out o{p.bias,     p.residual, p.z,        p.y,        p.residual_stride, p.z_stride,
-              p.y_stride, (int)p.m,   (int)p.n,   p.activation, p.y_dtype == D3S_DTYPE_F32};
-  const int t = p.m > 1024 && p.n > 1024 ? 256 : 128;
-  const TilePlan pl = plan(p, t, t);
-  if (p.x_transposed)
-    p.w_transposed ? launch_tiles<true, true>(a, o, pl, s) : launch_tiles<true, false>(a, o, pl, s);
+  Out o{p.bias,     p.residual, p.z,      p.y,          p.residual_stride,          p.z_stride,
+        p.y_stride, (int)p.m,   (int)p.n, p.activation, p.y_dtype == D3S_DTYPE_F32};
+  const Product pr = product_of(p, (uintptr_t)p.x, (uintptr_t)p.w);
+  Plan pl = plan(pr);
+  char *parts = ws ? (char *)ws + split_counter_bytes() : nullptr;
+  if (pl.few.tiles) {
+    pl.few.arrivals = (uint32_t *)ws;
+    pl.few.parts = (uint64_t *)parts;
+    launch_few(a, o, pr.x_turned, pr.w_turned, pl.few, s);
+  }
+  if (!pl.tile.tiles) return;
+  pl.tile.arrivals = (uint32_t *)ws;
+  pl.tile.parts = (float *)parts;
+  o.m = (int)pl.tile_rows;
+  if (pr.x_turned)
+    pr.w_turned ? launch_tiles<true, true>(a, o, pl.tile, s) : launch_tiles<true, false>(a, o, pl.tile, s);
   else
-    p.w_transposed ? launch_tiles<false, true>(a, o, pl, s) : launch_tiles<false, false>(a, o, pl, s);
+    pr.w_turned ? launch_tiles<false, true>(a, o, pl.tile, s) : launch_tiles<false, false>(a, o, pl.tile, s);
 }
 
 }  // namespace d3s

@@ -19,7 +19,7 @@
 
 #include <type_traits>
 
-#include "d3s_dense.h"
+#include "d3s_dense_load.h"
 #include "d3s_epilogue.h"
 
 namespace d3s {
@@ -35,31 +35,11 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define D3S_LDS __attribute__((address_space(3)))
 #define D3S_GLOBAL __attribute__((address_space(1)))
 
-/* elements [at, at + 8) of a stored row of `len`, zeros past its end (at < len) */
-__device__ __forceinline__ uint4 row_chunk(const uint16_t *row, int64_t at, int64_t len) {
-  uint64_t v[2] = {0u, 0u};
-  if (len >= 8) { /* near its end the row's last eight, moved down */
-    const int64_t from = at < len - 8 ? at : len - 8;
-    __builtin_memcpy(v, row + from, 16);
-    const int s = (int)(at - from) * 16; /* 0 .. 112 */
-    const uint64_t hi = v[1];
-    v[1] = s < 64 ? hi >> s : 0u;
-    v[0] = s == 0 ? v[0] : s < 64 ? v[0] >> s | hi << (64 - s) : hi >> (s - 64);
-  } else {
-#pragma nounroll
-    for (int64_t e = len - 1; e >= at; e--) {
-      v[1] = v[1] << 16 | v[0] >> 48;
-      v[0] = v[0] << 16 | row[e];
-    }
-  }
-  return make_uint4((uint32_t)v[0], (uint32_t)(v[0] >> 32), (uint32_t)v[1], (uint32_t)(v[1] >> 32));
-}
-
 /* how an operand's stages reach LDS */
 enum Way { DIRECT, ROWS, TURNED };
 
 /* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED: stored [k, rows]). */
-template <int R, Way WAY>
+template <int R, Way WAY, int SETS>
 struct Part {
   static constexpr int BYTES = R * TK * 2;
   static constexpr int PER = R * TK / 8 / TT;                      /* 16-byte loads a thread */
@@ -73,7 +53,7 @@ struct Part {
   __amdgpu_buffer_rsrc_t from;
   const uint16_t *mine;                  /* ROWS, TURNED: the thread's first chunk of stage 0 */
   int to;                                /* TURNED: its first row in LDS (below 0: not the tile's) */
-  uint4 q[PER];
+  uint4 q[SETS][PER];
 
   static __device__ __forceinline__ int tid() { return (int)threadIdx.x; }
   static __device__ __forceinline__ int turn(int r) { return (r ^ r >> 3) & 7; }
@@ -108,11 +88,11 @@ struct Part {
   __device__ __forceinline__ const uint16_t *start(int k0) const {
     return WAY == TURNED ? mine + (int64_t)k0 * stride : p + k0;
   }
-  __device__ __forceinline__ void load(int u, const uint16_t *at) {
+  __device__ __forceinline__ void load(int set, int u, const uint16_t *at) {
     if constexpr (WAY == ROWS)
-      q[u] = load16(at + ((int64_t)min(r0 + row(u), rows - 1) * stride + chunk(u) * 8));
+      q[set][u] = load16(at + ((int64_t)min(r0 + row(u), rows - 1) * stride + chunk(u) * 8));
     else
-      q[u] = load16(at + u * stride);
+      q[set][u] = load16(at + u * stride);
   }
   /* the same of any stage: something finite or not from k1 on */
   __device__ __forceinline__ void load_some(int k0, int k1) {
@@ -121,23 +101,23 @@ struct Part {
       if constexpr (WAY == TURNED) {
         const uint16_t *at = p + (int64_t)min(k0 + inner() + u, k1 - 1) * stride;
         if (rows >= 8)
-          q[u] = load16(at + (r0 + to));
+          q[0][u] = load16(at + (r0 + to));
         else
-          q[u] = r0 + to < rows ? row_chunk(at, r0 + to, rows) : make_uint4(0u, 0u, 0u, 0u);
+          q[0][u] = r0 + to < rows ? row_chunk(at, r0 + to, rows) : make_uint4(0u, 0u, 0u, 0u);
       } else {
         const int k = k0 + chunk(u) * 8;
         const uint16_t *at = p + (int64_t)min(r0 + row(u), rows - 1) * stride;
-        q[u] = k >= k1 ? make_uint4(0u, 0u, 0u, 0u) : WAY == DIRECT ? load16(at + k) : row_chunk(at, k, k1);
+        q[0][u] = k >= k1 ? make_uint4(0u, 0u, 0u, 0u) : WAY == DIRECT ? load16(at + k) : row_chunk(at, k, k1);
       }
     }
   }
   /* the v-th write of the registers into a stage (rows that are not the tile's: to `spare`) */
-  __device__ __forceinline__ void write(int v, char *lds, char *spare) const {
+  __device__ __forceinline__ void write(int set, int v, char *lds, char *spare) const {
     if constexpr (WAY != TURNED) {
-      *(uint4 *)(lds + (v * TT + tid()) * 16) = q[v];
+      *(uint4 *)(lds + (v * TT + tid()) * 16) = q[set][v];
     } else if constexpr (WAY == TURNED) {
       uint32_t w[PER > 1 ? PER / 2 : 1];
-      auto word = [&](int u) { return v < 2 ? q[u].x : v < 4 ? q[u].y : v < 6 ? q[u].z : q[u].w; };
+      auto word = [&](int u) { return v < 2 ? q[set][u].x : v < 4 ? q[set][u].y : v < 6 ? q[set][u].z : q[set][u].w; };
 #pragma unroll
       for (int u = 0; u + 1 < PER; u += 2)
         w[u / 2] = __builtin_amdgcn_perm(word(u + 1), word(u), v & 1 ? 0x07060302u : 0x05040100u);
@@ -155,7 +135,7 @@ struct Part {
   }
   __device__ __forceinline__ void write_all(char *lds, char *spare) const {
 #pragma unroll
-    for (int v = 0; v < (WAY == TURNED ? 8 : PER); v++) write(v, lds, spare);
+    for (int v = 0; v < (WAY == TURNED ? 8 : PER); v++) write(0, v, lds, spare);
   }
   /* the fragment of rows r .. r + 31 (r a multiple of 32), inner indices 16 step .. + 15 */
   static __device__ __forceinline__ bf16x8 fragment(const char *lds, int r, int step) {
@@ -173,28 +153,34 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <int TM, int TN, int WAVES_M, Way WX, Way WW>
-__global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operands a, Out o, TilePlan pl) {
+/* 16 bytes past the caches of one XCD */
+constexpr int DEVICE_SCOPE = 16;
+
+/* BUFS: stages in LDS.  AHEAD: stages through registers are loaded that many
+ * before the one that is written next. */
+template <int TM, int TN, int WAVES_M, int BUFS, int AHEAD, bool SPLIT, Way WX, Way WW>
+__global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) {
   constexpr int WAVES_N = 4 / WAVES_M;
   constexpr int WM = TM / WAVES_M, WN = TN / WAVES_N, FM = WM / 32, FN = WN / 32;
-  constexpr int STEPS = TK / STEP;
-  using PX = Part<TM, WX>;
-  using PW = Part<TN, WW>;
+  constexpr int STEPS = TK / STEP, SETS = AHEAD + 1;
+  using PX = Part<TM, WX, SETS>;
+  using PW = Part<TN, WW, SETS>;
   constexpr int STAGE = PX::BYTES + PW::BYTES;
   constexpr int OUT_ROW = WN + 4; /* a row of outputs in LDS, fp32 */
   constexpr int OUT_BYTES = 4 * 32 * OUT_ROW * 4;
-  constexpr int ROOM = 2 * STAGE > OUT_BYTES ? 2 * STAGE : OUT_BYTES;
+  constexpr int ROOM = BUFS * STAGE > OUT_BYTES ? BUFS * STAGE : OUT_BYTES;
   __shared__ __attribute__((aligned(1024))) char lds[ROOM + 16];
   char *spare = lds + ROOM;
+  static_assert(WX == DIRECT && WW == DIRECT ? AHEAD == 0 : BUFS == 2, "what the waits below count");
 
   /* workgroups go to the eight XCDs in turn: each takes a run of neighbouring
    * tiles, in columns of eight, whose operands its L2 then holds */
   const unsigned turn = blockIdx.x % 8, each = gridDim.x / 8;
   const unsigned t = pl.first + turn * each + min(turn, gridDim.x % 8) + blockIdx.x / 8;
-  const unsigned split = t / pl.tiles, tile = t % pl.tiles;
+  const unsigned split = SPLIT ? t / pl.tiles : 0u, tile = SPLIT ? t % pl.tiles : t;
   const unsigned wide = pl.group * pl.n_tiles, band = tile / wide, in = tile % wide;
   const unsigned high = min(pl.group, pl.m_tiles - band * pl.group); /* tiles in a column of the band */
-  const int i0 = pl.i0 + (int)(band * pl.group + in % high) * TM, j0 = pl.j0 + (int)(in / high) * TN;
+  const int i0 = (int)(band * pl.group + in % high) * TM, j0 = (int)(in / high) * TN;
 
   const int lane = lane_id(), wid = __builtin_amdgcn_readfirstlane((int)threadIdx.x / WAVE);
   const int wi = wid / WAVES_N * WM, wj = wid % WAVES_N * WN; /* the wave's rows and outputs */
@@ -234,17 +220,17 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
     const uint16_t *x, *w;
   };
   auto start = [&](int k0) { return Start{px.start(k0), pw.start(k0)}; };
-  auto load = [&](int u, const Start &at) {
+  auto load = [&](int set, int u, const Start &at) {
     if (u < PX::LOADS)
-      px.load(u, at.x);
+      px.load(set, u, at.x);
     else
-      pw.load(u - PX::LOADS, at.w);
+      pw.load(set, u - PX::LOADS, at.w);
   };
-  auto write = [&](int v, char *to) {
+  auto write = [&](int set, int v, char *to) {
     if (v < PX::WRITES)
-      px.write(v, to, spare);
+      px.write(set, v, to, spare);
     else
-      pw.write(v - PX::WRITES, to + PX::BYTES, spare);
+      pw.write(set, v - PX::WRITES, to + PX::BYTES, spare);
   };
   /* the products of fragments `from`; after the n-th of them, and pinned there,
    * beside(n): its share of what goes on meanwhile */
@@ -270,43 +256,62 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
    * step.  With operands through registers they come last (an LDS write behind
    * them would wait for them), all at once. */
   constexpr int LATE = LOADS == 0 ? DIRECTS / 2 : 0, SOON = DIRECTS - LATE, HALF = PRODUCTS / 2;
-  constexpr int WRITTEN = DIRECTS > 0 ? HALF : PRODUCTS;
+  constexpr int WRITTEN = DIRECTS > 0 && HALF > 0 ? HALF : PRODUCTS;
 
   /* TURNED operands of fewer than eight rows have no whole loads */
   const int full = (WX == TURNED && o.m < 8) || (WW == TURNED && o.n < 8) ? s0 : s1;
   if (s0 < full) {
+    auto k_of = [&](int s) { return min(s, s1 - 1) * TK; }; /* (loads past the end: the last stage's, not read) */
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-      const int k0 = min(s0 + b, s1 - 1) * TK;
-      const Start at = start(k0);
+    for (int b = 0; b < BUFS; b++) {
+      const Start at = start(k_of(s0 + b));
 #pragma unroll
-      for (int u = 0; u < LOADS; u++) load(u, at);
+      for (int u = 0; u < LOADS; u++) load(b % SETS, u, at);
 #pragma unroll
-      for (int u = 0; u < (b == 0 ? DIRECTS : SOON); u++) direct(u, k0, lds + b * STAGE);
+      for (int u = 0; u < (b < BUFS - 1 ? DIRECTS : SOON); u++) direct(u, k_of(s0 + b), lds + b * STAGE);
 #pragma unroll
-      for (int v = 0; v < WRITES; v++) write(v, lds + b * STAGE);
+      for (int v = 0; v < WRITES; v++) write(b % SETS, v, lds + b * STAGE);
     }
-    stage_barrier<SOON>();
+#pragma unroll
+    for (int b = 2; b < 2 + AHEAD; b++) {
+      const Start at = start(k_of(s0 + b));
+#pragma unroll
+      for (int u = 0; u < LOADS; u++) load(b % SETS, u, at);
+    }
+    stage_barrier<(BUFS - 2) * DIRECTS + SOON + AHEAD * LOADS>(); /* (registers' loads have been waited for) */
     read_all(0, lds, 0);
     char *here = lds;
-    for (int s = s0; s < s1; s++) { /* (the last two stages fill buffers that nothing reads) */
-      char *next = here == lds ? lds + STAGE : lds;
-      const int near = min(s + 1, s1 - 1) * TK, far = min(s + 2, s1 - 1) * TK;
-      const Start at = start(far);
+    /* stage s, `turn` stages after a multiple of SETS */
+    auto stage = [&](int s, auto turn) {
+      constexpr int V = decltype(turn)::value;
+      char *next = here == lds + (BUFS - 1) * STAGE ? lds : here + STAGE;
+      char *back = here == lds ? lds + (BUFS - 1) * STAGE : here - STAGE;
+      const int near = k_of(s + BUFS - 1), far = k_of(s + BUFS);
+      const Start at = start(k_of(s + 2 + AHEAD));
 #pragma unroll
       for (int j = 0; j < STEPS - 1; j++)
         multiply(j & 1, [&](int n) {
           share(n, 0, PRODUCTS, FM + FN, [&](int f) { read((j + 1) & 1, here, j + 1, f); });
-          if (j == 0) share(n, HALF, PRODUCTS, LATE, [&](int u) { direct(SOON + u, near, next); });
-          if (j == 0) share(n, 0, PRODUCTS, LOADS, [&](int u) { load(u, at); });
+          if (j == 0) share(n, HALF, PRODUCTS, LATE, [&](int u) { direct(SOON + u, near, back); });
+          if (j == 0) share(n, 0, PRODUCTS, LOADS, [&](int u) { load((V + 1) % SETS, u, at); });
         });
-      stage_barrier<LOADS>();
+      /* the next stage is there: loads after its own may still be on their way */
+      stage_barrier<(BUFS - 2) * DIRECTS + (AHEAD + 1) * LOADS>();
       multiply(1, [&](int n) {
         share(n, 0, PRODUCTS, FM + FN, [&](int f) { read(0, next, 0, f); });
-        share(n, 0, WRITTEN, WRITES, [&](int v) { write(v, here); });
+        share(n, 0, WRITTEN, WRITES, [&](int v) { write((V + 2) % SETS, v, here); });
         share(n, HALF, PRODUCTS, SOON, [&](int u) { direct(u, far, here); });
       });
       here = next;
+    };
+    for (int s = s0; s < s1; s += SETS) {
+      stage(s, std::integral_constant<int, 0>{});
+      if constexpr (SETS > 1)
+        if (s + 1 < s1) stage(s + 1, std::integral_constant<int, 1 % SETS>{});
+      if constexpr (SETS > 2)
+        if (s + 2 < s1) stage(s + 2, std::integral_constant<int, 2 % SETS>{});
+      if constexpr (SETS > 3)
+        if (s + 3 < s1) stage(s + 3, std::integral_constant<int, 3 % SETS>{});
     }
   }
   /* the rest of the inner length, what whole loads do not reach: zeros from its end on */
@@ -337,6 +342,35 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
     }
   }
 
+  /* A split's sums go to the workspace, complete before its arrival is counted;
+   * the last to arrive adds them below, in the order of the splits, so the bits
+   * do not depend on who that is. */
+  const int at = (int)threadIdx.x * 16;
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  auto block = [&](unsigned s) {
+    float *parts = pl.parts + ((size_t)tile * pl.splits + s) * (TM * TN);
+    return __builtin_amdgcn_make_buffer_rsrc(parts, 0, TM * TN * 4, 0x00020000);
+  };
+  if constexpr (SPLIT) {
+    const __amdgpu_buffer_rsrc_t own = block(split);
+#pragma unroll
+    for (int c = 0; c < FM * FN * 4; c++) {
+      const f32x16 &v = acc[c / 4 / FN][c / 4 % FN];
+      const f32x4 s = {v[c % 4 * 4], v[c % 4 * 4 + 1], v[c % 4 * 4 + 2], v[c % 4 * 4 + 3]};
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, s), own, at, c * (TT * 16), DEVICE_SCOPE);
+    }
+    stage_barrier<0>();
+    unsigned *last = (unsigned *)spare;
+    if (threadIdx.x == 0) {
+      uint32_t *count = pl.arrivals + (size_t)tile * 32;
+      const bool is = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pl.splits - 1;
+      if (is) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *last = is;
+    }
+    __syncthreads();
+    if (!*last) return;
+  }
+
   /* Each wave's outputs, 32 rows at a time, through its part of LDS, so that
    * a row leaves in whole lines.  Lane l holds row l % 32, and four neighbouring
    * outputs from 8 i + 4 (l / 32) in registers 4 i .. 4 i + 3.  One copy of the
@@ -354,16 +388,33 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
 #pragma nounroll
   for (int p = 0; p < FM; p++) {
     wave_lds_sync();
+    auto stage_out = [&](int q, int i, f32x4 v) {
+      *(f32x4 *)(mine + (lane & 31) * OUT_ROW + q * 32 + i * 8 + (lane >> 5) * 4) = v;
+    };
+    if constexpr (SPLIT) {
+      f32x4 sum[FN * 4];
 #pragma unroll
-    for (int c = 0; c < FM; c++)
-      if (c == p) {
+      for (int c = 0; c < FN * 4; c++) sum[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+      for (unsigned s = 0; s < pl.splits; s++) {
+        const __amdgpu_buffer_rsrc_t from = block(s);
 #pragma unroll
-        for (int q = 0; q < FN; q++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            *(f32x4 *)(mine + (lane & 31) * OUT_ROW + q * 32 + i * 8 + (lane >> 5) * 4) =
-                f32x4{acc[c][q][4 * i], acc[c][q][4 * i + 1], acc[c][q][4 * i + 2], acc[c][q][4 * i + 3]};
+        for (int c = 0; c < FN * 4; c++)
+          sum[c] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, at, (p * FN * 4 + c) * (TT * 16), DEVICE_SCOPE));
       }
+#pragma unroll
+      for (int c = 0; c < FN * 4; c++) stage_out(c / 4, c % 4, sum[c]);
+    } else {
+#pragma unroll
+      for (int c = 0; c < FM; c++)
+        if (c == p) {
+#pragma unroll
+          for (int q = 0; q < FN; q++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              stage_out(q, i, f32x4{acc[c][q][4 * i], acc[c][q][4 * i + 1], acc[c][q][4 * i + 2], acc[c][q][4 * i + 3]});
+        }
+    }
     wave_lds_sync();
     Eight now[ROUNDS];
 #pragma unroll
@@ -375,8 +426,8 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
     float *row = mine + lane / ACROSS * OUT_ROW + lane % ACROSS * 8;
     if (works) {
 #pragma nounroll
-      for (int r = 0; r < ROUNDS; r++)
-        activate_eight(o, i_at + p * 32 + r * DOWN, j_at, row + r * DOWN * OUT_ROW, bias);
+      for (int r = 0; r < ROUNDS; r += 2)
+        activate_twice_eight(o, i_at + p * 32 + r * DOWN, DOWN, j_at, row + r * DOWN * OUT_ROW, OUT_ROW, bias);
     }
 #pragma unroll
     for (int r = 0; r < ROUNDS; r++)
@@ -390,26 +441,43 @@ __global__ __launch_bounds__(TT, TM *TN >= 256 * 256 ? 1 : 2) void k_tile(Operan
   }
 }
 
-template <int TM, int TN, int WAVES_M, Way WX, Way WW>
+template <int TM, int TN, int WAVES_M, int BUFS, int AHEAD, Way WX, Way WW>
 void launch_ways(const Operands &a, const Out &o, TilePlan pl, hipStream_t s) {
   const unsigned all = pl.tiles * pl.splits;
-  for (pl.first = 0; pl.first < all; pl.first += TILE_GRID)
-    k_tile<TM, TN, WAVES_M, WX, WW><<<dim3(min(TILE_GRID, all - pl.first)), TT, 0, s>>>(a, o, pl);
+  for (pl.first = 0; pl.first < all; pl.first += TILE_GRID) {
+    const dim3 grid(min(TILE_GRID, all - pl.first));
+    bool split = false;
+    if constexpr (TM == 128 && TN == 128) {
+      split = pl.splits > 1;
+      if (split) k_tile<TM, TN, WAVES_M, BUFS, AHEAD, true, WX, WW><<<grid, TT, 0, s>>>(a, o, pl);
+    }
+    if (!split) k_tile<TM, TN, WAVES_M, BUFS, AHEAD, false, WX, WW><<<grid, TT, 0, s>>>(a, o, pl);
+  }
 }
 
-template <int TM, int TN, int WAVES_M, bool XT, bool WT>
-void launch_shape(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
+/* Small tiles: both operands directly, or both through registers (a write
+ * behind a direct load waits for it, and small tiles' loads are many stages ahead). */
+template <int TM, int TN, int WAVES_M, int BUFS, int AHEAD, bool XT, bool WT>
+void launch_small(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
+  if constexpr (!XT && !WT) {
+    if (pl.x_direct && pl.w_direct) return launch_ways<TM, TN, WAVES_M, BUFS, 0, DIRECT, DIRECT>(a, o, pl, s);
+  }
+  launch_ways<TM, TN, WAVES_M, 2, AHEAD, XT ? TURNED : ROWS, WT ? TURNED : ROWS>(a, o, pl, s);
+}
+
+template <bool XT, bool WT>
+void launch_large(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
   constexpr Way X = XT ? TURNED : DIRECT, W = WT ? TURNED : DIRECT, XR = XT ? TURNED : ROWS, WR = WT ? TURNED : ROWS;
   if (!XT && !pl.x_direct) {
     if (!WT && !pl.w_direct)
-      launch_ways<TM, TN, WAVES_M, XR, WR>(a, o, pl, s);
+      launch_ways<256, 256, 2, 2, 0, XR, WR>(a, o, pl, s);
     else
-      launch_ways<TM, TN, WAVES_M, XR, W>(a, o, pl, s);
+      launch_ways<256, 256, 2, 2, 0, XR, W>(a, o, pl, s);
   } else {
     if (!WT && !pl.w_direct)
-      launch_ways<TM, TN, WAVES_M, X, WR>(a, o, pl, s);
+      launch_ways<256, 256, 2, 2, 0, X, WR>(a, o, pl, s);
     else
-      launch_ways<TM, TN, WAVES_M, X, W>(a, o, pl, s);
+      launch_ways<256, 256, 2, 2, 0, X, W>(a, o, pl, s);
   }
 }
 
@@ -417,10 +485,12 @@ void launch_shape(const Operands &a, const Out &o, const TilePlan &pl, hipStream
 
 template <bool XT, bool WT>
 void launch_tiles(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
-  if (pl.tm == 256)
-    launch_shape<256, 256, 2, XT, WT>(a, o, pl, s);
+  if (pl.tm == 256 && pl.tn == 256)
+    launch_large<XT, WT>(a, o, pl, s);
+  else if (pl.tm == 256)
+    launch_small<256, 128, 2, 3, 1, XT, WT>(a, o, pl, s);
   else
-    launch_shape<128, 128, 2, XT, WT>(a, o, pl, s);
+    launch_small<128, 128, 2, 4, 3, XT, WT>(a, o, pl, s);
 }
 
 }  // namespace d3s
