@@ -379,12 +379,11 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
   stage_barrier<0>();
   constexpr int ACROSS = WN / 8, DOWN = WAVE / ACROSS, ROUNDS = 32 / DOWN;
   float *mine = (float *)lds + wid * 32 * OUT_ROW;
-  const int i_at = i0 + wi + lane / ACROSS, j_at = j0 + wj + lane % ACROSS * 8;
-  const uint4 bias = bias_eight(o, j_at);
+  float *row = mine + lane / ACROSS * OUT_ROW + lane % ACROSS * 8;
+  const Eights<ROUNDS, DOWN, OUT_ROW> out(o, i0 + wi + lane / ACROSS, j0 + wj + lane % ACROSS * 8);
   const bool works = o.bias || o.z || o.act != D3S_ACT_NONE;
-  Eight ahead[ROUNDS];
-#pragma unroll
-  for (int r = 0; r < ROUNDS; r++) get_eight(o, i_at + r * DOWN, j_at, ahead[r]);
+  typename Eights<ROUNDS, DOWN, OUT_ROW>::Residual now, ahead;
+  out.get(ahead, 0);
 #pragma nounroll
   for (int p = 0; p < FM; p++) {
     wave_lds_sync();
@@ -416,28 +415,11 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
         }
     }
     wave_lds_sync();
-    Eight now[ROUNDS];
-#pragma unroll
-    for (int r = 0; r < ROUNDS; r++) now[r] = ahead[r];
-    if (p + 1 < FM) {
-#pragma unroll
-      for (int r = 0; r < ROUNDS; r++) get_eight(o, i_at + (p + 1) * 32 + r * DOWN, j_at, ahead[r]);
-    }
-    float *row = mine + lane / ACROSS * OUT_ROW + lane % ACROSS * 8;
-    if (works) {
-#pragma nounroll
-      for (int r = 0; r < ROUNDS; r += 2)
-        activate_twice_eight(o, i_at + p * 32 + r * DOWN, DOWN, j_at, row + r * DOWN * OUT_ROW, OUT_ROW, bias);
-    }
-#pragma unroll
-    for (int r = 0; r < ROUNDS; r++)
-      put_eight(o, i_at + p * 32 + r * DOWN, j_at, row + r * DOWN * OUT_ROW, now[r]);
-    if (j_at < o.n && j_at + 8 > o.n) {
-#pragma nounroll
-      for (int r = 0; r < 32; r += DOWN)
-        for (int e = 0; e < o.n - j_at && i_at + p * 32 + r < o.m; e++)
-          put_one(o, i_at + p * 32 + r, j_at + e, row[r * OUT_ROW + e]);
-    }
+    now = ahead;
+    if (p + 1 < FM) out.get(ahead, (p + 1) * 32);
+    if (works) out.activate(row, p * 32);
+    out.put(row, p * 32, now);
+    out.put_rest(row, p * 32);
   }
 }
 

@@ -46,13 +46,13 @@ __device__ __forceinline__ float activated(float z) {
     float e;
     return fmaf(-u, normal_below(u, &e), __builtin_elementwise_maximum(z, 0.0f));
   }
-  /* far below, z times a probability that is 0 in fp32 (-inf times it would be NaN) */
-  if (ACT > D3S_ACT_RELU && z < -100.0f) return 0.0f;
+  /* (from -100 on down exp overflows and the products are -0; -inf times 0 would be NaN) */
+  const float zc = ACT > D3S_ACT_RELU ? __builtin_elementwise_maximum(z, -100.0f) : z;
   switch (ACT) {
-    case D3S_ACT_RELU: return z < 0.0f ? 0.0f : z; /* (a NaN stays one) */
-    case D3S_ACT_SILU: return z * logistic(z);
+    case D3S_ACT_RELU: return __builtin_elementwise_maximum(z, 0.0f); /* (a NaN stays one) */
+    case D3S_ACT_SILU: return zc * logistic(zc);
     case D3S_ACT_GELU_TANH: /* (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)) */
-      return z * logistic(2.0f * GELU_C * z * fmaf(GELU_A * z, z, 1.0f));
+      return zc * logistic(2.0f * GELU_C * zc * fmaf(GELU_A * zc, zc, 1.0f));
   }
   return z;
 }
@@ -145,24 +145,6 @@ __device__ __forceinline__ void put_some(const Out &o, int i, int j, int skip, f
   }
 }
 
-/* elements of y's type: eight neighbouring ones of a residual */
-struct Eight {
-  uint4 lo, hi; /* (bf16: lo alone) */
-};
-
-/* residual (i, j .. j + 7); nothing where the eight are not all there */
-__device__ __forceinline__ void get_eight(const Out &o, int i, int j, Eight &r) {
-  r.lo = r.hi = make_uint4(0u, 0u, 0u, 0u);
-  if (!o.residual || i >= o.m || j + 8 > o.n) return;
-  const int64_t at = (int64_t)i * o.residual_stride + j;
-  if (o.f32) {
-    r.lo = load16((const float *)o.residual + at);
-    r.hi = load16((const float *)o.residual + at + 4);
-  } else {
-    r.lo = load16((const uint16_t *)o.residual + at);
-  }
-}
-
 __device__ __forceinline__ void bf_eight(uint4 q, float *v) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -175,54 +157,95 @@ __device__ __forceinline__ uint4 pack_eight(const float *s) {
   return make_uint4(pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7]));
 }
 
-/* the bias of outputs j .. j + 7, zeros where the eight are not all there */
-__device__ __forceinline__ uint4 bias_eight(const Out &o, int j) {
-  return o.bias && j + 8 <= o.n ? load16(o.bias + j) : make_uint4(0u, 0u, 0u, 0u);
-}
+/* A lane's eight neighbouring outputs from j on, of rows i, i + DOWN, ... (ROUNDS
+ * of them, from `down` rows below i), whose sums lie ROW floats apart in LDS, 16-byte
+ * aligned.  The outputs' addresses may lie at any element. */
+template <int ROUNDS, int DOWN, int ROW>
+struct Eights {
+  const Out &o;
+  const int i, j;
+  const bool all; /* the eight are inside */
+  uint4 bias;
+  struct Residual {
+    uint4 lo[ROUNDS], hi[ROUNDS]; /* bf16: lo alone */
+  };
 
-/* Outputs (i, j .. j + 7), in two steps, so that the second, light, can be
- * unrolled over rows whose residuals are in flight: first the sums at `sum` (16-byte
- * aligned) of rows i and i + down become activations, with the bias as bias_eight
- * gave it ... */
-__device__ __forceinline__ void activate_twice_eight(const Out &o, int i, int down, int j, float *sum, int row, uint4 bias) {
-  if (i >= o.m || j + 8 > o.n) return;
-  float s[16], v[8];
-  bf_eight(bias, v);
-#pragma unroll
-  for (int h = 0; h < 2; h++) { /* (the second row's sums lie `down` rows of LDS further) */
-    const f32x4 a = *(const f32x4 *)(sum + h * down * row), b = *(const f32x4 *)(sum + h * down * row + 4);
-#pragma unroll
-    for (int e = 0; e < 4; e++) s[h * 8 + e] = a[e] + v[e], s[h * 8 + 4 + e] = b[e] + v[e + 4];
+  __device__ __forceinline__ Eights(const Out &out, int row, int column)
+      : o(out), i(row), j(column), all(row < out.m && column + 8 <= out.n) {
+    bias = o.bias && all ? load16(o.bias + j) : make_uint4(0u, 0u, 0u, 0u);
   }
-  if (o.z) {
-    store16(o.z + (int64_t)i * o.z_stride + j, pack_eight(s));
-    if (i + down < o.m) store16(o.z + (int64_t)(i + down) * o.z_stride + j, pack_eight(s + 8));
-  }
-  activate<16>(s, o.act);
+  /* rows past the last are the last again */
+  __device__ __forceinline__ void get(Residual &r, int down) const {
+    if (!o.residual || !all) return;
+    if (o.f32) {
+      const float *at = (const float *)o.residual + ((int64_t)i * o.residual_stride + j);
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    *(f32x4 *)(sum + h * down * row) = f32x4{s[h * 8], s[h * 8 + 1], s[h * 8 + 2], s[h * 8 + 3]};
-    *(f32x4 *)(sum + h * down * row + 4) = f32x4{s[h * 8 + 4], s[h * 8 + 5], s[h * 8 + 6], s[h * 8 + 7]};
-  }
-}
-/* ... then they are written, with the residual as get_eight gave it.  Where the
- * eight are not all there, `sum` still holds sums. */
-__device__ __forceinline__ void put_eight(const Out &o, int i, int j, const float *sum, const Eight &r) {
-  if (i >= o.m || j + 8 > o.n) return;
-  f32x4 a = *(const f32x4 *)sum, b = *(const f32x4 *)(sum + 4);
-  if (o.f32) {
-    if (o.residual) a += __builtin_bit_cast(f32x4, r.lo), b += __builtin_bit_cast(f32x4, r.hi);
-    float *y = (float *)o.y + (int64_t)i * o.y_stride + j;
-    store16(y, __builtin_bit_cast(uint4, a));
-    store16(y + 4, __builtin_bit_cast(uint4, b));
-  } else {
-    float s[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, v[8];
-    bf_eight(r.lo, v);
+      for (int c = 0; c < ROUNDS; c++) {
+        const float *p = at + (int64_t)min(down + c * DOWN, o.m - 1 - i) * o.residual_stride;
+        r.lo[c] = load16(p);
+        r.hi[c] = load16(p + 4);
+      }
+    } else {
+      const uint16_t *at = (const uint16_t *)o.residual + ((int64_t)i * o.residual_stride + j);
 #pragma unroll
-    for (int e = 0; e < 8; e++) s[e] = o.residual ? s[e] + v[e] : s[e];
-    store16((uint16_t *)o.y + (int64_t)i * o.y_stride + j, pack_eight(s));
+      for (int c = 0; c < ROUNDS; c++) r.lo[c] = load16(at + (int64_t)min(down + c * DOWN, o.m - 1 - i) * o.residual_stride);
+    }
   }
-}
+  /* sums become activations; z is written */
+  __device__ __forceinline__ void activate(float *sums, int down) const {
+    if (!all) return;
+    uint16_t *z = o.z + ((int64_t)(i + down) * o.z_stride + j);
+#pragma nounroll
+    for (int c = 0; c < ROUNDS; c++) {
+      float s[8], v[8];
+      const f32x4 a = *(const f32x4 *)(sums + c * DOWN * ROW), b = *(const f32x4 *)(sums + c * DOWN * ROW + 4);
+      bf_eight(bias, v);
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[e] = a[e] + v[e], s[e + 4] = b[e] + v[e + 4];
+      if (o.z && i + down + c * DOWN < o.m) store16(z + c * (DOWN * o.z_stride), pack_eight(s));
+      d3s::activate<8>(s, o.act);
+      *(f32x4 *)(sums + c * DOWN * ROW) = f32x4{s[0], s[1], s[2], s[3]};
+      *(f32x4 *)(sums + c * DOWN * ROW + 4) = f32x4{s[4], s[5], s[6], s[7]};
+    }
+  }
+  /* y from the activations and the residual */
+  __device__ __forceinline__ void put(const float *sums, int down, const Residual &r) const {
+    if (!all) return;
+    const int64_t y = (int64_t)(i + down) * o.y_stride + j;
+    if (o.f32) {
+#pragma unroll
+      for (int c = 0; c < ROUNDS; c++) {
+        f32x4 a = *(const f32x4 *)(sums + c * DOWN * ROW), b = *(const f32x4 *)(sums + c * DOWN * ROW + 4);
+        if (o.residual) a += __builtin_bit_cast(f32x4, r.lo[c]), b += __builtin_bit_cast(f32x4, r.hi[c]);
+        if (i + down + c * DOWN < o.m) {
+          float *at = (float *)o.y + y + c * (DOWN * o.y_stride);
+          store16(at, __builtin_bit_cast(uint4, a));
+          store16(at + 4, __builtin_bit_cast(uint4, b));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < ROUNDS; c++) {
+        const f32x4 a = *(const f32x4 *)(sums + c * DOWN * ROW), b = *(const f32x4 *)(sums + c * DOWN * ROW + 4);
+        float s[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}, v[8];
+        if (o.residual) {
+          bf_eight(r.lo[c], v);
+#pragma unroll
+          for (int e = 0; e < 8; e++) s[e] += v[e];
+        }
+        if (i + down + c * DOWN < o.m) store16((uint16_t *)o.y + y + c * (DOWN * o.y_stride), pack_eight(s));
+      }
+    }
+  }
+  /* columns that are not all there: from the sums, one by one */
+  __device__ __forceinline__ void put_rest(const float *sums, int down) const {
+    if (all || j >= o.n) return;
+#pragma nounroll
+    for (int c = 0; c < ROUNDS; c++)
+      for (int e = 0; e < o.n - j && i + down + c * DOWN < o.m; e++)
+        put_one(o, i + down + c * DOWN, j + e, sums[c * DOWN * ROW + e]);
+  }
+};
 
 }  // namespace
 }  // namespace d3s
