@@ -29,24 +29,23 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 /* Microseconds of m rows in tiles of tm x tn, one workgroup a CU: rounds of
  * workgroups, each its stages and what it spends before and after them.
  * Measured, by how many operands go to LDS directly: a stage of 256 x 256 1.45
- * (both), 1.55 (one, the other turned) and 1.72; of 256 x 128 0.93 and 1.27; of
- * 128 x 128 0.52 and 0.80, with half of the CUs idle 0.38 and 0.72.  Around them
- * 14, 10 and 6, and for split sums 3 and 1 a split.
+ * (both), 1.65 (one) and 2.2; of 128 x 256 0.93 and 1.2; of 128 x 128 0.52 and
+ * 0.75, with a quarter of the CUs idle 0.38 and 0.65.  Around them 14, 10 and 6, and
+ * for split sums 3 and 1 a split.
  * (8192 x 2048 x 2048, both direct: 63, 78 and 87 us in the three tiles;
- * 2048 x 2048 x 2048: 50, 29 and 22; 4096 x 2048 x 8192, both turned: 217, 163
- * and 210; 256 x 2048 x 8192: 128 x 128 with 1, 2, 4 and 8 splits 49, 31, 22
- * and 24.) */
+ * 2048 x 2048 x 2048: 50, 29 and 22; 4096 x 2048 x 8192, both by the inner
+ * index: 217, 160 and 210; 256 x 2048 x 8192: 128 x 128 with 1, 2, 4 and 8
+ * splits 49, 31, 22 and 24.)  Between 128 x 256 and 256 x 128 there is little,
+ * but rows of x that are not at 4 bytes cost less the fewer tiles load them (heads of
+ * 4097 outputs, their weights' gradient: 186 and 205 us). */
 double tile_us(const Product &p, int64_t m, int tm, int tn, int splits) {
   const int direct = p.x_direct + p.w_direct;
   const double wgs = (double)up(m, tm) * (double)up(p.n, tn) * splits;
   const double rounds = (double)(int64_t)((wgs + CUS - 1) / CUS), stages = (double)up(p.k, (int64_t)TILE_K * splits);
-  if (tn == 256) {
-    const bool mixed = direct == 1 && p.x_turned != p.w_turned;
-    return rounds * (stages * (direct == 2 ? 1.45 : mixed ? 1.55 : 1.72) + 14);
-  }
-  if (tm == 256) return rounds * (stages * (direct == 2 ? 0.93 : 1.27) + 10);
+  if (tm == 256) return rounds * (stages * (direct == 2 ? 1.45 : direct == 1 ? 1.65 : 2.2) + 14);
+  if (tn == 256) return rounds * (stages * (direct == 2 ? 0.93 : 1.2) + 10);
   const bool few = wgs <= CUS * 3 / 4;
-  const double stage = direct == 2 ? (few ? 0.38 : 0.52) : few ? 0.72 : 0.80;
+  const double stage = direct == 2 ? (few ? 0.38 : 0.52) : few ? 0.65 : 0.75;
   return rounds * (stages * stage + 6) + (splits > 1 ? 3 + splits : 0);
 }
 
@@ -83,7 +82,7 @@ Plan plan(const Product &p) {
       pl.tile.tm = tm, pl.tile.tn = tn, pl.tile.splits = (unsigned)splits;
     };
     offer(256, 256, 1);
-    offer(256, 128, 1);
+    offer(128, 256, 1);
     /* (every split has its stages, and fewer workgroups than twice the CUs) */
     for (int s = 1; s <= 8; s++)
       if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(p.n, 128) * s <= 2 * CUS)) offer(128, 128, s);

@@ -31,27 +31,28 @@ constexpr int STEP = 16;       /* ... of a matrix instruction */
 constexpr unsigned TILE_GRID = 1 << 22; /* workgroups a launch: their threads are counted in 32 bits */
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 #define D3S_LDS __attribute__((address_space(3)))
 #define D3S_GLOBAL __attribute__((address_space(1)))
 
-/* how an operand's stages reach LDS */
-enum Way { DIRECT, ROWS, TURNED };
+/* how an operand's stages reach LDS, and how they lie there (above) */
+enum Way { DIRECT, ROWS, TURNED, INNER };
 
-/* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED: stored [k, rows]). */
+/* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED, INNER: stored [k, rows]). */
 template <int R, Way WAY, int SETS>
 struct Part {
   static constexpr int BYTES = R * TK * 2;
   static constexpr int PER = R * TK / 8 / TT;                      /* 16-byte loads a thread */
   static constexpr int DIRECTS = WAY == DIRECT ? PER : 0;          /* of them into LDS */
   static constexpr int LOADS = WAY == DIRECT ? 0 : PER;            /* ... into registers */
-  static constexpr int WRITES = WAY == DIRECT ? 0 : WAY == ROWS ? PER : 8; /* and from them */
+  static constexpr int WRITES = WAY == DIRECT ? 0 : WAY == TURNED ? 8 : PER; /* and from them */
   const uint16_t *p;
   int64_t stride;
   int rows, r0;
   uint32_t off[WAY == DIRECT ? PER : 1]; /* bytes from the tile's first row, and where that is */
   __amdgpu_buffer_rsrc_t from;
-  const uint16_t *mine;                  /* ROWS, TURNED: the thread's first chunk of stage 0 */
+  const uint16_t *mine;                  /* TURNED, INNER: the thread's first chunk of stage 0 */
   int to;                                /* TURNED: its first row in LDS (below 0: not the tile's) */
   uint4 q[SETS][PER];
 
@@ -62,6 +63,12 @@ struct Part {
   static __device__ __forceinline__ int chunk(int u) { return tid() % 8 ^ turn(row(u)); }
   /* TURNED: the thread's inner indices inside a stage, PER of them from here */
   static __device__ __forceinline__ int inner() { return tid() / (R / 8) * PER; }
+  /* INNER: the u-th place's inner index, and its chunk: ACROSS places an index, in
+   * order (the same chunk for every u) */
+  static constexpr int ACROSS = R / 8;
+  static __device__ __forceinline__ int spin(int k) { return (k & 3) << 2 & (ACROSS - 1); }
+  static __device__ __forceinline__ int inner(int u) { return u * (TT / ACROSS) + tid() / ACROSS; }
+  static __device__ __forceinline__ int across() { return tid() % ACROSS ^ spin(inner(0)); }
 
   __device__ __forceinline__ Part(const uint16_t *base, int64_t st, int n, int first)
       : p(base), stride(st), rows(n), r0(first) {
@@ -75,6 +82,11 @@ struct Part {
       to = tid() % (R / 8) * 8;
       if (rows >= 8) to = min(to, rows - 8 - r0);
       mine = p + (int64_t)inner() * stride + (r0 + to);
+    } else if constexpr (WAY == INNER) {
+      /* (chunks past the rows are the last one again; one that is cut reads on into
+       * the next inner index: see whole()) */
+      to = min(across() * 8, (rows - 1 - r0) / 8 * 8);
+      mine = p + (int64_t)inner(0) * stride + (r0 + to);
     }
   }
   /* the u-th 16 bytes of stage k0, straight into LDS (a buffer load: one 32-bit
@@ -84,15 +96,18 @@ struct Part {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (D3S_LDS void *)(lds + (u * TT + wid * WAVE) * 16), 16, (int)off[u],
                                              k0 * 2, 0, 0);
   }
+  /* inner indices of which whole stages may be loaded: not the last where an
+   * INNER chunk is cut, it would read past the operand's end */
+  __device__ __forceinline__ int whole(int k) const { return WAY == INNER && r0 + R > rows && rows % 8 != 0 ? max(k - 1, 0) : k; }
   /* the same into registers, from start(k0): a whole stage, at least eight rows if TURNED */
   __device__ __forceinline__ const uint16_t *start(int k0) const {
-    return WAY == TURNED ? mine + (int64_t)k0 * stride : p + k0;
+    return WAY == TURNED || WAY == INNER ? mine + (int64_t)k0 * stride : p + k0;
   }
   __device__ __forceinline__ void load(int set, int u, const uint16_t *at) {
     if constexpr (WAY == ROWS)
       q[set][u] = load16(at + ((int64_t)min(r0 + row(u), rows - 1) * stride + chunk(u) * 8));
     else
-      q[set][u] = load16(at + u * stride);
+      q[set][u] = load16(at + u * (WAY == INNER ? TT / ACROSS * stride : stride));
   }
   /* the same of any stage: something finite or not from k1 on */
   __device__ __forceinline__ void load_some(int k0, int k1) {
@@ -104,6 +119,8 @@ struct Part {
           q[0][u] = load16(at + (r0 + to));
         else
           q[0][u] = r0 + to < rows ? row_chunk(at, r0 + to, rows) : make_uint4(0u, 0u, 0u, 0u);
+      } else if constexpr (WAY == INNER) {
+        q[0][u] = row_chunk(p + (int64_t)min(k0 + inner(u), k1 - 1) * stride, r0 + to, rows);
       } else {
         const int k = k0 + chunk(u) * 8;
         const uint16_t *at = p + (int64_t)min(r0 + row(u), rows - 1) * stride;
@@ -139,6 +156,14 @@ struct Part {
   }
   /* the fragment of rows r .. r + 31 (r a multiple of 32), inner indices 16 step .. + 15 */
   static __device__ __forceinline__ bf16x8 fragment(const char *lds, int r, int step) {
+    if constexpr (WAY == INNER) { /* two transposing reads: four inner indices of 16 rows a lane group */
+      const int g = lane_id() >> 4, i = lane_id() & 15, k = step * STEP + (g >> 1) * 8 + (i >> 2);
+      const int c = (r / 8 + (g & 1) * 2 + (i >> 1 & 1)) ^ spin(i >> 2);
+      const char *at = lds + k * (R * 2) + c * 16 + (i & 1) * 8;
+      const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((D3S_LDS bf16x4 *)at);
+      const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((D3S_LDS bf16x4 *)(at + 4 * R * 2));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
     const int at = r + (lane_id() & 31), c = (step * 2 + (lane_id() >> 5)) ^ turn(at);
     return *(const bf16x8 *)(lds + at * (TK * 2) + c * 16);
   }
@@ -195,7 +220,7 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
 #pragma unroll
       for (int i = 0; i < 16; i++) acc[p][q][i] = 0.0f;
 
-  const int whole = a.k / TK;
+  const int whole = min(px.whole(a.k), pw.whole(a.k)) / TK;
   const int s0 = min(whole, (int)split * pl.stages);
   const int s1 = split == pl.splits - 1 ? whole : min(whole, s0 + pl.stages);
   bf16x8 fx[2][FM], fw[2][FN];
@@ -444,22 +469,26 @@ void launch_small(const Operands &a, const Out &o, const TilePlan &pl, hipStream
   if constexpr (!XT && !WT) {
     if (pl.x_direct && pl.w_direct) return launch_ways<TM, TN, WAVES_M, BUFS, 0, DIRECT, DIRECT>(a, o, pl, s);
   }
-  launch_ways<TM, TN, WAVES_M, 2, AHEAD, XT ? TURNED : ROWS, WT ? TURNED : ROWS>(a, o, pl, s);
+  launch_ways<TM, TN, WAVES_M, 2, AHEAD, XT ? INNER : ROWS, WT ? INNER : ROWS>(a, o, pl, s);
 }
 
+/* The large tile turns (8192 x 2048 x 8192, both by the inner index: 305 us, as they
+ * are 335; one beside direct rows, k 4096: 121, as it is beside rows through
+ * registers 134), the small ones read transposed (4096 x 2048 x 8192 in 128 x 256:
+ * 160, turned 173; their writes have fewer products to hide behind). */
 template <bool XT, bool WT>
 void launch_large(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
-  constexpr Way X = XT ? TURNED : DIRECT, W = WT ? TURNED : DIRECT, XR = XT ? TURNED : ROWS, WR = WT ? TURNED : ROWS;
-  if (!XT && !pl.x_direct) {
-    if (!WT && !pl.w_direct)
-      launch_ways<256, 256, 2, 2, 0, XR, WR>(a, o, pl, s);
-    else
-      launch_ways<256, 256, 2, 2, 0, XR, W>(a, o, pl, s);
+  if constexpr (XT && WT) {
+    launch_ways<256, 256, 2, 2, 0, TURNED, TURNED>(a, o, pl, s);
+  } else if constexpr (XT) {
+    pl.w_direct ? launch_ways<256, 256, 2, 2, 0, TURNED, DIRECT>(a, o, pl, s) : launch_ways<256, 256, 2, 2, 0, TURNED, ROWS>(a, o, pl, s);
+  } else if constexpr (WT) {
+    pl.x_direct ? launch_ways<256, 256, 2, 2, 0, DIRECT, TURNED>(a, o, pl, s) : launch_ways<256, 256, 2, 2, 0, ROWS, TURNED>(a, o, pl, s);
   } else {
-    if (!WT && !pl.w_direct)
-      launch_ways<256, 256, 2, 2, 0, X, WR>(a, o, pl, s);
+    if (pl.x_direct)
+      pl.w_direct ? launch_ways<256, 256, 2, 2, 0, DIRECT, DIRECT>(a, o, pl, s) : launch_ways<256, 256, 2, 2, 0, DIRECT, ROWS>(a, o, pl, s);
     else
-      launch_ways<256, 256, 2, 2, 0, X, W>(a, o, pl, s);
+      pl.w_direct ? launch_ways<256, 256, 2, 2, 0, ROWS, DIRECT>(a, o, pl, s) : launch_ways<256, 256, 2, 2, 0, ROWS, ROWS>(a, o, pl, s);
   }
 }
 
@@ -469,10 +498,10 @@ template <bool XT, bool WT>
 void launch_tiles(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s) {
   if (pl.tm == 256 && pl.tn == 256)
     launch_large<XT, WT>(a, o, pl, s);
-  else if (pl.tm == 256)
-    launch_small<256, 128, 2, 3, 1, XT, WT>(a, o, pl, s);
+  else if (pl.tn == 256)
+    launch_small<128, 256, 2, 3, 1, XT, WT>(a, o, pl, s);
   else
-    launch_small<128, 128, 2, 4, 3, XT, WT>(a, o, pl, s);
+    launch_small<128, 128, 2, 4, 1, XT, WT>(a, o, pl, s);
 }
 
 }  // namespace d3s
