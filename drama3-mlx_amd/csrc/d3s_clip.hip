@@ -1,14 +1,15 @@
 /* k_norm, k_clip: the global L2 norm of many gradients, and the gradients
  * scaled to it (gfx950, wave64; include/d3s_train.h).
  *
- * The tensors' addresses and lengths travel as kernel arguments (up to
- * CLIP_TENSORS a launch), so the call keeps nothing and may be captured.  A
- * launch's elements are cut into chunks of one size; chunk i belongs to the
+ * The tensors' addresses and lengths travel as kernel arguments (as many a
+ * launch as 4 KiB hold: a launch costs more than a short tensor's work), so the
+ * call keeps nothing and may be captured; a tensor of more than 2^30 elements
+ * travels in pieces.  A launch's elements are cut into chunks of one size; chunk i belongs to the
  * tensor whose range of chunk numbers holds it (a search in the arguments).
  * k_norm: workgroups take chunks in turn, square in 64 bits (a bf16's square is
  * exact and an fp32's keeps its range: nothing overflows, and the order costs no
  * accuracy; the conversions hide behind the loads) and leave one partial sum
- * each.  k_clip: every workgroup adds all partial sums in one order (they are a
+ * each (a later launch of the same call adds to them).  k_clip: every workgroup adds all partial sums in one order (they are a
  * few kilobytes of L2; a launch of its own for it would cost more), and scales
  * its chunks, from the last to the first: the end of the norm's pass is what
  * the cache still holds.
@@ -21,30 +22,34 @@ namespace {
 
 constexpr int CT = 256;
 constexpr int CW = CT / WAVE;
-constexpr int CLIP_TENSORS = 128;  /* tensors a launch */
+constexpr int NORM_PIECES = 248;  /* a launch of k_norm */
+constexpr int CLIP_PIECES = 164;  /* a launch of k_clip */
+constexpr int64_t PIECE = (int64_t)1 << 30; /* elements, at most */
 constexpr int CLIP_GROUPS = 1024;  /* workgroups a launch of k_norm: its partial sums */
 constexpr int CU = 4;              /* 16-byte loads a lane has in flight */
 
-struct ClipArgs {
-  const void *src[CLIP_TENSORS];
-  uint32_t first[CLIP_TENSORS]; /* the tensor's first chunk */
-  uint64_t numel[CLIP_TENSORS]; /* elements << 1 | bf16 */
+template <int MOST>
+struct Pieces {
+  const void *src[MOST];
+  uint32_t first[MOST]; /* the piece's first chunk */
+  uint32_t numel[MOST]; /* elements << 1 | bf16 */
   int n;
   uint32_t chunks;
   uint32_t chunk; /* 16-byte units a chunk */
 };
 struct ClipOut {
-  void *dst[CLIP_TENSORS];
+  void *dst[CLIP_PIECES];
 };
 
-/* a chunk of a tensor: elements [j0, j1) from an aligned start, or cut by the tensor's ends */
+/* a chunk of a piece: elements [j0, j1) from an aligned start, or cut by the piece's ends */
 struct Chunk {
   int t;
   bool bf16;
   int64_t j0, j1;
 };
 
-__device__ __forceinline__ Chunk find_chunk(const ClipArgs &a, uint32_t i) {
+template <int MOST>
+__device__ __forceinline__ Chunk find_chunk(const Pieces<MOST> &a, uint32_t i) {
   int lo = 0, hi = a.n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -141,14 +146,14 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(CT) void k_norm(ClipArgs a, double *parts) {
+__global__ __launch_bounds__(CT) void k_norm(Pieces<NORM_PIECES> a, double *parts, int have) {
   double sum = 0.0;
   for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
     const Chunk c = find_chunk(a, i);
     sum += c.bf16 ? chunk_squares<true>(a.src[c.t], c) : chunk_squares<false>(a.src[c.t], c);
   }
   sum = block_sum(sum);
-  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+  if (threadIdx.x == 0) parts[blockIdx.x] = (int)blockIdx.x < have ? parts[blockIdx.x] + sum : sum;
 }
 
 /* the norm from its partial sums, in every thread */
@@ -217,7 +222,7 @@ __device__ __forceinline__ void chunk_scale(const void *p, void *d, const Chunk 
   if (e < s.tail1) scale_one<BF16>(p, d, e, scale, keep);
 }
 
-__global__ __launch_bounds__(CT) void k_clip(ClipArgs a, ClipOut out, const double *parts, int n_parts,
+__global__ __launch_bounds__(CT) void k_clip(Pieces<CLIP_PIECES> a, ClipOut out, const double *parts, int n_parts,
                                              float max_norm, float *norm) {
   const float v = norm_of(parts, n_parts);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
@@ -233,64 +238,76 @@ __global__ __launch_bounds__(CT) void k_clip(ClipArgs a, ClipOut out, const doub
   }
 }
 
-int launches(int n_tensors) { return (n_tensors + CLIP_TENSORS - 1) / CLIP_TENSORS; }
+/* walks the tensors' pieces, MOST at a time */
+struct Walk {
+  const void *const *src;
+  void *const *dst;
+  const int64_t *numel;
+  const int32_t *dtypes;
+  int n_tensors, t;
+  int64_t at; /* elements of tensor t that are behind */
 
-/* tensors [t0, t0 + n) and their chunks */
-void fill(ClipArgs &a, const void *const *src, const int64_t *numel, const int32_t *dtypes, int t0, int n) {
-  /* chunks of 4 KiB (a 16-byte unit a lane) up to 64 KiB, by what fills the workgroups */
-  auto units = [&](int i) {
-    const int size = dtypes[i] == D3S_DTYPE_BF16 ? 2 : 4;
-    return numel[i] == 0 ? (int64_t)0 : (numel[i] * size + (int64_t)((uintptr_t)src[i] & 15u) + 15) / 16;
-  };
-  int64_t total = 0;
-  for (int i = t0; i < t0 + n; i++) total += units(i);
-  int64_t chunk = CT;
-  while (chunk < 16 * CT && total > chunk * CLIP_GROUPS) chunk *= 2;
-  for (;;) { /* (chunk numbers are 32 bits) */
-    int64_t at = 0;
-    for (int i = 0; i < n; i++) {
-      a.src[i] = src[t0 + i];
-      a.first[i] = (uint32_t)at;
-      a.numel[i] = (uint64_t)numel[t0 + i] << 1 | (dtypes[t0 + i] == D3S_DTYPE_BF16 ? 1u : 0u);
-      at += (units(t0 + i) + chunk - 1) / chunk;
+  /* the next pieces and their chunks; false: there are none left */
+  template <int MOST>
+  bool fill(Pieces<MOST> &a, void **out) {
+    int64_t total = 0;
+    a.n = 0;
+    uint32_t units[MOST];
+    while (t < n_tensors && a.n < MOST) {
+      const int size = dtypes[t] == D3S_DTYPE_BF16 ? 2 : 4;
+      const int64_t left = numel[t] - at, n = left < PIECE ? left : PIECE;
+      if (n > 0) {
+        a.src[a.n] = (const char *)src[t] + at * size;
+        if (out) out[a.n] = (char *)dst[t] + at * size;
+        a.numel[a.n] = (uint32_t)n << 1 | (size == 2 ? 1u : 0u);
+        units[a.n] = (uint32_t)((n * size + (int64_t)((uintptr_t)a.src[a.n] & 15u) + 15) / 16);
+        total += units[a.n];
+        a.n++;
+      }
+      at += n;
+      if (at >= numel[t]) t++, at = 0;
     }
-    a.n = n;
-    a.chunks = (uint32_t)at;
-    a.chunk = (uint32_t)chunk;
-    if (at <= 0x7fffffff || chunk >= (int64_t)1 << 30) return;
-    chunk *= 2;
+    /* chunks of 4 KiB (a 16-byte unit a lane) up to 64 KiB, by what fills the workgroups */
+    uint32_t chunk = CT;
+    while (chunk < 16 * CT && total > (int64_t)chunk * CLIP_GROUPS) chunk *= 2;
+    uint32_t first = 0; /* (at most 248 pieces of 2^18 chunks) */
+    for (int i = 0; i < a.n; i++) {
+      a.first[i] = first;
+      first += (units[i] + chunk - 1) / chunk;
+    }
+    a.chunks = first;
+    a.chunk = chunk;
+    return a.n > 0;
   }
-}
+};
 
 }  // namespace
 
-size_t clip_workspace_bytes(int n_tensors) {
-  const size_t parts = (size_t)launches(n_tensors > 0 ? n_tensors : 1) * CLIP_GROUPS;
-  return split_counter_bytes() + parts * sizeof(double);
-}
+size_t clip_workspace_bytes() { return split_counter_bytes() + CLIP_GROUPS * sizeof(double); }
 
 void launch_clip(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int n_tensors,
                  float max_norm, float *norm, void *ws, hipStream_t s) {
   double *parts = (double *)((char *)ws + split_counter_bytes());
-  ClipArgs a;
   int n_parts = 0;
-  for (int t0 = 0; t0 < n_tensors; t0 += CLIP_TENSORS) {
-    fill(a, src, numel, dtypes, t0, min(n_tensors - t0, CLIP_TENSORS));
-    if (a.chunks == 0) continue;
-    const int groups = min((int)min(a.chunks, 0x7fffffffu), CLIP_GROUPS);
-    k_norm<<<groups, CT, 0, s>>>(a, parts + n_parts);
-    n_parts += groups;
+  {
+    Pieces<NORM_PIECES> a;
+    Walk w{src, dst, numel, dtypes, n_tensors, 0, 0};
+    while (w.fill(a, nullptr)) {
+      const int groups = a.chunks < CLIP_GROUPS ? (int)a.chunks : CLIP_GROUPS;
+      k_norm<<<groups, CT, 0, s>>>(a, parts, n_parts);
+      if (groups > n_parts) n_parts = groups;
+    }
   }
   bool written = false;
-  for (int t0 = 0; dst && n_parts > 0 && t0 < n_tensors; t0 += CLIP_TENSORS) {
-    const int n = min(n_tensors - t0, CLIP_TENSORS);
-    fill(a, src, numel, dtypes, t0, n);
-    if (a.chunks == 0) continue;
+  if (dst) {
+    Pieces<CLIP_PIECES> a;
     ClipOut o;
-    for (int i = 0; i < n; i++) o.dst[i] = dst[t0 + i];
-    const int groups = min((int)min(a.chunks, 0x7fffffffu), 2 * CLIP_GROUPS);
-    k_clip<<<groups, CT, 0, s>>>(a, o, parts, n_parts, max_norm, written ? nullptr : norm);
-    written = true;
+    Walk w{src, dst, numel, dtypes, n_tensors, 0, 0};
+    while (w.fill(a, o.dst)) {
+      const int groups = a.chunks < 2 * CLIP_GROUPS ? (int)a.chunks : 2 * CLIP_GROUPS;
+      k_clip<<<groups, CT, 0, s>>>(a, o, parts, n_parts, max_norm, written ? nullptr : norm);
+      written = true;
+    }
   }
   if (!written) k_norm_write<<<1, CT, 0, s>>>(parts, n_parts, norm);
 }

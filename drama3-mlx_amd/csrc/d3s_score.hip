@@ -39,9 +39,11 @@ constexpr int ST = 256;        /* threads of a workgroup */
 constexpr int SW = ST / WAVE;
 constexpr int GRID_MOST = 1 << 22; /* workgroups a launch: their threads are counted in 32 bits */
 constexpr int SU = 4;          /* chunks a lane takes at a time */
-constexpr int LIST = 1024;     /* keys a workgroup ranks */
+constexpr int SCORE_ARRIVALS = 2048; /* rows that have a counter of arrivals */
+constexpr int LIST = 512;      /* keys a workgroup files */
+constexpr int JOIN = 2048;     /* ... and the segments' that it joins */
 constexpr int SEG_MOST = 256;  /* segments a row */
-constexpr int SEG_TOP = 16;    /* the same with alternatives: their keys are ranked again */
+constexpr int SEG_TOP = 64;    /* the same with alternatives: their keys (at most JOIN) are ranked again */
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 /* the least exponent a term is given: 2^-1000 is 0 in fp32, and 0 times it is 0 where 0 * -inf is not */
 constexpr float LEAST = -1000.0f;
@@ -158,11 +160,11 @@ __device__ __forceinline__ void add_batch(Sums &s, const float *v, float c) {
 }
 
 struct ScoreLds {
-  alignas(16) uint64_t list[LIST + 2]; /* (read in pairs, the next in fours) */
+  alignas(16) uint64_t list[LIST + 2]; /* (read in pairs) */
   uint64_t ranked[D3S_MAX_TOP];
-  alignas(16) uint32_t lane_max[ST];
+  uint32_t least[SW];
   float wm[SW], wS[SW], wA[SW];
-  uint64_t bound;
+  uint64_t bound[SW];
   uint32_t count, last;
 };
 
@@ -178,11 +180,11 @@ __device__ __forceinline__ Sums join_block(ScoreLds &L, Sums s, float c) {
   return s;
 }
 
-/* ranks the list's n keys and leaves the best k in L.ranked (fewer: the rest 0) */
-__device__ __forceinline__ void rank_list(ScoreLds &L, uint32_t n, int k) {
+/* ranks a list's n keys (two places behind them) and leaves the best k in L.ranked (fewer: the rest 0) */
+__device__ __forceinline__ void rank_list(ScoreLds &L, uint64_t *list, uint32_t n, int k) {
   if (threadIdx.x < (unsigned)k) L.ranked[threadIdx.x] = 0ull;
   __syncthreads();
-  rank_by_count<ST>(L.list, n, k, L.ranked);
+  rank_by_count<ST>(list, n, k, L.ranked);
 }
 
 /* the row's outputs, by the whole workgroup: s the row's sums, L.ranked its alternatives */
@@ -219,7 +221,7 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, ScoreLds &L, const Ro
 /* words of a segment's record: (m, S), A, then its alternatives' keys */
 __host__ __device__ inline int record_words(int n_top) { return 2 + n_top; }
 
-template <bool BF16, bool ENT>
+template <bool BF16, bool ENT, bool TOP>
 __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chunks, uint32_t *arrivals,
                                               uint64_t *records, int row0) {
   constexpr int EPC = Row<BF16>::EPC;
@@ -244,58 +246,96 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
   const int lo = seg * seg_chunks, hi = min(R.chunks, lo + seg_chunks);
 
   Sums s{-FLT_MAX, 0.0f, 0.0f};
-  int ch = lo + tid;
-  for (; ch + (SU - 1) * ST < hi; ch += SU * ST) {
-    uint4 q[SU];
+  /* With alternatives the segment goes by blocks through LDS (a lane's own
+   * places), where the second pass finds it again: rolled loops, since the code of
+   * such short work has to be fetched while it runs. */
+  __shared__ uint4 block[TOP ? SU * ST + 1 : 1]; /* (later the segments' keys) */
+  static_assert(sizeof(uint64_t) * (JOIN + 2) <= sizeof(uint4) * (SU * ST + 1), "the join's list");
+  uint4 q[SU];
+  auto fetch = [&](int at) {
 #pragma unroll
-    for (int u = 0; u < SU; u++) q[u] = R.base[ch + u * ST];
-    float v[SU * EPC];
+    for (int u = 0; u < SU; u++) q[u] = R.base[min(at + tid + u * ST, hi - 1)];
 #pragma unroll
-    for (int u = 0; u < SU; u++) R.values(q[u], ch + u * ST, v + u * EPC);
-    add_batch<SU * EPC, ENT>(s, v, c);
-  }
-  for (; ch < hi; ch += ST) {
-    float v[EPC];
-    R.values(R.base[ch], ch, v);
-    add_batch<EPC, ENT>(s, v, c);
+    for (int u = 0; u < SU; u++) block[u * ST + tid] = q[u];
+  };
+  if (TOP) {
+    for (int at = lo; at < hi; at += SU * ST) {
+      fetch(at);
+      if (at + tid + (SU - 1) * ST < hi) {
+        float v[SU * EPC];
+#pragma unroll
+        for (int u = 0; u < SU; u++) R.values(q[u], at + tid + u * ST, v + u * EPC);
+        add_batch<SU * EPC, ENT>(s, v, c);
+        continue;
+      }
+#pragma nounroll
+      for (int i = tid; i < min(SU * ST, hi - at); i += ST) {
+        float v[EPC];
+        R.values(block[i], at + i, v);
+        add_batch<EPC, ENT>(s, v, c);
+      }
+    }
+  } else {
+    int ch = lo + tid;
+    for (; ch + (SU - 1) * ST < hi; ch += SU * ST) {
+#pragma unroll
+      for (int u = 0; u < SU; u++) q[u] = R.base[ch + u * ST];
+      float v[SU * EPC];
+#pragma unroll
+      for (int u = 0; u < SU; u++) R.values(q[u], ch + u * ST, v + u * EPC);
+      add_batch<SU * EPC, ENT>(s, v, c);
+    }
+    for (; ch < hi; ch += ST) {
+      float v[EPC];
+      R.values(R.base[ch], ch, v);
+      add_batch<EPC, ENT>(s, v, c);
+    }
   }
   const uint32_t mine = s.S > 0.0f ? d3s_ordkey(s.m) : 0u; /* (0: below every logit's key) */
-  s = join_block(L, s, c);
   const int k = a.n_top;
+  if (TOP) {
+    /* the wave's ceil(k / SW)-th greatest lane maximum, its upper 16 bits (0: there
+     * are not so many): k logits reach the least wave's */
+    const int want = (k + SW - 1) / SW;
+    uint32_t t = 0u;
+#pragma unroll
+    for (int b = 31; b >= 16; b--)
+      if (__popcll(__ballot(mine >= (t | 1u << b))) >= want) t |= 1u << b;
+    if (lane_id() == 0) L.least[tid / WAVE] = t;
+    if (tid == 0) L.count = 0u;
+  }
+  s = join_block(L, s, c);
   const bool live = s.m < __builtin_inff(); /* no NaN or +inf in the segment */
 
-  if (k > 0) {
-    L.lane_max[tid] = mine;
-    if (tid == 0) L.bound = 0ull, L.count = 0u;
-    __syncthreads();
-    uint32_t above = 0u, same = 0u;
-    const uint4 *m4 = (const uint4 *)L.lane_max;
-    for (int i = 0; i < ST / 4; i++) {
-      const uint4 q = m4[i];
-      above += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
-      same += (q.x == mine) + (q.y == mine) + (q.z == mine) + (q.w == mine);
-    }
-    if (above < (uint32_t)k && above + same >= (uint32_t)k) L.bound = (uint64_t)mine << 32;
-    __syncthreads();
+  if (TOP) {
+    uint32_t t = L.least[0];
+#pragma unroll
+    for (int w = 1; w < SW; w++) t = min(t, L.least[w]);
+    uint64_t bound = (uint64_t)t << 32;
     uint32_t n = 0u;
     while (live) { /* every thread of the workgroup agrees on `live` and n */
-      const uint64_t bound = L.bound;
       const float least = (bound >> 32) ? d3s_from_ordkey((uint32_t)(bound >> 32)) : -__builtin_inff();
-      for (int q = lo + tid; q < hi; q += ST) {
-        float v[EPC];
-        R.values(R.base[q], q, v);
-        float b = v[0];
+      for (int at = lo; at < hi; at += SU * ST) {
+        if (hi - lo > SU * ST) fetch(at);
+        uint32_t reach = 0u; /* a bit an element that may */
+#pragma nounroll
+        for (int u = 0; u < SU; u++) {
+          const int i = u * ST + tid;
+          if (at + i >= hi) break;
+          float v[EPC];
+          R.values(block[i], at + i, v);
 #pragma unroll
-        for (int i = 1; i < EPC; i++) b = fmaxf(b, v[i]);
-        if (b >= least) {
-#pragma unroll
-          for (int i = 0; i < EPC; i++) {
-            const int j = q * EPC + i - R.lead;
-            const uint64_t key = composite_key(v[i], j);
-            if (key >= bound && j >= 0 && j < a.vocab) {
-              const uint32_t at = atomicAdd(&L.count, 1u);
-              if (at < LIST) L.list[at] = key;
-            }
+          for (int e = 0; e < EPC; e++) reach |= (v[e] >= least ? 1u : 0u) << (u * EPC + e);
+        }
+        while (reach) {
+          const int b = __ffs(reach) - 1, i = b / EPC * ST + tid, j = (at + i) * EPC + b % EPC - R.lead;
+          reach &= reach - 1u;
+          float x = BF16 ? d3s_u2f((uint32_t)((const uint16_t *)&block[i])[b % EPC] << 16) : ((const float *)&block[i])[b % EPC];
+          if (j == R.banned) x = -__builtin_inff();
+          const uint64_t key = composite_key(x, j);
+          if (key >= bound && j >= 0 && j < a.vocab) {
+            const uint32_t place = atomicAdd(&L.count, 1u);
+            if (place < LIST) L.list[place] = key;
           }
         }
       }
@@ -304,11 +344,12 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
       __syncthreads();
       if (n <= LIST) break;
       /* at least k of the filed keys reach their k-th: none below it is among the best k */
-      rank_list(L, LIST, k);
-      if (tid == 0) L.bound = L.ranked[k - 1], L.count = 0u;
+      rank_list(L, L.list, LIST, k);
+      if (tid == 0) L.count = 0u;
+      bound = L.ranked[k - 1];
       __syncthreads();
     }
-    rank_list(L, n, k);
+    rank_list(L, L.list, n, k);
   }
   if (nseg == 1) {
     finish<BF16>(a, L, R, row, s, T, token_logit, token);
@@ -340,17 +381,31 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
     s = {d3s_u2f((uint32_t)w0), d3s_u2f((uint32_t)(w0 >> 32)), d3s_u2f((uint32_t)w1)};
   }
   s = join_block(L, s, c);
-  if (k > 0) {
-    /* every segment's ceil(k / nseg)-th key: at least k keys reach the least of them */
+  if (TOP) {
+    /* a wave's segments, lane i the i-th key (loads together); every segment's
+     * ceil(k / nseg)-th key: at least k keys reach the least of them */
+    uint64_t *list = (uint64_t *)block;
     const int kc = (k + nseg - 1) / nseg;
-    uint64_t least = ~0ull;
-    for (int q = 0; q < nseg; q++) least = min(least, ld_agent(rr + (size_t)q * words + 2 + kc - 1));
-    for (int i = tid; i < nseg * k; i += ST) {
-      const uint64_t key = ld_agent(rr + (size_t)(i / k) * words + 2 + i % k);
-      if (key != 0ull && key >= least) L.list[atomicAdd(&L.count, 1u)] = key;
+    uint64_t key[SEG_TOP / SW], least = ~0ull;
+#pragma unroll
+    for (int u = 0; u < SEG_TOP / SW; u++) {
+      const int q = tid / WAVE + u * SW;
+      key[u] = q < nseg && lane_id() < k ? ld_agent(rr + (size_t)q * words + 2 + lane_id()) : 0ull;
     }
+#pragma unroll
+    for (int u = 0; u < SEG_TOP / SW; u++) {
+      const uint64_t at = (uint64_t)readlane_u((uint32_t)(key[u] >> 32), kc - 1) << 32 | readlane_u((uint32_t)key[u], kc - 1);
+      if (tid / WAVE + u * SW < nseg) least = min(least, at);
+    }
+    if (lane_id() == 0) L.bound[tid / WAVE] = least;
     __syncthreads();
-    rank_list(L, L.count, k);
+#pragma unroll
+    for (int w = 0; w < SW; w++) least = min(least, L.bound[w]);
+#pragma unroll
+    for (int u = 0; u < SEG_TOP / SW; u++)
+      if (key[u] != 0ull && key[u] >= least) list[atomicAdd(&L.count, 1u)] = key[u];
+    __syncthreads();
+    rank_list(L, list, L.count, k);
   }
   finish<BF16>(a, L, R, row, s, T, token_logit, token);
 }
@@ -522,14 +577,19 @@ int chunks_of(int vocab) {
 }  // namespace
 
 /* Enough workgroups to fill the chip (eight of 256 threads a CU), each with at
- * least two chunks a lane. */
+ * least two chunks a lane.  With alternatives: segments that a workgroup's
+ * registers hold, so that filing them needs no second read, where those are few
+ * enough to be joined. */
 int score_segments(Dtype dt, int64_t n_rows, int vocab, int n_top) {
   const int chunks = dt == DT_BF16 ? chunks_of<true>(vocab) : chunks_of<false>(vocab);
+  if (n_rows > SCORE_ARRIVALS) return 1;
+  if (n_top > 0) {
+    const int held = (chunks + SU * ST - 1) / (SU * ST);
+    if (held <= SEG_TOP && held * n_top <= JOIN) return held;
+  }
   const int64_t want = n_rows > 0 ? 2048 / n_rows : 1;
-  int most = n_top > 0 ? SEG_TOP : SEG_MOST;
-  most = min(most, chunks / (2 * ST));
+  const int most = min(n_top > 0 ? min(SEG_TOP, JOIN / n_top) : SEG_MOST, chunks / (2 * ST));
   const int n = (int)(want < most ? want : most);
-  /* (the arrival counters hold 2048 rows; 2048 / n_rows is 1 from 1025 rows on) */
   return n > 1 ? n : 1;
 }
 
@@ -548,10 +608,11 @@ static void score_launch(const ScoreArgs &a, void *ws, hipStream_t s) {
   for (int row0 = 0; row0 < a.n_rows;) {
     const int rows = min(a.n_rows - row0, GRID_MOST / nseg);
     const dim3 grid((unsigned)(rows * nseg));
+    auto go = [&](auto kernel) { kernel<<<grid, ST, 0, s>>>(a, nseg, seg_chunks, arrivals, records, row0); };
     if (a.entropy)
-      k_score<BF16, true><<<grid, ST, 0, s>>>(a, nseg, seg_chunks, arrivals, records, row0);
+      a.n_top > 0 ? go(k_score<BF16, true, true>) : go(k_score<BF16, true, false>);
     else
-      k_score<BF16, false><<<grid, ST, 0, s>>>(a, nseg, seg_chunks, arrivals, records, row0);
+      a.n_top > 0 ? go(k_score<BF16, false, true>) : go(k_score<BF16, false, false>);
     row0 += rows;
   }
 }
