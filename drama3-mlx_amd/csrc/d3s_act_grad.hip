@@ -25,8 +25,9 @@ Split split_of(int64_t m, int64_t n) {
   while (s.lanes < WAVE && (int64_t)s.lanes * 8 < n) s.lanes *= 2;
   s.strips = (int)((n + s.lanes * 8 - 1) / (s.lanes * 8));
   const int at_once = AT / s.lanes;
-  /* about 1024 workgroups, each of at least four rounds of rows */
-  int64_t runs = 1024 / s.strips;
+  /* about 2048 workgroups (1024: 24.7 us for 8192 x 2048 with gelu, 2048: 22.5), each
+   * of at least four rounds of rows */
+  int64_t runs = 2048 / s.strips;
   if (runs < 1) runs = 1;
   int64_t rows = (m + runs - 1) / runs;
   rows = (rows + 4 * at_once - 1) / (4 * at_once) * (4 * at_once);
@@ -36,7 +37,7 @@ Split split_of(int64_t m, int64_t n) {
   return s;
 }
 
-template <bool SUM>
+template <bool SUM, int ACT>
 __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *parts, int block0) {
   __shared__ float sum[SUM ? AT * 8 : 1];
   const int block = block0 + (int)blockIdx.x;
@@ -46,13 +47,13 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
   const int64_t end = min((int64_t)a.m, (int64_t)(run + 1) * s.rows);
   float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   const int left = j < a.n ? (int)min((int64_t)8, a.n - j) : 0;
-  auto one = [&](float dy, float z) { return a.act == D3S_ACT_NONE ? dy : dy * slope(z, a.act); };
+  auto one = [&](float dy, float z) { return ACT == D3S_ACT_NONE ? dy : dy * slope<ACT>(z); };
   if (left == 8) {
 #pragma unroll 2
     for (int64_t i = (int64_t)run * s.rows + down; i < end; i += at_once) {
       uint32_t d[4], z[4] = {0u, 0u, 0u, 0u}, w[4];
       __builtin_memcpy(d, a.dy + i * a.dy_stride + j, 16);
-      if (a.z) __builtin_memcpy(z, a.z + i * a.z_stride + j, 16);
+      if (ACT != D3S_ACT_NONE) __builtin_memcpy(z, a.z + i * a.z_stride + j, 16);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const float x = one(d3s_u2f(d[e] << 16), d3s_u2f(z[e] << 16));
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
 #pragma unroll
       for (int e = 0; e < 8; e++)
         if (e < left) {
-          const float v = one(bf(a.dy[i * a.dy_stride + j + e]), a.z ? bf(a.z[i * a.z_stride + j + e]) : 0.0f);
+          const float v = one(bf(a.dy[i * a.dy_stride + j + e]), ACT != D3S_ACT_NONE ? bf(a.z[i * a.z_stride + j + e]) : 0.0f);
           acc[e] += v;
           if (a.dz) a.dz[i * a.dz_stride + j + e] = pack1(v);
         }
@@ -120,10 +121,18 @@ void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s) {
   const int64_t blocks = (int64_t)sp.strips * sp.runs;
   for (int64_t b = 0; b < blocks; b += GRID_MOST) {
     const dim3 grid((unsigned)min((int64_t)GRID_MOST, blocks - b));
-    if (a.dbias)
-      k_act_grad<true><<<grid, AT, 0, s>>>(a, sp, parts, (int)b);
-    else
-      k_act_grad<false><<<grid, AT, 0, s>>>(a, sp, parts, (int)b);
+    auto go = [&](auto kernel) { kernel<<<grid, AT, 0, s>>>(a, sp, parts, (int)b); };
+    auto pick = [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      a.dbias ? go(k_act_grad<true, ACT>) : go(k_act_grad<false, ACT>);
+    };
+    switch (a.act) {
+      case D3S_ACT_RELU: pick(std::integral_constant<int, D3S_ACT_RELU>{}); break;
+      case D3S_ACT_SILU: pick(std::integral_constant<int, D3S_ACT_SILU>{}); break;
+      case D3S_ACT_GELU: pick(std::integral_constant<int, D3S_ACT_GELU>{}); break;
+      case D3S_ACT_GELU_TANH: pick(std::integral_constant<int, D3S_ACT_GELU_TANH>{}); break;
+      default: pick(std::integral_constant<int, D3S_ACT_NONE>{});
+    }
   }
   if (!a.dbias) return;
   const int64_t groups = ((int64_t)a.n + 15) / 16;

@@ -72,14 +72,15 @@ __device__ __forceinline__ void activate(float *z, int act) {
   }
 }
 
-__device__ __forceinline__ float slope(float z, int act) {
-  /* far out the slope is 0 or 1 in fp32, and its terms could be 0 times infinity */
-  if (act > D3S_ACT_RELU && fabsf(z) > 100.0f) return z > 0.0f ? 1.0f : 0.0f;
-  switch (act) {
+template <int ACT>
+__device__ __forceinline__ float slope(float z) {
+  /* far out the slope is 0 or 1 in fp32 (and its terms could be 0 times infinity) */
+  const float zc = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 100.0f), -100.0f);
+  switch (ACT) {
     case D3S_ACT_RELU: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
     case D3S_ACT_SILU: {
-      const float f = logistic(z);
-      return f * fmaf(z, 1.0f - f, 1.0f);
+      const float f = logistic(zc);
+      return f * fmaf(zc, 1.0f - f, 1.0f);
     }
     case D3S_ACT_GELU: { /* the normal distribution's function and z times its density */
       const float u = fminf(fabsf(z), 15.0f);
@@ -88,8 +89,8 @@ __device__ __forceinline__ float slope(float z, int act) {
       return fmaf(z1 * 0.3989422804014327f, e, z > 0.0f ? 1.0f - q : q);
     }
     case D3S_ACT_GELU_TANH: { /* f + z f' of the logistic function f of 2 u */
-      const float f = logistic(2.0f * GELU_C * z * fmaf(GELU_A * z, z, 1.0f));
-      return fmaf(z * f * (1.0f - f), 2.0f * GELU_C * fmaf(3.0f * GELU_A * z, z, 1.0f), f);
+      const float f = logistic(2.0f * GELU_C * zc * fmaf(GELU_A * zc, zc, 1.0f));
+      return fmaf(zc * f * (1.0f - f), 2.0f * GELU_C * fmaf(3.0f * GELU_A * zc, zc, 1.0f), f);
     }
   }
   return 1.0f;
