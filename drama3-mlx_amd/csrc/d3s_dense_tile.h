@@ -96,9 +96,12 @@ struct Part {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (D3S_LDS void *)(lds + (u * TT + wid * WAVE) * 16), 16, (int)off[u],
                                              k0 * 2, 0, 0);
   }
-  /* inner indices of which whole stages may be loaded: not the last where an
-   * INNER chunk is cut, it would read past the operand's end */
-  __device__ __forceinline__ int whole(int k) const { return WAY == INNER && r0 + R > rows && rows % 8 != 0 ? max(k - 1, 0) : k; }
+  /* inner indices of which whole stages may be loaded: not the last, or of short
+   * rows the last eight, where an INNER chunk is cut: it would read past the operand's end */
+  __device__ __forceinline__ int whole(int k) const {
+    const bool cut = WAY == INNER && r0 + R > rows && rows % 8 != 0;
+    return cut ? max(k - (stride >= 8 ? 1 : 8), 0) : k;
+  }
   /* the same into registers, from start(k0): a whole stage, at least eight rows if TURNED */
   __device__ __forceinline__ const uint16_t *start(int k0) const {
     return WAY == TURNED || WAY == INNER ? mine + (int64_t)k0 * stride : p + k0;
