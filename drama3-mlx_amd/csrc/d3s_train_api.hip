@@ -99,8 +99,11 @@ int logprob_call(const void *logits, int dtype, int64_t n_rows, int64_t vocab, i
   return done();
 }
 
+/* (a tile or a stage past the end still counts in 32 bits) */
+constexpr int64_t SIZE_MOST = INT_MOST - 1023;
+
 bool product_shape(const d3s_dense_params *p) {
-  if (p->m < 0 || p->n < 0 || p->k < 0 || p->m > INT_MOST || p->n > INT_MOST || p->k > INT_MOST) return false;
+  if (p->m < 0 || p->n < 0 || p->k < 0 || p->m > SIZE_MOST || p->n > SIZE_MOST || p->k > SIZE_MOST) return false;
   return p->x_stride >= (p->x_transposed ? p->m : p->k) && p->w_stride >= (p->w_transposed ? p->n : p->k);
 }
 

@@ -95,7 +95,7 @@ int d3s_logprob_backward(const void *logits, int dtype, int64_t n_rows, int64_t 
  * [m, n] of y's type (it may be y itself: sums over micro-batches) and z [m, n]
  * bf16 (the pre-activation x w^T + bias, kept for the backward) may be NULL.
  * No other output may overlap an input.  y_dtype D3S_DTYPE_F32 or
- * D3S_DTYPE_BF16.  m, n, k from 0 up to 2^31 - 1; k = 0 sums nothing. */
+ * D3S_DTYPE_BF16.  m, n, k from 0 up to 2^31 - 1024; k = 0 sums nothing. */
 typedef struct {
   const uint16_t *x;
   int64_t x_stride;
