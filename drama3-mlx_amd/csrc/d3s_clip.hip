@@ -4,15 +4,14 @@
  * The tensors' addresses and lengths travel as kernel arguments (as many a
  * launch as 4 KiB hold: a launch costs more than a short tensor's work), so the
  * call keeps nothing and may be captured; a tensor of more than 2^30 elements
- * travels in pieces.  A launch's elements are cut into chunks of one size; chunk i belongs to the
- * tensor whose range of chunk numbers holds it (a search in the arguments).
+ * travels in pieces.  A launch's elements are cut into chunks of one size.
  * k_norm: workgroups take chunks in turn, square in 64 bits (a bf16's square is
  * exact and an fp32's keeps its range: nothing overflows, and the order costs no
  * accuracy; the conversions hide behind the loads) and leave one partial sum
- * each (a later launch of the same call adds to them).  k_clip: every workgroup adds all partial sums in one order (they are a
- * few kilobytes of L2; a launch of its own for it would cost more), and scales
- * its chunks, from the last to the first: the end of the norm's pass is what
- * the cache still holds.
+ * each (a later launch of the same call adds to them).  k_clip: every workgroup
+ * adds all partial sums in one order (they are 8 KiB of L2; a launch of its own for
+ * it would cost more), and scales its chunks, from the last to the first: the end
+ * of the norm's pass is what the cache still holds.
  * Bound: HBM; the second pass over the gradients is the operation's own. */
 #include "d3s_device.h"
 #include "d3s_train_internal.h"
@@ -48,16 +47,17 @@ struct Chunk {
   int64_t j0, j1;
 };
 
+/* chunk i's piece: the last of those that start at or before it, all starts loaded
+ * at once (they ascend; a search would wait for one load after the other) */
 template <int MOST>
 __device__ __forceinline__ Chunk find_chunk(const Pieces<MOST> &a, uint32_t i) {
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (a.first[mid] <= i)
-      lo = mid;
-    else
-      hi = mid - 1;
+  int lo = -1;
+#pragma unroll
+  for (int w = 0; w < MOST; w += WAVE) {
+    const int at = w + lane_id();
+    lo += (int)__popcll(__ballot(at < a.n && a.first[min(at, MOST - 1)] <= i));
   }
+  lo = __builtin_amdgcn_readfirstlane(lo);
   Chunk c;
   c.t = lo;
   c.bf16 = (a.numel[lo] & 1u) != 0u;

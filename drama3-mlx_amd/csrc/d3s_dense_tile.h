@@ -280,10 +280,11 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
       if (n >= from && n < to && i < of) each(i);
   };
   /* Direct loads: the issue of one takes longer than a product hides beside an
-   * LDS read, so they follow the reads, half of them in the next stage's first
-   * step.  With operands through registers they come last (an LDS write behind
+   * LDS read, so they follow the reads, half of them in the next stage's first two
+   * steps (8192 x 2048 x 8192: all in the last step 232 us, so 211).  With operands through registers they come last (an LDS write behind
    * them would wait for them), all at once. */
   constexpr int LATE = LOADS == 0 ? DIRECTS / 2 : 0, SOON = DIRECTS - LATE, HALF = PRODUCTS / 2;
+  static_assert(LATE % 2 == 0, "two steps' shares");
   constexpr int WRITTEN = DIRECTS > 0 && HALF > 0 ? HALF : PRODUCTS;
 
   /* TURNED operands of fewer than eight rows have no whole loads */
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
       for (int j = 0; j < STEPS - 1; j++)
         multiply(j & 1, [&](int n) {
           share(n, 0, PRODUCTS, FM + FN, [&](int f) { read((j + 1) & 1, here, j + 1, f); });
-          if (j == 0) share(n, HALF, PRODUCTS, LATE, [&](int u) { direct(SOON + u, near, back); });
+          if (j < 2) share(n, HALF, PRODUCTS, LATE / 2, [&](int u) { direct(SOON + u + j * (LATE / 2), near, back); });
           if (j == 0) share(n, 0, PRODUCTS, LOADS, [&](int u) { load((V + 1) % SETS, u, at); });
         });
       /* the next stage is there: loads after its own may still be on their way */

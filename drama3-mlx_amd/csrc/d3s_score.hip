@@ -425,6 +425,12 @@ __device__ __forceinline__ void store_one(void *p, int64_t at, float v) {
     ((float *)p)[at] = v;
 }
 
+__device__ __forceinline__ uint4 load16(const void *p) {
+  uint4 q;
+  __builtin_memcpy(&q, p, 16);
+  return q;
+}
+
 /* one row's numbers */
 struct GradRow {
   float m, c, c_lo, inv_S, log2S, G, gH, H, inv_T;
@@ -465,6 +471,11 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
   const int chunks = (lead + V + EPC - 1) / EPC;
   const int lo = seg * seg_chunks, hi = min(chunks, lo + seg_chunks);
   const int j0 = max(lo * EPC - lead, 0), j1 = min(hi * EPC - lead, V);
+  /* whole chunks, and single elements before and after them: a lane each */
+  const int first = max(lo, lead > 0 ? 1 : 0), end = min(hi, (lead + V) / EPC);
+  const int head = lead > 0 && lo == 0 ? min(EPC - lead, V) : 0;
+  const int tail = lo < chunks && hi == chunks ? max((lead + V) / EPC * EPC - lead, lead > 0 ? min(EPC - lead, V) : 0) : V;
+  auto get = [&](int ch) { return load16(src + ((int64_t)ch * EPC - lead) * ES); };
 
   float T = a.temperature ? a.temperature[row] : a.temperature_scalar;
   if (T < 1e-5f) T = 1e-5f;
@@ -500,38 +511,33 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  auto one = [&](int j) {
-    float v = 0.0f;
-    if (!zero) v = j == ban ? 0.0f : grad_at<BF16>(r, load_one<BF16>(src, j));
-    store_one<BF16>(dst, j, v);
-  };
-  auto whole = [&](int ch) { return ch * EPC >= lead && (ch + 1) * EPC <= lead + V; };
   auto put = [&](int ch, uint4 q) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    uint32_t o[4];
+    uint32_t o[4] = {0u, 0u, 0u, 0u};
+    if (!zero) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int j = (ch * EPC - lead) + i * (EPC / 4);
-      if constexpr (BF16) {
-        float x = grad_at<true>(r, d3s_u2f(w[i] << 16)), y = grad_at<true>(r, d3s_u2f(w[i] & 0xffff0000u));
-        if (j == ban) x = 0.0f;
-        if (j + 1 == ban) y = 0.0f;
-        o[i] = (uint32_t)d3s_f32_to_bf16_rn(x) | (uint32_t)d3s_f32_to_bf16_rn(y) << 16;
-      } else {
-        o[i] = j == ban ? 0u : d3s_f2u(grad_at<false>(r, d3s_u2f(w[i])));
+      for (int i = 0; i < 4; i++) {
+        const int j = (ch * EPC - lead) + i * (EPC / 4);
+        if constexpr (BF16) {
+          float x = grad_at<true>(r, d3s_u2f(w[i] << 16)), y = grad_at<true>(r, d3s_u2f(w[i] & 0xffff0000u));
+          if (j == ban) x = 0.0f;
+          if (j + 1 == ban) y = 0.0f;
+          o[i] = (uint32_t)d3s_f32_to_bf16_rn(x) | (uint32_t)d3s_f32_to_bf16_rn(y) << 16;
+        } else {
+          o[i] = j == ban ? 0u : d3s_f2u(grad_at<false>(r, d3s_u2f(w[i])));
+        }
       }
     }
     *(uint4 *)(dst + ((int64_t)ch * EPC - lead) * ES) = make_uint4(o[0], o[1], o[2], o[3]);
   };
-  auto get = [&](int ch) {
-    uint4 q;
-    __builtin_memcpy(&q, src + ((int64_t)ch * EPC - lead) * ES, 16);
-    return q;
-  };
-  int ch = lo + tid;
-  for (; ch < hi; ch += GU * ST) {
-    const bool all = whole(ch) && ch + (GU - 1) * ST < hi && whole(ch + (GU - 1) * ST);
-    if (all && !zero) {
+  const int j = tid < head ? tid : tail + (tid - head);
+  if (j < V && (tid < head || j >= tail)) {
+    float v = 0.0f;
+    if (!zero) v = j == ban ? 0.0f : grad_at<BF16>(r, load_one<BF16>(src, j));
+    store_one<BF16>(dst, j, v);
+  }
+  for (int ch = first + tid; ch < end; ch += GU * ST) {
+    if (ch + (GU - 1) * ST < end && !zero) {
       uint4 q[GU];
 #pragma unroll
       for (int u = 0; u < GU; u++) q[u] = get(ch + u * ST);
@@ -539,20 +545,8 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
       for (int u = 0; u < GU; u++) put(ch + u * ST, q[u]);
       continue;
     }
-    for (int u = 0; u < GU; u++) {
-      const int e = ch + u * ST;
-      if (e >= hi) break;
-      if (whole(e) && zero) {
-        *(uint4 *)(dst + ((int64_t)e * EPC - lead) * ES) = make_uint4(0u, 0u, 0u, 0u);
-      } else if (whole(e)) {
-        put(e, get(e));
-      } else {
-        for (int i = 0; i < EPC; i++) {
-          const int j = e * EPC + i - lead;
-          if (j >= 0 && j < V) one(j);
-        }
-      }
-    }
+    for (int u = 0; u < GU && ch + u * ST < end; u++)
+      put(ch + u * ST, zero ? make_uint4(0u, 0u, 0u, 0u) : get(ch + u * ST));
   }
   if (a.n_tokens == 0 || zero) return;
   /* the tokens' own places, after everything else is there */

@@ -70,7 +70,7 @@ int d3s_logprob_ws(const void *logits, int dtype, int64_t n_rows, int64_t vocab,
  * apart; computed in fp32, rounded once).  row_stats and entropy are what
  * d3s_logprob wrote (entropy may be NULL with grad_entropy NULL).  Tokens that
  * are none have no gradient; a token given twice has both.  A row all of whose
- * gradients are 0 gets zeros without being read; any other refused row gets
+ * gradients are 0 gets zeros whatever it holds; any other refused row gets
  * NaN (0 at masked places).  grad_logits may be logits itself (with the same row stride), else the
  * two must not overlap.  Needs no workspace. */
 int d3s_logprob_backward(const void *logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,
