@@ -36,8 +36,8 @@ struct TilePlan {
   bool x_direct, w_direct; /* operands by rows at 16 bytes: see Way */
 };
 
-/* k_few's: rows from i0 on (at most FEW_ROWS), the inner length cut into
- * `splits` of `batches` batches */
+/* k_few's: rows from i0 on (at most FEW_ROWS; or outputs, at most half as many:
+ * the operands' roles exchanged), the inner length cut into `splits` of `batches` batches */
 constexpr int FEW_ROWS = 64;
 struct FewPlan {
   unsigned tiles, splits;
@@ -45,11 +45,12 @@ struct FewPlan {
   uint64_t *parts;
   uint32_t *arrivals;
 };
-int few_outputs(bool w_transposed); /* a workgroup's */
+int few_outputs(bool w_transposed); /* a workgroup's (exchanged: rows, by how x lies) */
 int few_batch(bool w_transposed);
 int few_waves(bool w_transposed); /* batches at a time */
 size_t few_part_bytes(bool w_transposed, int rows); /* a split's sums of one workgroup */
-void launch_few(const Operands &a, const Out &o, bool x_transposed, bool w_transposed, const FewPlan &pl, hipStream_t s);
+void launch_few(const Operands &a, const Out &o, bool x_transposed, bool w_transposed, bool swap, const FewPlan &pl,
+                hipStream_t s);
 
 template <bool XT, bool WT>
 void launch_tiles(const Operands &a, const Out &o, const TilePlan &pl, hipStream_t s);

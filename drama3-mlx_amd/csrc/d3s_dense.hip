@@ -26,7 +26,7 @@ Product product_of(const d3s_dense_params &p, uintptr_t x, uintptr_t w) {
 
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-/* Microseconds of m rows in tiles of tm x tn, one workgroup a CU: rounds of
+/* Microseconds of m rows and n outputs in tiles of tm x tn, one workgroup a CU: rounds of
  * workgroups, each its stages and what it spends before and after them.
  * Measured, by how many operands go to LDS directly: a stage of 256 x 256 1.45
  * (both), 1.65 (one) and 2.2; of 128 x 256 0.93 and 1.2; of 128 x 128 0.52 and
@@ -38,9 +38,9 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
  * splits 49, 31, 22 and 24.)  Between 128 x 256 and 256 x 128 there is little,
  * but rows of x that are not at 4 bytes cost less the fewer tiles load them (heads of
  * 4097 outputs, their weights' gradient: 186 and 205 us). */
-double tile_us(const Product &p, int64_t m, int tm, int tn, int splits) {
+double tile_us(const Product &p, int64_t m, int64_t n, int tm, int tn, int splits) {
   const int direct = p.x_direct + p.w_direct;
-  const double wgs = (double)up(m, tm) * (double)up(p.n, tn) * splits;
+  const double wgs = (double)up(m, tm) * (double)up(n, tn) * splits;
   const double rounds = (double)(int64_t)((wgs + CUS - 1) / CUS), stages = (double)up(p.k, (int64_t)TILE_K * splits);
   if (tm == 256) return rounds * (stages * (direct == 2 ? 1.45 : direct == 1 ? 1.65 : 2.2) + 14);
   if (tn == 256) return rounds * (stages * (direct == 2 ? 0.93 : 1.2) + 10);
@@ -49,18 +49,34 @@ double tile_us(const Product &p, int64_t m, int tm, int tn, int splits) {
   return rounds * (stages * stage + 6) + (splits > 1 ? 3 + splits : 0);
 }
 
-/* ... and of k_few: the weights at 4 TB/s */
-double few_us(const Product &p) { return 6 + (double)p.n * (double)p.k * 2 / 4e6; }
+/* ... and of k_few, which reads `many` rows of the other operand at 4 TB/s */
+double few_us(const Product &p, int64_t many) { return 6 + (double)many * (double)p.k * 2 / 4e6; }
 
 struct Plan {
-  TilePlan tile; /* no tiles: no such launch */
-  FewPlan few;
-  int64_t tile_rows;
+  TilePlan tile;         /* no tiles: no such launch */
+  int64_t tile_m, tile_n;
+  FewPlan few, few_outs; /* the rows after the tiles', and the outputs after theirs of the tiles' rows */
 };
 
 size_t tile_bytes(const TilePlan &t) { return t.splits > 1 ? (size_t)t.tiles * t.splits * t.tm * t.tn * sizeof(float) : 0; }
-size_t few_bytes(const Plan &pl, const Product &p) {
-  return pl.few.splits > 1 ? (size_t)pl.few.tiles * pl.few.splits * few_part_bytes(p.w_turned, (int)(p.m - pl.few.i0)) : 0;
+size_t few_bytes(const FewPlan &f, bool turned, int64_t rows) {
+  return f.splits > 1 ? (size_t)f.tiles * f.splits * few_part_bytes(turned, (int)rows) : 0;
+}
+
+/* `few` rows from i0 on against `many` of the other operand, turned or not */
+FewPlan few_plan(int64_t i0, int64_t few, int64_t many, int64_t k, bool turned) {
+  FewPlan f{};
+  f.i0 = (int)i0;
+  f.tiles = (unsigned)up(many, few_outputs(turned));
+  /* the inner length over more workgroups while there are fewer than CUs, at
+   * least two batches a wave (one with four fragments of rows) */
+  const int64_t batches = up(k, few_batch(turned));
+  int64_t most = batches / (few_waves(turned) * (few > 32 ? 1 : 2)), want = CUS / (int64_t)f.tiles;
+  if (want < most) most = want;
+  if (most > 16) most = 16;
+  f.splits = most > 1 ? (unsigned)most : 1u;
+  f.batches = (int)up(batches, f.splits);
+  return f;
 }
 
 Plan plan(const Product &p) {
@@ -68,63 +84,52 @@ Plan plan(const Product &p) {
   /* Few rows: k_few, which turns weights eight outputs at a time.  33 to 64 rows
    * (64 x 2048 x 2048: 9.3 us, in tiles 14.2; 64 x 4097 x 2048: 19.8, in tiles 15.8) while
    * its workgroups of 16 outputs, each of which reads all of x, run at once. */
-  const bool can = !p.w_turned || p.n >= 8;
-  int64_t few = 0;
-  if (can && (p.m <= 32 || (p.m <= FEW_ROWS && !p.w_turned && p.n <= 16 * CUS))) few = p.m;
+  const bool rows_can = !p.w_turned || p.n >= 8;
+  if (rows_can && (p.m <= 32 || (p.m <= FEW_ROWS && !p.w_turned && p.n <= 16 * CUS))) {
+    pl.few = few_plan(0, p.m, p.n, p.k, p.w_turned);
+    return pl;
+  }
 
+  /* A last row or column of tiles that is nearly empty may cost a round of its
+   * own: its rows, or outputs, are k_few's too. */
   double best = 1e300;
-  auto choose = [&](int64_t m, double also) {
+  TilePlan &t = pl.tile;
+  for (int cut = 0; cut < 4; cut++) {
+    const int64_t dm = cut & 1 ? p.m % 128 : 0, dn = cut & 2 ? p.n % 128 : 0, m = p.m - dm, n = p.n - dn;
+    if ((cut & 1) && !(rows_can && dm > 0 && dm <= 32 && m >= 256)) continue;
+    if ((cut & 2) && !(dn > 0 && dn <= 32 && n >= 256 && (!p.x_turned || m >= 8))) continue;
+    const double also = (dm ? few_us(p, p.n) : 0) + (dn ? few_us(p, m) : 0);
     auto offer = [&](int tm, int tn, int splits) {
-      const double us = tile_us(p, m, tm, tn, splits) + also;
+      const double us = tile_us(p, m, n, tm, tn, splits) + also;
       if (us >= best) return;
       best = us;
-      pl.tile_rows = m;
-      pl.tile.tm = tm, pl.tile.tn = tn, pl.tile.splits = (unsigned)splits;
+      pl.tile_m = m, pl.tile_n = n;
+      t.tm = tm, t.tn = tn, t.splits = (unsigned)splits;
     };
     offer(256, 256, 1);
     offer(128, 256, 1);
     /* (every split has its stages, and fewer workgroups than twice the CUs) */
     for (int s = 1; s <= 8; s++)
-      if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(p.n, 128) * s <= 2 * CUS)) offer(128, 128, s);
-  };
-  if (few == 0) {
-    choose(p.m, 0);
-    /* a last row of tiles that is nearly empty may cost a round of its own */
-    const int64_t rest = p.m % 128;
-    if (can && rest > 0 && rest <= 32 && p.m > 256) {
-      const double with = best;
-      choose(p.m - rest, few_us(p));
-      if (best < with) few = rest;
-    }
-    TilePlan &t = pl.tile;
-    t.m_tiles = (unsigned)up(pl.tile_rows, t.tm);
-    t.n_tiles = (unsigned)up(p.n, t.tn);
-    t.tiles = t.m_tiles * t.n_tiles;
-    t.group = 8;
-    t.stages = (int)up(p.k / TILE_K, t.splits);
-    t.x_direct = p.x_direct;
-    t.w_direct = p.w_direct;
+      if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(n, 128) * s <= 2 * CUS)) offer(128, 128, s);
   }
-  if (few > 0) {
-    FewPlan &f = pl.few;
-    f.i0 = (int)(p.m - few);
-    f.tiles = (unsigned)up(p.n, few_outputs(p.w_turned));
-    /* the inner length over more workgroups while there are fewer than CUs, at
-     * least two batches a wave (one with four fragments of rows) */
-    const int64_t batches = up(p.k, few_batch(p.w_turned));
-    int64_t most = batches / (few_waves(p.w_turned) * (few > 32 ? 1 : 2)), want = CUS / (int64_t)f.tiles;
-    if (want < most) most = want;
-    if (most > 16) most = 16;
-    f.splits = most > 1 ? (unsigned)most : 1u;
-    f.batches = (int)up(batches, f.splits);
-  }
+  t.m_tiles = (unsigned)up(pl.tile_m, t.tm);
+  t.n_tiles = (unsigned)up(pl.tile_n, t.tn);
+  t.tiles = t.m_tiles * t.n_tiles;
+  t.group = 8;
+  t.stages = (int)up(p.k / TILE_K, t.splits);
+  t.x_direct = p.x_direct;
+  t.w_direct = p.w_direct;
+  if (pl.tile_m < p.m) pl.few = few_plan(pl.tile_m, p.m - pl.tile_m, p.n, p.k, p.w_turned);
+  if (pl.tile_n < p.n) pl.few_outs = few_plan(pl.tile_n, p.n - pl.tile_n, pl.tile_m, p.k, p.x_turned);
   return pl;
 }
 
 size_t bytes_of(const Product &p) {
   const Plan pl = plan(p);
-  const size_t a = tile_bytes(pl.tile), b = pl.few.tiles ? few_bytes(pl, p) : 0;
-  return a > b ? a : b; /* (one launch after the other) */
+  const size_t a = tile_bytes(pl.tile), b = few_bytes(pl.few, p.w_turned, p.m - pl.few.i0),
+               c = few_bytes(pl.few_outs, p.x_turned, p.n - pl.few_outs.i0);
+  const size_t ab = a > b ? a : b;
+  return ab > c ? ab : c; /* (one launch after the other) */
 }
 
 }  // namespace
@@ -149,12 +154,18 @@ void launch_dense(const d3s_dense_params &p, void *ws, hipStream_t s) {
   if (pl.few.tiles) {
     pl.few.arrivals = (uint32_t *)ws;
     pl.few.parts = (uint64_t *)parts;
-    launch_few(a, o, pr.x_turned, pr.w_turned, pl.few, s);
+    launch_few(a, o, pr.x_turned, pr.w_turned, false, pl.few, s);
   }
   if (!pl.tile.tiles) return;
+  o.m = (int)pl.tile_m;
+  if (pl.few_outs.tiles) {
+    pl.few_outs.arrivals = (uint32_t *)ws;
+    pl.few_outs.parts = (uint64_t *)parts;
+    launch_few(a, o, pr.x_turned, pr.w_turned, true, pl.few_outs, s);
+  }
+  o.n = (int)pl.tile_n;
   pl.tile.arrivals = (uint32_t *)ws;
   pl.tile.parts = (float *)parts;
-  o.m = (int)pl.tile_rows;
   if (pr.x_turned)
     pr.w_turned ? launch_tiles<true, true>(a, o, pl.tile, s) : launch_tiles<true, false>(a, o, pl.tile, s);
   else

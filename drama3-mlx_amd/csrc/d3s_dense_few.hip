@@ -1,5 +1,5 @@
-/* k_few: dense layers of up to 64 rows of x (gfx950, wave64;
- * include/d3s_train.h).
+/* k_few: dense layers of up to 64 rows of x, or, with the operands' roles
+ * exchanged, of up to 32 outputs (gfx950, wave64; include/d3s_train.h).
  *
  * Bound: the weights' bytes, which are read once, straight into the fragments
  * of 16 x 16 x 32 products (no LDS: nothing is shared between waves but x,
@@ -10,7 +10,9 @@
  * Weights by rows: a wave's 16 outputs, lane l row l % 16 and inner indices
  * 8 (l / 16) .. + 7 of a step.  Weights by the inner index: 128 outputs, lane l
  * eight of them (l % 16) at eight inner indices, turned in registers: fragment
- * e is outputs 8 r + e. */
+ * e is outputs 8 r + e.
+ * Rows that start between 4-byte words are loaded from the word below, with the word
+ * behind, and moved down: a 16-byte load there takes far longer. */
 #include "d3s_dense_load.h"
 #include "d3s_epilogue.h"
 #include "d3s_rowcore.h"
@@ -29,8 +31,17 @@ struct Shape {
   static constexpr int FRAGMENTS = WT ? 8 : 1;  /* of 16 outputs */
 };
 
+/* eight elements at p, `odd` (0, 1) elements behind a 4-byte word */
+__device__ __forceinline__ uint4 load_odd(const uint16_t *p, int odd) {
+  const uint4 q = load16(p - odd);
+  const uint32_t behind = *(const uint32_t *)(p - odd + 6 + 2 * odd);
+  const int s = odd * 16;
+  return make_uint4(__builtin_amdgcn_alignbit(q.y, q.x, s), __builtin_amdgcn_alignbit(q.z, q.y, s),
+                    __builtin_amdgcn_alignbit(q.w, q.z, s), __builtin_amdgcn_alignbit(behind, q.w, s));
+}
+
 /* elements [at, at + 8) of row i of x, zeros past its end */
-template <bool XT>
+template <bool XT, bool ODD>
 __device__ __forceinline__ bf16x8 x_fragment(const Operands &a, int i, int at, bool whole) {
   uint4 q = make_uint4(0u, 0u, 0u, 0u);
   if constexpr (XT) {
@@ -41,29 +52,30 @@ __device__ __forceinline__ bf16x8 x_fragment(const Operands &a, int i, int at, b
   } else {
     const uint16_t *row = a.x + (int64_t)i * a.x_stride;
     if (whole)
-      q = load16(row + at);
+      q = ODD ? load_odd(row + at, (int)((uintptr_t)row >> 1 & 1)) : load16(row + at);
     else if (at < a.k)
       q = row_chunk(row, at, a.k);
   }
   return __builtin_bit_cast(bf16x8, q);
 }
 
-template <int FR, bool XT, bool WT>
+template <int FR, bool XT, bool WT, bool ODD, bool SWAP>
 __global__ __launch_bounds__(Shape<WT>::THREADS) void k_few(Operands a, Out o, FewPlan pl, unsigned first) {
   using S = Shape<WT>;
   constexpr int FG = S::FRAGMENTS, BATCH = S::STEPS * 32;
   __shared__ f32x4 sums[S::WAVES][FG][FR][WAVE];
   __shared__ unsigned last;
   const int lane = lane_id(), wid = (int)threadIdx.x / WAVE, g = lane >> 4, r = lane & 15;
+  const int rows = SWAP ? o.n : o.m, outputs = SWAP ? o.m : o.n;
   const unsigned tile = (first + blockIdx.x) / pl.splits, split = (first + blockIdx.x) % pl.splits;
   const int j0 = (int)tile * S::OUTPUTS;
   const int batches = (int)(((int64_t)a.k + BATCH - 1) / BATCH);
   const int b1 = (int)min((int64_t)batches, (int64_t)(split + 1) * pl.batches);
   /* outputs past the end are the last again, and not written (turned: the last eight) */
-  const int j = WT ? min(j0 + r * 8, o.n - 8) : min(j0 + r, o.n - 1);
+  const int j = WT ? min(j0 + r * 8, outputs - 8) : min(j0 + r, outputs - 1);
   int xi[FR];
 #pragma unroll
-  for (int f = 0; f < FR; f++) xi[f] = min(pl.i0 + f * 16 + r, o.m - 1);
+  for (int f = 0; f < FR; f++) xi[f] = min(pl.i0 + f * 16 + r, rows - 1);
   f32x4 acc[FG][FR];
 #pragma unroll
   for (int e = 0; e < FG; e++)
@@ -79,7 +91,7 @@ __global__ __launch_bounds__(Shape<WT>::THREADS) void k_few(Operands a, Out o, F
 #pragma unroll
       for (int u = 0; u < 8; u++) q[u] = load16(a.w + (int64_t)(whole ? k + u : min(k + u, a.k - 1)) * a.w_stride + j);
 #pragma unroll
-      for (int f = 0; f < FR; f++) fx[0][f] = x_fragment<XT>(a, xi[f], k, whole);
+      for (int f = 0; f < FR; f++) fx[0][f] = x_fragment<XT, ODD>(a, xi[f], k, whole);
       const int n = a.k - k;
       auto some = [&](int d) { return whole || n >= 2 * d + 2 ? ~0u : n == 2 * d + 1 ? 0xffffu : 0u; };
 #pragma unroll
@@ -96,12 +108,13 @@ __global__ __launch_bounds__(Shape<WT>::THREADS) void k_few(Operands a, Out o, F
     } else {
       bf16x8 fw[S::STEPS];
       const uint16_t *row = a.w + (int64_t)j * a.w_stride;
+      const int odd = (int)((uintptr_t)row >> 1 & 1);
 #pragma unroll
       for (int s = 0; s < S::STEPS; s++) {
         const int k = k0 + s * 32 + g * 8;
-        fw[s] = __builtin_bit_cast(bf16x8, whole ? load16(row + k) : k < a.k ? row_chunk(row, k, a.k) : make_uint4(0u, 0u, 0u, 0u));
+        fw[s] = __builtin_bit_cast(bf16x8, whole ? (ODD ? load_odd(row + k, odd) : load16(row + k)) : k < a.k ? row_chunk(row, k, a.k) : make_uint4(0u, 0u, 0u, 0u));
 #pragma unroll
-        for (int f = 0; f < FR; f++) fx[s][f] = x_fragment<XT>(a, xi[f], k, whole);
+        for (int f = 0; f < FR; f++) fx[s][f] = x_fragment<XT, ODD>(a, xi[f], k, whole);
       }
 #pragma unroll
       for (int s = 0; s < S::STEPS; s++)
@@ -132,8 +145,8 @@ __global__ __launch_bounds__(Shape<WT>::THREADS) void k_few(Operands a, Out o, F
     const int t = c * S::THREADS + (int)threadIdx.x;
     /* items in order of rows, then outputs */
     const int i = t / (S::OUTPUTS / EACH) % 16, f = t / (S::OUTPUTS / EACH) / 16 % FR, across = t % (S::OUTPUTS / EACH);
-    at_i[c] = t < ITEMS ? pl.i0 + f * 16 + i : o.m;
-    at_j[c] = WT ? (int)min((int64_t)j0 + across * 8, (int64_t)o.n - 8) : j0 + across * 4;
+    at_i[c] = t < ITEMS ? pl.i0 + f * 16 + i : rows;
+    at_j[c] = WT ? (int)min((int64_t)j0 + across * 8, (int64_t)outputs - 8) : j0 + across * 4;
     skip[c] = j0 + across * EACH - at_j[c]; /* (what the item before writes: a residual in place is added once) */
     const int from = WT ? (across >> 2) * 16 + i : across * 16 + i;
 #pragma unroll
@@ -185,24 +198,36 @@ __global__ __launch_bounds__(Shape<WT>::THREADS) void k_few(Operands a, Out o, F
         }
   }
 #pragma unroll
-  for (int c = 0; c < ROUNDS; c++) put_some<EACH>(o, at_i[c], at_j[c], skip[c], v[c]);
+  for (int c = 0; c < ROUNDS; c++) put_some<EACH, SWAP>(o, at_i[c], at_j[c], skip[c], v[c]);
 }
 
-template <int FR, bool XT, bool WT>
+template <int FR, bool XT, bool WT, bool SWAP>
 void few_launch(const Operands &a, const Out &o, const FewPlan &pl, hipStream_t s) {
   const unsigned all = pl.tiles * pl.splits;
-  for (unsigned first = 0; first < all; first += FEW_GRID)
-    k_few<FR, XT, WT><<<dim3(min(FEW_GRID, all - first)), Shape<WT>::THREADS, 0, s>>>(a, o, pl, first);
+  /* (transposed loads are not moved: x's are single elements, the weights' eight rows each) */
+  const bool odd = (!XT && ((uintptr_t)a.x % 4 != 0 || a.x_stride % 2 != 0)) || (!WT && ((uintptr_t)a.w % 4 != 0 || a.w_stride % 2 != 0));
+  for (unsigned first = 0; first < all; first += FEW_GRID) {
+    const dim3 grid(min(FEW_GRID, all - first));
+    if constexpr (!(XT && WT)) {
+      if (odd) {
+        k_few<FR, XT, WT, true, SWAP><<<grid, Shape<WT>::THREADS, 0, s>>>(a, o, pl, first);
+        continue;
+      }
+    }
+    k_few<FR, XT, WT, false, SWAP><<<grid, Shape<WT>::THREADS, 0, s>>>(a, o, pl, first);
+  }
 }
 template <bool XT, bool WT>
-void few_rows(const Operands &a, const Out &o, const FewPlan &pl, hipStream_t s) {
-  const int rows = o.m - pl.i0;
-  if (rows <= 16)
-    few_launch<1, XT, WT>(a, o, pl, s);
+void few_rows(const Operands &a, const Out &o, bool swap, const FewPlan &pl, hipStream_t s) {
+  const int rows = (swap ? o.n : o.m) - pl.i0;
+  if (swap)
+    rows <= 16 ? few_launch<1, XT, WT, true>(a, o, pl, s) : few_launch<2, XT, WT, true>(a, o, pl, s);
+  else if (rows <= 16)
+    few_launch<1, XT, WT, false>(a, o, pl, s);
   else if (rows <= 32)
-    few_launch<2, XT, WT>(a, o, pl, s);
+    few_launch<2, XT, WT, false>(a, o, pl, s);
   else
-    few_launch<4, XT, WT>(a, o, pl, s);
+    few_launch<4, XT, WT, false>(a, o, pl, s);
 }
 
 }  // namespace
@@ -217,11 +242,15 @@ size_t few_part_bytes(bool w_transposed, int rows) {
   return (items / each + threads - 1) / threads * threads * each * sizeof(float);
 }
 
-void launch_few(const Operands &a, const Out &o, bool x_transposed, bool w_transposed, const FewPlan &pl, hipStream_t s) {
-  if (x_transposed)
-    w_transposed ? few_rows<true, true>(a, o, pl, s) : few_rows<true, false>(a, o, pl, s);
+void launch_few(const Operands &a, const Out &o, bool x_transposed, bool w_transposed, bool swap, const FewPlan &pl,
+                hipStream_t s) {
+  const Operands b{a.w, a.x, a.w_stride, a.x_stride, a.k};
+  const Operands &in = swap ? b : a;
+  const bool xt = swap ? w_transposed : x_transposed, wt = swap ? x_transposed : w_transposed;
+  if (xt)
+    wt ? few_rows<true, true>(in, o, swap, pl, s) : few_rows<true, false>(in, o, swap, pl, s);
   else
-    w_transposed ? few_rows<false, true>(a, o, pl, s) : few_rows<false, false>(a, o, pl, s);
+    wt ? few_rows<false, true>(in, o, swap, pl, s) : few_rows<false, false>(in, o, swap, pl, s);
 }
 
 }  // namespace d3s

@@ -120,29 +120,33 @@ __device__ __forceinline__ void put_one(const Out &o, int i, int j, float s) {
   }
 }
 
-/* outputs (i, j + skip .. j + N - 1), their sums s: those that are inside */
-template <int N>
+/* N neighbouring outputs of row i from j on (DOWN: N neighbouring rows from j on of
+ * output i), their sums s: those from `skip` on that are inside */
+template <int N, bool DOWN>
 __device__ __forceinline__ void put_some(const Out &o, int i, int j, int skip, float *s) {
-  if (i >= o.m) return;
-  const int n = o.n - j;
+  if (i >= (DOWN ? o.n : o.m)) return;
+  const int n = (DOWN ? o.m : o.n) - j;
+  auto at = [&](int64_t stride, int e) { return DOWN ? (int64_t)(j + e) * stride + i : (int64_t)i * stride + j + e; };
 #pragma unroll
   for (int e = 0; e < N; e++)
-    if (o.bias && e >= skip && e < n) s[e] += bf(o.bias[j + e]);
+    if (o.bias && e >= skip && e < n) s[e] += bf(o.bias[DOWN ? i : j + e]);
   if (o.z) {
 #pragma unroll
     for (int e = 0; e < N; e++)
-      if (e >= skip && e < n) o.z[(int64_t)i * o.z_stride + j + e] = pack1(s[e]);
+      if (e >= skip && e < n) o.z[at(o.z_stride, e)] = pack1(s[e]);
   }
   activate<N>(s, o.act);
-  const int64_t y = (int64_t)i * o.y_stride + j, r = (int64_t)i * o.residual_stride + j;
   if (o.f32) {
 #pragma unroll
     for (int e = 0; e < N; e++)
-      if (e >= skip && e < n) ((float *)o.y)[y + e] = o.residual ? s[e] + ((const float *)o.residual)[r + e] : s[e];
+      if (e >= skip && e < n)
+        ((float *)o.y)[at(o.y_stride, e)] = o.residual ? s[e] + ((const float *)o.residual)[at(o.residual_stride, e)] : s[e];
   } else {
 #pragma unroll
     for (int e = 0; e < N; e++)
-      if (e >= skip && e < n) ((uint16_t *)o.y)[y + e] = pack1(o.residual ? s[e] + bf(((const uint16_t *)o.residual)[r + e]) : s[e]);
+      if (e >= skip && e < n)
+        ((uint16_t *)o.y)[at(o.y_stride, e)] =
+            pack1(o.residual ? s[e] + bf(((const uint16_t *)o.residual)[at(o.residual_stride, e)]) : s[e]);
   }
 }
 

@@ -202,3 +202,18 @@ def test_infinite_activations(gpu):
             got, d = y.download((4,), np.float32), R.from_bits(dz.download((4,), np.uint16))
         assert got[0] == inf and got[1] == 0 and np.isnan(got[2]), (act, got)
         assert d[0] == 1 and d[1] == 0 and np.isnan(d[2]), (act, d)
+
+
+@pytest.mark.parametrize("xt,wt", [(False, False), (False, True), (True, False), (True, True)])
+def test_outputs_peeled(gpu, xt, wt):
+    """outputs, and rows and outputs, that a last tile would leave nearly empty"""
+    product(gpu, 4096, 4097, 130, xt, wt, bias=True, act="silu", keep=True, residual=True)
+    product(gpu, 4096, 2070, 136, xt, wt, residual=True, out="f32", in_place=True)
+    product(gpu, 4097, 4098, 97, xt, wt, bias=True, residual=True, pads=(1, 1, 3), offset=1)
+
+
+@pytest.mark.parametrize("m,n,k", [(9, 513, 1025), (1, 4097, 4097), (33, 200, 999), (64, 300, 513)])
+def test_few_rows_at_any_element(gpu, m, n, k):
+    for xt, wt in ((False, False), (False, True), (True, False)):
+        product(gpu, m, n, k, xt, wt, bias=True, act="gelu", residual=True)
+        product(gpu, m, n, k, xt, wt, pads=(2, 1, 0), offset=1, out="f32")
