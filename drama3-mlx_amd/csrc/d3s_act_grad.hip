@@ -62,7 +62,7 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
         acc[2 * e + 1] += y;
         w[e] = pack2(x, y);
       }
-      if (a.dz) __builtin_memcpy(a.dz + i * a.dz_stride + j, w, 16);
+      if (a.dz) stream16(a.dz + i * a.dz_stride + j, make_uint4(w[0], w[1], w[2], w[3]));
     }
   } else if (left > 0) {
     for (int64_t i = (int64_t)run * s.rows + down; i < end; i += at_once)

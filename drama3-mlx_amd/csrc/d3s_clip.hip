@@ -11,9 +11,10 @@
  * each (a later launch of the same call adds to them).  k_clip: every workgroup
  * adds all partial sums in one order (they are 8 KiB of L2; a launch of its own for
  * it would cost more), and scales its chunks, from the last to the first: the end
- * of the norm's pass is what the cache still holds.
+ * of the norm's pass is what the cache still holds, and the stores leave it there.
  * Bound: HBM; the second pass over the gradients is the operation's own. */
 #include "d3s_device.h"
+#include "d3s_stream.h"
 #include "d3s_train_internal.h"
 
 namespace d3s {
@@ -205,17 +206,17 @@ __device__ __forceinline__ void chunk_scale(const void *p, void *d, const Chunk 
   for (; i + (CU - 1) * CT < s.units; i += CU * CT) {
     uint4 q[CU];
 #pragma unroll
-    for (int u = 0; u < CU; u++) q[u] = b[i + u * CT];
+    for (int u = 0; u < CU; u++) q[u] = last16(b + i + u * CT);
 #pragma unroll
     for (int u = 0; u < CU; u++) {
       if (!keep) q[u] = scaled<BF16>(q[u], scale);
-      __builtin_memcpy(o + (int64_t)(i + u * CT) * 16, &q[u], 16);
+      stream16(o + (int64_t)(i + u * CT) * 16, q[u]);
     }
   }
   for (; i < s.units; i += CT) {
     uint4 q = b[i];
     if (!keep) q = scaled<BF16>(q, scale);
-    __builtin_memcpy(o + (int64_t)i * 16, &q, 16);
+    stream16(o + (int64_t)i * 16, q);
   }
   const int64_t h = s.head0 + threadIdx.x, e = s.tail0 + threadIdx.x;
   if (h < s.head1) scale_one<BF16>(p, d, h, scale, keep);

@@ -4,6 +4,7 @@
 
 #include "d3s_dense.h"
 #include "d3s_device.h"
+#include "d3s_stream.h"
 
 namespace d3s {
 namespace {
@@ -17,8 +18,6 @@ __device__ __forceinline__ uint4 load16(const void *p) {
   __builtin_memcpy(&q, p, 16);
   return q;
 }
-__device__ __forceinline__ void store16(void *p, uint4 q) { __builtin_memcpy(p, &q, 16); }
-
 /* elements [at, at + 8) of a stored row of `len`, zeros past its end (at < len) */
 __device__ __forceinline__ uint4 row_chunk(const uint16_t *row, int64_t at, int64_t len) {
   uint64_t v[2] = {0u, 0u};

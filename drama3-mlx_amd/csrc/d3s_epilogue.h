@@ -207,7 +207,7 @@ struct Eights {
       bf_eight(bias, v);
 #pragma unroll
       for (int e = 0; e < 4; e++) s[e] = a[e] + v[e], s[e + 4] = b[e] + v[e + 4];
-      if (o.z && i + down + c * DOWN < o.m) store16(z + c * (DOWN * o.z_stride), pack_eight(s));
+      if (o.z && i + down + c * DOWN < o.m) stream16(z + c * (DOWN * o.z_stride), pack_eight(s));
       d3s::activate<8>(s, o.act);
       *(f32x4 *)(sums + c * DOWN * ROW) = f32x4{s[0], s[1], s[2], s[3]};
       *(f32x4 *)(sums + c * DOWN * ROW + 4) = f32x4{s[4], s[5], s[6], s[7]};
@@ -224,8 +224,9 @@ struct Eights {
         if (o.residual) a += __builtin_bit_cast(f32x4, r.lo[c]), b += __builtin_bit_cast(f32x4, r.hi[c]);
         if (i + down + c * DOWN < o.m) {
           float *at = (float *)o.y + y + c * (DOWN * o.y_stride);
-          store16(at, __builtin_bit_cast(uint4, a));
-          store16(at + 4, __builtin_bit_cast(uint4, b));
+          /* (the caches join the halves of 32 bytes a lane: not past them) */
+          __builtin_memcpy(at, &a, 16);
+          __builtin_memcpy(at + 4, &b, 16);
         }
       }
     } else {
@@ -238,7 +239,7 @@ struct Eights {
 #pragma unroll
           for (int e = 0; e < 8; e++) s[e] += v[e];
         }
-        if (i + down + c * DOWN < o.m) store16((uint16_t *)o.y + y + c * (DOWN * o.y_stride), pack_eight(s));
+        if (i + down + c * DOWN < o.m) stream16((uint16_t *)o.y + y + c * (DOWN * o.y_stride), pack_eight(s));
       }
     }
   }

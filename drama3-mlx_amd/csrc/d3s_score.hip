@@ -30,6 +30,7 @@
 #include <float.h>
 
 #include "d3s_rowcore.h"
+#include "d3s_stream.h"
 #include "d3s_train_internal.h"
 
 namespace d3s {
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
         }
       }
     }
-    *(uint4 *)(dst + ((int64_t)ch * EPC - lead) * ES) = make_uint4(o[0], o[1], o[2], o[3]);
+    stream16(dst + ((int64_t)ch * EPC - lead) * ES, make_uint4(o[0], o[1], o[2], o[3]));
   };
   const int j = tid < head ? tid : tail + (tid - head);
   if (j < V && (tid < head || j >= tail)) {
