@@ -18,15 +18,24 @@
  * segments' records go to the workspace and the last to arrive joins them (in
  * segment order, so the bits do not depend on who is last).
  *
- * Alternatives.  The n-th greatest of the 256 lane maxima is at most the n-th
- * greatest logit, and few logits reach it: a second pass over the segment
- * (from L2) files those, and the filed keys (order-preserving logit bits, then
+ * Alternatives.  Of the n best, each of the four waves finds by ballots the
+ * ceil(n / 4)-th greatest of its lanes' maxima (its upper 16 bits); at least n
+ * logits reach the least of the four, and few others do: a second pass over
+ * the segment files those, and the filed keys (order-preserving logit bits, then
  * the complement of the index) are ranked by counting.  More than the list
  * holds (ties, masked rows): the n-th of the filed keys is a bound at least as
- * high, and the pass is run again with it.
+ * high, and the pass is run again with it.  The segment passes through LDS in
+ * blocks of 16 KiB; one that is a single block is not loaded again.  The join
+ * of the segments bounds their keys the same way and ranks what reaches it.
  *
  * Gradient.  Every element needs its own logit and four numbers of its row:
- * one streaming pass, rows cut into segments that share nothing. */
+ * one streaming pass, rows cut into segments that share nothing, stores past the
+ * caches (through them: 2 to 20 % slower).
+ *
+ * Bound: long rows HBM (bf16 [4096, 151936]: 219 us, 5.7 TB/s; the gradient of
+ * [2048, 151936] 229 us, 5.4 TB/s; of fp32 [4096, 4097] 25 us, 5.3 TB/s); few
+ * rows the chain of dependent steps (bf16 [1, 4097] with five alternatives 6.7 us;
+ * [64, 151936] with twenty 18.3 us, of which the bytes are 4). */
 #include <float.h>
 
 #include "d3s_rowcore.h"
@@ -38,6 +47,7 @@ namespace {
 
 constexpr int ST = 256;        /* threads of a workgroup */
 constexpr int SW = ST / WAVE;
+constexpr int CUS = 256;
 constexpr int GRID_MOST = 1 << 22; /* workgroups a launch: their threads are counted in 32 bits */
 constexpr int SU = 4;          /* chunks a lane takes at a time */
 constexpr int SCORE_ARRIVALS = 2048; /* rows that have a counter of arrivals */
@@ -571,19 +581,18 @@ int chunks_of(int vocab) {
 
 }  // namespace
 
-/* Enough workgroups to fill the chip (eight of 256 threads a CU), each with at
- * least two chunks a lane.  With alternatives: segments that a workgroup's
- * registers hold, so that filing them needs no second read, where those are few
- * enough to be joined. */
+/* Four workgroups a CU, each with at least two chunks a lane (bf16, four and eight
+ * a CU: 64 rows of 151936 9.8 and 12.5 us, 1024 of them 53 and 60, 1024 rows of
+ * 32000 15 and 20; with ten alternatives 512 rows of 151936 56 and 64).  With alternatives
+ * at least a block of LDS, so that filing needs no second read ([16, 151936], twenty
+ * alternatives: 14 us, 17 with two chunks a lane), and more of them only while
+ * there are few rows (ten alternatives, a block each: 128 rows 27 us, so 24; 512
+ * rows 89, so 56). */
 int score_segments(Dtype dt, int64_t n_rows, int vocab, int n_top) {
   const int chunks = dt == DT_BF16 ? chunks_of<true>(vocab) : chunks_of<false>(vocab);
   if (n_rows > SCORE_ARRIVALS) return 1;
-  if (n_top > 0) {
-    const int held = (chunks + SU * ST - 1) / (SU * ST);
-    if (held <= SEG_TOP && held * n_top <= JOIN) return held;
-  }
-  const int64_t want = n_rows > 0 ? 2048 / n_rows : 1;
-  const int most = min(n_top > 0 ? min(SEG_TOP, JOIN / n_top) : SEG_MOST, chunks / (2 * ST));
+  const int64_t want = n_rows > 0 ? 4 * CUS / n_rows : 1;
+  const int most = n_top > 0 ? min(min(SEG_TOP, JOIN / n_top), (chunks + SU * ST - 1) / (SU * ST)) : min(SEG_MOST, chunks / (2 * ST));
   const int n = (int)(want < most ? want : most);
   return n > 1 ? n : 1;
 }
@@ -622,9 +631,11 @@ void launch_score(const ScoreArgs &a, Dtype dt, void *ws, hipStream_t s) {
 template <bool BF16>
 static void grad_launch(const ScoreArgs &a, hipStream_t s) {
   const int chunks = chunks_of<BF16>(a.vocab);
-  /* a segment is a few rounds of the workgroup's GU chunks a lane (the row's
-   * numbers are read once a segment), fewer when there are few rows */
-  const int64_t room = (4096 + a.n_rows - 1) / a.n_rows;
+  /* a segment is two rounds of the workgroup's GU chunks a lane (bf16 [2048, 151936]:
+   * 228 us; one 241, four 258, twenty 273), less when there would be fewer than
+   * four workgroups a CU ([64, 151936] 9.9 us, 12.8 with sixteen a CU; 1000 rows of
+   * 32000 25 and 30.5) */
+  const int64_t room = (4 * CUS + a.n_rows - 1) / a.n_rows;
   int64_t nseg = (chunks + 2 * GU * ST - 1) / (2 * GU * ST);
   const int64_t least = (chunks + ST - 1) / ST;
   if (nseg < room) nseg = room < least ? room : least;
