@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import train_ref as R
+import test_score as S
 from test_dense import product, slopes
 
 pytestmark = pytest.mark.gpu
@@ -217,3 +218,22 @@ def test_few_rows_at_any_element(gpu, m, n, k):
     for xt, wt in ((False, False), (False, True), (True, False)):
         product(gpu, m, n, k, xt, wt, bias=True, act="gelu", residual=True)
         product(gpu, m, n, k, xt, wt, pads=(2, 1, 0), offset=1, out="f32")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,V,top,pad,offset", [(700, 10001, 33, 0, 0), (130, 60003, 64, 1, 3), (1025, 8200, 2, 0, 1)])
+def test_alternatives_of_long_segments(gpu, n, V, top, pad, offset, dtype):
+    """so many rows that a segment is more than is held at once: it is read again for
+    the alternatives, several times where there are more ties than are filed"""
+    rng = np.random.default_rng([n, V])
+    x = rng.standard_normal((n, V), np.float32) * 2.5
+    x[1::8] = 0
+    x[2::8] = rng.integers(0, 2, x[2::8].shape)
+    x[3::8] = np.round(x[3::8])
+    x[4::8, : V - 5] = -np.inf
+    x[5] = -np.inf
+    x[6, V - 1] = np.nan
+    bits, l = R.to_bits(x, dtype)
+    tokens = rng.integers(0, V, (n, 1))
+    banned = np.where(rng.random(n) < 0.5, l.argmax(1), -1)
+    S.check(S.run(gpu, bits, 0.8, banned, tokens, top, pad, offset), R.score(l, S.temperatures(0.8, n), banned, tokens, top))
