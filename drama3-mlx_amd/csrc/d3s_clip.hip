@@ -2,8 +2,9 @@
  * scaled to it (gfx950, wave64; include/d3s_train.h).
  *
  * The tensors' addresses and lengths travel as kernel arguments (as many a
- * launch as 4 KiB hold: a launch costs more than a short tensor's work), so the
- * call keeps nothing and may be captured; a tensor of more than 2^30 elements
+ * launch as 4 KiB hold: a launch costs more than a short tensor's work), those of
+ * many tensors on to k_clip in the workspace, so the call keeps nothing and may be
+ * captured; a tensor of more than 2^30 elements
  * travels in pieces.  A launch's elements are cut into chunks of one size.
  * k_norm: workgroups take chunks in turn, square in 64 bits (a bf16's square is
  * exact and an fp32's keeps its range: nothing overflows, and the order costs no
@@ -16,6 +17,8 @@
  * tensors of 8.4 million fp32: the norm 59 us (5.7 TB/s), the scaling 103 (6.5 TB/s;
  * with stores through the caches 200 in all, so 162); 150 ragged tensors of 2
  * million elements in all: 14 us, two launches. */
+#include <type_traits>
+
 #include "d3s_device.h"
 #include "d3s_stream.h"
 #include "d3s_train_internal.h"
@@ -44,12 +47,41 @@ struct ClipOut {
   void *dst[CLIP_PIECES];
 };
 
+/* the pieces of many tensors, in the workspace */
+struct Table {
+  const void **src;
+  void **dst;
+  uint32_t *first, *numel;
+  int n;
+  uint32_t chunks, chunk;
+};
+
+/* what a launch of k_norm files there: its pieces from `at` on, chunks from `chunk0` */
+struct Filed {
+  void *dst[CLIP_PIECES];
+  Table to;
+  int at;
+  uint32_t chunk0;
+};
+struct Nothing {};
+
 /* a chunk of a piece: elements [j0, j1) from an aligned start, or cut by the piece's ends */
 struct Chunk {
   int t;
   bool bf16;
   int64_t j0, j1;
 };
+
+/* chunk i of a piece that starts with chunk `first` */
+__device__ __forceinline__ Chunk chunk_of(const void *src, uint32_t numel, uint32_t first, uint32_t chunk, uint32_t i) {
+  Chunk c;
+  c.bf16 = (numel & 1u) != 0u;
+  const int64_t n = (int64_t)(numel >> 1), per = (int64_t)chunk * (c.bf16 ? 8 : 4);
+  const int64_t lead = (int64_t)((uintptr_t)src & 15u) / (c.bf16 ? 2 : 4);
+  c.j0 = (int64_t)(i - first) * per - lead;
+  c.j1 = c.j0 + per < n ? c.j0 + per : n;
+  return c;
+}
 
 /* chunk i's piece: the last of those that start at or before it, all starts loaded
  * at once (they ascend; a search would wait for one load after the other) */
@@ -62,13 +94,23 @@ __device__ __forceinline__ Chunk find_chunk(const Pieces<MOST> &a, uint32_t i) {
     lo += (int)__popcll(__ballot(at < a.n && a.first[min(at, MOST - 1)] <= i));
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
-  Chunk c;
+  Chunk c = chunk_of(a.src[lo], a.numel[lo], a.first[lo], a.chunk, i);
   c.t = lo;
-  c.bf16 = (a.numel[lo] & 1u) != 0u;
-  const int64_t n = (int64_t)(a.numel[lo] >> 1), per = (int64_t)a.chunk * (c.bf16 ? 8 : 4);
-  const int64_t lead = (int64_t)((uintptr_t)a.src[lo] & 15u) / (c.bf16 ? 2 : 4);
-  c.j0 = (int64_t)(i - a.first[lo]) * per - lead;
-  c.j1 = c.j0 + per < n ? c.j0 + per : n;
+  return c;
+}
+
+/* the same in a table: the last 64th piece that starts at or before it, then the last of the 64 from there */
+__device__ __forceinline__ Chunk find_chunk(const Table &a, uint32_t i) {
+  int lo = -1;
+  for (int w = 0; w < a.n; w += WAVE * WAVE) {
+    const int at = w + lane_id() * WAVE;
+    lo += (int)__popcll(__ballot(at < a.n && a.first[min(at, a.n - 1)] <= i));
+  }
+  const int at = lo * WAVE + lane_id();
+  lo = lo * WAVE - 1 + (int)__popcll(__ballot(at < a.n && a.first[min(at, a.n - 1)] <= i));
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  Chunk c = chunk_of(a.src[lo], a.numel[lo], a.first[lo], a.chunk, i);
+  c.t = lo;
   return c;
 }
 
@@ -150,8 +192,19 @@ __device__ __forceinline__ double block_sum(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(CT) void k_norm(Pieces<NORM_PIECES> a, double *parts, int have) {
+template <int MOST, class F>
+__global__ __launch_bounds__(CT) void k_norm(Pieces<MOST> a, F filed, double *parts, int have) {
   double sum = 0.0;
+  if constexpr (!std::is_same_v<F, Nothing>) {
+    if (blockIdx.x == 0 && (int)threadIdx.x < a.n) {
+      static_assert(MOST <= CT, "a thread a piece");
+      const int i = (int)threadIdx.x;
+      filed.to.src[filed.at + i] = a.src[i];
+      filed.to.dst[filed.at + i] = filed.dst[i];
+      filed.to.first[filed.at + i] = filed.chunk0 + a.first[i];
+      filed.to.numel[filed.at + i] = a.numel[i];
+    }
+  }
   for (uint32_t i = blockIdx.x; i < a.chunks; i += gridDim.x) {
     const Chunk c = find_chunk(a, i);
     sum += c.bf16 ? chunk_squares<true>(a.src[c.t], c) : chunk_squares<false>(a.src[c.t], c);
@@ -226,8 +279,8 @@ __device__ __forceinline__ void chunk_scale(const void *p, void *d, const Chunk 
   if (e < s.tail1) scale_one<BF16>(p, d, e, scale, keep);
 }
 
-__global__ __launch_bounds__(CT) void k_clip(Pieces<CLIP_PIECES> a, ClipOut out, const double *parts, int n_parts,
-                                             float max_norm, float *norm) {
+template <class P, class O>
+__global__ __launch_bounds__(CT) void k_clip(P a, O out, const double *parts, int n_parts, float max_norm, float *norm) {
   const float v = norm_of(parts, n_parts);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   const bool keep = !(v > max_norm && v < __builtin_inff());
@@ -242,6 +295,13 @@ __global__ __launch_bounds__(CT) void k_clip(Pieces<CLIP_PIECES> a, ClipOut out,
   }
 }
 
+/* chunks of 4 KiB (a 16-byte unit a lane) up to 64 KiB, by what fills the workgroups of some launches */
+uint32_t chunk_for(int64_t units, int64_t launches) {
+  uint32_t chunk = CT;
+  while (chunk < 16 * CT && units > (int64_t)chunk * CLIP_GROUPS * launches) chunk *= 2;
+  return chunk;
+}
+
 /* walks the tensors' pieces, MOST at a time */
 struct Walk {
   const void *const *src;
@@ -251,9 +311,9 @@ struct Walk {
   int n_tensors, t;
   int64_t at; /* elements of tensor t that are behind */
 
-  /* the next pieces and their chunks; false: there are none left */
+  /* the next pieces and their chunks, of `chunk` units (0: by the pieces' lengths); false: there are none left */
   template <int MOST>
-  bool fill(Pieces<MOST> &a, void **out) {
+  bool fill(Pieces<MOST> &a, void **out, uint32_t chunk = 0) {
     int64_t total = 0;
     a.n = 0;
     uint32_t units[MOST];
@@ -271,9 +331,7 @@ struct Walk {
       at += n;
       if (at >= numel[t]) t++, at = 0;
     }
-    /* chunks of 4 KiB (a 16-byte unit a lane) up to 64 KiB, by what fills the workgroups */
-    uint32_t chunk = CT;
-    while (chunk < 16 * CT && total > (int64_t)chunk * CLIP_GROUPS) chunk *= 2;
+    if (chunk == 0) chunk = chunk_for(total, 1);
     uint32_t first = 0; /* (at most 248 pieces of 2^18 chunks) */
     for (int i = 0; i < a.n; i++) {
       a.first[i] = first;
@@ -287,18 +345,60 @@ struct Walk {
 
 }  // namespace
 
-size_t clip_workspace_bytes() { return split_counter_bytes() + CLIP_GROUPS * sizeof(double); }
+/* More tensors than a launch of k_clip holds: the launches of k_norm file their
+ * pieces in a table, and one launch of k_clip takes them from there (700000 fp32
+ * elements in 260 tensors 14.3 us, 18.6 with a launch for every 164 of them, in 1000
+ * 39 and 53, in 170 12.7 and 13.5; 8 million bf16 in 214: 20.7 and 21.9).  A tensor of several pieces:
+ * launch by launch (the table's room is by the tensors' number). */
+bool tabled(const int64_t *numel, const int32_t *dtypes, int n_tensors, int64_t *units) {
+  int n = 0;
+  *units = 0;
+  for (int t = 0; t < n_tensors; t++) {
+    if (numel[t] > PIECE) return false;
+    n += numel[t] > 0;
+    *units += (numel[t] * (dtypes[t] == D3S_DTYPE_BF16 ? 2 : 4) + 15) / 16;
+  }
+  return n > CLIP_PIECES;
+}
+
+size_t clip_workspace_bytes(int n_tensors) {
+  const size_t table = n_tensors > CLIP_PIECES ? (size_t)n_tensors * (2 * sizeof(void *) + 2 * sizeof(uint32_t)) : 0;
+  return split_counter_bytes() + CLIP_GROUPS * sizeof(double) + table;
+}
 
 void launch_clip(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int n_tensors,
                  float max_norm, float *norm, void *ws, hipStream_t s) {
   double *parts = (double *)((char *)ws + split_counter_bytes());
   int n_parts = 0;
+  int64_t units;
+  if (dst && tabled(numel, dtypes, n_tensors, &units)) {
+    Table to;
+    to.src = (const void **)(parts + CLIP_GROUPS);
+    to.dst = (void **)(to.src + n_tensors);
+    to.first = (uint32_t *)(to.dst + n_tensors);
+    to.numel = to.first + n_tensors;
+    to.n = 0, to.chunks = 0;
+    to.chunk = chunk_for(units, (n_tensors + CLIP_PIECES - 1) / CLIP_PIECES);
+    Pieces<CLIP_PIECES> a;
+    Filed f;
+    Walk w{src, dst, numel, dtypes, n_tensors, 0, 0};
+    while (w.fill(a, f.dst, to.chunk)) {
+      f.to = to, f.at = to.n, f.chunk0 = to.chunks;
+      const int groups = a.chunks < CLIP_GROUPS ? (int)a.chunks : CLIP_GROUPS;
+      k_norm<<<groups, CT, 0, s>>>(a, f, parts, n_parts);
+      if (groups > n_parts) n_parts = groups;
+      to.n += a.n, to.chunks += a.chunks;
+    }
+    const int groups = to.chunks < 2 * CLIP_GROUPS ? (int)to.chunks : 2 * CLIP_GROUPS;
+    k_clip<<<groups, CT, 0, s>>>(to, to, parts, n_parts, max_norm, norm);
+    return;
+  }
   {
     Pieces<NORM_PIECES> a;
     Walk w{src, dst, numel, dtypes, n_tensors, 0, 0};
     while (w.fill(a, nullptr)) {
       const int groups = a.chunks < CLIP_GROUPS ? (int)a.chunks : CLIP_GROUPS;
-      k_norm<<<groups, CT, 0, s>>>(a, parts, n_parts);
+      k_norm<<<groups, CT, 0, s>>>(a, Nothing{}, parts, n_parts);
       if (groups > n_parts) n_parts = groups;
     }
   }

@@ -162,7 +162,7 @@ int clip_call(const void *const *src, void *const *dst, const int64_t *numel, co
   }
   hipStream_t s = (hipStream_t)stream;
   void *ws = nullptr;
-  if (const int rc = take_room(room, d3s::clip_workspace_bytes(), s, &ws)) return rc;
+  if (const int rc = take_room(room, d3s::clip_workspace_bytes(n_tensors), s, &ws)) return rc;
   d3s::launch_clip(src, dst, numel, dtypes, n_tensors, max_norm, norm, ws, s);
   return done();
 }
@@ -274,7 +274,7 @@ int d3s_clip_grads(const void *const *src, void *const *dst, const int64_t *nume
 }
 
 int64_t d3s_clip_grads_workspace_bytes(int n_tensors) {
-  return n_tensors < 0 ? D3S_ERR_ARG : (int64_t)d3s::clip_workspace_bytes();
+  return n_tensors < 0 ? D3S_ERR_ARG : (int64_t)d3s::clip_workspace_bytes(n_tensors);
 }
 
 int d3s_clip_grads_ws(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes,

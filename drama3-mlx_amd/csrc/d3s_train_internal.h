@@ -56,7 +56,7 @@ struct ActGradArgs {
 size_t act_grad_workspace_bytes(int64_t m, int64_t n, bool dbias);
 void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s);
 
-size_t clip_workspace_bytes();
+size_t clip_workspace_bytes(int n_tensors);
 void launch_clip(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int n_tensors,
                  float max_norm, float *norm, void *ws, hipStream_t s);
 

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import train_ref as R
+import test_clip as C
 import test_score as S
 from test_dense import product, slopes
 
@@ -237,3 +238,17 @@ def test_alternatives_of_long_segments(gpu, n, V, top, pad, offset, dtype):
     tokens = rng.integers(0, V, (n, 1))
     banned = np.where(rng.random(n) < 0.5, l.argmax(1), -1)
     S.check(S.run(gpu, bits, 0.8, banned, tokens, top, pad, offset), R.score(l, S.temperatures(0.8, n), banned, tokens, top))
+
+
+@pytest.mark.parametrize("sizes", [[3] * 248, [3] * 249, [0, 7] * 260, list(range(1, 500)) + [300000, 0, 70001] + [9] * 300,
+                                   [1, 2, 8] * 1366, [5] * 4160 + [100000] + [2] * 4160])
+def test_many_tensors(gpu, sizes):
+    """more tensors than travel with one launch, with every number of 64s and of 4096s of them"""
+    t = C.tensors_of(sizes)
+    norm = float(np.sqrt(sum(float((R.from_bits(b) ** 2).sum()) for b, _ in t)))
+    for limit in (norm / 3, norm * 2):
+        limit = float(np.float32(limit))
+        C.check(*C.run(gpu, t, limit, shift=3, use_ws=True), t, limit)
+        C.check(*C.run(gpu, t, limit, in_place=True), t, limit)
+    n, _ = C.run(gpu, t, 1.0, norm_only=True)
+    C.check(n, [], t, 1.0)
