@@ -29,9 +29,9 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 /* Microseconds of m rows and n outputs in tiles of tm x tn, one workgroup a CU: rounds of
  * workgroups, each its stages and what it spends before and after them.
  * Measured, by how many operands go to LDS directly: a stage of 256 x 256 1.45
- * (both), 1.65 (one) and 2.2; of 128 x 256 0.93 and 1.2; of 128 x 128 0.52 and
- * 0.75, with a quarter of the CUs idle 0.38 and 0.65.  Around them 14, 10 and 6, and
- * for split sums 3 and 1 a split.
+ * (both), 1.65 (one) and 2.2, with an eighth of the CUs idle 1.1, 1.35 and 1.6; of
+ * 128 x 256 0.93 and 1.2 (0.65 and 0.95); of 128 x 128 0.52 and 0.75 (with a
+ * quarter idle 0.38 and 0.65).  Around them 14, 10 and 6, and for split sums 3 and 1 a split.
  * (8192 x 2048 x 2048, both direct: 63, 78 and 87 us in the three tiles;
  * 2048 x 2048 x 2048: 50, 29 and 22; 4096 x 2048 x 8192, both by the inner
  * index: 217, 160 and 210; 256 x 2048 x 8192: 128 x 128 with 1, 2, 4 and 8
@@ -42,9 +42,15 @@ double tile_us(const Product &p, int64_t m, int64_t n, int tm, int tn, int split
   const int direct = p.x_direct + p.w_direct;
   const double wgs = (double)up(m, tm) * (double)up(n, tn) * splits;
   const double rounds = (double)(int64_t)((wgs + CUS - 1) / CUS), stages = (double)up(p.k, (int64_t)TILE_K * splits);
-  if (tm == 256) return rounds * (stages * (direct == 2 ? 1.45 : direct == 1 ? 1.65 : 2.2) + 14);
-  if (tn == 256) return rounds * (stages * (direct == 2 ? 0.93 : 1.2) + 10);
-  const bool few = wgs <= CUS * 3 / 4;
+  const bool few = wgs <= (tn == 256 ? CUS * 7 / 8 : CUS * 3 / 4);
+  if (tm == 256) {
+    const double full = direct == 2 ? 1.45 : direct == 1 ? 1.65 : 2.2, some = direct == 2 ? 1.1 : direct == 1 ? 1.35 : 1.6;
+    return rounds * (stages * (few ? some : full) + 14);
+  }
+  if (tn == 256) {
+    const double full = direct == 2 ? 0.93 : 1.2, some = direct == 2 ? 0.65 : 0.95;
+    return rounds * (stages * (few ? some : full) + 10);
+  }
   const double stage = direct == 2 ? (few ? 0.38 : 0.52) : few ? 0.65 : 0.75;
   return rounds * (stages * stage + 6) + (splits > 1 ? 3 + splits : 0);
 }
@@ -56,6 +62,7 @@ struct Plan {
   TilePlan tile;         /* no tiles: no such launch */
   int64_t tile_m, tile_n;
   FewPlan few, few_outs; /* the rows after the tiles', and the outputs after theirs of the tiles' rows */
+  double us;             /* what it should take */
 };
 
 size_t tile_bytes(const TilePlan &t) { return t.splits > 1 ? (size_t)t.tiles * t.splits * t.tm * t.tn * sizeof(float) : 0; }
@@ -87,6 +94,7 @@ Plan plan(const Product &p) {
   const bool rows_can = !p.w_turned || p.n >= 8;
   if (rows_can && (p.m <= 32 || (p.m <= FEW_ROWS && !p.w_turned && p.n <= 16 * CUS))) {
     pl.few = few_plan(0, p.m, p.n, p.k, p.w_turned);
+    pl.us = few_us(p, p.n);
     return pl;
   }
 
@@ -112,6 +120,7 @@ Plan plan(const Product &p) {
     for (int s = 1; s <= 8; s++)
       if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(n, 128) * s <= 2 * CUS)) offer(128, 128, s);
   }
+  pl.us = best;
   t.m_tiles = (unsigned)up(pl.tile_m, t.tm);
   t.n_tiles = (unsigned)up(pl.tile_n, t.tn);
   t.tiles = t.m_tiles * t.n_tiles;
@@ -124,12 +133,54 @@ Plan plan(const Product &p) {
   return pl;
 }
 
-size_t bytes_of(const Product &p) {
+/* A product in two: the first part's rows and outputs, one of them the whole's.
+ * Where the last round of tiles would be less than half full, what fills the rounds
+ * before is a product of its own, and the rest another, in smaller tiles and
+ * split sums (1500 x 11008 x 4096, w by the inner index, 258 tiles of 256 x 256: 205
+ * us, so 135; 3000 x 11008 x 4096 by rows 271 and 216).  Whole rounds of whole tiles: both parts start where the
+ * operands' alignment is the same. */
+struct Cut {
+  int64_t m, n;
+};
+Cut cut_of(const Product &p) {
+  Cut best{p.m, p.n};
+  const Plan whole = plan(p);
+  if (!whole.tile.tiles) return best;
+  double least = 0.92 * whole.us; /* (a launch more, and costs that are estimates) */
+  const int tiles[3][2] = {{256, 256}, {128, 256}, {128, 128}};
+  for (const auto &t : tiles) {
+    const int64_t mt = up(p.m, t[0]), nt = up(p.n, t[1]), rounds = mt * nt / CUS;
+    if (rounds < 1 || mt * nt % CUS == 0 || mt * nt % CUS >= CUS / 2) continue;
+    const int64_t n = rounds * CUS / mt * t[1], m = rounds * CUS / nt * t[0];
+    auto offer = [&](int64_t m1, int64_t n1, int64_t m2, int64_t n2) {
+      Product a = p, b = p;
+      a.m = m1, a.n = n1, b.m = m2, b.n = n2;
+      const double us = plan(a).us + plan(b).us;
+      if (us < least) least = us, best = {m1, n1};
+    };
+    if (n > 0 && n < p.n) offer(p.m, n, p.m, p.n - n);
+    if (m > 0 && m < p.m) offer(m, p.n, p.m - m, p.n);
+  }
+  return best;
+}
+
+size_t bytes_of_part(const Product &p) {
   const Plan pl = plan(p);
   const size_t a = tile_bytes(pl.tile), b = few_bytes(pl.few, p.w_turned, p.m - pl.few.i0),
                c = few_bytes(pl.few_outs, p.x_turned, p.n - pl.few_outs.i0);
   const size_t ab = a > b ? a : b;
   return ab > c ? ab : c; /* (one launch after the other) */
+}
+
+size_t bytes_of(const Product &p) {
+  const Cut c = cut_of(p);
+  Product first = p, rest = p;
+  first.m = c.m, first.n = c.n;
+  const size_t a = bytes_of_part(first);
+  if (c.m == p.m && c.n == p.n) return a;
+  c.n < p.n ? rest.n -= c.n : rest.m -= c.m;
+  const size_t b = bytes_of_part(rest);
+  return a > b ? a : b;
 }
 
 }  // namespace
@@ -144,7 +195,7 @@ size_t dense_workspace_bytes(const d3s_dense_params &p) {
   return most ? split_counter_bytes() + most : 0;
 }
 
-void launch_dense(const d3s_dense_params &p, void *ws, hipStream_t s) {
+static void launch_part(const d3s_dense_params &p, void *ws, hipStream_t s) {
   const Operands a{p.x, p.w, p.x_stride, p.w_stride, (int)p.k};
   Out o{p.bias,     p.residual, p.z,      p.y,          p.residual_stride,          p.z_stride,
         p.y_stride, (int)p.m,   (int)p.n, p.activation, p.y_dtype == D3S_DTYPE_F32};
@@ -170,6 +221,30 @@ void launch_dense(const d3s_dense_params &p, void *ws, hipStream_t s) {
     pr.w_turned ? launch_tiles<true, true>(a, o, pl.tile, s) : launch_tiles<true, false>(a, o, pl.tile, s);
   else
     pr.w_turned ? launch_tiles<false, true>(a, o, pl.tile, s) : launch_tiles<false, false>(a, o, pl.tile, s);
+}
+
+void launch_dense(const d3s_dense_params &p, void *ws, hipStream_t s) {
+  const Cut c = cut_of(product_of(p, (uintptr_t)p.x, (uintptr_t)p.w));
+  d3s_dense_params first = p, rest = p;
+  first.m = c.m, first.n = c.n;
+  launch_part(first, ws, s);
+  const int64_t es = p.y_dtype == D3S_DTYPE_F32 ? 4 : 2;
+  if (c.n < p.n) {
+    rest.n -= c.n;
+    rest.w += p.w_transposed ? c.n : c.n * p.w_stride;
+    if (p.bias) rest.bias += c.n;
+    if (p.z) rest.z += c.n;
+    if (p.residual) rest.residual = (const char *)p.residual + c.n * es;
+    rest.y = (char *)p.y + c.n * es;
+    launch_part(rest, ws, s);
+  } else if (c.m < p.m) {
+    rest.m -= c.m;
+    rest.x += p.x_transposed ? c.m : c.m * p.x_stride;
+    if (p.z) rest.z += c.m * p.z_stride;
+    if (p.residual) rest.residual = (const char *)p.residual + c.m * p.residual_stride * es;
+    rest.y = (char *)p.y + c.m * p.y_stride * es;
+    launch_part(rest, ws, s);
+  }
 }
 
 }  // namespace d3s

@@ -252,3 +252,12 @@ def test_many_tensors(gpu, sizes):
         C.check(*C.run(gpu, t, limit, in_place=True), t, limit)
     n, _ = C.run(gpu, t, 1.0, norm_only=True)
     C.check(n, [], t, 1.0)
+
+
+@pytest.mark.parametrize("xt,wt", [(False, False), (False, True), (True, False), (True, True)])
+def test_last_round_of_tiles_apart(gpu, xt, wt):
+    """outputs or rows whose tiles would begin one more round of the whole chip are a product of their own"""
+    product(gpu, 1500, 11008, 130, xt, wt, bias=True, act="silu", keep=True, residual=True)
+    product(gpu, 11008, 1500, 70, xt, wt, bias=True, act="gelu", keep=True, residual=True, out="f32", in_place=True)
+    product(gpu, 11010, 1501, 65, xt, wt, bias=True, keep=True, residual=True, pads=(1, 1, 3), offset=1)
+    product(gpu, 1537, 11011, 200, xt, wt, residual=True, out="f32")
