@@ -119,6 +119,8 @@ int dense_call(const d3s_dense_params *p, Room room, void *stream) {
   if (p->y_stride < p->n || (p->residual && p->residual_stride < p->n) || (p->z && p->z_stride < p->n))
     return D3S_ERR_ARG;
   if (p->m == 0 || p->n == 0) return D3S_OK;
+  /* (at another stride one workgroup's outputs would be rows that another has yet to read) */
+  if (p->residual == p->y && p->residual && p->residual_stride != p->y_stride && p->m > 1) return D3S_ERR_ARG;
   const size_t ys = size_of(p->y_dtype);
   if (!p->y || off(p->y, ys) || off(p->residual, ys) || off(p->bias, 2) || off(p->z, 2)) return D3S_ERR_ARG;
   if (p->k > 0 && (!p->x || !p->w || off(p->x, 2) || off(p->w, 2))) return D3S_ERR_ARG;

@@ -92,8 +92,9 @@ int d3s_logprob_backward(const void *logits, int dtype, int64_t n_rows, int64_t 
  * gradients are the same call: dx [m, k'] = dz w (w_transposed, inner length
  * n), dw [n, k'] = dz^T x (both transposed, inner length m).
  * Strides are in elements between two stored rows.  bias [n] bf16, residual
- * [m, n] of y's type (it may be y itself: sums over micro-batches) and z [m, n]
- * bf16 (the pre-activation x w^T + bias, kept for the backward) may be NULL.
+ * [m, n] of y's type (it may be y itself, with y's stride: sums over
+ * micro-batches) and z [m, n] bf16 (the pre-activation x w^T + bias, kept for the
+ * backward) may be NULL.
  * No other output may overlap an input.  y_dtype D3S_DTYPE_F32 or
  * D3S_DTYPE_BF16.  m, n, k from 0 up to 2^31 - 1024; k = 0 sums nothing. */
 typedef struct {

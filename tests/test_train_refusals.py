@@ -1,0 +1,24 @@
+"""More of what the scoring and training entry points refuse, and what their
+workspace queries promise (no GPU needed: no pointer below is looked at)."""
+import pytest
+
+P = 4096  # an aligned address that is never read
+
+
+@pytest.fixture(scope="module")
+def d3s():
+    import d3s
+    d3s.lib()
+    return d3s
+
+
+@pytest.mark.parametrize("y_dtype", [0, 1])
+@pytest.mark.parametrize("residual_stride", [32, 41, 100])
+def test_dense_in_place_at_another_stride(d3s, y_dtype, residual_stride):
+    """a residual that is y itself lies where y does: at another stride one workgroup's
+    outputs would be rows that another has yet to read"""
+    call = dict(x=P, x_stride=64, w=P, w_stride=64, m=8, n=32, k=64, y=2 * P, y_stride=40, y_dtype=y_dtype,
+                residual=2 * P, residual_stride=residual_stride)
+    assert d3s.dense_raw(**call) == -1
+    assert d3s.dense_raw(**call, workspace=(P, 1 << 30)) == -1
+    assert d3s.dense_raw(**dict(call, m=2)) == -1
