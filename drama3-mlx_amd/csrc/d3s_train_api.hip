@@ -137,6 +137,7 @@ int act_grad_call(const uint16_t *dy, int64_t dy_stride, const uint16_t *z, int6
       dy_stride < n || (z && z_stride < n) || (dz && dz_stride < n))
     return D3S_ERR_ARG;
   if (n == 0 || (!dz && !dbias)) return D3S_OK;
+  if (dz && dz == dy && dz_stride != dy_stride && m > 1) return D3S_ERR_ARG; /* (as a residual in place, above) */
   if (off(dbias, 4)) return D3S_ERR_ARG;
   if (m > 0 && (!dy || (!z && activation != D3S_ACT_NONE) || off(dy, 2) || off(z, 2) || off(dz, 2)))
     return D3S_ERR_ARG;

@@ -126,9 +126,9 @@ int64_t d3s_dense_workspace_bytes(const d3s_dense_params *params);
 int d3s_dense_bf16_ws(const d3s_dense_params *params, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* The gradient through a dense layer's epilogue: dz [m, n] = dy act'(z) (bf16,
- * rounded once; it may be dy itself or NULL) and dbias[n] = the column sums of
- * dy act'(z) in fp32, before the rounding (may be NULL).  z may be NULL with
- * D3S_ACT_NONE. */
+ * rounded once; it may be dy itself, with dy's stride, or NULL) and dbias[n] =
+ * the column sums of dy act'(z) in fp32, before the rounding (may be NULL).  z may
+ * be NULL with D3S_ACT_NONE. */
 int d3s_dense_activation_backward_bf16(const uint16_t *dy, int64_t dy_stride, const uint16_t *z, int64_t z_stride,
                                        int64_t m, int64_t n, int activation, uint16_t *dz, int64_t dz_stride,
                                        float *dbias, void *stream);

@@ -22,3 +22,13 @@ def test_dense_in_place_at_another_stride(d3s, y_dtype, residual_stride):
     assert d3s.dense_raw(**call) == -1
     assert d3s.dense_raw(**call, workspace=(P, 1 << 30)) == -1
     assert d3s.dense_raw(**dict(call, m=2)) == -1
+
+
+@pytest.mark.parametrize("dz_stride", [32, 41, 100])
+def test_activation_gradient_in_place_at_another_stride(d3s, dz_stride):
+    """the same of a dz that is dy itself"""
+    call = dict(dy=P, dy_stride=40, z=2 * P, z_stride=32, m=8, n=32, activation=2, dz=P, dz_stride=dz_stride, dbias=3 * P)
+    assert d3s.dense_activation_backward_raw(**call) == -1
+    assert d3s.dense_activation_backward_raw(**dict(call, dbias=None)) == -1
+    assert d3s.dense_activation_backward_raw(**call, workspace=(P, 1 << 30)) == -1
+    assert d3s.dense_activation_backward_raw(**dict(call, m=2, z=None, activation=0)) == -1
