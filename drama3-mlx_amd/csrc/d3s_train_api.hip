@@ -188,7 +188,10 @@ int d3s_logprob(const void *logits, int dtype, int64_t n_rows, int64_t vocab, in
 int64_t d3s_logprob_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int n_top) {
   if (const int rc = check_rows(dtype, n_rows, vocab)) return rc;
   if (n_top < 0 || n_top > D3S_MAX_TOP || n_top > vocab) return D3S_ERR_ARG;
-  return (int64_t)d3s::score_workspace_bytes(type_of(dtype), n_rows, (int)vocab, n_top);
+  /* (a call with neither array of alternatives has none: other segments) */
+  const size_t with = d3s::score_workspace_bytes(type_of(dtype), n_rows, (int)vocab, n_top);
+  const size_t without = d3s::score_workspace_bytes(type_of(dtype), n_rows, (int)vocab, 0);
+  return (int64_t)(with > without ? with : without);
 }
 
 int d3s_logprob_ws(const void *logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

@@ -53,7 +53,8 @@ int d3s_logprob(const void *logits, int dtype, int64_t n_rows, int64_t vocab, in
                 int n_tokens, float *logprobs, float *entropy, float *row_stats, int n_top, int32_t *top_ids,
                 float *top_logprobs, uint32_t *counters, void *stream);
 
-/* Bytes of workspace d3s_logprob_ws needs (0: none), or a negative status. */
+/* Bytes of workspace d3s_logprob_ws needs (0: none), with n_top alternatives or
+ * with top_ids and top_logprobs both NULL, or a negative status. */
 int64_t d3s_logprob_workspace_bytes(int dtype, int64_t n_rows, int64_t vocab, int n_top);
 
 /* d3s_logprob with the workspace given: never allocates, may be captured. */

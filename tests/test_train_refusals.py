@@ -32,3 +32,14 @@ def test_activation_gradient_in_place_at_another_stride(d3s, dz_stride):
     assert d3s.dense_activation_backward_raw(**dict(call, dbias=None)) == -1
     assert d3s.dense_activation_backward_raw(**call, workspace=(P, 1 << 30)) == -1
     assert d3s.dense_activation_backward_raw(**dict(call, m=2, z=None, activation=0)) == -1
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_scores_workspace_covers_a_call_without_alternatives(d3s, dtype):
+    """n_top with neither top_ids nor top_logprobs is a call without alternatives,
+    which is cut into other segments: what was queried with n_top serves it too"""
+    size = d3s.lib().d3s_logprob_workspace_bytes
+    for rows in (1, 2, 7, 64, 500, 1024, 2048, 2049):
+        for vocab in (64, 4097, 8185, 16384, 60000, 151936, 1000003):
+            for n_top in (1, 5, 20, 64):
+                assert size(dtype, rows, vocab, n_top) >= size(dtype, rows, vocab, 0), (rows, vocab, n_top)
