@@ -64,6 +64,12 @@ constexpr float SHIFT_MOST = 1048576.0f;
 
 __device__ __forceinline__ float maximum(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+/* a row's temperature; one that is not finite (the row is refused) stays as it is */
+__device__ __forceinline__ float row_temperature(const ScoreArgs &a, int row) {
+  const float T = a.temperature ? a.temperature[row] : a.temperature_scalar;
+  return T < 1e-5f && T > -__builtin_inff() ? 1e-5f : T;
+}
+__device__ __forceinline__ bool finite(float T) { return fabsf(T) < __builtin_inff(); }
 /* a - b for the exponents of maxima: both may be -FLT_MAX, neither is -inf */
 __device__ __forceinline__ float drop(float a, float b, float c) { return fmaxf((a - b) * c, LEAST); }
 
@@ -204,7 +210,7 @@ __device__ __forceinline__ void finish(const ScoreArgs &a, ScoreLds &L, const Ro
                                        float token_logit, int token) {
   const int tid = (int)threadIdx.x;
   const float nan = __builtin_nanf(""), ninf = -__builtin_inff();
-  const bool refused = !(s.m < __builtin_inff()) || !(T < __builtin_inff());
+  const bool refused = !(s.m < __builtin_inff()) || !finite(T);
   const bool masked = !refused && s.S == 0.0f;
   const float logS = refused ? nan : masked ? ninf : d3s_logf(s.S);
   if (tid == 0) {
@@ -239,8 +245,7 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
   __shared__ ScoreLds L;
   const int tid = (int)threadIdx.x;
   const int row = row0 + (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
-  float T = a.temperature ? a.temperature[row] : a.temperature_scalar;
-  if (T < 1e-5f) T = 1e-5f;
+  const float T = row_temperature(a, row);
   const float c = LOG2E / T;
   const Row<BF16> R(a.logits, a.row_stride, row, a.vocab, a.banned ? a.banned[row] : -1);
   int token = -1;
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
     if (tid == 0) L.count = 0u;
   }
   s = join_block(L, s, c);
-  const bool live = s.m < __builtin_inff(); /* no NaN or +inf in the segment */
+  const bool live = s.m < __builtin_inff() && finite(T); /* no NaN or +inf in the segment: the row may be scored */
 
   if (TOP) {
     uint32_t t = L.least[0];
@@ -488,8 +493,7 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
   const int tail = lo < chunks && hi == chunks ? max((lead + V) / EPC * EPC - lead, lead > 0 ? min(EPC - lead, V) : 0) : V;
   auto get = [&](int ch) { return load16(src + ((int64_t)ch * EPC - lead) * ES); };
 
-  float T = a.temperature ? a.temperature[row] : a.temperature_scalar;
-  if (T < 1e-5f) T = 1e-5f;
+  const float T = row_temperature(a, row);
   const int ban = a.banned ? a.banned[row] : -1;
   GradRow r;
   r.m = a.stats_in[2 * (size_t)row];
@@ -513,7 +517,7 @@ __global__ __launch_bounds__(ST) void k_score_grad(ScoreArgs a, int nseg, int se
   r.inv_S = d3s_expf(-logS);
   r.log2S = logS * LOG2E;
   r.inv_T = 1.0f / T;
-  if (!(T < __builtin_inff())) r.inv_T = __builtin_nanf("");
+  if (!finite(T)) r.inv_T = __builtin_nanf("");
 
   /* a token's logit, before its place may be overwritten (grad may be logits) */
   const bool here = token >= j0 && token < j1 && threadIdx.x < WAVE;

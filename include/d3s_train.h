@@ -44,8 +44,9 @@ extern "C" {
  * min(D3S_MAX_TOP, vocab).  logprobs (with n_tokens), entropy, row_stats
  * [n_rows, 2] and top_ids / top_logprobs [n_rows, n_top] may each be NULL.
  * counters: as d3s_sample's, the first two slots.
- * A row with a NaN or +inf logit, or a temperature that is not finite, is
- * refused: every number NaN (log probabilities of no token too), top_ids -1.
+ * A row with a NaN or +inf logit, or a temperature that is not finite (-infinity
+ * too, which a draw takes as 1e-5), is refused: every number NaN (log
+ * probabilities of no token too), top_ids -1.
  * A row whose logits are all masked has log probabilities -inf (0 for no
  * token), entropy 0, row_stats -inf and top_ids 0, 1, ... */
 int d3s_logprob(const void *logits, int dtype, int64_t n_rows, int64_t vocab, int64_t row_stride,

@@ -35,3 +35,30 @@ def test_alternatives_that_nobody_takes(gpu, n, V, top):
         hiprt.synchronize()
         R.assert_near(lp.download((n, 1), np.float32), ref["logprobs"], R.score_tol(ref, ref["logprobs"]))
         R.assert_near(st.download((n, 2), np.float32)[:, 0], ref["m"], 0)
+
+
+@pytest.mark.parametrize("per_row", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [3, 4097, 60001])
+def test_temperatures_that_are_not_finite(gpu, V, dtype, per_row):
+    """infinities of both signs and NaN refuse a row, and its gradient"""
+    n, inf = 6, np.inf
+    T = np.float32([-inf, 0.8, inf, -inf, np.nan, -1e30])
+    rng, bits, l = S.make(n, V, dtype, 12)
+    l[3, 1] = -inf
+    bits, l = R.to_bits(l, dtype)
+    tokens = np.stack([rng.integers(0, V, n), np.full(n, -1)], 1)
+    # (the plain form clamps before it looks: any temperature that it refuses stands for those)
+    ref = R.score(l, np.where(np.isfinite(T), T, inf).astype(np.float64), None, tokens, 3)
+    refused = ~np.isfinite(T)
+    assert np.array_equal(ref["refused"], refused)
+    g, gH = rng.standard_normal((n, 2)).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    dx, err = R.score_grad(ref, tokens, g.astype(np.float64), gH)
+    dx[refused] = np.where(np.isneginf(l[refused]), 0.0, np.nan)
+    if per_row:
+        S.check(S.run(gpu, bits, T, None, tokens, 3), ref)
+        S.check_grad(S.run_grad(gpu, bits, T, None, tokens, ref, g, gH), dx, np.nan_to_num(err, nan=0.0) + 1e-37)
+        return
+    for r in range(n):
+        one = {k: v[r:r + 1] for k, v in ref.items()}
+        S.check(S.run(gpu, bits[r:r + 1], T[r], None, tokens[r:r + 1], 3), one)
