@@ -23,8 +23,9 @@
  * logits reach the least of the four, and few others do: a second pass over
  * the segment files those, and the filed keys (order-preserving logit bits, then
  * the complement of the index) are ranked by counting.  More than the list
- * holds (ties, masked rows): the n-th of the filed keys is a bound at least as
- * high, and the pass is run again with it.  The segment passes through LDS in
+ * holds (ties, masked rows, logits that agree in their upper 16 bits): the n-th of
+ * the filed keys is a bound at least as high, and the pass is run again with it, and
+ * with a sample filed where that leaves out too few.  The segment passes through LDS in
  * blocks of 16 KiB; one that is a single block is not loaded again.  The join
  * of the segments bounds their keys the same way and ranks what reaches it.
  *
@@ -328,8 +329,8 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
 #pragma unroll
     for (int w = 1; w < SW; w++) t = min(t, L.least[w]);
     uint64_t bound = (uint64_t)t << 32;
-    uint32_t n = 0u;
-    while (live) { /* every thread of the workgroup agrees on `live` and n */
+    uint32_t n = 0u, shift = 0u, before = ~0u; /* of those that reach, every 2^shift-th to arrive is filed */
+    while (live) { /* every thread of the workgroup agrees on `live`, n and shift */
       const float least = (bound >> 32) ? d3s_from_ordkey((uint32_t)(bound >> 32)) : -__builtin_inff();
       for (int at = lo; at < hi; at += SU * ST) {
         if (hi - lo > SU * ST) fetch(at);
@@ -350,19 +351,31 @@ __global__ __launch_bounds__(ST) void k_score(ScoreArgs a, int nseg, int seg_chu
           if (j == R.banned) x = -__builtin_inff();
           const uint64_t key = composite_key(x, j);
           if (key >= bound && j >= 0 && j < a.vocab) {
-            const uint32_t place = atomicAdd(&L.count, 1u);
-            if (place < LIST) L.list[place] = key;
+            const uint32_t place = atomicAdd(&L.count, 1u), slot = place >> shift;
+            if (slot << shift == place && slot < LIST) L.list[slot] = key;
           }
         }
       }
       __syncthreads();
       n = L.count;
       __syncthreads();
-      if (n <= LIST) break;
+      if (n <= LIST && shift == 0u) break;
       /* at least k of the filed keys reach their k-th: none below it is among the best k */
-      rank_list(L, L.list, LIST, k);
+      const uint32_t filed = min((uint32_t)LIST, ((n - 1u) >> shift) + 1u);
+      rank_list(L, L.list, filed, k);
       if (tid == 0) L.count = 0u;
-      bound = L.ranked[k - 1];
+      if (filed >= (uint32_t)k) bound = L.ranked[k - 1];
+      /* The first to arrive are a good sample of rows in no order, the best of ties, and
+       * the least of a rising row, 448 a pass: where they did not leave out half, every
+       * 2^shift-th of all n is filed, which leaves about k << shift. */
+      if (shift > 0u && filed >= (uint32_t)k) {
+        shift -= min(shift, 31u - __clz(LIST / 2 / k));
+      } else if (shift > 0u) { /* (fewer were left) */
+        shift = n <= LIST ? 0u : 32u - __clz(n / LIST);
+      } else {
+        shift = n <= before / 2u ? 0u : 32u - __clz(n / LIST);
+        before = n;
+      }
       __syncthreads();
     }
     rank_list(L, L.list, n, k);

@@ -62,3 +62,44 @@ def test_temperatures_that_are_not_finite(gpu, V, dtype, per_row):
     for r in range(n):
         one = {k: v[r:r + 1] for k, v in ref.items()}
         S.check(S.run(gpu, bits[r:r + 1], T[r], None, tokens[r:r + 1], 3), one)
+
+
+def flat_rows(n, V, order):
+    """rows whose logits share their upper 16 bits, each value a few times"""
+    row = np.float32(1) + (np.arange(V) // (V // 65536 + 1)).astype(np.float32) * np.float32(2.0 ** -23)
+    row = row[::-1] if order == "falling" else np.random.default_rng(13).permutation(row) if order == "mixed" else row
+    return np.ascontiguousarray(np.broadcast_to(row, (n, V)))
+
+
+@pytest.mark.parametrize("top", [1, 20, 64])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("n,V", [(2, 60000), (700, 30011), (1100, 9001)])
+def test_alternatives_of_rows_that_rise_a_little(gpu, n, V, order, top):
+    l = flat_rows(n, V, order)
+    tokens = np.zeros((n, 1), np.int64)
+    S.check(S.run(gpu, l, 1.0, None, tokens, top), R.score(l.astype(np.float64), np.ones(n), None, tokens, top))
+
+
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_passes_over_rows_that_rise_a_little(gpu, top):
+    """the segment's passes for its alternatives are few whatever its order: rising rows
+    take the time of falling ones, whose first pass files the best, a few times over
+    (each pass that files the first of those that reach leaves out 448 elements of
+    131072 at most, 292 passes)"""
+    import time
+
+    import hiprt
+    n, V = 600, 131072
+    times = {}
+    with R.Arena() as D:
+        tok, lp, ids = D.put(np.zeros((n, 1), np.int32)), D.room(4 * n), D.room(4 * n * top)
+        for order in ("falling", "rising"):
+            lg = D.put(flat_rows(n, V, order))
+            for _ in range(4):
+                hiprt.synchronize()
+                start = time.perf_counter()
+                assert gpu.logprob_raw(lg.ptr, gpu.DTYPE_F32, n, V, V, 1.0, None, tok.ptr, 1, lp.ptr, None, None, top,
+                                       ids.ptr) == 0
+                hiprt.synchronize()
+                times[order] = min(times.get(order, 1e9), time.perf_counter() - start)
+    assert times["rising"] < 12 * times["falling"], times
