@@ -103,3 +103,42 @@ def test_passes_over_rows_that_rise_a_little(gpu, top):
                 hiprt.synchronize()
                 times[order] = min(times.get(order, 1e9), time.perf_counter() - start)
     assert times["rising"] < 12 * times["falling"], times
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_more_rows_than_a_launch(gpu, dtype):
+    """2^22 workgroups a launch, one a row: the second launch's rows, tokens,
+    temperatures, statistics, alternatives and gradients"""
+    import hiprt
+    n, V = (1 << 22) + 5, 3
+    rng = np.random.default_rng(16)
+    code = gpu.DTYPE_F32 if dtype == "f32" else gpu.DTYPE_BF16
+    bits, l = R.to_bits(rng.standard_normal((n, V)).astype(np.float32), dtype)
+    T = rng.uniform(0.5, 1.5, n).astype(np.float32)
+    tokens, banned = rng.integers(0, V, (n, 1)), rng.integers(-1, V, n)
+    g, gH = rng.standard_normal((n, 1)).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    with R.Arena() as D:
+        lg, tok, temp, ban = D.put(bits), D.put(tokens.astype(np.int32)), D.put(T), D.put(banned.astype(np.int32))
+        lp, ent, st = D.room(4 * n, 0xee), D.room(4 * n, 0xee), D.room(8 * n, 0xee)
+        ids, tlp, grad = D.room(8 * n, 0xee), D.room(8 * n, 0xee), D.room(bits.nbytes, 0xee)
+        assert gpu.logprob_raw(lg.ptr, code, n, V, V, ("ptr", temp.ptr), ban.ptr, tok.ptr, 1, lp.ptr, ent.ptr, st.ptr, 2,
+                               ids.ptr, tlp.ptr) == 0
+        assert gpu.logprob_backward_raw(lg.ptr, code, n, V, V, ("ptr", temp.ptr), ban.ptr, tok.ptr, 1, st.ptr, ent.ptr,
+                                        D.put(g).ptr, D.put(gH).ptr, grad.ptr, V) == 0
+        hiprt.synchronize()
+        got = dict(logprobs=lp.download((n, 1), np.float32), H=ent.download((n,), np.float32),
+                   stats=st.download((n, 2), np.float32), top_ids=ids.download((n, 2), np.int32),
+                   top_logprobs=tlp.download((n, 2), np.float32), counters=np.zeros(4, np.uint32))
+        dl = grad.download((n, V), bits.dtype)
+    # whole, coarsely: no row is another's
+    x = np.where(np.arange(V) == banned[:, None], -np.inf, l) / T[:, None]
+    x -= x.max(1, keepdims=True)
+    logp = x - np.log(np.exp(x).sum(1, keepdims=True))
+    R.assert_near(got["logprobs"], np.take_along_axis(logp, tokens, 1), 1e-4)
+    # on both sides of the launches' border, and here and there
+    at = np.unique(np.concatenate([np.arange(300), np.arange(n - 300, n), rng.integers(0, n, 2000)]))
+    ref = R.score(l[at], T[at].astype(np.float64), banned[at], tokens[at], 2)
+    S.check({k: v if k == "counters" else v[at] for k, v in got.items()}, ref)
+    dx, err = R.score_grad(ref, tokens[at], g[at].astype(np.float64), gH[at])
+    # (from the kernel's own fp32 statistics: their roundings move every p alike)
+    S.check_grad(dl[at], dx, 2 * err)
