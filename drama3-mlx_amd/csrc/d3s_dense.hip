@@ -114,7 +114,8 @@ Plan plan(const Product &p) {
       pl.tile_m = m, pl.tile_n = n;
       t.tm = tm, t.tn = tn, t.splits = (unsigned)splits;
     };
-    offer(256, 256, 1);
+    /* (256 x 256 turns eight rows at a time) */
+    if (!(p.x_turned && m < 8) && !(p.w_turned && n < 8)) offer(256, 256, 1);
     offer(128, 256, 1);
     /* (every split has its stages, and fewer workgroups than twice the CUs) */
     for (int s = 1; s <= 8; s++)

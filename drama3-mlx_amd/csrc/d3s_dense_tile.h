@@ -47,7 +47,8 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 /* how an operand's stages reach LDS, and how they lie there (above) */
 enum Way { DIRECT, ROWS, TURNED, INNER };
 
-/* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED, INNER: stored [k, rows]). */
+/* One operand's part of a tile: R rows from r0 of [rows, k] (TURNED, INNER: stored [k, rows];
+ * TURNED: eight rows at least). */
 template <int R, Way WAY, int SETS>
 struct Part {
   static constexpr int BYTES = R * TK * 2;
@@ -86,9 +87,8 @@ struct Part {
 #pragma unroll
       for (int u = 0; u < PER; u++) off[u] = (uint32_t)(min(row(u), rows - 1 - r0) * stride + chunk(u) * 8) * 2u;
     } else if constexpr (WAY == TURNED) {
-      /* eight rows that end with the last (written twice, the same), where there are eight */
-      to = tid() % (R / 8) * 8;
-      if (rows >= 8) to = min(to, rows - 8 - r0);
+      /* eight rows that end with the last (written twice, the same) */
+      to = min(tid() % (R / 8) * 8, rows - 8 - r0);
       mine = p + (int64_t)inner() * stride + (r0 + to);
     } else if constexpr (WAY == INNER) {
       /* (chunks past the rows are the last one again; one that is cut reads on into
@@ -110,7 +110,7 @@ struct Part {
     const bool cut = WAY == INNER && r0 + R > rows && rows % 8 != 0;
     return cut ? max(k - (stride >= 8 ? 1 : 8), 0) : k;
   }
-  /* the same into registers, from start(k0): a whole stage, at least eight rows if TURNED */
+  /* the same into registers, from start(k0): a whole stage */
   __device__ __forceinline__ const uint16_t *start(int k0) const {
     return WAY == TURNED || WAY == INNER ? mine + (int64_t)k0 * stride : p + k0;
   }
@@ -125,11 +125,7 @@ struct Part {
 #pragma unroll
     for (int u = 0; u < PER; u++) {
       if constexpr (WAY == TURNED) {
-        const uint16_t *at = p + (int64_t)min(k0 + inner() + u, k1 - 1) * stride;
-        if (rows >= 8)
-          q[0][u] = load16(at + (r0 + to));
-        else
-          q[0][u] = r0 + to < rows ? row_chunk(at, r0 + to, rows) : make_uint4(0u, 0u, 0u, 0u);
+        q[0][u] = load16(p + (int64_t)min(k0 + inner() + u, k1 - 1) * stride + (r0 + to));
       } else if constexpr (WAY == INNER) {
         q[0][u] = row_chunk(p + (int64_t)min(k0 + inner(u), k1 - 1) * stride, r0 + to, rows);
       } else {
@@ -295,9 +291,7 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
   static_assert(LATE % 2 == 0, "two steps' shares");
   constexpr int WRITTEN = DIRECTS > 0 && HALF > 0 ? HALF : PRODUCTS;
 
-  /* TURNED operands of fewer than eight rows have no whole loads */
-  const int full = (WX == TURNED && o.m < 8) || (WW == TURNED && o.n < 8) ? s0 : s1;
-  if (s0 < full) {
+  if (s0 < s1) {
     auto k_of = [&](int s) { return min(s, s1 - 1) * TK; }; /* (loads past the end: the last stage's, not read) */
 #pragma unroll
     for (int b = 0; b < BUFS; b++) {
@@ -353,7 +347,7 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
   }
   /* the rest of the inner length, what whole loads do not reach: zeros from its end on */
   const int end = split == pl.splits - 1 ? a.k : s1 * TK;
-  for (int k0 = full * TK; k0 < end; k0 += TK) {
+  for (int k0 = s1 * TK; k0 < end; k0 += TK) {
     px.load_some(k0, end);
     pw.load_some(k0, end);
     stage_barrier<0>();

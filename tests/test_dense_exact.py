@@ -131,3 +131,38 @@ def test_one_row_in_place_has_no_stride(gpu):
         hiprt.synchronize()
         assert np.array_equal(y.download((n,), np.float32), r + (x @ w.T)[0])
         assert np.array_equal(dy.download((n,), np.uint16), gb[0])
+
+
+@pytest.mark.parametrize("n", [1, 5, 7, 8, 9])
+def test_very_few_outputs_by_the_inner_index(gpu, n):
+    """so many rows that large tiles pay, outputs fewer than what those turn at a time"""
+    product(gpu, 57344, n, 1024, False, True)
+    product(gpu, 50000, n, 1090, False, True, added=True)
+
+
+def test_the_time_of_very_few_outputs(gpu):
+    """five outputs by the inner index take no longer than eight, a few per cent aside (they took 3.3 times
+    as long in tiles whose loads are made for eight)"""
+    import ctypes
+
+    import hiprt
+    m, k = 57344, 8192
+    H = hiprt.hip()
+    start, stop = ctypes.c_void_p(), ctypes.c_void_p()
+    hiprt.check(H.hipEventCreate(ctypes.byref(start)))
+    hiprt.check(H.hipEventCreate(ctypes.byref(stop)))
+    times = {}
+    with R.Arena() as D:
+        x, w, y = D.room(2 * m * k, 0), D.room(2 * 8 * k, 0), D.room(4 * 8 * m)
+        for n in (5, 8):
+            for _ in range(4):
+                hiprt.check(H.hipEventRecord(start, None))
+                assert gpu.dense_raw(x.ptr, k, w.ptr, n, m, n, k, y.ptr, n, gpu.DTYPE_F32, w_transposed=True) == 0
+                hiprt.check(H.hipEventRecord(stop, None))
+                hiprt.synchronize()
+                ms = ctypes.c_float()
+                hiprt.check(H.hipEventElapsedTime(ctypes.byref(ms), start, stop))
+                times[n] = min(times.get(n, 1e9), ms.value)
+    H.hipEventDestroy(start)
+    H.hipEventDestroy(stop)
+    assert times[5] < 1.7 * times[8], times
