@@ -102,6 +102,20 @@ def test_more_outputs_than_a_launch_of_few_rows(gpu):
     product(gpu, 1, (1 << 24) + 21, 8)
 
 
+@pytest.mark.parametrize("xt", [False, True])
+def test_more_tiles_than_a_launch(gpu, xt):
+    """128 rows a tile, 2^22 tiles a launch: the second launch's rows"""
+    import hiprt
+    m = (1 << 29) + 300
+    i = np.random.default_rng(17).integers(0, 5, m, np.uint8)
+    with R.Arena() as D:
+        y = D.room(4 * m, 0xee)
+        assert gpu.dense_raw(D.put(BITS[i]).ptr, m if xt else 1, D.put(BITS[4:]).ptr, 1, m, 1, 1, y.ptr, 1, gpu.DTYPE_F32,
+                             x_transposed=xt) == 0
+        hiprt.synchronize()
+        assert np.array_equal(y.download((m,), np.float32), (2 * VALUES)[i])
+
+
 def test_more_columns_than_a_launch_of_sums(gpu):
     """the bias gradient of 2^26 columns and 37: 16 a workgroup, 2^22 workgroups a launch"""
     import hiprt
