@@ -42,7 +42,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 #define D3S_LDS __attribute__((address_space(3)))
-#define D3S_GLOBAL __attribute__((address_space(1)))
 
 /* how an operand's stages reach LDS, and how they lie there (above) */
 enum Way { DIRECT, ROWS, TURNED, INNER };
@@ -139,22 +138,16 @@ struct Part {
   __device__ __forceinline__ void write(int set, int v, char *lds, char *spare) const {
     if constexpr (WAY != TURNED) {
       *(uint4 *)(lds + (v * TT + tid()) * 16) = q[set][v];
-    } else if constexpr (WAY == TURNED) {
-      uint32_t w[PER > 1 ? PER / 2 : 1];
+    } else {
+      static_assert(PER == 8, "a row's eight inner indices are one chunk");
+      uint32_t w[4];
       auto word = [&](int u) { return v < 2 ? q[set][u].x : v < 4 ? q[set][u].y : v < 6 ? q[set][u].z : q[set][u].w; };
 #pragma unroll
-      for (int u = 0; u + 1 < PER; u += 2)
+      for (int u = 0; u < 8; u += 2)
         w[u / 2] = __builtin_amdgcn_perm(word(u + 1), word(u), v & 1 ? 0x07060302u : 0x05040100u);
       const int r = to + v, k = inner();
-      char *at = r < 0 ? spare : lds + (r * (TK * 2) + (k / 8 ^ turn(r)) * 16 + k % 8 * 2);
-      if constexpr (PER == 8)
-        *(uint4 *)at = make_uint4(w[0], w[1], w[2], w[3]);
-      else if constexpr (PER == 4)
-        *(uint2 *)at = make_uint2(w[0], w[1]);
-      else if constexpr (PER == 2)
-        *(uint32_t *)at = w[0];
-      else
-        *(uint16_t *)at = (uint16_t)(word(0) >> (16 * (v & 1)));
+      char *at = r < 0 ? spare : lds + (r * (TK * 2) + (k / 8 ^ turn(r)) * 16);
+      *(uint4 *)at = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   __device__ __forceinline__ void write_all(char *lds, char *spare) const {
@@ -204,6 +197,7 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
   __shared__ __attribute__((aligned(1024))) char lds[ROOM + 16];
   char *spare = lds + ROOM;
   static_assert(WX == DIRECT && WW == DIRECT ? AHEAD == 0 : BUFS == 2, "what the waits below count");
+  static_assert(SETS <= 2, "the loop over stages takes two at a time");
 
   /* workgroups go to the eight XCDs in turn: each takes a run of neighbouring
    * tiles, in columns of eight, whose operands its L2 then holds */
@@ -339,10 +333,6 @@ __global__ __launch_bounds__(TT, 1) void k_tile(Operands a, Out o, TilePlan pl) 
       stage(s, std::integral_constant<int, 0>{});
       if constexpr (SETS > 1)
         if (s + 1 < s1) stage(s + 1, std::integral_constant<int, 1 % SETS>{});
-      if constexpr (SETS > 2)
-        if (s + 2 < s1) stage(s + 2, std::integral_constant<int, 2 % SETS>{});
-      if constexpr (SETS > 3)
-        if (s + 3 < s1) stage(s + 3, std::integral_constant<int, 3 % SETS>{});
     }
   }
   /* the rest of the inner length, what whole loads do not reach: zeros from its end on */
