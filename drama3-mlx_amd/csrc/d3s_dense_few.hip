@@ -224,20 +224,18 @@ void few_launch(const Operands &a, const Out &o, const FewPlan &pl, hipStream_t 
 template <bool XT, bool WT>
 void few_rows(const Operands &a, const Out &o, bool swap, const FewPlan &pl, hipStream_t s) {
   const int rows = (swap ? o.n : o.m) - pl.i0;
-  if (swap)
-    rows <= 16 ? few_launch<1, XT, WT, true>(a, o, pl, s) : few_launch<2, XT, WT, true>(a, o, pl, s);
-  else if (rows <= 16)
-    few_launch<1, XT, WT, false>(a, o, pl, s);
-  else if (rows <= 32)
-    few_launch<2, XT, WT, false>(a, o, pl, s);
-  else
-    few_launch<4, XT, WT, false>(a, o, pl, s);
+  if (swap) return rows <= 16 ? few_launch<1, XT, WT, true>(a, o, pl, s) : few_launch<2, XT, WT, true>(a, o, pl, s);
+  if (rows <= 16) return few_launch<1, XT, WT, false>(a, o, pl, s);
+  if constexpr (!WT) { /* (33 rows and more: weights by rows only) */
+    if (rows > 32) return few_launch<4, XT, WT, false>(a, o, pl, s);
+  }
+  few_launch<2, XT, WT, false>(a, o, pl, s);
 }
 
 }  // namespace
 
 int few_outputs(bool w_transposed) { return w_transposed ? Shape<true>::OUTPUTS : Shape<false>::OUTPUTS; }
-int few_batch(bool w_transposed) { return w_transposed ? 32 : 128; }
+int few_batch(bool w_transposed) { return 32 * (w_transposed ? Shape<true>::STEPS : Shape<false>::STEPS); }
 int few_waves(bool w_transposed) { return w_transposed ? Shape<true>::WAVES : Shape<false>::WAVES; }
 size_t few_part_bytes(bool w_transposed, int rows) {
   const size_t fr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
