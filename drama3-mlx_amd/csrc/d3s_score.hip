@@ -88,12 +88,6 @@ __device__ __forceinline__ void join(Sums &a, float m, float S, float A, float c
   a.m = M;
 }
 
-template <int CTRL, int ROWM>
-__device__ __forceinline__ void join_dpp(Sums &a, float c) {
-  const float m = dpp_f<CTRL, ROWM>(-FLT_MAX, a.m), S = dpp_f<CTRL, ROWM>(0.0f, a.S), A = dpp_f<CTRL, ROWM>(0.0f, a.A);
-  join(a, m, S, A, c);
-}
-
 /* the whole wave's, in every lane */
 __device__ __forceinline__ void join_wave(Sums &a, float c) {
   const float M = wave_max_f(a.m);
