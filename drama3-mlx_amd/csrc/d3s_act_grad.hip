@@ -40,10 +40,9 @@ Split split_of(int64_t m, int64_t n) {
 }
 
 template <bool SUM, int ACT>
-__global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *parts, int block0) {
+__global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *parts) {
   __shared__ float sum[SUM ? AT * 8 : 1];
-  const int block = block0 + (int)blockIdx.x;
-  const int strip = block % s.strips, run = block / s.strips;
+  const int strip = (int)blockIdx.x % s.strips, run = (int)blockIdx.x / s.strips;
   const int across = (int)threadIdx.x % s.lanes, down = (int)threadIdx.x / s.lanes, at_once = AT / s.lanes;
   const int64_t j = ((int64_t)strip * s.lanes + across) * 8;
   const int64_t end = min((int64_t)a.m, (int64_t)(run + 1) * s.rows);
@@ -120,14 +119,14 @@ size_t act_grad_workspace_bytes(int64_t m, int64_t n, bool dbias) {
 void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s) {
   const Split sp = split_of(a.m, a.n);
   float *parts = ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
-  const int64_t blocks = (int64_t)sp.strips * sp.runs;
-  for (int64_t b = 0; b < blocks; b += GRID_MOST) {
-    const dim3 grid((unsigned)min((int64_t)GRID_MOST, blocks - b));
-    auto go = [&](auto kernel) { kernel<<<grid, AT, 0, s>>>(a, sp, parts, (int)b); };
-    auto pick = [&](auto act) {
-      constexpr int ACT = decltype(act)::value;
-      a.dbias ? go(k_act_grad<true, ACT>) : go(k_act_grad<false, ACT>);
-    };
+  /* at most 2048 workgroups, or a strip of 512 columns each: 2^22 */
+  const unsigned blocks = (unsigned)sp.strips * (unsigned)sp.runs;
+  auto go = [&](auto kernel) { kernel<<<dim3(blocks), AT, 0, s>>>(a, sp, parts); };
+  auto pick = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    a.dbias ? go(k_act_grad<true, ACT>) : go(k_act_grad<false, ACT>);
+  };
+  if (blocks) {
     switch (a.act) {
       case D3S_ACT_RELU: pick(std::integral_constant<int, D3S_ACT_RELU>{}); break;
       case D3S_ACT_SILU: pick(std::integral_constant<int, D3S_ACT_SILU>{}); break;
@@ -138,7 +137,7 @@ void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s) {
   }
   if (!a.dbias) return;
   const int64_t groups = ((int64_t)a.n + 15) / 16;
-  /* (at most 2^27 workgroups: 2^35 threads would pass the launch's count) */
+  /* (up to 2^27 workgroups: 2^35 threads would pass the launch's count) */
   for (int64_t g = 0; g < groups; g += GRID_MOST)
     k_column_sums<<<dim3((unsigned)min((int64_t)GRID_MOST, groups - g)), AT, 0, s>>>(
         parts, sp.runs, a.n, (int)g, a.dbias);
