@@ -350,7 +350,7 @@ struct Walk {
  * elements in 260 tensors 14.3 us, 18.6 with a launch for every 164 of them, in 1000
  * 39 and 53, in 170 12.7 and 13.5; 8 million bf16 in 214: 20.7 and 21.9).  A tensor of several pieces:
  * launch by launch (the table's room is by the tensors' number). */
-bool tabled(const int64_t *numel, const int32_t *dtypes, int n_tensors, int64_t *units) {
+static bool tabled(const int64_t *numel, const int32_t *dtypes, int n_tensors, int64_t *units) {
   int n = 0;
   *units = 0;
   for (int t = 0; t < n_tensors; t++) {
