@@ -35,9 +35,9 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
  * (8192 x 2048 x 2048, both direct: 63, 78 and 87 us in the three tiles;
  * 2048 x 2048 x 2048: 50, 29 and 22; 4096 x 2048 x 8192, both by the inner
  * index: 217, 160 and 210; 256 x 2048 x 8192: 128 x 128 with 1, 2, 4 and 8
- * splits 49, 31, 22 and 24.)  Between 128 x 256 and 256 x 128 there is little,
- * but rows of x that are not at 4 bytes cost less the fewer tiles load them (heads of
- * 4097 outputs, their weights' gradient: 186 and 205 us). */
+ * splits 49, 31, 22 and 24.)  The middle tile is the wide one: few rows of tiles load
+ * rows of x that are not at 4 bytes less often (heads of 4097 outputs, their weights'
+ * gradient: 186 us, in tiles of 256 x 128 it was 205). */
 double tile_us(const Product &p, int64_t m, int64_t n, int tm, int tn, int splits) {
   const int direct = p.x_direct + p.w_direct;
   const double wgs = (double)up(m, tm) * (double)up(n, tn) * splits;
@@ -80,7 +80,7 @@ FewPlan few_plan(int64_t i0, int64_t few, int64_t many, int64_t k, bool turned) 
   const int64_t batches = up(k, few_batch(turned));
   int64_t most = batches / (few_waves(turned) * (few > 32 ? 1 : 2)), want = CUS / (int64_t)f.tiles;
   if (want < most) most = want;
-  if (most > 16) most = 16;
+  if (most > 16) most = 16; /* (32 splits of turned weights, 34 MB of them: 19.6 us, sixteen 15.4) */
   f.splits = most > 1 ? (unsigned)most : 1u;
   f.batches = (int)up(batches, f.splits);
   return f;
@@ -117,7 +117,10 @@ Plan plan(const Product &p) {
     /* (256 x 256 turns eight rows at a time) */
     if (!(p.x_turned && m < 8) && !(p.w_turned && n < 8)) offer(256, 256, 1);
     offer(128, 256, 1);
-    /* (every split has its stages, and fewer workgroups than twice the CUs) */
+    /* (Every split has its stages, and fewer workgroups than twice the CUs.  Eight at
+     * most: the last to arrive reads every split's sums, so by the costs above more
+     * only pay past an inner length of 8192; 256 x 256 x 16384, both by the inner
+     * index, 32 us and with sixteen 29, 256 x 256 x 8192 23 either way.) */
     for (int s = 1; s <= 8; s++)
       if (s == 1 || (p.k >= (int64_t)4 * s * TILE_K && up(m, 128) * up(n, 128) * s <= 2 * CUS)) offer(128, 128, s);
   }

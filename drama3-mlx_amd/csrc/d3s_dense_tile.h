@@ -18,10 +18,10 @@
  * is stored by the inner index, [inner][row], to be read transposed.
  *
  * Bound: the matrix pipe, as far as LDS reads and the loads' issue leave it busy: 35 (both
- * operands by the inner index) to 51 % of a call.  8192 x 2048 x 2048 64 us
- * (1050 TFLOP/s; with every part of the epilogue 79), 8192 x 8192 x 8192 840 to
- * 890 us (1270 TFLOP/s), 4096 x 2048 x 8192 with both by the inner index 154 us
- * (890 TFLOP/s). */
+ * operands by the inner index) to 51 % of a call.  On operands that are used again:
+ * 8192 x 2048 x 2048 59 us (1160 TFLOP/s; from cold operands with every part of the
+ * epilogue 77), 8192 x 8192 x 8192 805 us (1370 TFLOP/s), 8192 x 4097 x 2048 128 us (1070),
+ * 4096 x 2048 x 8192 with both by the inner index 152 us (900 TFLOP/s). */
 #ifndef D3S_DENSE_TILE_H
 #define D3S_DENSE_TILE_H
 

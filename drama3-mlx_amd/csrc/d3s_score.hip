@@ -33,7 +33,8 @@
  * one streaming pass, rows cut into segments that share nothing, stores past the
  * caches (through them: 2 to 20 % slower).
  *
- * Bound: long rows HBM (bf16 [4096, 151936]: 219 us, 5.7 TB/s; the gradient of
+ * Bound: long rows HBM (bf16 [4096, 151936]: 219 us, 5.7 TB/s; fp32 [2048, 151936]
+ * 212 us, 5.9 TB/s; the gradient of fp32 [1024, 151936] 233 us, 5.3 TB/s, and of bf16
  * [2048, 151936] 229 us, 5.4 TB/s; of fp32 [4096, 4097] 25 us, 5.3 TB/s); few
  * rows the chain of dependent steps (bf16 [1, 4097] with five alternatives 6.7 us;
  * [64, 151936] with twenty 18.3 us, of which the bytes are 4). */
