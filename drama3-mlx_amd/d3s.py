@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "libd3sampler.so")
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_E4M3 = 2  # outputs of rms_norm_raw only
 FLAG_GENERIC = 1
 FLAG_EXACT_LSE = 2
 FLAG_EXACT_SELECT = 4
@@ -30,6 +31,9 @@ SCRATCH_BYTES = 4 << 20
 MAX_VOCAB = (1 << 24) - 1
 MAX_TOKENS = 64
 MAX_TOP = 64
+MAX_DRAFT = 64
+MAX_RANKED = 1024
+MAX_IDS = 64
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # D3S_ACT_*
 
 _lib = None
@@ -52,6 +56,18 @@ class DenseParams(ctypes.Structure):
                 ("activation", ctypes.c_int), ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
                 ("z", ctypes.c_void_p), ("z_stride", ctypes.c_int64), ("y", ctypes.c_void_p),
                 ("y_stride", ctypes.c_int64), ("y_dtype", ctypes.c_int)]
+
+
+class VerifyParams(ctypes.Structure):
+    """d3s_verify_params (include/d3s_step.h)"""
+    _fields_ = [("target", ctypes.c_void_p), ("target_dtype", ctypes.c_int), ("target_stride", ctypes.c_int64),
+                ("draft", ctypes.c_void_p), ("draft_dtype", ctypes.c_int), ("draft_stride", ctypes.c_int64),
+                ("n_seqs", ctypes.c_int64), ("n_draft", ctypes.c_int), ("vocab", ctypes.c_int64),
+                ("drafted", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("temperature", ctypes.c_void_p),
+                ("temperature_scalar", ctypes.c_float), ("draft_temperature", ctypes.c_void_p),
+                ("draft_temperature_scalar", ctypes.c_float), ("u_accept", ctypes.c_void_p), ("u_draw", ctypes.c_void_p),
+                ("tokens", ctypes.c_void_p), ("n_accepted", ctypes.c_void_p), ("accept", ctypes.c_void_p),
+                ("counters", ctypes.c_void_p)]
 
 
 def ras_params(**kw):
@@ -143,6 +159,30 @@ def lib():
             f.restype = i32
         for f in (L.d3s_logprob_workspace_bytes, L.d3s_dense_workspace_bytes,
                   L.d3s_dense_activation_backward_workspace_bytes, L.d3s_clip_grads_workspace_bytes):
+            f.restype = i64
+        verify = ctypes.POINTER(VerifyParams)
+        u64 = ctypes.c_uint64
+        L.d3s_verify.argtypes = [verify, vp]
+        L.d3s_verify_ws.argtypes = [verify, vp, i64, vp]
+        L.d3s_verify_workspace_bytes.argtypes = [verify]
+        L.d3s_verify_ranked.argtypes = [vp, vp, i32, vp, vp, i32, i64, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+        L.d3s_embed.argtypes = [vp, i64, i32, vp, i32, i64, i64, i64, i64, f32, vp, i32, i64, vp]
+        embed = [vp, i64, i32, vp, i32, i64, i64, i64, i64, f32, i32, vp, i32, i64]
+        L.d3s_embed_backward.argtypes = embed + [vp]
+        L.d3s_embed_backward_ws.argtypes = embed + [vp, i64, vp]
+        L.d3s_embed_backward_workspace_bytes.argtypes = [i64, i32, i64, i64, i64]
+        L.d3s_rms_norm.argtypes = [vp, i32, i64, vp, i64, vp, i64, vp, f32, i64, i64, vp, i32, i64, i32, vp, vp, vp]
+        norm = [vp, i32, i64, vp, i64, vp, vp, vp, i64, i64, i64, vp, i64, vp]
+        L.d3s_rms_norm_backward.argtypes = norm + [vp]
+        L.d3s_rms_norm_backward_ws.argtypes = norm + [vp, i64, vp]
+        L.d3s_rms_norm_backward_workspace_bytes.argtypes = [i64, i64, i32]
+        L.d3s_dropout.argtypes = [vp, i32, i64, vp, i64, i64, i64, f32, u64, u64, vp, vp, i64, vp]
+        for f in (L.d3s_verify, L.d3s_verify_ws, L.d3s_verify_ranked, L.d3s_embed, L.d3s_embed_backward,
+                  L.d3s_embed_backward_ws, L.d3s_rms_norm, L.d3s_rms_norm_backward, L.d3s_rms_norm_backward_ws,
+                  L.d3s_dropout):
+            f.restype = i32
+        for f in (L.d3s_verify_workspace_bytes, L.d3s_embed_backward_workspace_bytes,
+                  L.d3s_rms_norm_backward_workspace_bytes):
             f.restype = i64
         L.d3s_version.argtypes = []
         L.d3s_version.restype = ctypes.c_char_p
@@ -514,3 +554,70 @@ def clip_grads_raw(src, dst, numel, dtypes, n_tensors, max_norm, norm, stream=No
     if workspace is not None:
         return lib().d3s_clip_grads_ws(*args, workspace[0], workspace[1], stream)
     return lib().d3s_clip_grads(*args, stream)
+
+
+# ---- between ids and logits (include/d3s_step.h), on device pointers (ints) ----
+def verify_params(target, target_dtype, target_stride, draft, draft_dtype, draft_stride, n_seqs, n_draft, vocab, drafted,
+                  lengths, temperature, draft_temperature, u_accept, u_draw, tokens, n_accepted, accept=None,
+                  counters=None):
+    """VerifyParams; temperatures as in logprob_raw."""
+    t_ptr, t_s = _temperature(temperature)
+    d_ptr, d_s = _temperature(draft_temperature)
+    return VerifyParams(target, target_dtype, target_stride, draft, draft_dtype, draft_stride, n_seqs, n_draft, vocab,
+                        drafted, lengths, t_ptr, t_s, d_ptr, d_s, u_accept, u_draw, tokens, n_accepted, accept, counters)
+
+
+def verify_raw(*args, stream=None, workspace=None, **kw):
+    """d3s_verify, or d3s_verify_ws with workspace = (address, bytes); the other
+    arguments are verify_params'."""
+    p = verify_params(*args, **kw)
+    if workspace is not None:
+        return lib().d3s_verify_ws(ctypes.byref(p), workspace[0], workspace[1], stream)
+    return lib().d3s_verify(ctypes.byref(p), stream)
+
+
+def verify_ranked_raw(target_cand, target_probs, target_k, draft_cand, draft_probs, draft_k, n_seqs, n_draft, drafted,
+                      lengths, u_accept, u_draw, tokens, n_accepted, accept=None, counters=None, stream=None):
+    """d3s_verify_ranked."""
+    return lib().d3s_verify_ranked(target_cand, target_probs, target_k, draft_cand, draft_probs, draft_k, n_seqs, n_draft,
+                                   drafted, lengths, u_accept, u_draw, tokens, n_accepted, accept, counters, stream)
+
+
+def embed_raw(ids, n_rows, n_ids, table, dtype, table_stride, vocab, slot_rows, width, scale, y, y_dtype, y_stride,
+              stream=None):
+    """d3s_embed: y[r] = scale * the sum of the ids' rows of the table."""
+    return lib().d3s_embed(ids, n_rows, n_ids, table, dtype, table_stride, vocab, slot_rows, width, scale, y, y_dtype,
+                           y_stride, stream)
+
+
+def embed_backward_raw(ids, n_rows, n_ids, dy, dtype, dy_stride, vocab, slot_rows, width, scale, accumulate, grad,
+                       grad_dtype, grad_stride, stream=None, workspace=None):
+    """d3s_embed_backward, or its _ws form with workspace = (address, bytes)."""
+    args = (ids, n_rows, n_ids, dy, dtype, dy_stride, vocab, slot_rows, width, scale, accumulate, grad, grad_dtype,
+            grad_stride)
+    if workspace is not None:
+        return lib().d3s_embed_backward_ws(*args, workspace[0], workspace[1], stream)
+    return lib().d3s_embed_backward(*args, stream)
+
+
+def rms_norm_raw(x, dtype, x_stride, residual, residual_stride, sum, sum_stride, gain, eps, n_rows, width, y, y_dtype,
+                 y_stride, group=0, scales=None, rstd=None, stream=None):
+    """d3s_rms_norm."""
+    return lib().d3s_rms_norm(x, dtype, x_stride, residual, residual_stride, sum, sum_stride, gain, eps, n_rows, width, y,
+                              y_dtype, y_stride, group, scales, rstd, stream)
+
+
+def rms_norm_backward_raw(dy, dtype, dy_stride, h, h_stride, gain, rstd, dsum, dsum_stride, n_rows, width, dx, dx_stride,
+                          dgain, stream=None, workspace=None):
+    """d3s_rms_norm_backward, or its _ws form with workspace = (address, bytes)."""
+    args = (dy, dtype, dy_stride, h, h_stride, gain, rstd, dsum, dsum_stride, n_rows, width, dx, dx_stride, dgain)
+    if workspace is not None:
+        return lib().d3s_rms_norm_backward_ws(*args, workspace[0], workspace[1], stream)
+    return lib().d3s_rms_norm_backward(*args, stream)
+
+
+def dropout_raw(x, dtype, x_stride, residual, residual_stride, n_rows, width, p, seed, draw, draw_add, y, y_stride,
+                stream=None):
+    """d3s_dropout; its own gradient with x = dy and no residual."""
+    return lib().d3s_dropout(x, dtype, x_stride, residual, residual_stride, n_rows, width, p, seed, draw, draw_add, y,
+                             y_stride, stream)
