@@ -8,13 +8,13 @@
  * depend on which workgroup ends first.  Bound: HBM (two reads, one
  * write): 8192 x 2048 with silu and the sums 18 to 20 us (5.3 TB/s) and 3.9 of the second
  * launch; dz goes past the caches (through them 22.5 in all, so 21). */
+#include "d3s_colsums.h"
 #include "d3s_epilogue.h"
 
 namespace d3s {
 namespace {
 
 constexpr int AT = 256;
-constexpr int GRID_MOST = 1 << 22;
 
 struct Split {
   int lanes, strips; /* lanes across, strips of 8 * lanes columns */
@@ -89,26 +89,6 @@ __global__ __launch_bounds__(AT) void k_act_grad(ActGradArgs a, Split s, float *
   }
 }
 
-/* 16 columns a workgroup, 16 threads a column, each a sixteenth of the runs */
-__global__ __launch_bounds__(AT) void k_column_sums(const float *parts, int runs, int n, int group0, float *dbias) {
-  __shared__ float sum[16][17];
-  const int c = (int)threadIdx.x % 16, q = (int)threadIdx.x / 16;
-  const int64_t col = ((int64_t)group0 + blockIdx.x) * 16 + c;
-  const int per = (runs + 15) / 16, r1 = min(runs, (q + 1) * per);
-  float v = 0.0f;
-  if (col < n) {
-#pragma unroll 8
-    for (int r = q * per; r < r1; r++) v += parts[(int64_t)r * n + col];
-  }
-  sum[q][c] = v;
-  __syncthreads();
-  if (q == 0 && col < n) {
-    v = 0.0f;
-    for (int i = 0; i < 16; i++) v += sum[i][c];
-    dbias[col] = v;
-  }
-}
-
 }  // namespace
 
 size_t act_grad_workspace_bytes(int64_t m, int64_t n, bool dbias) {
@@ -136,11 +116,7 @@ void launch_act_grad(const ActGradArgs &a, void *ws, hipStream_t s) {
     }
   }
   if (!a.dbias) return;
-  const int64_t groups = ((int64_t)a.n + 15) / 16;
-  /* (up to 2^27 workgroups: 2^35 threads would pass the launch's count) */
-  for (int64_t g = 0; g < groups; g += GRID_MOST)
-    k_column_sums<<<dim3((unsigned)min((int64_t)GRID_MOST, groups - g)), AT, 0, s>>>(
-        parts, sp.runs, a.n, (int)g, a.dbias);
+  launch_column_sums(parts, sp.runs, a.n, a.dbias, s);
 }
 
 }  // namespace d3s

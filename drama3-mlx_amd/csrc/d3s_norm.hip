@@ -1,5 +1,6 @@
 /* k_norm_rows, k_norm_grad_rows: root-mean-square norm with the residual's addition
  * and an output in 8 bits, and its gradient (gfx950, wave64; include/d3s_step.h). */
+#include "d3s_colsums.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
 
@@ -32,15 +33,19 @@ __device__ __forceinline__ float block_max(float v, float *part) {
   return t;
 }
 
-/* eight values over their group's greatest, as 8 bits (saturating: a quotient is
- * at most 448 and a rounding) */
+/* eight values over their group's scale, as 8 bits.  By the scale's reciprocal, whose
+ * rounding moves a quotient by 2^-23 of itself where a step is 2^-3, except where it
+ * would overflow; saturating: the greatest quotient is 448 and a rounding. */
 __device__ __forceinline__ uint64_t pack_e4m3(const float *v, float scale) {
   uint32_t w[2] = {0u, 0u};
   float q[8];
+  const float inv = 1.0f / scale;
+  const bool tiny = !(scale >= 0x1p-100f); /* (zero and NaN too) */
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    q[e] = scale > 0.0f ? v[e] / scale : scale == 0.0f ? 0.0f : __builtin_nanf("");
-    if (scale > 0.0f) q[e] = fminf(fmaxf(q[e], -E4M3_MOST), E4M3_MOST);
+    q[e] = v[e] * inv;
+    if (tiny) q[e] = scale > 0.0f ? v[e] / scale : scale == 0.0f ? 0.0f : __builtin_nanf("");
+    q[e] = __builtin_elementwise_minimum(__builtin_elementwise_maximum(q[e], -E4M3_MOST), E4M3_MOST); /* (NaN stays) */
   }
 #pragma unroll
   for (int i = 0; i < 2; i++) {
@@ -54,6 +59,213 @@ __device__ __forceinline__ uint64_t pack_e4m3(const float *v, float scale) {
  * is one too) */
 __device__ __forceinline__ float e4m3_scale(float most) {
   return most < __builtin_inff() ? most / E4M3_MOST : __builtin_nanf("");
+}
+
+/* the sum (or greatest) over the G threads of a row, in each of them, added in one order */
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float *part) {
+  if constexpr (G == NT) return block_sum(v, part);
+  if constexpr (G == WAVE) return readlane_f(wave_scan_add_f32(v), 63);
+#pragma unroll
+  for (int d = 1; d < G; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float row_max(float v, float *part) {
+  if constexpr (G == NT) return block_max(v, part);
+  if constexpr (G == WAVE) return wave_max_f(v);
+#pragma unroll
+  for (int d = 1; d < G; d *= 2) v = __builtin_elementwise_maximum(v, __shfl_xor(v, d));
+  return v;
+}
+
+/* G threads hold a row, U chunks of eight elements each, in registers: one read of
+ * everything, all of it in flight together. */
+template <bool BF16, int OUT, int G, int U>
+__global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
+  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G;
+  __shared__ float part[NW];
+  const int g = (int)threadIdx.x % G;
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
+    const bool mine = row0 + threadIdx.x / G < a.n_rows; /* (the others shadow the last row and store nothing) */
+    const int width = (int)a.width;
+    const char *x = (const char *)a.x + row * a.x_stride * ES;
+    Vec8<BF16> q[U], r[U], w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) q[u].load_some(x, (u * G + g) * 8, width - (u * G + g) * 8);
+    if (a.residual) {
+      const char *res = (const char *)a.residual + row * a.residual_stride * ES;
+#pragma unroll
+      for (int u = 0; u < U; u++) r[u].load_some(res, (u * G + g) * 8, width - (u * G + g) * 8);
+    }
+    if (a.gain) {
+#pragma unroll
+      for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * 8, width - (u * G + g) * 8);
+    }
+    float h[U][8], s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      q[u].values(h[u]);
+      if (a.residual) {
+        float t[8];
+        r[u].values(t);
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[u][e] += t[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) s = fmaf(h[u][e], h[u][e], s);
+    }
+    if (a.sum && mine) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        store8<BF16>((char *)a.sum + row * a.sum_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8, h[u]);
+    }
+    s = row_sum<G>(s, part);
+    const float rstd = 1.0f / sqrtf(s / (float)width + a.eps);
+    if (g == 0 && a.rstd && mine) a.rstd[row] = rstd;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float t[8];
+      if (a.gain) w[u].values(t);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        h[u][e] *= rstd;
+        if (a.gain) h[u][e] *= t[e];
+      }
+    }
+    if constexpr (OUT != D3S_DTYPE_E4M3) {
+      constexpr int YS = OUT == D3S_DTYPE_BF16 ? 2 : 4;
+      if (mine) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          store8<OUT == D3S_DTYPE_BF16>((char *)a.y + row * a.y_stride * YS, (u * G + g) * 8, width - (u * G + g) * 8, h[u]);
+      }
+    } else {
+      /* (places past the row hold x = 0 and, where rstd is infinite, 0 times it: not looked at) */
+      float most[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        most[u] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          most[u] = __builtin_elementwise_maximum(most[u], (u * G + g) * 8 + e < width ? fabsf(h[u][e]) : 0.0f);
+      }
+      if (a.group == 0) {
+#pragma unroll
+        for (int u = 1; u < U; u++) most[0] = __builtin_elementwise_maximum(most[0], most[u]);
+        most[0] = row_max<G>(most[0], part);
+#pragma unroll
+        for (int u = 1; u < U; u++) most[u] = most[0];
+      } else {
+        for (int d = 1; d < min(a.group / 8, G); d *= 2)
+#pragma unroll
+          for (int u = 0; u < U; u++) most[u] = __builtin_elementwise_maximum(most[u], __shfl_xor(most[u], d));
+      }
+      const int size = a.group ? a.group : width;
+      const int64_t groups = (width + size - 1) / size;
+      uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int j = (u * G + g) * 8, left = width - j;
+        const float scale = e4m3_scale(most[u]);
+        if (left <= 0 || !mine) continue;
+        if (a.group ? j % a.group == 0 : j == 0) a.scales[row * groups + (a.group ? j / a.group : 0)] = scale;
+        const uint64_t p = pack_e4m3(h[u], scale);
+        if (left >= 8)
+          __builtin_memcpy(y + j, &p, 8);
+        else
+          for (int e = 0; e < left; e++) y[j + e] = (uint8_t)(p >> 8 * e);
+      }
+    }
+  }
+}
+
+/* The gradient, rows held the same way; a workgroup takes every gridDim.x-th set of
+ * rows and keeps their columns' sums of dy xhat in registers. */
+template <bool BF16, int G, int U, bool SUM>
+__global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) {
+  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G;
+  __shared__ float part[NW];
+  __shared__ float sums[SUM && ROWS > 1 ? NT * U * 8 : 1];
+  const int g = (int)threadIdx.x % G, width = (int)a.width;
+  Vec8<BF16> w[U];
+  if (a.gain) {
+#pragma unroll
+    for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * 8, width - (u * G + g) * 8);
+  }
+  float acc[U][8];
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) acc[u][e] = 0.0f;
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
+    const bool mine = row0 + threadIdx.x / G < a.n_rows;
+    Vec8<BF16> d[U], h[U], r[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      d[u].load_some((const char *)a.dy + row * a.dy_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
+      h[u].load_some((const char *)a.h + row * a.h_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
+    }
+    if (a.dsum && a.dx) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        r[u].load_some((const char *)a.dsum + row * a.dsum_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
+    }
+    const float rstd = a.rstd[row];
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float p[8], t[8], k[8];
+      d[u].values(p);
+      h[u].values(t);
+      if (a.gain) w[u].values(k);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float xhat = t[e] * rstd;
+        if (SUM && mine && (u * G + g) * 8 + e < width) acc[u][e] = fmaf(p[e], xhat, acc[u][e]);
+        s = fmaf(a.gain ? p[e] * k[e] : p[e], (u * G + g) * 8 + e < width ? xhat : 0.0f, s);
+      }
+    }
+    if (!a.dx) continue; /* (uniform) */
+    const float mean = row_sum<G>(s, part) / (float)width;
+    if (!mine) continue; /* (G == NT: always its own) */
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float p[8], t[8], k[8], o[8];
+      d[u].values(p);
+      h[u].values(t);
+      if (a.gain) w[u].values(k);
+      if (a.dsum) r[u].values(o);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float v = rstd * ((a.gain ? p[e] * k[e] : p[e]) - t[e] * rstd * mean);
+        o[e] = a.dsum ? v + o[e] : v;
+      }
+      store8<BF16>((char *)a.dx + row * a.dx_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8, o);
+    }
+  }
+  if constexpr (SUM) {
+    float *out = parts + (int64_t)blockIdx.x * a.width;
+    if constexpr (ROWS == 1) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        store8<false, false>(out, (u * G + g) * 8, width - (u * G + g) * 8, acc[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) sums[(threadIdx.x / G) * (G * U * 8) + (u * G + g) * 8 + e] = acc[u][e];
+      __syncthreads();
+      for (int j = (int)threadIdx.x; j < width; j += NT) {
+        float v = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < ROWS; i++) v += sums[i * (G * U * 8) + j];
+        out[j] = v;
+      }
+    }
+  }
 }
 
 template <bool BF16>
@@ -176,39 +388,117 @@ __global__ __launch_bounds__(NT) void k_norm_grad_rows(NormGradArgs a) {
   }
 }
 
-/* dgain: a thread a column, the rows in order */
+/* dgain of rows too long for registers: a thread a column, a run of rows each */
 template <bool BF16>
-__global__ __launch_bounds__(NT) void k_norm_dgain(NormGradArgs a) {
-  for (int64_t j = (int64_t)blockIdx.x * NT + threadIdx.x; j < a.width; j += (int64_t)gridDim.x * NT) {
-    float s = 0.0f;
-    for (int64_t r = 0; r < a.n_rows; r++)
-      s = fmaf(load_at<BF16>(a.dy, r * a.dy_stride + j), load_at<BF16>(a.h, r * a.h_stride + j) * a.rstd[r], s);
-    a.dgain[j] = s;
+__global__ __launch_bounds__(NT) void k_norm_dgain(NormGradArgs a, int64_t strips, int rows, float *parts) {
+  const int64_t j = (int64_t)blockIdx.x % strips * NT + threadIdx.x, run = blockIdx.x / strips;
+  if (j >= a.width) return;
+  float s = 0.0f;
+#pragma unroll 4
+  for (int64_t r = run * rows; r < min(a.n_rows, (run + 1) * rows); r++)
+    s = fmaf(load_at<BF16>(a.dy, r * a.dy_stride + j), load_at<BF16>(a.h, r * a.h_stride + j) * a.rstd[r], s);
+  parts[run * a.width + j] = s;
+}
+
+/* the threads and chunks that hold a row: f(G, U), or false for one that is streamed */
+template <class F>
+bool in_registers(int64_t width, F f) {
+  auto c = [](auto v) { return v; };
+#define D3S_ROW(G, U) return f(c(std::integral_constant<int, G>{}), c(std::integral_constant<int, U>{})), true
+  if (width <= 64) D3S_ROW(8, 1);
+  if (width <= 128) D3S_ROW(16, 1);
+  if (width <= 256) D3S_ROW(32, 1);
+  if (width <= 512) D3S_ROW(64, 1);
+  if (width <= 1024) D3S_ROW(64, 2);
+  if (width <= 2048) D3S_ROW(64, 4);
+  if (width <= 4096) D3S_ROW(256, 2);
+  if (width <= 8192) D3S_ROW(256, 4);
+  if (width <= 16384) D3S_ROW(256, 8);
+#undef D3S_ROW
+  return false;
+}
+
+/* workgroups of the gradient: the runs of its column sums */
+constexpr int GRAD_RUNS = 512;
+struct GradSplit {
+  int64_t strips;
+  int rows, runs;
+};
+GradSplit grad_split(int64_t n_rows, int64_t width) {
+  GradSplit p{1, 0, 0};
+  const bool held = in_registers(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
+  if (held) {
+    const int64_t sets = (n_rows + p.rows - 1) / p.rows;
+    p.runs = (int)(sets < GRAD_RUNS ? sets : GRAD_RUNS);
+  } else {
+    p.strips = (width + NT - 1) / NT;
+    int64_t runs = 1024 / p.strips;
+    if (runs < 1) runs = 1;
+    p.rows = (int)((n_rows + runs - 1) / runs);
+    p.runs = p.rows ? (int)((n_rows + p.rows - 1) / p.rows) : 0;
   }
+  return p;
 }
 
 }  // namespace
 
 void launch_norm(const NormArgs &args, Dtype dt, hipStream_t s) {
   const NormArgs a = args;
-  const dim3 grid((unsigned)(a.n_rows < STEP_GRID ? a.n_rows : STEP_GRID));
+  auto grid = [&](int rows) {
+    const int64_t n = (a.n_rows + rows - 1) / rows;
+    return dim3((unsigned)(n < STEP_GRID ? n : STEP_GRID));
+  };
+  const bool held = in_registers(a.width, [&](auto g, auto u) {
+    constexpr int G = decltype(g)::value, U = decltype(u)::value;
+    auto go = [&](auto kernel) { kernel<<<grid(NT / G), NT, 0, s>>>(a); };
+    auto out = [&](auto bf16) {
+      constexpr bool B = decltype(bf16)::value;
+      if (a.y_dtype == D3S_DTYPE_BF16)
+        go(k_norm<B, D3S_DTYPE_BF16, G, U>);
+      else if (a.y_dtype == D3S_DTYPE_F32)
+        go(k_norm<B, D3S_DTYPE_F32, G, U>);
+      else
+        go(k_norm<B, D3S_DTYPE_E4M3, G, U>);
+    };
+    dt == DT_BF16 ? out(std::true_type{}) : out(std::false_type{});
+  });
+  if (held) return;
   if (dt == DT_BF16)
-    k_norm_rows<true><<<grid, NT, 0, s>>>(a);
+    k_norm_rows<true><<<grid(1), NT, 0, s>>>(a);
   else
-    k_norm_rows<false><<<grid, NT, 0, s>>>(a);
+    k_norm_rows<false><<<grid(1), NT, 0, s>>>(a);
 }
 
-size_t norm_grad_workspace_bytes(int64_t, int64_t, bool) { return 0; }
+size_t norm_grad_workspace_bytes(int64_t n_rows, int64_t width, bool dgain) {
+  if (!dgain || n_rows == 0 || width == 0) return 0;
+  return split_counter_bytes() + (size_t)grad_split(n_rows, width).runs * (size_t)width * sizeof(float);
+}
 
-void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *, hipStream_t s) {
+void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t s) {
   const NormGradArgs a = args;
-  /* (dgain first: dx may be dy or h) */
-  const int64_t cols = (a.width + NT - 1) / NT;
-  const dim3 strips((unsigned)(cols < STEP_GRID ? cols : STEP_GRID));
-  const dim3 grid((unsigned)(a.n_rows < STEP_GRID ? a.n_rows : STEP_GRID));
-  if (a.dgain) dt == DT_BF16 ? k_norm_dgain<true><<<strips, NT, 0, s>>>(a) : k_norm_dgain<false><<<strips, NT, 0, s>>>(a);
-  if (!a.dx || a.n_rows == 0) return;
-  dt == DT_BF16 ? k_norm_grad_rows<true><<<grid, NT, 0, s>>>(a) : k_norm_grad_rows<false><<<grid, NT, 0, s>>>(a);
+  const GradSplit p = grad_split(a.n_rows, a.width);
+  float *parts = ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
+  bool held = false;
+  if (p.runs)
+    held = in_registers(a.width, [&](auto g, auto u) {
+      constexpr int G = decltype(g)::value, U = decltype(u)::value;
+      auto go = [&](auto kernel) { kernel<<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts); };
+      if (dt == DT_BF16)
+        a.dgain ? go(k_norm_grad<true, G, U, true>) : go(k_norm_grad<true, G, U, false>);
+      else
+        a.dgain ? go(k_norm_grad<false, G, U, true>) : go(k_norm_grad<false, G, U, false>);
+    });
+  if (!held && p.runs) { /* (dgain first: dx may be dy or h) */
+    const dim3 strips((unsigned)(p.strips * p.runs)), rows((unsigned)(a.n_rows < STEP_GRID ? a.n_rows : STEP_GRID));
+    if (a.dgain) {
+      if (dt == DT_BF16)
+        k_norm_dgain<true><<<strips, NT, 0, s>>>(a, p.strips, p.rows, parts);
+      else
+        k_norm_dgain<false><<<strips, NT, 0, s>>>(a, p.strips, p.rows, parts);
+    }
+    if (a.dx) dt == DT_BF16 ? k_norm_grad_rows<true><<<rows, NT, 0, s>>>(a) : k_norm_grad_rows<false><<<rows, NT, 0, s>>>(a);
+  }
+  if (a.dgain) launch_column_sums(parts, p.runs, (int)a.width, a.dgain, s);
 }
 
 }  // namespace d3s

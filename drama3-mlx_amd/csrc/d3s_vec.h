@@ -24,6 +24,25 @@ struct Vec8 {
     __builtin_memcpy(&q[0], p, 16);
     if constexpr (!BF16) __builtin_memcpy(&q[1], p + 16, 16);
   }
+  /* elements j .. j + 7 of which `left` (0 .. 8) are inside, the rest +0 */
+  __device__ __forceinline__ void load_some(const void *row, int64_t j, int left) {
+    if (left >= 8) {
+      load(row, j);
+      return;
+    }
+    uint32_t *w = (uint32_t *)q;
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 4 : 8); i++) w[i] = 0u;
+    if (left <= 0) return;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (e >= left) continue;
+      if constexpr (BF16)
+        w[e / 2] |= (uint32_t)((const uint16_t *)row)[j + e] << 16 * (e % 2);
+      else
+        w[e] = ((const uint32_t *)row)[j + e];
+    }
+  }
   __device__ __forceinline__ void values(float *v) const {
     const uint32_t *w = (const uint32_t *)q;
 #pragma unroll
