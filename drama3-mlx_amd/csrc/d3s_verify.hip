@@ -1,5 +1,6 @@
 /* k_verify_one, k_verify_ranked: verification of drafted tokens (gfx950, wave64;
  * include/d3s_step.h). */
+#include "d3s_rowcore.h"
 #include "d3s_rowsums.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
@@ -7,67 +8,57 @@
 namespace d3s {
 namespace {
 
-constexpr int VT = 1024;
-constexpr int VW = VT / WAVE;
+constexpr int VT = 1024;       /* threads of k_verify_one */
+constexpr int ST = 256;        /* ... of the split kernels */
+constexpr int SU = 4;          /* chunks a lane takes at a time */
+constexpr int GRID_MOST = 1 << 22;
 constexpr double LOG2E_64 = 1.4426950408889634074;
 
 __device__ __forceinline__ float least_T(float T) { return T < 1e-5f && T > -__builtin_inff() ? 1e-5f : T; }
 
-/* 2^t for t <= 0 (0 below -1100): the Taylor series of 2^f on |f| <= 1 / 2 to the
- * 11th power (the rest below 2^-46), in 64 bits */
+/* 2^t for t <= 0 (0 from -1100 down): 2^f on |f| <= 1 / 2 by the polynomial that
+ * agrees with it at ten Chebyshev nodes (fitted here; 2e-14 relative) */
 __device__ __forceinline__ double exp2_64(double t) {
   t = fmax(t, -1100.0);
   const double n = rint(t), f = t - n;
-  double p = 4.4455382718708116e-10; /* (ln 2)^k / k!, k = 11 .. 0 */
-  p = fma(p, f, 7.0549116208011234e-09);
-  p = fma(p, f, 1.0178086009239699e-07);
-  p = fma(p, f, 1.3215486790144310e-06);
-  p = fma(p, f, 1.5252733804059841e-05);
-  p = fma(p, f, 1.5403530393381609e-04);
-  p = fma(p, f, 1.3333558146428443e-03);
-  p = fma(p, f, 9.6181291076284772e-03);
-  p = fma(p, f, 5.5504108664821580e-02);
-  p = fma(p, f, 2.4022650695910072e-01);
-  p = fma(p, f, 6.9314718055994531e-01);
-  p = fma(p, f, 1.0);
+  double p = 1.0205905308574628e-07;
+  p = fma(p, f, 1.3259645243778838e-06);
+  p = fma(p, f, 1.5252672925435629e-05);
+  p = fma(p, f, 0.0001540343375125619);
+  p = fma(p, f, 0.0013333558200793471);
+  p = fma(p, f, 0.009618129193934302);
+  p = fma(p, f, 0.05550410866465168);
+  p = fma(p, f, 0.2402265069564034);
+  p = fma(p, f, 0.6931471805599462);
+  p = fma(p, f, 1.0000000000000135);
   return ldexp(p, (int)n);
 }
 
-/* a row's greatest logit and sum, and what they say of it */
+/* a row's greatest logit and sum (m = NaN: refused) */
 struct RowStat {
   float m, S;
 };
 __device__ __forceinline__ bool refused(RowStat r) { return !(r.m < __builtin_inff()); }
-/* the probability of a logit (S > 0 unless all is masked) */
-__device__ __forceinline__ float prob_of(RowStat r, float l, float T) {
-  return r.S > 0.0f ? d3s_expf_nonpos((l - r.m) / T) / r.S : 0.0f;
-}
 
-/* What a sequence comes to: its drafts accepted, and how the token after them is drawn */
+/* what a sequence comes to: its drafts accepted, and how the token after them is drawn */
 struct Outcome {
   int accepted;
   bool refuse, rejected;
 };
 
-__device__ __forceinline__ float accept_of(float p, float q) { return q > 0.0f ? fminf(p / q, 1.0f) : p > 0.0f ? 1.0f : 0.0f; }
+__device__ __forceinline__ float accept_of(float p, float q) {
+  return p != p || q != q ? __builtin_nanf("") : q > 0.0f ? fminf(p / q, 1.0f) : p > 0.0f ? 1.0f : 0.0f;
+}
 
-/* p, q (NaN: a refused row) of L drafts; last: p's row behind them is refused */
-template <class P, class Q>
-__device__ __forceinline__ Outcome decide(int L, const float *u, P p, Q q, bool last_refused) {
-  Outcome o{0, false, false};
-  for (int i = 0; i < L; i++) {
-    const float pi = p(i), qi = q(i);
-    if (pi != pi || qi != qi) {
-      o.refuse = true;
-      return o;
-    }
-    if (!(u[i] * qi < pi)) {
-      o.rejected = true;
-      return o;
-    }
-    o.accepted++;
-  }
-  o.refuse = last_refused;
+/* Lane i of every wave holds u, p and q (NaN: a refused row) of draft i < L <= 64;
+ * last_refused: the target's row behind them. */
+__device__ __forceinline__ Outcome decide(int L, float u, float p, float q, bool last_refused) {
+  const bool inside = lane_id() < L, odd = p != p || q != q;
+  const uint64_t refusing = __ballot(inside && odd), stops = __ballot(inside && (odd || !(u * q < p)));
+  Outcome o;
+  o.accepted = stops ? (int)__builtin_ctzll(stops) : L;
+  o.refuse = stops ? (refusing >> o.accepted & 1ull) != 0ull : last_refused;
+  o.rejected = stops && !o.refuse;
   return o;
 }
 
@@ -80,233 +71,614 @@ __device__ __forceinline__ void write_tokens(int b, int n_draft, Outcome o, int 
   if (threadIdx.x == 0) n_accepted[b] = o.accepted;
 }
 
-__device__ __forceinline__ double shfl_up_f64(double v, int d) { return __shfl_up(v, d); }
+/* A sequence: its length and temperatures, its rows (0 .. n_draft the target's, then the
+ * draft model's) */
+struct Seq {
+  int b, len, rows;
+  float T, Td;
 
+  __device__ __forceinline__ Seq(const d3s_verify_params &a, int b_) : b(b_) {
+    len = a.lengths ? min(max(a.lengths[b], 0), a.n_draft) : a.n_draft;
+    T = least_T(a.temperature ? a.temperature[b] : a.temperature_scalar);
+    Td = least_T(a.draft_temperature ? a.draft_temperature[b] : a.draft_temperature_scalar);
+    rows = a.n_draft + 1 + (a.draft ? a.n_draft : 0);
+  }
+  __device__ __forceinline__ bool target(const d3s_verify_params &a, int r) const { return r <= a.n_draft; }
+  __device__ __forceinline__ int place(const d3s_verify_params &a, int r) const { return target(a, r) ? r : r - a.n_draft - 1; }
+  __device__ __forceinline__ int row(const d3s_verify_params &a, int r) const {
+    return target(a, r) ? b * (a.n_draft + 1) + r : b * a.n_draft + r - a.n_draft - 1;
+  }
+  /* whether the row can count: a target's up to the one behind the drafts */
+  __device__ __forceinline__ bool there(const d3s_verify_params &a, int r) const {
+    return target(a, r) ? r <= len : place(a, r) < len;
+  }
+  __device__ __forceinline__ float temperature(const d3s_verify_params &a, int r) const { return target(a, r) ? T : Td; }
+};
+
+/* A lane's share of a row's chunks, every `step`-th from `ch` on, up to `hi`; a batch
+ * is loaded while the one before it is added. */
+template <bool BF16>
+__device__ __forceinline__ void lane_sums(Sums &s, const Row<BF16> &R, int ch, int hi, int step, float c) {
+  constexpr int EPC = Row<BF16>::EPC;
+  uint4 q[SU], next[SU];
+  bool whole = ch + (SU - 1) * step < hi;
+  if (whole) {
+#pragma unroll
+    for (int u = 0; u < SU; u++) q[u] = R.base[ch + u * step];
+  }
+  while (whole) {
+    const int after = ch + SU * step;
+    whole = after + (SU - 1) * step < hi;
+    if (whole) {
+#pragma unroll
+      for (int u = 0; u < SU; u++) next[u] = R.base[after + u * step];
+    }
+    float v[SU * EPC];
+#pragma unroll
+    for (int u = 0; u < SU; u++) R.values(q[u], ch + u * step, v + u * EPC);
+    add_batch<SU * EPC, false>(s, v, c);
+#pragma unroll
+    for (int u = 0; u < SU; u++) q[u] = next[u];
+    ch = after;
+  }
+  if (ch >= hi) return;
+  /* the rest, less than a batch: a place past the end is the last chunk again, masked */
+  float v[SU * EPC];
+#pragma unroll
+  for (int u = 0; u < SU; u++) q[u] = R.base[min(ch + u * step, hi - 1)];
+#pragma unroll
+  for (int u = 0; u < SU; u++) {
+    R.values(q[u], min(ch + u * step, hi - 1), v + u * EPC);
+    if (ch + u * step >= hi) {
+#pragma unroll
+      for (int e = 0; e < EPC; e++) v[u * EPC + e] = -__builtin_inff();
+    }
+  }
+  add_batch<SU * EPC, false>(s, v, c);
+}
+
+/* LDS of a sequence's decision */
+struct Settled {
+  RowStat stat[2 * D3S_MAX_DRAFT + 1];
+  float prob[2 * D3S_MAX_DRAFT + 1];
+};
+
+/* the logit of row r's draft (-inf: not a token, or none) */
+template <bool TB, bool DB>
+__device__ __forceinline__ float draft_logit(const d3s_verify_params &a, const Seq &q, int r) {
+  const int i = q.place(a, r);
+  if (r >= q.rows || i >= q.len) return -__builtin_inff();
+  const int x = a.drafted[(size_t)q.b * a.n_draft + i];
+  if ((unsigned)x >= (unsigned)a.vocab) return -__builtin_inff();
+  return q.target(a, r) ? load_at<TB>(a.target, (int64_t)q.row(a, r) * a.target_stride + x)
+                        : load_at<DB>(a.draft, (int64_t)q.row(a, r) * a.draft_stride + x);
+}
+
+/* A thread a row: the probability of its draft's logit, from the row's statistics (S > 0
+ * unless all of the row is masked). */
+__device__ __forceinline__ void settle_row(const d3s_verify_params &a, const Seq &q, int r, RowStat st, float l, Settled &L) {
+  const float T = q.temperature(a, r);
+  if (!finite(T)) st.m = __builtin_nanf("");
+  L.stat[r] = st;
+  L.prob[r] = refused(st) ? __builtin_nanf("") : st.S > 0.0f ? d3s_expf_nonpos((l - st.m) / T) / st.S : 0.0f;
+}
+
+__device__ __forceinline__ float lane_u(const d3s_verify_params &a, const Seq &s) {
+  return lane_id() < s.len ? a.u_accept[(size_t)s.b * a.n_draft + lane_id()] : 0.0f;
+}
+
+/* the whole workgroup, the rows settled; u: lane_u */
+__device__ __forceinline__ Outcome settle(const d3s_verify_params &a, const Seq &s, const Settled &L, float u, bool write_accept) {
+  const int i = lane_id();
+  const bool inside = i < s.len;
+  const float p = inside ? L.prob[i] : 0.0f, q = !inside ? 0.0f : a.draft ? L.prob[a.n_draft + 1 + i] : 1.0f;
+  if (write_accept && a.accept && (int)threadIdx.x < a.n_draft)
+    a.accept[(size_t)s.b * a.n_draft + i] = inside ? accept_of(p, q) : 0.0f;
+  return decide(s.len, u, p, q, refused(L.stat[s.len]));
+}
+
+/* The weights r_j that a token is drawn from, in 64 bits. */
+template <bool TB, bool DB>
+struct Weights {
+  const char *tp, *dp; /* the rows (dp null: none, or a certain draft) */
+  int V, gone;         /* the certain draft's token, or -1 */
+  double mp, mq, cp, cq, ip, iq; /* greatest logits, log2(e) / T, the sums' reciprocals */
+
+  /* sp, sq: what the sequence's rows hold */
+  __device__ __forceinline__ Weights(const d3s_verify_params &a, const Seq &s, int accepted, bool rejected, float m_p, float m_q) {
+    tp = (const char *)a.target + ((int64_t)s.b * (a.n_draft + 1) + accepted) * a.target_stride * (TB ? 2 : 4);
+    dp = rejected && a.draft ? (const char *)a.draft + ((int64_t)s.b * a.n_draft + accepted) * a.draft_stride * (DB ? 2 : 4) : nullptr;
+    V = (int)a.vocab;
+    gone = rejected && !a.draft ? a.drafted[(size_t)s.b * a.n_draft + accepted] : -1;
+    mp = m_p, mq = m_q;
+    cp = LOG2E_64 / s.T, cq = LOG2E_64 / s.Td;
+    ip = iq = 1.0;
+  }
+  __device__ __forceinline__ int left(int j) const { return min(8, V - j); }
+  /* eight terms of each sum from j on (0 past the end), j < V */
+  __device__ __forceinline__ void terms(int j, double *p, double *q) const {
+    float v[8], w[8];
+    load8<TB>(tp, j, left(j), v, -__builtin_inff());
+    if (dp) load8<DB>(dp, j, left(j), w, -__builtin_inff());
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = exp2_64(((double)v[e] - mp) * cp);
+    if (dp) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) q[e] = exp2_64(((double)w[e] - mq) * cq);
+    }
+  }
+  /* eight weights from j on; plain: p alone */
+  __device__ __forceinline__ void at(int j, bool plain, double *r) const {
+    double p[8], q[8];
+    terms(j, p, q);
+    weights(j, plain, p, q, r);
+  }
+  __device__ __forceinline__ void weights(int j, bool plain, const double *p, const double *q, double *r) const {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      r[e] = p[e] * ip;
+      if (plain) continue;
+      if (dp)
+        r[e] = fmax(r[e] - q[e] * iq, 0.0);
+      else if (j + e == gone)
+        r[e] = fmax(r[e] - 1.0, 0.0);
+    }
+  }
+};
+
+template <int NT>
 struct DrawLds {
-  double wave[VW];
+  double wave[NT / WAVE];
+  double from;
   int at;
 };
 
-/* the workgroup's sum in one order, in every thread */
-__device__ __forceinline__ double block_sum64(double v, DrawLds &L) {
-#pragma unroll
-  for (int d = 1; d < WAVE; d *= 2) v += __shfl_xor(v, d);
+template <int CTRL, int ROWM>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t w = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = dpp_u<CTRL, ROWM>(0u, (uint32_t)w), hi = dpp_u<CTRL, ROWM>(0u, (uint32_t)(w >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+/* inclusive sums over the wave (wave_scan_add_f32 in 64 bits) */
+__device__ __forceinline__ double wave_scan64(double v) {
+  v += dpp_f64<DPP_SHR1, 0xf>(v);
+  v += dpp_f64<DPP_SHR2, 0xf>(v);
+  v += dpp_f64<DPP_SHR4, 0xf>(v);
+  v += dpp_f64<DPP_SHR8, 0xf>(v);
+  v += dpp_f64<DPP_BCAST15, 0xa>(v);
+  v += dpp_f64<DPP_BCAST31, 0xc>(v);
+  return v;
+}
+template <int NT>
+__device__ __forceinline__ double block_sum64(double v, DrawLds<NT> &L) {
+  v = wave_scan64(v);
   __syncthreads();
-  if (lane_id() == 0) L.wave[threadIdx.x / WAVE] = v;
+  if (lane_id() == WAVE - 1) L.wave[threadIdx.x / WAVE] = v;
   __syncthreads();
   double t = 0.0;
-  for (int w = 0; w < VW; w++) t += L.wave[w];
+#pragma unroll
+  for (int w = 0; w < NT / WAVE; w++) t += L.wave[w];
   return t;
 }
+/* the sum of the threads before, and of all */
+template <int NT>
+__device__ __forceinline__ double block_scan64(double v, DrawLds<NT> &L, double *total) {
+  const double incl = wave_scan64(v);
+  __syncthreads();
+  if (lane_id() == WAVE - 1) L.wave[threadIdx.x / WAVE] = incl;
+  __syncthreads();
+  double before = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < NT / WAVE; w++) {
+    if (w == (int)threadIdx.x / WAVE) before = all;
+    all += L.wave[w];
+  }
+  *total = all;
+  return before + (incl - v);
+}
 
-template <bool TB, bool DB>
-__global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
-  __shared__ RowStat stat[2 * D3S_MAX_DRAFT + 1];
-  __shared__ float prob[2 * D3S_MAX_DRAFT];
-  __shared__ DrawLds L;
-  const int b = (int)blockIdx.x, tid = (int)threadIdx.x, V = (int)a.vocab;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.n_draft) : a.n_draft;
-  const float T = least_T(a.temperature ? a.temperature[b] : a.temperature_scalar);
-  const float Td = least_T(a.draft_temperature ? a.draft_temperature[b] : a.draft_temperature_scalar);
-  const int32_t *x = a.drafted + (size_t)b * a.n_draft;
-  const float nan = __builtin_nanf("");
-
-  /* a wave a row: target 0 .. len, then draft 0 .. len - 1 */
-  auto row_sums = [&](auto bf16, const void *logits, int64_t stride, int row, float T_) {
-    constexpr bool BF16 = decltype(bf16)::value;
-    const Row<BF16> R(logits, stride, row, V, -1);
-    Sums s{-FLT_MAX, 0.0f, 0.0f};
-    const float c = LOG2E / T_;
-    for (int ch = lane_id(); ch < R.chunks; ch += WAVE) {
-      float v[Row<BF16>::EPC];
-      R.values(R.base[ch], ch, v);
-      add_batch<Row<BF16>::EPC, false>(s, v, c);
-    }
-    join_wave(s, c);
-    return s;
-  };
-  const int n_rows = len + 1 + (a.draft ? len : 0);
-  for (int r = tid / WAVE; r < n_rows; r += VW) {
-    const bool target = r <= len;
-    const int i = target ? r : r - len - 1;
-    const int row = target ? b * (a.n_draft + 1) + i : b * a.n_draft + i;
-    const float Tr = target ? T : Td;
-    const Sums s = target ? row_sums(std::integral_constant<bool, TB>{}, a.target, a.target_stride, row, Tr)
-                          : row_sums(std::integral_constant<bool, DB>{}, a.draft, a.draft_stride, row, Tr);
-    if (lane_id() == 0) {
-      RowStat st{s.m, s.S};
-      if (!finite(Tr)) st.m = nan;
-      stat[r] = st;
-      if (i < len) {
-        float pr = 0.0f;
-        if (refused(st)) {
-          pr = nan;
-        } else if ((unsigned)x[i] < (unsigned)V) {
-          const float l = target ? load_at<TB>(a.target, (int64_t)row * a.target_stride + x[i])
-                                 : load_at<DB>(a.draft, (int64_t)row * a.draft_stride + x[i]);
-          pr = prob_of(st, l, Tr);
-        }
-        prob[target ? i : D3S_MAX_DRAFT + i] = pr;
-      }
+/* The first place whose sum passes bar, else (LAST) the last with a weight, else -1, in
+ * every thread: a thread's eight weights r follow each other from j on, `before` is the sum of
+ * those before them. */
+template <int NT>
+__device__ __forceinline__ int first_past(const double *r, int j, double before, double bar, bool last_too, DrawLds<NT> &L) {
+  int over = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    before += r[e];
+    if (r[e] > 0.0) {
+      last = j + e;
+      if (before > bar) over = min(over, j + e);
     }
   }
+  if (threadIdx.x == 0) L.at = 0x7fffffff;
   __syncthreads();
-  auto p = [&](int i) { return prob[i]; };
-  auto q = [&](int i) { return a.draft ? prob[D3S_MAX_DRAFT + i] : 1.0f; };
-  const Outcome o = decide(len, a.u_accept + (size_t)b * a.n_draft, p, q, refused(stat[len]));
-  if (a.accept)
-    for (int i = tid; i < a.n_draft; i += VT)
-      a.accept[(size_t)b * a.n_draft + i] = i >= len ? 0.0f : p(i) != p(i) || q(i) != q(i) ? nan : accept_of(p(i), q(i));
-  int token = -1;
-  const RowStat sp = stat[o.accepted];
-  if (o.refuse) {
-    if (tid == 0 && a.counters) atomicAdd(&a.counters[CNT_REFUSED], 1u);
-  } else if (sp.S == 0.0f) {
-    token = 0;
-    if (tid == 0 && a.counters) atomicAdd(&a.counters[CNT_ALL_MASKED], 1u);
-  } else {
-    /* the draw in 64 bits, a thread a run of the row */
-    const int per = ((V + VT - 1) / VT + 7) / 8 * 8, lo = min(V, tid * per), hi = min(V, lo + per);
-    const bool pair = o.rejected && a.draft;
-    const RowStat sq = pair ? stat[len + 1 + o.accepted] : RowStat{0.0f, 0.0f};
-    const int gone = o.rejected && !a.draft ? x[o.accepted] : -1;
-    const char *tp = (const char *)a.target + ((int64_t)b * (a.n_draft + 1) + o.accepted) * a.target_stride * (TB ? 2 : 4);
-    const char *dp = (const char *)a.draft + ((int64_t)b * a.n_draft + o.accepted) * a.draft_stride * (DB ? 2 : 4);
-    const double cp = LOG2E_64 / T, cq = LOG2E_64 / Td;
-    auto ep = [&](float l) { return exp2_64(((double)l - sp.m) * cp); };
-    auto eq = [&](float l) { return exp2_64(((double)l - sq.m) * cq); };
-    double Sp = 0.0, Sq = 0.0;
-    for (int j = lo; j < hi; j++) {
-      Sp += ep(load_at<TB>(tp, j));
-      if (pair) Sq += eq(load_at<DB>(dp, j));
+  if (over != 0x7fffffff) atomicMin(&L.at, over);
+  __syncthreads();
+  int at = L.at;
+  if (at != 0x7fffffff || !last_too) {
+    __syncthreads();
+    return at != 0x7fffffff ? at : -1;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) L.at = -1;
+  __syncthreads();
+  if (last >= 0) atomicMax(&L.at, last);
+  __syncthreads();
+  at = L.at;
+  __syncthreads();
+  return at;
+}
+
+/* the token among [lo, hi), `base` the weights before them */
+template <int NT, bool TB, bool DB>
+__device__ __forceinline__ int pick(const Weights<TB, DB> &W, int lo, int hi, double base, double bar, bool plain, DrawLds<NT> &L) {
+  int last = -1;
+  for (int c = lo; c < hi; c += NT * 8) {
+    const int j = c + (int)threadIdx.x * 8;
+    double r[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0}, mine = 0.0, total;
+    if (j < hi) W.at(j, plain, r);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if (j + e >= hi) r[e] = 0.0;
+      mine += r[e];
     }
-    Sp = 1.0 / block_sum64(Sp, L);
-    if (pair) {
-      Sq = block_sum64(Sq, L);
-      Sq = Sq > 0.0 ? 1.0 / Sq : 0.0;
+    const double before = base + block_scan64(mine, L, &total);
+    const int at = first_past(r, j, before, bar, false, L);
+    if (at >= 0) return at;
+    const int end = first_past(r, j, before, __builtin_inf(), true, L);
+    if (end >= 0) last = end;
+    base += total;
+  }
+  return last;
+}
+
+/* A workgroup a sequence: a wave a row of logits, then the draw.  HELD: rows of which a
+ * thread's eight elements are all (VT * 8): their terms stay in registers from the sums to the
+ * token; else three passes. */
+template <bool TB, bool DB, bool HELD>
+__global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
+  __shared__ Settled S;
+  __shared__ DrawLds<VT> L;
+  const int tid = (int)threadIdx.x, V = (int)a.vocab;
+  const Seq q(a, (int)blockIdx.x);
+  const float u = lane_u(a, q), ud = a.u_draw[q.b];
+  for (int r = tid / WAVE; r < q.rows; r += VT / WAVE) {
+    if (!q.there(a, r)) continue;
+    const float l = draft_logit<TB, DB>(a, q, r);
+    Sums s{-FLT_MAX, 0.0f, 0.0f};
+    const float c = LOG2E / q.temperature(a, r);
+    if (q.target(a, r)) {
+      const Row<TB> R(a.target, a.target_stride, q.row(a, r), V, -1);
+      lane_sums(s, R, lane_id(), R.chunks, WAVE, c);
+    } else {
+      const Row<DB> R(a.draft, a.draft_stride, q.row(a, r), V, -1);
+      lane_sums(s, R, lane_id(), R.chunks, WAVE, c);
+    }
+    join_wave(s, c);
+    if (lane_id() == 0) settle_row(a, q, r, RowStat{s.m, s.S}, l, S);
+  }
+  __syncthreads();
+  const Outcome o = settle(a, q, S, u, true);
+  const RowStat P = S.stat[o.accepted];
+  const bool masked = !o.refuse && P.S == 0.0f;
+  int token = masked ? 0 : -1;
+  if (o.refuse || masked) {
+    if (tid == 0 && a.counters) atomicAdd(&a.counters[masked ? CNT_ALL_MASKED : CNT_REFUSED], 1u);
+  } else {
+    Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, S.stat[o.rejected && a.draft ? a.n_draft + 1 + o.accepted : 0].m);
+    double sp = 0.0, sq = 0.0, p[8], t[8];
+    if (HELD) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = t[e] = 0.0;
+    }
+    for (int j = tid * 8; j < V; j += VT * 8) {
+      W.terms(j, p, t);
+#pragma unroll
+      for (int e = 0; e < 8; e++) sp += p[e];
+      if (W.dp) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) sq += t[e];
+      }
+      if (HELD) break;
+    }
+    W.ip = 1.0 / block_sum64(sp, L);
+    if (W.dp) {
+      sq = block_sum64(sq, L);
+      W.iq = sq > 0.0 ? 1.0 / sq : 0.0;
     }
     bool plain = !o.rejected;
-    auto weight = [&](int j) {
-      const double w = ep(load_at<TB>(tp, j)) * Sp;
-      if (plain) return w;
-      if (!pair) return j == gone ? fmax(w - 1.0, 0.0) : w;
-      return fmax(w - eq(load_at<DB>(dp, j)) * Sq, 0.0);
-    };
-    double mine, base, Z;
+    double r[8], Z;
     for (;;) {
-      mine = 0.0;
-      for (int j = lo; j < hi; j++) mine += weight(j);
-      double incl = mine;
+      if (HELD) {
+        double mine = 0.0;
+        W.weights(tid * 8, plain, p, t, r);
 #pragma unroll
-      for (int d = 1; d < WAVE; d *= 2) {
-        const double t = shfl_up_f64(incl, d);
-        if (lane_id() >= d) incl += t;
+        for (int e = 0; e < 8; e++) mine += r[e];
+        const double before = block_scan64(mine, L, &Z);
+        if (Z > 0.0 || plain) {
+          token = first_past(r, tid * 8, before, (double)ud * Z, true, L);
+          break;
+        }
+      } else {
+        Z = 0.0;
+        for (int j = tid * 8; j < V; j += VT * 8) {
+          W.at(j, plain, r);
+#pragma unroll
+          for (int e = 0; e < 8; e++) Z += r[e];
+        }
+        Z = block_sum64(Z, L);
+        if (Z > 0.0 || plain) {
+          token = pick<VT>(W, 0, V, 0.0, (double)ud * Z, plain, L);
+          break;
+        }
       }
-      __syncthreads();
-      if (lane_id() == WAVE - 1) L.wave[tid / WAVE] = incl;
-      if (tid == 0) L.at = 0x7fffffff;
-      __syncthreads();
-      double before = 0.0;
-      Z = 0.0;
-      for (int w = 0; w < VW; w++) {
-        if (w < tid / WAVE) before += L.wave[w];
-        Z += L.wave[w];
-      }
-      base = before + (incl - mine);
-      if (Z > 0.0 || plain) break;
-      plain = true; /* (p <= q everywhere: rounding alone) */
+      plain = true; /* (p <= q everywhere: by rounding alone) */
     }
-    const double bar = (double)a.u_draw[b] * Z;
-    if (mine > 0.0 && base + mine > bar) atomicMin(&L.at, tid);
+  }
+  write_tokens(q.b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
+}
+
+/* ---- long rows: two launches ---- */
+
+constexpr int SWV = ST / WAVE;
+
+/* how the rows are cut: nseg segments of 16-byte chunks for the statistics, nblk blocks of `block`
+ * elements for the draw, SWV parts each */
+struct VerifySplit {
+  int nseg, nblk, block;
+};
+
+struct VerifyRoom {
+  RowStat *stats; /* [n_seqs, rows, nseg] */
+  uint64_t *parts; /* [n_seqs, nblk, SWV, 4]: doubles */
+  uint32_t *arrivals;
+  int spacing; /* words between two sequences' counters */
+};
+
+/* 1: greatest logit and sum of a segment of a row */
+template <bool TB, bool DB>
+__global__ __launch_bounds__(ST) void k_verify_rows(d3s_verify_params a, VerifySplit sp, VerifyRoom w, int64_t wg0) {
+  __shared__ float wm[ST / WAVE], wS[ST / WAVE];
+  const int64_t wg = wg0 + blockIdx.x;
+  const int rows = a.n_draft + 1 + (a.draft ? a.n_draft : 0);
+  const int seg = (int)(wg % sp.nseg), r = (int)(wg / sp.nseg % rows);
+  const Seq q(a, (int)(wg / sp.nseg / rows));
+  if (!q.there(a, r)) return;
+  Sums s{-FLT_MAX, 0.0f, 0.0f};
+  const float c = LOG2E / q.temperature(a, r);
+  auto go = [&](const auto &R) {
+    const int per = (R.chunks + sp.nseg - 1) / sp.nseg;
+    lane_sums(s, R, seg * per + (int)threadIdx.x, min(R.chunks, (seg + 1) * per), ST, c);
+  };
+  if (q.target(a, r))
+    go(Row<TB>(a.target, a.target_stride, q.row(a, r), (int)a.vocab, -1));
+  else
+    go(Row<DB>(a.draft, a.draft_stride, q.row(a, r), (int)a.vocab, -1));
+  join_wave(s, c);
+  if (lane_id() == 0) wm[threadIdx.x / WAVE] = s.m, wS[threadIdx.x / WAVE] = s.S;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  s = {wm[0], wS[0], 0.0f};
+#pragma unroll
+  for (int i = 1; i < ST / WAVE; i++) join(s, wm[i], wS[i], 0.0f, c);
+  w.stats[wg] = RowStat{s.m, s.S};
+}
+
+/* 2: the decision (by every block), and the sums of the rows that the token is drawn from, in 64
+ * bits and in one pass.  With P and Q the rows' sums, the weights are p_j / P - q_j / Q =
+ * (p_j - rho q_j) / P where that is positive, rho = P / Q.  P and Q are known only behind the pass,
+ * but the 32-bit sums give rho0, 1e-6 off at most, and with z = sum max(p_j - rho0 q_j, 0) and
+ * B = sum of q_j over the same places, z - (rho - rho0) B is the sum at rho, but for places where
+ * p_j - rho q_j changes its sign in between: those are 1e-6 q_j off at most and few.  Each wave leaves
+ * P, Q, z and B of its part; the last block of a sequence to arrive finds the part
+ * that passes u Z, and the place in it by the weights themselves.  (A pass for P and Q and another
+ * for the weights: 64 sequences of 151936, 49 us where this takes 32.) */
+template <bool TB, bool DB>
+__global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifySplit sp, VerifyRoom w) {
+  __shared__ Settled S;
+  __shared__ DrawLds<ST> L;
+  __shared__ uint32_t last;
+  const int tid = (int)threadIdx.x;
+  const int blk = (int)(blockIdx.x % (unsigned)sp.nblk);
+  const Seq q(a, (int)(blockIdx.x / (unsigned)sp.nblk));
+  const float u = lane_u(a, q), ud = a.u_draw[q.b];
+  if (tid < q.rows && q.there(a, tid)) {
+    const float l = draft_logit<TB, DB>(a, q, tid);
+    const float c = LOG2E / q.temperature(a, tid);
+    const RowStat *st = w.stats + ((int64_t)q.b * q.rows + tid) * sp.nseg;
+    Sums s{-FLT_MAX, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int i = 0; i < sp.nseg; i++) join(s, st[i].m, st[i].S, 0.0f, c);
+    settle_row(a, q, tid, RowStat{s.m, s.S}, l, S);
+  }
+  __syncthreads();
+  const Outcome o = settle(a, q, S, u, blk == 0);
+  const RowStat P = S.stat[o.accepted], Q = S.stat[o.rejected && a.draft ? a.n_draft + 1 + o.accepted : 0];
+  const bool masked = !o.refuse && P.S == 0.0f;
+  if (o.refuse || masked) {
+    if (blk != 0) return;
+    write_tokens(q.b, a.n_draft, o, masked ? 0 : -1, a.drafted, a.tokens, a.n_accepted);
+    if (tid == 0 && a.counters) atomicAdd(&a.counters[masked ? CNT_ALL_MASKED : CNT_REFUSED], 1u);
+    return;
+  }
+  Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, Q.m);
+  const double rho0 = W.dp && Q.S > 0.0f ? (double)P.S / Q.S : 0.0;
+  const int part = sp.block / SWV;
+  {
+    const int lo = blk * sp.block + tid / WAVE * part, hi = (int)min((int64_t)a.vocab, (int64_t)lo + part);
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int j = lo + lane_id() * 8; j < hi; j += WAVE * 8) {
+      double x[8], y[8];
+      W.terms(j, x, y);
+      if (W.dp) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const double d = fma(-rho0, y[e], x[e]);
+          sum[0] += x[e];
+          sum[1] += y[e];
+          sum[2] += d > 0.0 ? d : 0.0;
+          sum[3] += d > 0.0 ? y[e] : 0.0;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          sum[0] += x[e];
+          sum[2] += j + e == W.gone ? 0.0 : x[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] = wave_scan64(sum[i]);
+    uint64_t *out = w.parts + (((int64_t)q.b * sp.nblk + blk) * SWV + tid / WAVE) * 4;
+    if (lane_id() == WAVE - 1) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) st_agent(out + i, __builtin_bit_cast(uint64_t, sum[i]));
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t *cnt = w.arrivals + (int64_t)q.b * w.spacing;
+    last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(sp.nblk - 1);
+    if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  /* a thread the parts of a block (nblk <= ST) */
+  double at[SWV][4];
+#pragma unroll
+  for (int i = 0; i < SWV; i++)
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      at[i][k] = tid < sp.nblk ? __builtin_bit_cast(double, ld_agent(w.parts + (((int64_t)q.b * sp.nblk + tid) * SWV + i) * 4 + k)) : 0.0;
+  double p = 0.0, t = 0.0;
+#pragma unroll
+  for (int i = 0; i < SWV; i++) p += at[i][0], t += at[i][1];
+  const double sum_p = block_sum64(p, L), sum_q = W.dp ? block_sum64(t, L) : 0.0;
+  W.ip = 1.0 / sum_p;
+  W.iq = sum_q > 0.0 ? 1.0 / sum_q : 0.0;
+  const double shift = sum_q > 0.0 ? sum_p / sum_q - rho0 : 0.0;
+  int token = -1;
+  for (bool plain = !o.rejected; token < 0; plain = true) {
+    double mine[SWV], all = 0.0, Z;
+#pragma unroll
+    for (int i = 0; i < SWV; i++) {
+      mine[i] = W.ip * (plain ? at[i][0] : fmax(at[i][2] - shift * at[i][3], 0.0));
+      all += mine[i];
+    }
+    double from = block_scan64(all, L, &Z);
+    /* (p <= q everywhere, or by rounding alone not so: p's own draw) */
+    if (!(Z > 0.0) && !plain) continue;
+    const double bar = (double)ud * Z;
+    int over = 0x7fffffff, some = -1;
+    double over_from = 0.0, some_from = 0.0;
+#pragma unroll
+    for (int i = 0; i < SWV; i++) {
+      if (mine[i] > 0.0) {
+        some = tid * SWV + i, some_from = from;
+        if (over == 0x7fffffff && from + mine[i] > bar) over = some, over_from = from;
+      }
+      from += mine[i];
+    }
+    if (tid == 0) L.at = 0x7fffffff;
+    __syncthreads();
+    if (over != 0x7fffffff) atomicMin(&L.at, over);
     __syncthreads();
     if (L.at == 0x7fffffff) { /* none by rounding: the last that has any */
       __syncthreads();
       if (tid == 0) L.at = -1;
       __syncthreads();
-      if (mine > 0.0) atomicMax(&L.at, tid);
+      if (some >= 0) atomicMax(&L.at, some);
+      over = some, over_from = some_from;
       __syncthreads();
     }
-    const int who = L.at;
+    const int which = L.at;
+    if (over == which) L.from = over_from;
     __syncthreads();
-    if (tid == who) {
-      int at = -1;
-      for (int j = lo; j < hi; j++) {
-        const double w = weight(j);
-        base += w;
-        if (w > 0.0) {
-          at = j;
-          if (base > bar) break;
-        }
-      }
-      L.at = at;
-    }
-    __syncthreads();
-    token = L.at;
+    const double base = L.from;
+    token = pick<ST>(W, which * part, (int)min((int64_t)a.vocab, (int64_t)(which + 1) * part), base, bar, plain, L);
+    if (plain) break;
   }
-  write_tokens(b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
+  write_tokens(q.b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
 }
 
 /* ------------------------------------------------------------------------ */
 
 constexpr int RT = 256;
 
+/* A workgroup a sequence.  All its candidates are loaded at once where HELD entries hold
+ * them; else the drawn rows' again. */
 __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
+  constexpr int HELD = 2048;
   __shared__ float prob[2 * D3S_MAX_DRAFT];
-  __shared__ int cand[D3S_MAX_RANKED];
-  __shared__ float qs[D3S_MAX_RANKED];
+  __shared__ int cand[HELD];
+  __shared__ float qs[HELD];
   __shared__ float best[RT / WAVE];
   __shared__ int best_at[RT / WAVE];
   const int b = (int)blockIdx.x, tid = (int)threadIdx.x;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.n_draft) : a.n_draft;
-  const int32_t *x = a.drafted + (size_t)b * a.n_draft;
+  const int i = lane_id();
+  const int mine = i < a.n_draft ? a.drafted[(size_t)b * a.n_draft + i] : -1; /* lane i: draft i */
+  const float u = i < a.n_draft ? a.u_accept[(size_t)b * a.n_draft + i] : 0.0f;
   const size_t t0 = (size_t)b * (a.n_draft + 1) * a.target_k, d0 = (size_t)b * a.n_draft * a.draft_k;
+  const int nt = (len + 1) * a.target_k, nd = a.draft_cand ? len * a.draft_k : 0;
+  const bool held = nt + nd <= HELD;
   const float nan = __builtin_nanf("");
+  if (tid < 2 * D3S_MAX_DRAFT) prob[tid] = !a.draft_cand && tid >= D3S_MAX_DRAFT ? 1.0f : 0.0f;
+  __syncthreads();
   /* (a refused row's candidates are -1; a masked one's probabilities NaN, taken as 0) */
-  auto refused_t = [&](int i) { return a.target_cand[t0 + (size_t)i * a.target_k] < 0; };
-  for (int i = tid; i < len; i += RT) {
-    prob[i] = refused_t(i) ? nan : 0.0f;
-    prob[D3S_MAX_DRAFT + i] = !a.draft_cand ? 1.0f : a.draft_cand[d0 + (size_t)i * a.draft_k] < 0 ? nan : 0.0f;
-  }
-  __syncthreads();
-  for (int e = tid; e < len * a.target_k; e += RT) {
-    const int i = e / a.target_k;
-    if (x[i] >= 0 && a.target_cand[t0 + e] == x[i] && a.target_probs[t0 + e] > 0.0f) prob[i] = a.target_probs[t0 + e];
-  }
-  if (a.draft_cand)
-    for (int e = tid; e < len * a.draft_k; e += RT) {
-      const int i = e / a.draft_k;
-      if (x[i] >= 0 && a.draft_cand[d0 + e] == x[i] && a.draft_probs[d0 + e] > 0.0f)
-        prob[D3S_MAX_DRAFT + i] = a.draft_probs[d0 + e];
+  auto look = [&](const int32_t *c, const float *p, int k, int n, float *out, int at) {
+    for (int e0 = 0; e0 < n; e0 += RT) {
+      const int e = e0 + tid, row = e / k;
+      const int x = __shfl(mine, row & (WAVE - 1)); /* (row <= len <= 64: the row behind 63 drafts has none) */
+      if (e >= n) continue;
+      const int id = c[e];
+      const float pr = p[e];
+      if (held) cand[at + e] = id, qs[at + e] = pr;
+      if (row < len) {
+        if (id < 0) {
+          if (e == row * k) out[row] = nan;
+        } else if (id == x && pr > 0.0f) {
+          out[row] = pr;
+        }
+      }
     }
+  };
+  look(a.target_cand + t0, a.target_probs + t0, a.target_k, nt, prob, 0);
+  if (a.draft_cand) look(a.draft_cand + d0, a.draft_probs + d0, a.draft_k, nd, prob + D3S_MAX_DRAFT, nt);
+  const bool last_refused = a.target_cand[t0 + (size_t)len * a.target_k] < 0;
   __syncthreads();
-  auto p = [&](int i) { return prob[i]; };
-  auto q = [&](int i) { return prob[D3S_MAX_DRAFT + i]; };
-  const Outcome o = decide(len, a.u_accept + (size_t)b * a.n_draft, p, q, refused_t(len));
-  if (a.accept)
-    for (int i = tid; i < a.n_draft; i += RT)
-      a.accept[(size_t)b * a.n_draft + i] = i >= len ? 0.0f : p(i) != p(i) || q(i) != q(i) ? nan : accept_of(p(i), q(i));
+  const float p = i < len ? prob[i] : 0.0f, q = i < len ? prob[D3S_MAX_DRAFT + i] : 0.0f;
+  const Outcome o = decide(len, u, p, q, last_refused);
+  if (a.accept && tid < a.n_draft) a.accept[(size_t)b * a.n_draft + i] = i < len ? accept_of(p, q) : 0.0f;
   int token = -1;
   if (o.refuse) {
     if (tid == 0 && a.counters) atomicAdd(&a.counters[CNT_REFUSED], 1u);
   } else {
     const int32_t *tc = a.target_cand + t0 + (size_t)o.accepted * a.target_k;
     const float *tp = a.target_probs + t0 + (size_t)o.accepted * a.target_k;
-    if (o.rejected && a.draft_cand)
+    const bool pair = o.rejected && a.draft_cand;
+    const int qa = held ? nt + o.accepted * a.draft_k : 0; /* the draft's row in LDS */
+    if (pair && !held) { /* (draft_k <= D3S_MAX_RANKED <= HELD) */
       for (int e = tid; e < a.draft_k; e += RT) {
         cand[e] = a.draft_cand[d0 + (size_t)o.accepted * a.draft_k + e];
         qs[e] = a.draft_probs[d0 + (size_t)o.accepted * a.draft_k + e];
       }
-    __syncthreads();
+      __syncthreads();
+    }
+    const int x = o.rejected ? __shfl(mine, o.accepted) : -1;
     bool plain = !o.rejected;
     for (;;) {
       float sc = -2.0f;
       int at = 0x7fffffff;
       for (int r = tid; r < a.target_k; r += RT) {
-        float w = tp[r];
-        if (!plain && a.draft_cand) {
+        const int id = held ? cand[o.accepted * a.target_k + r] : tc[r];
+        float w = held ? qs[o.accepted * a.target_k + r] : tp[r];
+        if (!plain && pair) {
           for (int e = 0; e < a.draft_k; e++)
-            if (cand[e] == tc[r] && qs[e] > 0.0f) w -= qs[e];
-        } else if (!plain && tc[r] == x[o.accepted]) {
+            if (cand[qa + e] == id && qs[qa + e] > 0.0f) w -= qs[qa + e];
+        } else if (!plain && id == x) {
           w -= 1.0f;
         }
         if (!(w > 0.0f)) continue;
@@ -337,16 +709,70 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
 
 }  // namespace
 
-size_t verify_workspace_bytes(const d3s_verify_params &) { return 0; }
+/* Long rows of not too many sequences are split over the chip (beyond, a workgroup a
+ * sequence fills it). */
+static bool verify_split(const d3s_verify_params &a, VerifySplit *sp) {
+  if (a.vocab <= 16384 || a.n_seqs > 2048) return false;
+  const int64_t rows = a.n_seqs * (2 * a.n_draft + 1);
+  /* segments of two batches of bf16 chunks a lane, one where there are few */
+  const int64_t batches = ((a.vocab + 7) / 8 + SU * ST - 1) / (SU * ST);
+  sp->nseg = (int)(rows * batches <= 2048 ? batches : (batches + 1) / 2);
+  /* blocks of whole rounds of eight elements a thread: at most ST of them a row, about 1024 or more in all */
+  int64_t block = ST * 8;
+  while ((a.vocab + block - 1) / block > ST || (block < 16384 && a.n_seqs * ((a.vocab + block - 1) / block) > 2048)) block *= 2;
+  sp->block = (int)block;
+  sp->nblk = (int)((a.vocab + block - 1) / block);
+  return true;
+}
 
-void launch_verify(const d3s_verify_params &a, void *, hipStream_t s) {
-  const dim3 grid((unsigned)a.n_seqs);
-  auto go = [&](auto kernel) { kernel<<<grid, VT, 0, s>>>(a); };
+static size_t verify_layout(const d3s_verify_params &a, const VerifySplit &sp, char *base, VerifyRoom *w) {
+  size_t at = split_counter_bytes();
+  auto take = [&](size_t bytes) {
+    char *p = base + at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  const size_t n = (size_t)a.n_seqs;
+  w->arrivals = (uint32_t *)base;
+  w->spacing = 32;
+  w->stats = (RowStat *)take(n * (2 * (size_t)a.n_draft + 1) * sp.nseg * sizeof(RowStat));
+  w->parts = (uint64_t *)take(n * sp.nblk * SWV * 4 * sizeof(uint64_t));
+  return at;
+}
+
+size_t verify_workspace_bytes(const d3s_verify_params &a) {
+  VerifySplit sp;
+  VerifyRoom w;
+  return verify_split(a, &sp) ? verify_layout(a, sp, nullptr, &w) : 0;
+}
+
+template <bool TB, bool DB>
+static void verify_launch(const d3s_verify_params &a, void *ws, hipStream_t s) {
+  VerifySplit sp;
+  if (!verify_split(a, &sp)) {
+    const dim3 grid((unsigned)a.n_seqs);
+    if (a.vocab <= VT * 8)
+      k_verify_one<TB, DB, true><<<grid, VT, 0, s>>>(a);
+    else
+      k_verify_one<TB, DB, false><<<grid, VT, 0, s>>>(a);
+    return;
+  }
+  VerifyRoom w;
+  verify_layout(a, sp, (char *)ws, &w);
+  const int64_t wgs = a.n_seqs * (a.n_draft + 1 + (a.draft ? a.n_draft : 0)) * sp.nseg;
+  for (int64_t g = 0; g < wgs; g += GRID_MOST)
+    k_verify_rows<TB, DB><<<dim3((unsigned)(wgs - g < GRID_MOST ? wgs - g : GRID_MOST)), ST, 0, s>>>(a, sp, w, g);
+  const dim3 blocks((unsigned)(a.n_seqs * sp.nblk)); /* (at most 2048 * 256) */
+  k_verify_draw<TB, DB><<<blocks, ST, 0, s>>>(a, sp, w);
+}
+
+void launch_verify(const d3s_verify_params &params, void *ws, hipStream_t s) {
+  const d3s_verify_params a = params;
   const bool db = a.draft && a.draft_dtype == D3S_DTYPE_BF16;
   if (a.target_dtype == D3S_DTYPE_BF16)
-    db ? go(k_verify_one<true, true>) : go(k_verify_one<true, false>);
+    db ? verify_launch<true, true>(a, ws, s) : verify_launch<true, false>(a, ws, s);
   else
-    db ? go(k_verify_one<false, true>) : go(k_verify_one<false, false>);
+    db ? verify_launch<false, true>(a, ws, s) : verify_launch<false, false>(a, ws, s);
 }
 
 void launch_verify_ranked(const RankedArgs &args, hipStream_t s) {
