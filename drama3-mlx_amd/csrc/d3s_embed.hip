@@ -1,5 +1,6 @@
 /* k_embed, k_embed_grad: the rows that ids stand for, and their gradient in the
  * table (gfx950, wave64; include/d3s_step.h). */
+#include "d3s_rowcore.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
 
@@ -31,79 +32,334 @@ __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, int lanes, int64_t st
   }
 }
 
-constexpr int GR = 8;         /* rows of the table that a workgroup sums */
-constexpr int GC = ET * 8;    /* by columns */
-constexpr int LOOK = ET * 4;  /* ids looked at together */
+/* ---- the gradient ----
+ * k_embed_group: a workgroup takes a range of the table's rows, looks through all ids (of its
+ * slot) and writes the positions of its rows' ids, grouped by row and in their order:
+ * the positions follow each other in `order` behind those of lower rows, which it counts
+ * as it goes (a counter that each workgroup raises takes 23 ns a workgroup: 26 us for 1187), and seg
+ * says for each row where and how many.
+ * k_embed_sum: a row's positions are summed in that order, by lanes across its columns;
+ * rows that no id names are filled with zeros.  A row of more than `hot` positions is cut into chunks
+ * of as many, filed in a list; workgroups of their own sum the chunks in fp32, and the last
+ * of a row to arrive adds its chunks in order.  No atomics on floating-point values. */
 
-/* GR rows of one slot's part by GC columns, summed in LDS: the ids are looked
- * through in order, and those of these rows gathered in that order. */
-template <bool DB, bool GB>
-__global__ __launch_bounds__(ET) void k_embed_grad(EmbedArgs a, int64_t slots, int64_t part, int64_t blocks_part,
-                                                   int64_t strips, int64_t blocks) {
-  __shared__ float sum[GR][GC];
-  __shared__ int64_t found[LOOK];
-  __shared__ int which[LOOK];
-  __shared__ int counts[ET / WAVE];
-  const int tid = (int)threadIdx.x;
-  const int64_t n = slots > 1 ? a.n_rows : a.n_rows * a.n_ids; /* ids to look through */
-  for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-    const int64_t strip = blk % strips, slot = blk / strips / blocks_part;
-    const int64_t v0 = blk / strips % blocks_part * GR;
-    const int64_t j = strip * GC + tid * 8;
-    const int left = j < a.width ? (int)min((int64_t)8, a.width - j) : 0;
-    for (int r = 0; r < GR; r++)
-      for (int e = 0; e < 8; e++) sum[r][e * ET + tid] = 0.0f;
-    for (int64_t base = 0; base < n; base += LOOK) {
-      /* a thread's four ids follow each other */
-      int hit[4], mine = 0;
-      for (int u = 0; u < 4; u++) {
-        const int64_t i = base + tid * 4 + u;
-        hit[u] = -1;
-        if (i < n) {
-          const int id = a.ids[slots > 1 ? i * a.n_ids + slot : i];
-          if (id >= v0 && id < v0 + GR && id < a.vocab) hit[u] = (int)(id - v0), mine++;
-        }
-      }
-      const uint32_t incl = wave_scan_add_u32((uint32_t)mine);
-      __syncthreads();
-      if (lane_id() == WAVE - 1) counts[tid / WAVE] = (int)incl;
-      __syncthreads();
-      int at = (int)incl - mine, total = 0;
-      for (int w = 0; w < ET / WAVE; w++) {
-        if (w < tid / WAVE) at += counts[w];
-        total += counts[w];
-      }
-      for (int u = 0; u < 4; u++)
-        if (hit[u] >= 0) {
-          const int64_t i = base + tid * 4 + u;
-          found[at] = slots > 1 ? i : i / a.n_ids;
-          which[at++] = hit[u];
-        }
-      __syncthreads();
-      for (int f = 0; f < total && left > 0; f++) {
-        float d[8];
-        load8<DB>((const char *)a.in + found[f] * a.in_stride * (DB ? 2 : 4), j, left, d);
+constexpr int GW = ET / WAVE;
+constexpr int LIST = 512;         /* positions that a wave keeps in LDS (more: the ids are looked through again) */
+constexpr int AHEAD = 16;         /* ids that a lane loads at a time */
+constexpr int RANGE_MOST = 2048;  /* rows of the table that a workgroup takes: 32 KiB of counts */
+constexpr int HOT_GROUPS = 512;   /* workgroups for the chunks */
+constexpr int HOT_MOST = 4096;    /* rows that are cut, at most: a counter of arrivals each */
+constexpr int HOT_COUNTERS = 64;  /* words before them */
+
+struct Seg {
+  int start, count; /* count < 0: cut into chunks */
+};
+struct Chunk {
+  int64_t row;
+  int start, count, first, chunks, hot, pad; /* first: the row's first chunk */
+};
+/* the counters that the calls leave at zero: chunks, rows cut, arrivals */
+enum { CNT_CHUNKS = 0, CNT_HOT = 16, CNT_DONE = 32 };
+
+struct GradPlan {
+  int64_t slots, part, rows, n; /* parts of the table, rows of each and in all, ids of each */
+  int range, hot;               /* rows of a range; a row of more positions is cut */
+  int64_t ranges;               /* of each part */
+};
+struct GradRoom {
+  uint32_t *counters;
+  Seg *seg;
+  int *order;
+  Chunk *chunks;
+  float *sums; /* a chunk's, [.., width] */
+};
+
+GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) {
+  GradPlan p;
+  p.slots = slot_rows ? n_ids : 1;
+  p.part = slot_rows ? slot_rows : vocab;
+  p.rows = vocab + (n_ids - 1) * slot_rows;
+  p.n = slot_rows ? n_rows : n_rows * n_ids;
+  /* ranges of 64 rows, wider while looking through the ids for each would read more than 128 MB and
+   * there are more ranges than CUs (TBD) */
+  p.range = 64;
+  auto count = [&](int64_t r) { return (vocab + r - 1) / r; };
+  while (p.range < RANGE_MOST && p.slots * count(p.range) > 512 && p.slots * count(p.range) * p.n > (int64_t)32 << 20) p.range *= 2;
+  p.ranges = count(p.range);
+  p.hot = 64;
+  while ((int64_t)p.hot * HOT_MOST < p.n * p.slots) p.hot *= 2;
+  return p;
+}
+/* chunks at most: each full, but the last of a row that is cut */
+int64_t chunks_most(const GradPlan &p) { return 2 * (p.n * p.slots / p.hot) + 1; }
+
+size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
+  size_t at = split_counter_bytes();
+  auto take = [&](size_t bytes) {
+    char *q = base + at;
+    at += (bytes + 255) / 256 * 256;
+    return q;
+  };
+  w->counters = (uint32_t *)base;
+  w->seg = (Seg *)take((size_t)p.rows * sizeof(Seg));
+  w->order = (int *)take((size_t)(p.n * p.slots) * sizeof(int));
+  w->chunks = (Chunk *)take((size_t)chunks_most(p) * sizeof(Chunk));
+  w->sums = (float *)take((size_t)chunks_most(p) * (size_t)((width + 7) / 8 * 8) * sizeof(float));
+  return at;
+}
+
+__global__ __launch_bounds__(ET) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
+  extern __shared__ int cnt[]; /* [GW][range]: a wave's count of a row, then its place */
+  __shared__ int list_pos[GW][LIST];
+  __shared__ uint16_t list_row[GW][LIST];
+  __shared__ int wave_sum[GW], wave_less[GW];
+  const int tid = (int)threadIdx.x, wid = tid / WAVE, lane = lane_id();
+  int bits = 0;
+  while ((1 << bits) < p.range) bits++;
+  const int n = (int)p.n, each = (n / GW + WAVE) / WAVE * WAVE; /* ids of a wave */
+  const int step = a.slot_rows ? a.n_ids : 1;                   /* (the last is below 2^31) */
+  for (int64_t blk = blockIdx.x; blk < p.slots * p.ranges; blk += gridDim.x) {
+    const int64_t slot = blk / p.ranges, v0 = blk % p.ranges * p.range;
+    const uint32_t rows = (uint32_t)min((int64_t)p.range, a.vocab - v0);
+    const int i0 = (int)min((int64_t)n, (int64_t)wid * each), i1 = (int)min((int64_t)n, (int64_t)i0 + each);
+    const int32_t *ids = a.slot_rows ? a.ids + slot : a.ids;
+    for (int i = tid; i < GW * p.range; i += ET) cnt[i] = 0;
+    __syncthreads();
+    int *mine = cnt + wid * p.range;
+    /* f(position, row, whether it is this range's, which lanes' are) for the wave's ids in their order, 64 at a time
+     * (an id below 0 is a row past 2^31 - v0 here); and the number of ids of lower rows */
+    int less = 0;
+    auto look = [&](auto f) {
+      int id[AHEAD];
+      int i = i0;
+      less = 0;
+      for (; i1 - i >= AHEAD * WAVE; i += AHEAD * WAVE) {
+        bool any = false;
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum[which[f]][e * ET + tid] += d[e];
+        for (int u = 0; u < AHEAD; u++) id[u] = ids[(uint32_t)(i + u * WAVE + lane) * (uint32_t)step];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+          any |= (uint32_t)id[u] - (uint32_t)v0 < rows;
+          less += (int)__popcll(__ballot((uint32_t)id[u] < (uint32_t)v0));
+        }
+        if (__ballot(any) == 0ull) continue;
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+          const uint32_t row = (uint32_t)id[u] - (uint32_t)v0;
+          const uint64_t hits = __ballot(row < rows);
+          if (hits) f(i + u * WAVE + lane, (int)row, row < rows, hits);
+        }
       }
-    }
-    for (int r = 0; r < GR && left > 0; r++) {
-      if (v0 + r >= part) break;
+      for (; i < i1; i += WAVE) {
+        const int at = i + lane;
+        const uint32_t one = at < i1 ? (uint32_t)ids[(uint32_t)at * (uint32_t)step] : 0xffffffffu, row = one - (uint32_t)v0;
+        const uint64_t hits = __ballot(row < rows);
+        less += (int)__popcll(__ballot(one < (uint32_t)v0));
+        if (hits) f(at, (int)row, row < rows, hits);
+      }
+    };
+    auto below = [&](uint64_t m) {
+      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+    };
+    int found = 0;
+    look([&](int at, int row, bool hit, uint64_t hits) {
+      const int k = found + below(hits);
+      if (hit) {
+        atomicAdd(&mine[row], 1);
+        if (k < LIST) list_pos[wid][k] = at, list_row[wid][k] = row;
+      }
+      found += (int)__popcll(hits);
+    });
+    __syncthreads();
+    /* the rows' places: a thread `per` rows in a row */
+    const int per = (p.range + ET - 1) / ET, r0 = min(p.range, tid * per), r1 = min(p.range, r0 + per);
+    int total = 0;
+    for (int r = r0; r < r1; r++)
+      for (int g = 0; g < GW; g++) total += cnt[g * p.range + r];
+    const int incl = (int)wave_scan_add_u32((uint32_t)total);
+    if (lane == WAVE - 1) wave_sum[wid] = incl, wave_less[wid] = less;
+    __syncthreads();
+    int start = (int)(slot * p.n) + incl - total;
+    for (int g = 0; g < GW; g++) start += wave_less[g] + (g < wid ? wave_sum[g] : 0);
+    for (int r = r0; r < r1 && (uint32_t)r < rows; r++) {
+      const int from = start;
+      for (int g = 0; g < GW; g++) {
+        const int c = cnt[g * p.range + r];
+        cnt[g * p.range + r] = start;
+        start += c;
+      }
+      const int n = start - from;
       const int64_t row = slot * a.slot_rows + v0 + r;
-      if (a.slot_rows && slot == slots - 1 && v0 + r >= a.vocab) break;
-      if (a.accumulate && v0 + r >= a.vocab) break;
-      char *out = (char *)a.out + row * a.out_stride * (GB ? 2 : 4);
-      float v[8], o[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = sum[r][e * ET + tid] * a.scale;
-      if (a.accumulate) {
-        load8<GB>(out, j, left, o);
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += o[e];
+      w.seg[row] = Seg{from, n > p.hot ? -n : n};
+      if (n > p.hot) {
+        const int chunks = (n + p.hot - 1) / p.hot;
+        const int hot = (int)atomicAdd(&w.counters[CNT_HOT], 1u), first = (int)atomicAdd(&w.counters[CNT_CHUNKS], (uint32_t)chunks);
+        for (int c = 0; c < chunks; c++)
+          w.chunks[first + c] = Chunk{row, from + c * p.hot, min(p.hot, n - c * p.hot), first, chunks, hot, 0};
       }
-      store8<GB>(out, j, left, v);
     }
     __syncthreads();
+    /* the positions: lanes of one row find each other by ballots of its bits */
+    auto place = [&](int at, int row, bool hit, uint64_t hits) {
+      uint64_t peers = hits;
+      for (int b = 0; b < bits; b++) {
+        const uint64_t m = __ballot(hit && (row >> b & 1));
+        peers &= row >> b & 1 ? m : ~m;
+      }
+      const int k = below(peers);
+      if (hit) {
+        const int to = mine[row] + k;
+        w.order[to] = a.slot_rows ? at : at / a.n_ids;
+      }
+      wave_lds_sync();
+      if (hit && (peers >> lane) >> 1 == 0ull) mine[row] += k + 1; /* the last of them */
+      wave_lds_sync();
+    };
+    if (found <= LIST) {
+      for (int e = 0; e < found; e += WAVE) {
+        const bool hit = e + lane < found;
+        const int at = hit ? list_pos[wid][e + lane] : 0, row = hit ? list_row[wid][e + lane] : 0;
+        place(at, row, hit, __ballot(hit));
+      }
+    } else {
+      look(place);
+    }
+    __syncthreads();
+  }
+}
+
+/* the sum of n rows of dy, at the positions `at`, eight columns from j on */
+template <bool DB>
+__device__ __forceinline__ void add_rows(const EmbedArgs &a, const int *at, int n, int64_t j, int left, float *v) {
+  constexpr int UN = 4;
+  int k = 0;
+  auto row = [&](int i) { return (const char *)a.in + (int64_t)at[i] * a.in_stride * (DB ? 2 : 4); };
+  for (; k + UN <= n; k += UN) {
+    Vec8<DB> q[UN];
+#pragma unroll
+    for (int u = 0; u < UN; u++) q[u].load_some(row(k + u), j, left);
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      float d[8];
+      q[u].values(d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += d[e];
+    }
+  }
+  for (; k < n; k++) {
+    Vec8<DB> q;
+    float d[8];
+    q.load_some(row(k), j, left);
+    q.values(d);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += d[e];
+  }
+}
+
+template <bool GB>
+__device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t j, int left, float *v) {
+  char *out = (char *)a.out + row * a.out_stride * (GB ? 2 : 4);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] *= a.scale;
+  if (a.accumulate) {
+    float o[8];
+    load8<GB>(out, j, left, o);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += o[e];
+  }
+  store8<GB>(out, j, left, v);
+}
+
+/* Rows that a thread takes one after the other: a workgroup writes 16 KiB.  (40970 rows of 2048 fp32: one
+ * 75 us, two 74, four 110; 151936 of 1024 bf16: one 85 us, two 71, four 64, eight 66.  Loading
+ * the rows' first positions and their dy together, 64 to 70; a strip of columns for each
+ * XCD, so that dy stays in its L2, 110 to 132; stores through the caches, 74 to 80 and 64 to 128.) */
+template <bool GB>
+constexpr int sum_rows() { return GB ? 4 : 2; }
+
+template <bool DB, bool GB>
+__global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
+                                                  int hot_groups) {
+  constexpr int SUM_ROWS = sum_rows<GB>();
+  const int tid = (int)threadIdx.x;
+  if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut */
+    __shared__ uint32_t last;
+    const int64_t stride = (a.width + 7) / 8 * 8;
+    const int chunks = (int)w.counters[CNT_CHUNKS];
+    for (int c = (int)blockIdx.x; c < chunks; c += hot_groups) {
+      const Chunk k = w.chunks[c];
+      for (int64_t j = tid * 8; j < a.width; j += ET * 8) {
+        const int left = (int)min((int64_t)8, a.width - j);
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        add_rows<DB>(a, w.order + k.start, k.count, j, left, v);
+        uint64_t *out = (uint64_t *)(w.sums + c * stride + j);
+#pragma unroll
+        for (int e = 0; e < 4; e++) st_agent(out + e, (uint64_t)d3s_f2u(v[2 * e]) | (uint64_t)d3s_f2u(v[2 * e + 1]) << 32);
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) {
+        uint32_t *cnt = w.counters + HOT_COUNTERS + k.hot;
+        last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.chunks - 1);
+        if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+      if (last)
+        for (int64_t j = tid * 8; j < a.width; j += ET * 8) {
+          const int left = (int)min((int64_t)8, a.width - j);
+          float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+          for (int i = 0; i < k.chunks; i++) {
+            const uint64_t *in = (const uint64_t *)(w.sums + (k.first + i) * stride + j);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint64_t q = ld_agent(in + e);
+              v[2 * e] += d3s_u2f((uint32_t)q);
+              v[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
+            }
+          }
+          put_row<GB>(a, k.row, j, left, v);
+        }
+      __syncthreads();
+    }
+    /* the last to end clears what k_embed_group counted */
+    if (tid == 0 && __hip_atomic_fetch_add(w.counters + CNT_DONE, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(hot_groups - 1)) {
+      for (int c : {CNT_CHUNKS, CNT_HOT, CNT_DONE})
+        __hip_atomic_store(w.counters + c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return;
+  }
+  const int across = tid % lanes, down = tid / lanes, at_once = ET / lanes;
+  for (int64_t blk = blockIdx.x - hot_groups; blk < blocks; blk += gridDim.x - hot_groups) {
+    const int64_t row0 = blk / strips * (at_once * SUM_ROWS) + down;
+    const int64_t j = (blk % strips * lanes + across) * 8;
+    if (j >= a.width) continue;
+    const int left = (int)min((int64_t)8, a.width - j);
+    Seg seg[SUM_ROWS];
+#pragma unroll
+    for (int i = 0; i < SUM_ROWS; i++) {
+      const int64_t row = row0 + i * at_once;
+      const bool named = row < p.rows && (a.slot_rows == a.vocab || a.slot_rows == 0 || row % a.slot_rows < a.vocab);
+      seg[i] = named ? w.seg[row] : Seg{0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < SUM_ROWS; i++) {
+      const int64_t row = row0 + i * at_once;
+      if (row >= p.rows || seg[i].count < 0 || (a.accumulate && seg[i].count == 0)) continue;
+      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      add_rows<DB>(a, w.order + seg[i].start, seg[i].count, j, left, v);
+      put_row<GB>(a, row, j, left, v);
+    }
+  }
+}
+
+/* the table's gradient where there are no ids */
+template <bool GB>
+__global__ __launch_bounds__(ET) void k_embed_zero(EmbedArgs a, int64_t rows, int64_t strips) {
+  const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t blk = blockIdx.x; blk < rows * strips; blk += gridDim.x) {
+    const int64_t j = (blk % strips * ET + threadIdx.x) * 8;
+    if (j < a.width) store8<GB>((char *)a.out + blk / strips * a.out_stride * (GB ? 2 : 4), j, (int)min((int64_t)8, a.width - j), zero);
   }
 }
 
@@ -123,19 +379,40 @@ void launch_embed(const EmbedArgs &args, Dtype in, Dtype out, hipStream_t s) {
     out == DT_BF16 ? go(k_embed<false, true>) : go(k_embed<false, false>);
 }
 
-size_t embed_grad_workspace_bytes(int64_t, int, int64_t, int64_t, int64_t) { return 0; }
+size_t embed_grad_workspace_bytes(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, int64_t width) {
+  if (n_rows == 0 || width == 0) return 0;
+  GradRoom w;
+  return grad_layout(grad_plan(n_rows, n_ids, vocab, slot_rows), width, nullptr, &w);
+}
 
-void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *, hipStream_t s) {
+void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hipStream_t s) {
   const EmbedArgs a = args;
-  const int64_t slots = a.slot_rows ? a.n_ids : 1, part = a.slot_rows ? a.slot_rows : a.vocab;
-  const int64_t blocks_part = (part + GR - 1) / GR, strips = (a.width + GC - 1) / GC;
-  const int64_t blocks = slots * blocks_part * strips;
-  const dim3 grid((unsigned)(blocks < STEP_GRID ? blocks : STEP_GRID));
-  auto go = [&](auto kernel) { kernel<<<grid, ET, 0, s>>>(a, slots, part, blocks_part, strips, blocks); };
+  auto grid = [](int64_t n) { return dim3((unsigned)(n < STEP_GRID ? n : STEP_GRID)); };
+  const GradPlan p = grad_plan(a.n_rows, a.n_ids, a.vocab, a.slot_rows);
+  if (a.n_rows == 0) {
+    const int64_t strips = (a.width + ET * 8 - 1) / (ET * 8);
+    if (out == DT_BF16)
+      k_embed_zero<true><<<grid(p.rows * strips), ET, 0, s>>>(a, p.rows, strips);
+    else
+      k_embed_zero<false><<<grid(p.rows * strips), ET, 0, s>>>(a, p.rows, strips);
+    return;
+  }
+  GradRoom w;
+  grad_layout(p, a.width, (char *)ws, &w);
+  k_embed_group<<<grid(p.slots * p.ranges), ET, GW * p.range * sizeof(int), s>>>(a, p, w);
+  int lanes = 1;
+  while (lanes < ET && (int64_t)lanes * 8 < a.width) lanes *= 2;
+  const int64_t strips = (a.width + lanes * 8 - 1) / (lanes * 8), rows = ET / lanes * (out == DT_BF16 ? sum_rows<true>() : sum_rows<false>());
+  const int64_t blocks = strips * ((p.rows + rows - 1) / rows);
+  const int64_t most = chunks_most(p);
+  const int hot_groups = (int)(most < HOT_GROUPS ? most : HOT_GROUPS);
+  auto go = [&](auto kernel) {
+    kernel<<<dim3((unsigned)(hot_groups + (blocks < STEP_GRID ? blocks : STEP_GRID))), ET, 0, s>>>(a, p, w, lanes, strips, blocks, hot_groups);
+  };
   if (in == DT_BF16)
-    out == DT_BF16 ? go(k_embed_grad<true, true>) : go(k_embed_grad<true, false>);
+    out == DT_BF16 ? go(k_embed_sum<true, true>) : go(k_embed_sum<true, false>);
   else
-    out == DT_BF16 ? go(k_embed_grad<false, true>) : go(k_embed_grad<false, false>);
+    out == DT_BF16 ? go(k_embed_sum<false, true>) : go(k_embed_sum<false, false>);
 }
 
 }  // namespace d3s

@@ -50,7 +50,7 @@ int embed_grad_check(const int32_t *ids, int64_t n_rows, int n_ids, const void *
                      int64_t grad_stride) {
   if (!known(dtype) || !known(grad_dtype)) return D3S_ERR_DTYPE;
   if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || (slot_rows != 0 && slot_rows < vocab) ||
-      !stride_ok(dy_stride, width) || !stride_ok(grad_stride, width))
+      n_rows > INT_MOST / n_ids || !stride_ok(dy_stride, width) || !stride_ok(grad_stride, width))
     return D3S_ERR_ARG;
   if (width == 0) return D3S_OK;
   if (!grad || off(grad, size_of(grad_dtype))) return D3S_ERR_ARG;
@@ -160,7 +160,9 @@ int d3s_embed_backward(const int32_t *ids, int64_t n_rows, int n_ids, const void
 }
 
 int64_t d3s_embed_backward_workspace_bytes(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, int64_t width) {
-  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || (slot_rows != 0 && slot_rows < vocab)) return D3S_ERR_ARG;
+  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || (slot_rows != 0 && slot_rows < vocab) ||
+      n_rows > INT_MOST / n_ids)
+    return D3S_ERR_ARG;
   return (int64_t)embed_grad_workspace_bytes(n_rows, n_ids, vocab, slot_rows, width);
 }
 

@@ -118,7 +118,7 @@ int d3s_embed(const int32_t *ids, int64_t n_rows, int n_ids, const void *table, 
  * accumulate not 0, added to what is there before the rounding, else rows that no id
  * names are zeros (those between two slots' parts too).  dy [n_rows, width], grad
  * [vocab (+ (n_ids - 1) slot_rows), width]; fp32 or bf16 each.  slot_rows is 0
- * or at least vocab. */
+ * or at least vocab; n_rows * n_ids is below 2^31. */
 int d3s_embed_backward(const int32_t *ids, int64_t n_rows, int n_ids, const void *dy, int dtype, int64_t dy_stride,
                        int64_t vocab, int64_t slot_rows, int64_t width, float scale, int accumulate, void *grad,
                        int grad_dtype, int64_t grad_stride, void *stream);
