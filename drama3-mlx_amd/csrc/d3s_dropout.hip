@@ -8,63 +8,82 @@ namespace {
 
 constexpr int DT_ = 256;
 
-/* a workgroup takes DT_ / lanes rows by 8 * lanes columns */
+/* a workgroup takes DT_ / lanes rows by E * lanes columns */
 struct DropSplit {
   int lanes;
   int64_t strips, blocks;
 };
 
-DropSplit drop_split(int64_t rows, int64_t width) {
+DropSplit drop_split(int64_t rows, int64_t width, int E) {
   DropSplit s;
   s.lanes = 1;
-  while (s.lanes < DT_ && (int64_t)s.lanes * 8 < width) s.lanes *= 2;
-  s.strips = (width + s.lanes * 8 - 1) / (s.lanes * 8);
+  while (s.lanes < DT_ && (int64_t)s.lanes * E < width) s.lanes *= 2;
+  s.strips = (width + s.lanes * E - 1) / (s.lanes * E);
   s.blocks = s.strips * ((rows + DT_ / s.lanes - 1) / (DT_ / s.lanes));
   return s;
 }
 
-template <bool BF16>
+/* WHOLE: every lane's first element is a multiple of four in the generator's count, so that its
+ * words are whole blocks of Philox; else it draws one block more and takes its words from
+ * among them. */
+template <bool BF16, bool WHOLE>
 __global__ __launch_bounds__(DT_) void k_dropout(DropoutArgs a, DropSplit sp) {
+  constexpr int E = BF16 ? 8 : 4, ES = BF16 ? 2 : 4, B = E / 4 + (WHOLE ? 0 : 1);
   const int across = (int)threadIdx.x % sp.lanes, down = (int)threadIdx.x / sp.lanes;
   const uint64_t draw = a.draw + (a.draw_add ? *a.draw_add : 0u);
   for (int64_t blk = blockIdx.x; blk < sp.blocks; blk += gridDim.x) {
     const int64_t row = blk / sp.strips * (DT_ / sp.lanes) + down;
-    const int64_t j = (blk % sp.strips * sp.lanes + across) * 8;
-    if (row >= a.n_rows || j >= a.width) continue;
-    const int left = (int)min((int64_t)8, a.width - j);
-    const char *x = (const char *)a.x + row * a.x_stride * (BF16 ? 2 : 4);
-    char *y = (char *)a.y + row * a.y_stride * (BF16 ? 2 : 4);
-    float v[8], r[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    load8<BF16>(x, j, left, v);
-    if (a.residual) load8<BF16>((const char *)a.residual + row * a.residual_stride * (BF16 ? 2 : 4), j, left, r);
+    const int64_t j = (blk % sp.strips * sp.lanes + across) * E, left = a.width - j;
+    if (row >= a.n_rows || left <= 0) continue;
+    Vec<BF16, E> x, r;
+    x.load_some((const char *)a.x + row * a.x_stride * ES, j, left);
+    if (a.residual) r.load_some((const char *)a.residual + row * a.residual_stride * ES, j, left);
     const uint64_t at = (uint64_t)row * (uint64_t)a.width + (uint64_t)j;
+    uint32_t w[4 * B];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      d3s_u32x4 c;
-      const uint64_t q = (at + e) >> 2;
-      c.v[0] = (uint32_t)q;
-      c.v[1] = (uint32_t)(q >> 32);
-      c.v[2] = (uint32_t)draw;
-      c.v[3] = (uint32_t)(draw >> 32);
-      const d3s_u32x4 o = d3s_philox4x32_10(c, (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
-      const uint32_t i = (uint32_t)(at + e) & 3u;
-      const uint32_t w = i == 0 ? o.v[0] : i == 1 ? o.v[1] : i == 2 ? o.v[2] : o.v[3];
-      v[e] = ((w >> 8) >= a.least ? v[e] * a.scale : 0.0f) + r[e];
+    for (int b = 0; b < B; b++) {
+      const uint64_t q = (at >> 2) + b;
+      const d3s_u32x4 o = d3s_philox4x32_10({{(uint32_t)q, (uint32_t)(q >> 32), (uint32_t)draw, (uint32_t)(draw >> 32)}},
+                                            (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[4 * b + i] = o.v[i];
     }
-    store8<BF16>(y, j, left, v);
+    if constexpr (!WHOLE) { /* the words from at & 3 on */
+      const uint32_t s = (uint32_t)at & 3u;
+#pragma unroll
+      for (int e = 0; e < E + 2; e++) w[e] = s & 1u ? w[e + 1] : w[e];
+#pragma unroll
+      for (int e = 0; e < E; e++) w[e] = s & 2u ? w[e + 2] : w[e];
+    }
+    float v[E], o[E];
+    x.values(v);
+    if (a.residual) r.values(o);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      v[e] = (w[e] >> 8) >= a.least ? v[e] * a.scale : 0.0f;
+      if (a.residual) v[e] += o[e];
+    }
+    store_row<BF16, E>((char *)a.y + row * a.y_stride * ES, j, left, v);
   }
 }
 
 }  // namespace
 
 void launch_dropout(const DropoutArgs &args, Dtype dt, hipStream_t s) {
-  const DropoutArgs a = args;
-  const DropSplit sp = drop_split(a.n_rows, a.width);
+  DropoutArgs a = args;
+  /* rows that follow each other are one */
+  if (a.x_stride == a.width && a.y_stride == a.width && (!a.residual || a.residual_stride == a.width)) {
+    a.width *= a.n_rows;
+    a.n_rows = 1;
+  }
+  const DropSplit sp = drop_split(a.n_rows, a.width, dt == DT_BF16 ? 8 : 4);
   const dim3 grid((unsigned)(sp.blocks < STEP_GRID ? sp.blocks : STEP_GRID));
+  auto go = [&](auto kernel) { kernel<<<grid, DT_, 0, s>>>(a, sp); };
+  const bool whole = a.n_rows == 1 || a.width % 4 == 0;
   if (dt == DT_BF16)
-    k_dropout<true><<<grid, DT_, 0, s>>>(a, sp);
+    whole ? go(k_dropout<true, true>) : go(k_dropout<true, false>);
   else
-    k_dropout<false><<<grid, DT_, 0, s>>>(a, sp);
+    whole ? go(k_dropout<false, true>) : go(k_dropout<false, false>);
 }
 
 }  // namespace d3s

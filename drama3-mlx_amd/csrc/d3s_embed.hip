@@ -9,26 +9,41 @@ namespace {
 
 constexpr int ET = 256;
 
-template <bool TB, bool YB>
+/* A thread E columns of a row, its ids' rows loaded together (UN at a time). */
+template <bool TB, bool YB, int UN>
 __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, int lanes, int64_t strips, int64_t blocks) {
+  constexpr int E = YB ? 8 : 4;
   const int across = (int)threadIdx.x % lanes, down = (int)threadIdx.x / lanes;
   for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
     const int64_t row = blk / strips * (ET / lanes) + down;
-    const int64_t j = (blk % strips * lanes + across) * 8;
+    const int64_t j = (blk % strips * lanes + across) * E;
     if (row >= a.n_rows || j >= a.width) continue;
-    const int left = (int)min((int64_t)8, a.width - j);
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    for (int t = 0; t < a.n_ids; t++) {
-      const int id = a.ids[row * a.n_ids + t];
-      if ((uint32_t)id >= (uint64_t)a.vocab) continue;
-      float w[8];
-      load8<TB>((const char *)a.in + (t * a.slot_rows + id) * a.in_stride * (TB ? 2 : 4), j, left, w);
+    const int64_t left = a.width - j;
+    const int32_t *ids = a.ids + row * a.n_ids;
+    float v[E];
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] += w[e];
+    for (int e = 0; e < E; e++) v[e] = 0.0f;
+    for (int t = 0; t < a.n_ids; t += UN) {
+      int id[UN];
+      Vec<TB, E> q[UN];
+#pragma unroll
+      for (int u = 0; u < UN; u++) id[u] = t + u < a.n_ids ? ids[t + u] : -1;
+#pragma unroll
+      for (int u = 0; u < UN; u++) {
+        const bool live = (uint32_t)id[u] < (uint64_t)a.vocab;
+        q[u].load_some((const char *)a.in + ((t + u) * a.slot_rows + (live ? id[u] : 0)) * a.in_stride * (TB ? 2 : 4), j, live ? left : 0);
+      }
+#pragma unroll
+      for (int u = 0; u < UN; u++) {
+        float w[E];
+        q[u].values(w);
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] += w[e];
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= a.scale;
-    store8<YB>((char *)a.out + row * a.out_stride * (YB ? 2 : 4), j, left, v);
+    for (int e = 0; e < E; e++) v[e] *= a.scale;
+    store_row<YB, E>((char *)a.out + row * a.out_stride * (YB ? 2 : 4), j, left, v);
   }
 }
 
@@ -228,59 +243,60 @@ __global__ __launch_bounds__(ET) void k_embed_group(EmbedArgs a, GradPlan p, Gra
   }
 }
 
-/* the sum of n rows of dy, at the positions `at`, eight columns from j on */
-template <bool DB>
-__device__ __forceinline__ void add_rows(const EmbedArgs &a, const int *at, int n, int64_t j, int left, float *v) {
+/* the sum of n rows of dy, at the positions `at`, E columns from j on */
+template <bool DB, int E>
+__device__ __forceinline__ void add_rows(const EmbedArgs &a, const int *at, int n, int64_t j, int64_t left, float *v) {
   constexpr int UN = 4;
   int k = 0;
   auto row = [&](int i) { return (const char *)a.in + (int64_t)at[i] * a.in_stride * (DB ? 2 : 4); };
   for (; k + UN <= n; k += UN) {
-    Vec8<DB> q[UN];
+    Vec<DB, E> q[UN];
 #pragma unroll
     for (int u = 0; u < UN; u++) q[u].load_some(row(k + u), j, left);
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-      float d[8];
+      float d[E];
       q[u].values(d);
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] += d[e];
+      for (int e = 0; e < E; e++) v[e] += d[e];
     }
   }
   for (; k < n; k++) {
-    Vec8<DB> q;
-    float d[8];
-    q.load_some(row(k), j, left);
-    q.values(d);
+    float d[E];
+    load_row<DB, E>(row(k), j, left, d);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] += d[e];
+    for (int e = 0; e < E; e++) v[e] += d[e];
   }
 }
 
-template <bool GB>
-__device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t j, int left, float *v) {
+template <bool GB, int E>
+__device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t j, int64_t left, float *v) {
   char *out = (char *)a.out + row * a.out_stride * (GB ? 2 : 4);
 #pragma unroll
-  for (int e = 0; e < 8; e++) v[e] *= a.scale;
+  for (int e = 0; e < E; e++) v[e] *= a.scale;
   if (a.accumulate) {
-    float o[8];
-    load8<GB>(out, j, left, o);
+    float o[E];
+    load_row<GB, E>(out, j, left, o);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] += o[e];
+    for (int e = 0; e < E; e++) v[e] += o[e];
   }
-  store8<GB>(out, j, left, v);
+  store_row<GB, E>(out, j, left, v);
 }
 
-/* Rows that a thread takes one after the other: a workgroup writes 16 KiB.  (40970 rows of 2048 fp32: one
- * 75 us, two 74, four 110; 151936 of 1024 bf16: one 85 us, two 71, four 64, eight 66.  Loading
- * the rows' first positions and their dy together, 64 to 70; a strip of columns for each
- * XCD, so that dy stays in its L2, 110 to 132; stores through the caches, 74 to 80 and 64 to 128.) */
+#ifndef SRB
+#define SRB 4
+#define SRF 4
+#endif
+#ifndef LMAX
+#define LMAX 256
+#endif
 template <bool GB>
-constexpr int sum_rows() { return GB ? 4 : 2; }
+constexpr int sum_rows() { return GB ? SRB : SRF; }
 
 template <bool DB, bool GB>
 __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
                                                   int hot_groups) {
-  constexpr int SUM_ROWS = sum_rows<GB>();
+  constexpr int SUM_ROWS = sum_rows<GB>(), E = GB ? 8 : 4;
   const int tid = (int)threadIdx.x;
   if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut */
     __shared__ uint32_t last;
@@ -288,13 +304,14 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
     const int chunks = (int)w.counters[CNT_CHUNKS];
     for (int c = (int)blockIdx.x; c < chunks; c += hot_groups) {
       const Chunk k = w.chunks[c];
-      for (int64_t j = tid * 8; j < a.width; j += ET * 8) {
-        const int left = (int)min((int64_t)8, a.width - j);
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        add_rows<DB>(a, w.order + k.start, k.count, j, left, v);
+      for (int64_t j = tid * E; j < a.width; j += ET * E) {
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = 0.0f;
+        add_rows<DB, E>(a, w.order + k.start, k.count, j, a.width - j, v);
         uint64_t *out = (uint64_t *)(w.sums + c * stride + j);
 #pragma unroll
-        for (int e = 0; e < 4; e++) st_agent(out + e, (uint64_t)d3s_f2u(v[2 * e]) | (uint64_t)d3s_f2u(v[2 * e + 1]) << 32);
+        for (int e = 0; e < E / 2; e++) st_agent(out + e, (uint64_t)d3s_f2u(v[2 * e]) | (uint64_t)d3s_f2u(v[2 * e + 1]) << 32);
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
@@ -305,20 +322,21 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
       }
       __syncthreads();
       if (last)
-        for (int64_t j = tid * 8; j < a.width; j += ET * 8) {
-          const int left = (int)min((int64_t)8, a.width - j);
-          float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t j = tid * E; j < a.width; j += ET * E) {
+          float v[E];
+#pragma unroll
+          for (int e = 0; e < E; e++) v[e] = 0.0f;
 #pragma unroll 4
           for (int i = 0; i < k.chunks; i++) {
             const uint64_t *in = (const uint64_t *)(w.sums + (k.first + i) * stride + j);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int e = 0; e < E / 2; e++) {
               const uint64_t q = ld_agent(in + e);
               v[2 * e] += d3s_u2f((uint32_t)q);
               v[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
             }
           }
-          put_row<GB>(a, k.row, j, left, v);
+          put_row<GB, E>(a, k.row, j, a.width - j, v);
         }
       __syncthreads();
     }
@@ -332,9 +350,8 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
   const int across = tid % lanes, down = tid / lanes, at_once = ET / lanes;
   for (int64_t blk = blockIdx.x - hot_groups; blk < blocks; blk += gridDim.x - hot_groups) {
     const int64_t row0 = blk / strips * (at_once * SUM_ROWS) + down;
-    const int64_t j = (blk % strips * lanes + across) * 8;
+    const int64_t j = (blk % strips * lanes + across) * E;
     if (j >= a.width) continue;
-    const int left = (int)min((int64_t)8, a.width - j);
     Seg seg[SUM_ROWS];
 #pragma unroll
     for (int i = 0; i < SUM_ROWS; i++) {
@@ -346,9 +363,11 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
     for (int i = 0; i < SUM_ROWS; i++) {
       const int64_t row = row0 + i * at_once;
       if (row >= p.rows || seg[i].count < 0 || (a.accumulate && seg[i].count == 0)) continue;
-      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      add_rows<DB>(a, w.order + seg[i].start, seg[i].count, j, left, v);
-      put_row<GB>(a, row, j, left, v);
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) v[e] = 0.0f;
+      add_rows<DB, E>(a, w.order + seg[i].start, seg[i].count, j, a.width - j, v);
+      put_row<GB, E>(a, row, j, a.width - j, v);
     }
   }
 }
@@ -356,10 +375,11 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
 /* the table's gradient where there are no ids */
 template <bool GB>
 __global__ __launch_bounds__(ET) void k_embed_zero(EmbedArgs a, int64_t rows, int64_t strips) {
+  constexpr int E = GB ? 8 : 4;
   const float zero[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   for (int64_t blk = blockIdx.x; blk < rows * strips; blk += gridDim.x) {
-    const int64_t j = (blk % strips * ET + threadIdx.x) * 8;
-    if (j < a.width) store8<GB>((char *)a.out + blk / strips * a.out_stride * (GB ? 2 : 4), j, (int)min((int64_t)8, a.width - j), zero);
+    const int64_t j = (blk % strips * ET + threadIdx.x) * E;
+    if (j < a.width) store_row<GB, E>((char *)a.out + blk / strips * a.out_stride * (GB ? 2 : 4), j, a.width - j, zero);
   }
 }
 
@@ -367,16 +387,21 @@ __global__ __launch_bounds__(ET) void k_embed_zero(EmbedArgs a, int64_t rows, in
 
 void launch_embed(const EmbedArgs &args, Dtype in, Dtype out, hipStream_t s) {
   const EmbedArgs a = args;
+  const int E = out == DT_BF16 ? 8 : 4;
   int lanes = 1;
-  while (lanes < ET && (int64_t)lanes * 8 < a.width) lanes *= 2;
-  const int64_t strips = (a.width + lanes * 8 - 1) / (lanes * 8);
+  while (lanes < ET && (int64_t)lanes * E < a.width) lanes *= 2;
+  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E);
   const int64_t blocks = strips * ((a.n_rows + ET / lanes - 1) / (ET / lanes));
   const dim3 grid((unsigned)(blocks < STEP_GRID ? blocks : STEP_GRID));
   auto go = [&](auto kernel) { kernel<<<grid, ET, 0, s>>>(a, lanes, strips, blocks); };
+  auto many = [&](auto tb, auto yb) {
+    constexpr bool T = decltype(tb)::value, Y = decltype(yb)::value;
+    a.n_ids == 1 ? go(k_embed<T, Y, 1>) : go(k_embed<T, Y, 4>);
+  };
   if (in == DT_BF16)
-    out == DT_BF16 ? go(k_embed<true, true>) : go(k_embed<true, false>);
+    out == DT_BF16 ? many(std::true_type{}, std::true_type{}) : many(std::true_type{}, std::false_type{});
   else
-    out == DT_BF16 ? go(k_embed<false, true>) : go(k_embed<false, false>);
+    out == DT_BF16 ? many(std::false_type{}, std::true_type{}) : many(std::false_type{}, std::false_type{});
 }
 
 size_t embed_grad_workspace_bytes(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, int64_t width) {
@@ -389,8 +414,9 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   const EmbedArgs a = args;
   auto grid = [](int64_t n) { return dim3((unsigned)(n < STEP_GRID ? n : STEP_GRID)); };
   const GradPlan p = grad_plan(a.n_rows, a.n_ids, a.vocab, a.slot_rows);
+  const int E = out == DT_BF16 ? 8 : 4;
   if (a.n_rows == 0) {
-    const int64_t strips = (a.width + ET * 8 - 1) / (ET * 8);
+    const int64_t strips = (a.width + ET * E - 1) / (ET * E);
     if (out == DT_BF16)
       k_embed_zero<true><<<grid(p.rows * strips), ET, 0, s>>>(a, p.rows, strips);
     else
@@ -401,8 +427,8 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   grad_layout(p, a.width, (char *)ws, &w);
   k_embed_group<<<grid(p.slots * p.ranges), ET, GW * p.range * sizeof(int), s>>>(a, p, w);
   int lanes = 1;
-  while (lanes < ET && (int64_t)lanes * 8 < a.width) lanes *= 2;
-  const int64_t strips = (a.width + lanes * 8 - 1) / (lanes * 8), rows = ET / lanes * (out == DT_BF16 ? sum_rows<true>() : sum_rows<false>());
+  while (lanes < LMAX && (int64_t)lanes * E < a.width) lanes *= 2;
+  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * (out == DT_BF16 ? sum_rows<true>() : sum_rows<false>());
   const int64_t blocks = strips * ((p.rows + rows - 1) / rows);
   const int64_t most = chunks_most(p);
   const int hot_groups = (int)(most < HOT_GROUPS ? most : HOT_GROUPS);

@@ -81,9 +81,13 @@ __device__ __forceinline__ float row_max(float v, float *part) {
 
 /* G threads hold a row, U chunks of eight elements each, in registers: one read of
  * everything, all of it in flight together. */
+/* elements that follow each other in a lane: as many as make a store of 16 bytes; eight for 8 bits */
+template <bool BF16, int OUT>
+constexpr int norm_elements() { return OUT != D3S_DTYPE_E4M3 && (!BF16 || OUT == D3S_DTYPE_F32) ? 4 : 8; }
+
 template <bool BF16, int OUT, int G, int U>
 __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
-  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G;
+  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G, E = norm_elements<BF16, OUT>();
   __shared__ float part[NW];
   const int g = (int)threadIdx.x % G;
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
@@ -91,45 +95,45 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
     const bool mine = row0 + threadIdx.x / G < a.n_rows; /* (the others shadow the last row and store nothing) */
     const int width = (int)a.width;
     const char *x = (const char *)a.x + row * a.x_stride * ES;
-    Vec8<BF16> q[U], r[U], w[U];
+    Vec<BF16, E> q[U], r[U], w[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) q[u].load_some(x, (u * G + g) * 8, width - (u * G + g) * 8);
+    for (int u = 0; u < U; u++) q[u].load_some(x, (u * G + g) * E, width - (u * G + g) * E);
     if (a.residual) {
       const char *res = (const char *)a.residual + row * a.residual_stride * ES;
 #pragma unroll
-      for (int u = 0; u < U; u++) r[u].load_some(res, (u * G + g) * 8, width - (u * G + g) * 8);
+      for (int u = 0; u < U; u++) r[u].load_some(res, (u * G + g) * E, width - (u * G + g) * E);
     }
     if (a.gain) {
 #pragma unroll
-      for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * 8, width - (u * G + g) * 8);
+      for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * E, width - (u * G + g) * E);
     }
-    float h[U][8], s = 0.0f;
+    float h[U][E], s = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
       q[u].values(h[u]);
       if (a.residual) {
-        float t[8];
+        float t[E];
         r[u].values(t);
 #pragma unroll
-        for (int e = 0; e < 8; e++) h[u][e] += t[e];
+        for (int e = 0; e < E; e++) h[u][e] += t[e];
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) s = fmaf(h[u][e], h[u][e], s);
+      for (int e = 0; e < E; e++) s = fmaf(h[u][e], h[u][e], s);
     }
     if (a.sum && mine) {
 #pragma unroll
       for (int u = 0; u < U; u++)
-        store8<BF16>((char *)a.sum + row * a.sum_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8, h[u]);
+        store_row<BF16, E, BF16 || E == 4>((char *)a.sum + row * a.sum_stride * ES, (u * G + g) * E, width - (u * G + g) * E, h[u]);
     }
     s = row_sum<G>(s, part);
     const float rstd = 1.0f / sqrtf(s / (float)width + a.eps);
     if (g == 0 && a.rstd && mine) a.rstd[row] = rstd;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      float t[8];
+      float t[E];
       if (a.gain) w[u].values(t);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
+      for (int e = 0; e < E; e++) {
         h[u][e] *= rstd;
         if (a.gain) h[u][e] *= t[e];
       }
@@ -139,7 +143,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
       if (mine) {
 #pragma unroll
         for (int u = 0; u < U; u++)
-          store8<OUT == D3S_DTYPE_BF16>((char *)a.y + row * a.y_stride * YS, (u * G + g) * 8, width - (u * G + g) * 8, h[u]);
+          store_row<OUT == D3S_DTYPE_BF16, E>((char *)a.y + row * a.y_stride * YS, (u * G + g) * E, width - (u * G + g) * E, h[u]);
       }
     } else {
       /* (places past the row hold x = 0 and, where rstd is infinite, 0 times it: not looked at) */
@@ -148,8 +152,8 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
       for (int u = 0; u < U; u++) {
         most[u] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          most[u] = __builtin_elementwise_maximum(most[u], (u * G + g) * 8 + e < width ? fabsf(h[u][e]) : 0.0f);
+        for (int e = 0; e < E; e++)
+          most[u] = __builtin_elementwise_maximum(most[u], (u * G + g) * E + e < width ? fabsf(h[u][e]) : 0.0f);
       }
       if (a.group == 0) {
 #pragma unroll
@@ -167,7 +171,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
       uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int j = (u * G + g) * 8, left = width - j;
+        const int j = (u * G + g) * E, left = width - j;
         const float scale = e4m3_scale(most[u]);
         if (left <= 0 || !mine) continue;
         if (a.group ? j % a.group == 0 : j == 0) a.scales[row * groups + (a.group ? j / a.group : 0)] = scale;
@@ -185,47 +189,47 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
  * rows and keeps their columns' sums of dy xhat in registers. */
 template <bool BF16, int G, int U, bool SUM>
 __global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) {
-  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G;
+  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G, E = BF16 ? 8 : 4;
   __shared__ float part[NW];
-  __shared__ float sums[SUM && ROWS > 1 ? NT * U * 8 : 1];
+  __shared__ float sums[SUM && ROWS > 1 ? NT * U * E : 1];
   const int g = (int)threadIdx.x % G, width = (int)a.width;
-  Vec8<BF16> w[U];
+  Vec<BF16, E> w[U];
   if (a.gain) {
 #pragma unroll
-    for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * 8, width - (u * G + g) * 8);
+    for (int u = 0; u < U; u++) w[u].load_some(a.gain, (u * G + g) * E, width - (u * G + g) * E);
   }
-  float acc[U][8];
+  float acc[U][E];
 #pragma unroll
   for (int u = 0; u < U; u++)
 #pragma unroll
-    for (int e = 0; e < 8; e++) acc[u][e] = 0.0f;
+    for (int e = 0; e < E; e++) acc[u][e] = 0.0f;
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
     const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
     const bool mine = row0 + threadIdx.x / G < a.n_rows;
-    Vec8<BF16> d[U], h[U], r[U];
+    Vec<BF16, E> d[U], h[U], r[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      d[u].load_some((const char *)a.dy + row * a.dy_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
-      h[u].load_some((const char *)a.h + row * a.h_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
+      d[u].load_some((const char *)a.dy + row * a.dy_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
+      h[u].load_some((const char *)a.h + row * a.h_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
     }
     if (a.dsum && a.dx) {
 #pragma unroll
       for (int u = 0; u < U; u++)
-        r[u].load_some((const char *)a.dsum + row * a.dsum_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8);
+        r[u].load_some((const char *)a.dsum + row * a.dsum_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
     }
     const float rstd = a.rstd[row];
     float s = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      float p[8], t[8], k[8];
+      float p[E], t[E], k[E];
       d[u].values(p);
       h[u].values(t);
       if (a.gain) w[u].values(k);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
+      for (int e = 0; e < E; e++) {
         const float xhat = t[e] * rstd;
-        if (SUM && mine && (u * G + g) * 8 + e < width) acc[u][e] = fmaf(p[e], xhat, acc[u][e]);
-        s = fmaf(a.gain ? p[e] * k[e] : p[e], (u * G + g) * 8 + e < width ? xhat : 0.0f, s);
+        if (SUM && mine && (u * G + g) * E + e < width) acc[u][e] = fmaf(p[e], xhat, acc[u][e]);
+        s = fmaf(a.gain ? p[e] * k[e] : p[e], (u * G + g) * E + e < width ? xhat : 0.0f, s);
       }
     }
     if (!a.dx) continue; /* (uniform) */
@@ -233,17 +237,17 @@ __global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) 
     if (!mine) continue; /* (G == NT: always its own) */
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      float p[8], t[8], k[8], o[8];
+      float p[E], t[E], k[E], o[E];
       d[u].values(p);
       h[u].values(t);
       if (a.gain) w[u].values(k);
       if (a.dsum) r[u].values(o);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
+      for (int e = 0; e < E; e++) {
         const float v = rstd * ((a.gain ? p[e] * k[e] : p[e]) - t[e] * rstd * mean);
         o[e] = a.dsum ? v + o[e] : v;
       }
-      store8<BF16>((char *)a.dx + row * a.dx_stride * ES, (u * G + g) * 8, width - (u * G + g) * 8, o);
+      store_row<BF16, E>((char *)a.dx + row * a.dx_stride * ES, (u * G + g) * E, width - (u * G + g) * E, o);
     }
   }
   if constexpr (SUM) {
@@ -251,17 +255,17 @@ __global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) 
     if constexpr (ROWS == 1) {
 #pragma unroll
       for (int u = 0; u < U; u++)
-        store8<false, false>(out, (u * G + g) * 8, width - (u * G + g) * 8, acc[u]);
+        store_row<false, E, false>(out, (u * G + g) * E, width - (u * G + g) * E, acc[u]);
     } else {
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) sums[(threadIdx.x / G) * (G * U * 8) + (u * G + g) * 8 + e] = acc[u][e];
+        for (int e = 0; e < E; e++) sums[(threadIdx.x / G) * (G * U * E) + (u * G + g) * E + e] = acc[u][e];
       __syncthreads();
       for (int j = (int)threadIdx.x; j < width; j += NT) {
         float v = 0.0f;
 #pragma unroll 4
-        for (int i = 0; i < ROWS; i++) v += sums[i * (G * U * 8) + j];
+        for (int i = 0; i < ROWS; i++) v += sums[i * (G * U * E) + j];
         out[j] = v;
       }
     }
@@ -277,10 +281,10 @@ __global__ __launch_bounds__(NT) void k_norm_rows(NormArgs a) {
     const char *x = (const char *)a.x + row * a.x_stride * ES;
     const char *res = a.residual ? (const char *)a.residual + row * a.residual_stride * ES : nullptr;
     auto get = [&](int64_t j, int left, float *h) {
-      load8<BF16>(x, j, left, h);
+      load_row<BF16, 8>(x, j, left, h);
       if (res) {
         float r[8];
-        load8<BF16>(res, j, left, r);
+        load_row<BF16, 8>(res, j, left, r);
 #pragma unroll
         for (int e = 0; e < 8; e++) h[e] += r[e];
       }
@@ -298,7 +302,7 @@ __global__ __launch_bounds__(NT) void k_norm_rows(NormArgs a) {
     if (tid == 0 && a.rstd) a.rstd[row] = rstd;
     auto scaled = [&](int64_t j, int left, float *h) {
       float g[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-      if (a.gain) load8<BF16>(a.gain, j, left, g);
+      if (a.gain) load_row<BF16, 8>(a.gain, j, left, g);
 #pragma unroll
       for (int e = 0; e < 8; e++) h[e] = h[e] * rstd * g[e];
     };
@@ -326,12 +330,12 @@ __global__ __launch_bounds__(NT) void k_norm_rows(NormArgs a) {
       const int left = left_at(j);
       float h[8];
       get(j, left, h);
-      if (a.sum && left > 0) store8<BF16>((char *)a.sum + row * a.sum_stride * ES, j, left, h);
+      if (a.sum && left > 0) store_row<BF16, 8, BF16>((char *)a.sum + row * a.sum_stride * ES, j, left, h);
       scaled(j, left, h);
       if (a.y_dtype == D3S_DTYPE_BF16) {
-        if (left > 0) store8<true>((char *)a.y + row * a.y_stride * 2, j, left, h);
+        if (left > 0) store_row<true, 8>((char *)a.y + row * a.y_stride * 2, j, left, h);
       } else if (a.y_dtype == D3S_DTYPE_F32) {
-        if (left > 0) store8<false>((char *)a.y + row * a.y_stride * 4, j, left, h);
+        if (left > 0) store_row<false, 8, false>((char *)a.y + row * a.y_stride * 4, j, left, h);
       } else {
         float scale = row_scale;
         if (!whole) {
@@ -362,9 +366,9 @@ __global__ __launch_bounds__(NT) void k_norm_grad_rows(NormGradArgs a) {
     const float rstd = a.rstd[row];
     auto get = [&](int64_t j, int left, float *p, float *xhat) {
       float g[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-      load8<BF16>(dy, j, left, p);
-      load8<BF16>(h, j, left, xhat);
-      if (a.gain) load8<BF16>(a.gain, j, left, g);
+      load_row<BF16, 8>(dy, j, left, p);
+      load_row<BF16, 8>(h, j, left, xhat);
+      if (a.gain) load_row<BF16, 8>(a.gain, j, left, g);
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] *= g[e], xhat[e] *= rstd;
     };
@@ -380,10 +384,10 @@ __global__ __launch_bounds__(NT) void k_norm_grad_rows(NormGradArgs a) {
       const int left = (int)min((int64_t)8, a.width - j);
       float p[8], xhat[8], d[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
       get(j, left, p, xhat);
-      if (a.dsum) load8<BF16>((const char *)a.dsum + row * a.dsum_stride * ES, j, left, d);
+      if (a.dsum) load_row<BF16, 8>((const char *)a.dsum + row * a.dsum_stride * ES, j, left, d);
 #pragma unroll
       for (int e = 0; e < 8; e++) p[e] = rstd * (p[e] - xhat[e] * mean) + d[e];
-      store8<BF16>((char *)a.dx + row * a.dx_stride * ES, j, left, p);
+      store_row<BF16, 8, BF16>((char *)a.dx + row * a.dx_stride * ES, j, left, p);
     }
   }
 }
@@ -400,11 +404,12 @@ __global__ __launch_bounds__(NT) void k_norm_dgain(NormGradArgs a, int64_t strip
   parts[run * a.width + j] = s;
 }
 
-/* the threads and chunks that hold a row: f(G, U), or false for one that is streamed */
-template <class F>
+/* the threads and chunks of E elements that hold a row: f(G, U), or false for one that is streamed */
+template <int E, class F>
 bool in_registers(int64_t width, F f) {
+  constexpr int M = 8 / E;
   auto c = [](auto v) { return v; };
-#define D3S_ROW(G, U) return f(c(std::integral_constant<int, G>{}), c(std::integral_constant<int, U>{})), true
+#define D3S_ROW(G, U) return f(c(std::integral_constant<int, G>{}), c(std::integral_constant<int, U * M>{})), true
   if (width <= 64) D3S_ROW(8, 1);
   if (width <= 128) D3S_ROW(16, 1);
   if (width <= 256) D3S_ROW(32, 1);
@@ -426,7 +431,7 @@ struct GradSplit {
 };
 GradSplit grad_split(int64_t n_rows, int64_t width) {
   GradSplit p{1, 0, 0};
-  const bool held = in_registers(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
+  const bool held = in_registers<8>(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
   if (held) {
     const int64_t sets = (n_rows + p.rows - 1) / p.rows;
     p.runs = (int)(sets < GRAD_RUNS ? sets : GRAD_RUNS);
@@ -448,21 +453,20 @@ void launch_norm(const NormArgs &args, Dtype dt, hipStream_t s) {
     const int64_t n = (a.n_rows + rows - 1) / rows;
     return dim3((unsigned)(n < STEP_GRID ? n : STEP_GRID));
   };
-  const bool held = in_registers(a.width, [&](auto g, auto u) {
-    constexpr int G = decltype(g)::value, U = decltype(u)::value;
-    auto go = [&](auto kernel) { kernel<<<grid(NT / G), NT, 0, s>>>(a); };
-    auto out = [&](auto bf16) {
-      constexpr bool B = decltype(bf16)::value;
-      if (a.y_dtype == D3S_DTYPE_BF16)
-        go(k_norm<B, D3S_DTYPE_BF16, G, U>);
-      else if (a.y_dtype == D3S_DTYPE_F32)
-        go(k_norm<B, D3S_DTYPE_F32, G, U>);
-      else
-        go(k_norm<B, D3S_DTYPE_E4M3, G, U>);
-    };
-    dt == DT_BF16 ? out(std::true_type{}) : out(std::false_type{});
-  });
-  if (held) return;
+  auto held = [&](auto bf16, auto type) {
+    constexpr bool B = decltype(bf16)::value;
+    constexpr int OUT = decltype(type)::value;
+    return in_registers<norm_elements<B, OUT>()>(a.width, [&](auto g, auto u) {
+      constexpr int G = decltype(g)::value;
+      k_norm<B, OUT, G, decltype(u)::value><<<grid(NT / G), NT, 0, s>>>(a);
+    });
+  };
+  auto of_type = [&](auto bf16) {
+    return a.y_dtype == D3S_DTYPE_BF16  ? held(bf16, std::integral_constant<int, D3S_DTYPE_BF16>{})
+           : a.y_dtype == D3S_DTYPE_F32 ? held(bf16, std::integral_constant<int, D3S_DTYPE_F32>{})
+                                        : held(bf16, std::integral_constant<int, D3S_DTYPE_E4M3>{});
+  };
+  if (dt == DT_BF16 ? of_type(std::true_type{}) : of_type(std::false_type{})) return;
   if (dt == DT_BF16)
     k_norm_rows<true><<<grid(1), NT, 0, s>>>(a);
   else
@@ -478,16 +482,17 @@ void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t 
   const NormGradArgs a = args;
   const GradSplit p = grad_split(a.n_rows, a.width);
   float *parts = ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
-  bool held = false;
-  if (p.runs)
-    held = in_registers(a.width, [&](auto g, auto u) {
+  auto rows_held = [&](auto bf16) {
+    constexpr bool B = decltype(bf16)::value;
+    return in_registers<B ? 8 : 4>(a.width, [&](auto g, auto u) {
       constexpr int G = decltype(g)::value, U = decltype(u)::value;
-      auto go = [&](auto kernel) { kernel<<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts); };
-      if (dt == DT_BF16)
-        a.dgain ? go(k_norm_grad<true, G, U, true>) : go(k_norm_grad<true, G, U, false>);
+      if (a.dgain)
+        k_norm_grad<B, G, U, true><<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts);
       else
-        a.dgain ? go(k_norm_grad<false, G, U, true>) : go(k_norm_grad<false, G, U, false>);
+        k_norm_grad<B, G, U, false><<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts);
     });
+  };
+  const bool held = p.runs && (dt == DT_BF16 ? rows_held(std::true_type{}) : rows_held(std::false_type{}));
   if (!held && p.runs) { /* (dgain first: dx may be dy or h) */
     const dim3 strips((unsigned)(p.strips * p.runs)), rows((unsigned)(a.n_rows < STEP_GRID ? a.n_rows : STEP_GRID));
     if (a.dgain) {

@@ -1,4 +1,8 @@
-/* Eight elements of a row, fp32 or bf16, at any element.  Device code only. */
+/* A lane's elements of a row, fp32 or bf16, at any element.  Device code only.
+ *
+ * A lane takes E elements that follow each other, so that a store of 16 bytes a lane writes
+ * whole lines: 8 where the output is bf16, 4 where it is fp32.  (8 fp32 elements are two
+ * stores of half lines each: past the caches 40970 x 2048 of them took 110 us, so 74.) */
 #ifndef D3S_VEC_H
 #define D3S_VEC_H
 
@@ -16,48 +20,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 
 template <bool BF16>
-struct Vec8 {
-  uint4 q[BF16 ? 1 : 2];
-
-  __device__ __forceinline__ void load(const void *row, int64_t j) {
-    const char *p = (const char *)row + j * (BF16 ? 2 : 4);
-    __builtin_memcpy(&q[0], p, 16);
-    if constexpr (!BF16) __builtin_memcpy(&q[1], p + 16, 16);
-  }
-  /* elements j .. j + 7 of which `left` (0 .. 8) are inside, the rest +0 */
-  __device__ __forceinline__ void load_some(const void *row, int64_t j, int left) {
-    if (left >= 8) {
-      load(row, j);
-      return;
-    }
-    uint32_t *w = (uint32_t *)q;
-#pragma unroll
-    for (int i = 0; i < (BF16 ? 4 : 8); i++) w[i] = 0u;
-    if (left <= 0) return;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      if (e >= left) continue;
-      if constexpr (BF16)
-        w[e / 2] |= (uint32_t)((const uint16_t *)row)[j + e] << 16 * (e % 2);
-      else
-        w[e] = ((const uint32_t *)row)[j + e];
-    }
-  }
-  __device__ __forceinline__ void values(float *v) const {
-    const uint32_t *w = (const uint32_t *)q;
-#pragma unroll
-    for (int i = 0; i < (BF16 ? 4 : 8); i++) {
-      if constexpr (BF16) {
-        v[2 * i] = d3s_u2f(w[i] << 16);
-        v[2 * i + 1] = d3s_u2f(w[i] & 0xffff0000u);
-      } else {
-        v[i] = d3s_u2f(w[i]);
-      }
-    }
-  }
-};
-
-template <bool BF16>
 __device__ __forceinline__ float load_at(const void *row, int64_t j) {
   if constexpr (BF16) return d3s_u2f((uint32_t)((const uint16_t *)row)[j] << 16);
   return ((const float *)row)[j];
@@ -70,41 +32,71 @@ __device__ __forceinline__ void store_at(void *row, int64_t j, float v) {
     ((float *)row)[j] = v;
 }
 
-/* elements j .. j + 7 of a row, of which `left` are inside (the rest: `fill`) */
-template <bool BF16>
-__device__ __forceinline__ void load8(const void *row, int64_t j, int left, float *v, float fill = 0.0f) {
-  if (left >= 8) {
-    Vec8<BF16> q;
-    q.load(row, j);
-    q.values(v);
-  } else {
+/* E elements as they are stored */
+template <bool BF16, int E>
+struct Vec {
+  static constexpr int W = E * (BF16 ? 2 : 4) / 4;
+  uint32_t w[W];
+
+  __device__ __forceinline__ void load(const void *row, int64_t j) { __builtin_memcpy(w, (const char *)row + j * (BF16 ? 2 : 4), 4 * W); }
+  /* elements j .. j + E - 1 of which `left` (any number) are inside, the rest +0 */
+  __device__ __forceinline__ void load_some(const void *row, int64_t j, int64_t left) {
+    if (left >= E) {
+      load(row, j);
+      return;
+    }
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = e < left ? load_at<BF16>(row, j + e) : fill;
+    for (int i = 0; i < W; i++) w[i] = 0u;
+    if (left <= 0) return;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (e >= left) continue;
+      if constexpr (BF16)
+        w[e / 2] |= (uint32_t)((const uint16_t *)row)[j + e] << 16 * (e % 2);
+      else
+        w[e] = ((const uint32_t *)row)[j + e];
+    }
   }
+  __device__ __forceinline__ void values(float *v) const {
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      if constexpr (BF16) {
+        v[2 * i] = d3s_u2f(w[i] << 16);
+        v[2 * i + 1] = d3s_u2f(w[i] & 0xffff0000u);
+      } else {
+        v[i] = d3s_u2f(w[i]);
+      }
+    }
+  }
+};
+
+/* elements j .. j + E - 1 of a row, of which `left` are inside (the rest: 0) */
+template <bool BF16, int E>
+__device__ __forceinline__ void load_row(const void *row, int64_t j, int64_t left, float *v) {
+  Vec<BF16, E> q;
+  q.load_some(row, j, left);
+  q.values(v);
 }
 
-/* PAST: past the caches, for what is not read again soon */
-template <bool PAST>
-__device__ __forceinline__ void put16(void *p, uint4 q) {
-  if constexpr (PAST)
-    stream16(p, q);
-  else
-    __builtin_memcpy(p, &q, 16);
-}
-
-template <bool BF16, bool PAST = true>
-__device__ __forceinline__ void store8(void *row, int64_t j, int left, const float *v) {
-  if (left >= 8) {
+/* the first `left` of E elements, to j .. of a row.  PAST: past the caches, for what is not
+ * read again soon */
+template <bool BF16, int E, bool PAST = true>
+__device__ __forceinline__ void store_row(void *row, int64_t j, int64_t left, const float *v) {
+  if (left >= E) {
     char *p = (char *)row + j * (BF16 ? 2 : 4);
-    if constexpr (BF16) {
-      put16<PAST>(p, make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])));
+    constexpr int W = Vec<BF16, E>::W;
+    uint32_t w[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = BF16 ? pack_bf16(v[2 * i], v[2 * i + 1]) : d3s_f2u(v[i]);
+    if constexpr (PAST && W >= 4) { /* (a loop over the stores would lose their being non-temporal) */
+      stream16(p, make_uint4(w[0], w[1], w[2], w[3]));
+      if constexpr (W > 4) stream16(p + 16, make_uint4(w[W - 4], w[W - 3], w[W - 2], w[W - 1]));
     } else {
-      put16<PAST>(p, make_uint4(d3s_f2u(v[0]), d3s_f2u(v[1]), d3s_f2u(v[2]), d3s_f2u(v[3])));
-      put16<PAST>(p + 16, make_uint4(d3s_f2u(v[4]), d3s_f2u(v[5]), d3s_f2u(v[6]), d3s_f2u(v[7])));
+      __builtin_memcpy(p, w, 4 * W);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
+    for (int e = 0; e < E; e++)
       if (e < left) store_at<BF16>(row, j + e, v[e]);
   }
 }

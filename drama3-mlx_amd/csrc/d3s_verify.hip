@@ -198,8 +198,13 @@ struct Weights {
   /* eight terms of each sum from j on (0 past the end), j < V */
   __device__ __forceinline__ void terms(int j, double *p, double *q) const {
     float v[8], w[8];
-    load8<TB>(tp, j, left(j), v, -__builtin_inff());
-    if (dp) load8<DB>(dp, j, left(j), w, -__builtin_inff());
+    load_row<TB, 8>(tp, j, left(j), v);
+    if (dp) load_row<DB, 8>(dp, j, left(j), w);
+    if (left(j) < 8) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (e >= left(j)) v[e] = w[e] = -__builtin_inff();
+    }
 #pragma unroll
     for (int e = 0; e < 8; e++) p[e] = exp2_64(((double)v[e] - mp) * cp);
     if (dp) {
