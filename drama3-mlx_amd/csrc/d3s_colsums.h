@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void k_column_sums(const float *parts, int run
   const int per = (runs + 15) / 16, r1 = min(runs, (q + 1) * per);
   float v = 0.0f;
   if (col < n) {
-#pragma unroll 8
+#pragma unroll 16
     for (int r = q * per; r < r1; r++) v += parts[(int64_t)r * n + col];
   }
   sum[q][c] = v;

@@ -203,21 +203,40 @@ __global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) 
   for (int u = 0; u < U; u++)
 #pragma unroll
     for (int e = 0; e < E; e++) acc[u][e] = 0.0f;
-  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
-    const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
-    const bool mine = row0 + threadIdx.x / G < a.n_rows;
+  /* a row's inputs; the next row's are loaded while this one is worked on, where registers allow */
+  constexpr bool AHEAD = U * E <= 16;
+  struct In {
     Vec<BF16, E> d[U], h[U], r[U];
+    float rstd;
+  };
+  auto get = [&](int64_t row0, In &in) {
+    const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      d[u].load_some((const char *)a.dy + row * a.dy_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
-      h[u].load_some((const char *)a.h + row * a.h_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
+      in.d[u].load_some((const char *)a.dy + row * a.dy_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
+      in.h[u].load_some((const char *)a.h + row * a.h_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
     }
     if (a.dsum && a.dx) {
 #pragma unroll
       for (int u = 0; u < U; u++)
-        r[u].load_some((const char *)a.dsum + row * a.dsum_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
+        in.r[u].load_some((const char *)a.dsum + row * a.dsum_stride * ES, (u * G + g) * E, width - (u * G + g) * E);
     }
-    const float rstd = a.rstd[row];
+    in.rstd = a.rstd[row];
+  };
+  In in, next;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  if (AHEAD) get((int64_t)blockIdx.x * ROWS, in); /* (there is no workgroup without a row) */
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += step) {
+    const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
+    const bool mine = row0 + threadIdx.x / G < a.n_rows;
+    if (!AHEAD) {
+      get(row0, in);
+    } else {
+      if (row0 > (int64_t)blockIdx.x * ROWS) in = next;
+      if (row0 + step < a.n_rows) get(row0 + step, next);
+    }
+    const auto &d = in.d, &h = in.h, &r = in.r;
+    const float rstd = in.rstd;
     float s = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -423,15 +442,25 @@ bool in_registers(int64_t width, F f) {
   return false;
 }
 
-/* workgroups of the gradient: the runs of its column sums */
-constexpr int GRAD_RUNS = 512;
+/* The same for the gradient, whose inputs are three rows and whose sums stay: a workgroup a row
+ * beyond 1024, so that the next row's loads fit beside them (8192 x 2048 bf16: 32 us; a wave a row,
+ * without loads ahead, 43). */
+template <int E, class F>
+bool grad_in_registers(int64_t width, F f) {
+  if (width > 1024 && width <= 2048) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8 / E>{}), true;
+  return in_registers<E>(width, f);
+}
+
+/* Workgroups of the gradient: the runs of its column sums.  As many as are resident (512: 36 us for
+ * 8192 x 2048, 768 and 1024: 32, 1280 and 2048: 38). */
+constexpr int GRAD_RUNS = 1024;
 struct GradSplit {
   int64_t strips;
   int rows, runs;
 };
 GradSplit grad_split(int64_t n_rows, int64_t width) {
   GradSplit p{1, 0, 0};
-  const bool held = in_registers<8>(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
+  const bool held = grad_in_registers<8>(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
   if (held) {
     const int64_t sets = (n_rows + p.rows - 1) / p.rows;
     p.runs = (int)(sets < GRAD_RUNS ? sets : GRAD_RUNS);
@@ -484,7 +513,7 @@ void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t 
   float *parts = ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
   auto rows_held = [&](auto bf16) {
     constexpr bool B = decltype(bf16)::value;
-    return in_registers<B ? 8 : 4>(a.width, [&](auto g, auto u) {
+    return grad_in_registers<B ? 8 : 4>(a.width, [&](auto g, auto u) {
       constexpr int G = decltype(g)::value, U = decltype(u)::value;
       if (a.dgain)
         k_norm_grad<B, G, U, true><<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts);
