@@ -58,10 +58,11 @@ __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, int lanes, int64_t st
  * of as many, filed in a list; workgroups of their own sum the chunks in fp32, and the last
  * of a row to arrive adds its chunks in order.  No atomics on floating-point values. */
 
-constexpr int GW = ET / WAVE;
+constexpr int GT = 512; /* threads of k_embed_group */
+constexpr int GW = GT / WAVE;
 constexpr int LIST = 512;         /* positions that a wave keeps in LDS (more: the ids are looked through again) */
-constexpr int AHEAD = 16;         /* ids that a lane loads at a time */
-constexpr int RANGE_MOST = 2048;  /* rows of the table that a workgroup takes: 32 KiB of counts */
+constexpr int AHEAD = 8;          /* ids that a lane looks at at a time */
+constexpr int RANGE_MOST = 1024;  /* rows of the table that a workgroup takes: 32 KiB of counts */
 constexpr int HOT_GROUPS = 512;   /* workgroups for the chunks */
 constexpr int HOT_MOST = 4096;    /* rows that are cut, at most: a counter of arrivals each */
 constexpr int HOT_COUNTERS = 64;  /* words before them */
@@ -95,9 +96,9 @@ GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) 
   p.part = slot_rows ? slot_rows : vocab;
   p.rows = vocab + (n_ids - 1) * slot_rows;
   p.n = slot_rows ? n_rows : n_rows * n_ids;
-  /* ranges of 64 rows, wider while looking through the ids for each would read more than 128 MB and
-   * there are more ranges than CUs (TBD) */
-  p.range = 64;
+  /* Ranges of 256 rows (16384 ids for 151936 rows: 12 us; 64 and 128 rows 21), wider while looking through the ids
+   * for each would read more than 128 MB and there are more ranges than CUs. */
+  p.range = 256;
   auto count = [&](int64_t r) { return (vocab + r - 1) / r; };
   while (p.range < RANGE_MOST && p.slots * count(p.range) > 512 && p.slots * count(p.range) * p.n > (int64_t)32 << 20) p.range *= 2;
   p.ranges = count(p.range);
@@ -123,7 +124,7 @@ size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
   return at;
 }
 
-__global__ __launch_bounds__(ET) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
+__global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
   extern __shared__ int cnt[]; /* [GW][range]: a wave's count of a row, then its place */
   __shared__ int list_pos[GW][LIST];
   __shared__ uint16_t list_row[GW][LIST];
@@ -138,56 +139,74 @@ __global__ __launch_bounds__(ET) void k_embed_group(EmbedArgs a, GradPlan p, Gra
     const uint32_t rows = (uint32_t)min((int64_t)p.range, a.vocab - v0);
     const int i0 = (int)min((int64_t)n, (int64_t)wid * each), i1 = (int)min((int64_t)n, (int64_t)i0 + each);
     const int32_t *ids = a.slot_rows ? a.ids + slot : a.ids;
-    for (int i = tid; i < GW * p.range; i += ET) cnt[i] = 0;
+    for (int i = tid; i < GW * p.range; i += GT) cnt[i] = 0;
     __syncthreads();
     int *mine = cnt + wid * p.range;
-    /* f(position, row, whether it is this range's, which lanes' are) for the wave's ids in their order, 64 at a time
-     * (an id below 0 is a row past 2^31 - v0 here); and the number of ids of lower rows */
-    int less = 0;
-    auto look = [&](auto f) {
-      int id[AHEAD];
-      int i = i0;
-      less = 0;
-      for (; i1 - i >= AHEAD * WAVE; i += AHEAD * WAVE) {
-        bool any = false;
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++) id[u] = ids[(uint32_t)(i + u * WAVE + lane) * (uint32_t)step];
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-          any |= (uint32_t)id[u] - (uint32_t)v0 < rows;
-          less += (int)__popcll(__ballot((uint32_t)id[u] < (uint32_t)v0));
-        }
-        if (__ballot(any) == 0ull) continue;
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-          const uint32_t row = (uint32_t)id[u] - (uint32_t)v0;
-          const uint64_t hits = __ballot(row < rows);
-          if (hits) f(i + u * WAVE + lane, (int)row, row < rows, hits);
-        }
-      }
-      for (; i < i1; i += WAVE) {
-        const int at = i + lane;
-        const uint32_t one = at < i1 ? (uint32_t)ids[(uint32_t)at * (uint32_t)step] : 0xffffffffu, row = one - (uint32_t)v0;
-        const uint64_t hits = __ballot(row < rows);
-        less += (int)__popcll(__ballot(one < (uint32_t)v0));
-        if (hits) f(at, (int)row, row < rows, hits);
-      }
-    };
     auto below = [&](uint64_t m) {
       return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
     };
-    int found = 0;
-    look([&](int at, int row, bool hit, uint64_t hits) {
-      const int k = found + below(hits);
-      if (hit) {
-        atomicAdd(&mine[row], 1);
-        if (k < LIST) list_pos[wid][k] = at, list_row[wid][k] = row;
+    /* The wave's ids, AHEAD in a row for each lane: those of this range's rows go to its list, those of
+     * lower rows are counted (an id below 0 is a row past 2^31 - v0 here).  Most of the kernel's time is this
+     * chain; the code has to be short, since it is fetched while it runs (64 ids at a time by ballots,
+     * unrolled 16, 32 and 64 times: 15, 26 and 71 us). */
+    int less = 0, found = 0;
+    int next[AHEAD]; /* (loaded while those before are looked at) */
+    auto load = [&](int i) {
+      const int at = i + lane * AHEAD;
+      if (step == 1 && i1 - i >= AHEAD * WAVE) {
+        __builtin_memcpy(next, ids + at, sizeof(next));
+      } else if (i < i1) {
+        const int32_t *q = ids + (uint32_t)at * (uint32_t)step;
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++, q += step) next[e] = at + e < i1 ? *q : -1;
       }
-      found += (int)__popcll(hits);
+    };
+    load(i0);
+    for (int i = i0; i < i1; i += AHEAD * WAVE) {
+      const int at = i + lane * AHEAD;
+      int id[AHEAD];
+#pragma unroll
+      for (int e = 0; e < AHEAD; e++) id[e] = next[e];
+      load(i + AHEAD * WAVE);
+      uint32_t hits = 0u;
+#pragma unroll
+      for (int e = 0; e < AHEAD; e++) {
+        hits |= ((uint32_t)id[e] - (uint32_t)v0 < rows ? 1u : 0u) << e;
+        less += (uint32_t)id[e] < (uint32_t)v0 ? 1 : 0;
+      }
+      if (__ballot(hits != 0u) == 0ull) continue;
+      const int mine_here = __popc(hits), incl = (int)wave_scan_add_u32((uint32_t)mine_here);
+      int k = found + incl - mine_here;
+      found += (int)readlane_u((uint32_t)incl, WAVE - 1);
+      for (; hits; hits &= hits - 1u, k++) { /* (loaded again: no register is found by a number) */
+        const int e = at + __ffs(hits) - 1;
+        if (k < LIST) list_pos[wid][k] = e, list_row[wid][k] = (uint16_t)((uint32_t)ids[(uint32_t)e * (uint32_t)step] - (uint32_t)v0);
+      }
+    }
+    less = (int)wave_sum_u32((uint32_t)less);
+    /* f(position, row, whether it is this range's, which lanes' are) for them in their order: from the list, or
+     * where it does not hold them from the ids again */
+    auto each_hit = [&](auto f) {
+      if (found <= LIST) {
+        for (int e = 0; e < found; e += WAVE) {
+          const bool hit = e + lane < found;
+          f(hit ? list_pos[wid][e + lane] : 0, hit ? (int)list_row[wid][e + lane] : 0, hit, __ballot(hit));
+        }
+        return;
+      }
+#pragma nounroll
+      for (int at = i0 + lane; at - lane < i1; at += WAVE) {
+        const uint32_t row = at < i1 ? (uint32_t)ids[(uint32_t)at * (uint32_t)step] - (uint32_t)v0 : rows;
+        const uint64_t hits = __ballot(row < rows);
+        if (hits) f(at, (int)row, row < rows, hits);
+      }
+    };
+    each_hit([&](int, int row, bool hit, uint64_t) {
+      if (hit) atomicAdd(&mine[row], 1);
     });
     __syncthreads();
     /* the rows' places: a thread `per` rows in a row */
-    const int per = (p.range + ET - 1) / ET, r0 = min(p.range, tid * per), r1 = min(p.range, r0 + per);
+    const int per = (p.range + GT - 1) / GT, r0 = min(p.range, tid * per), r1 = min(p.range, r0 + per);
     int total = 0;
     for (int r = r0; r < r1; r++)
       for (int g = 0; g < GW; g++) total += cnt[g * p.range + r];
@@ -230,15 +249,7 @@ __global__ __launch_bounds__(ET) void k_embed_group(EmbedArgs a, GradPlan p, Gra
       if (hit && (peers >> lane) >> 1 == 0ull) mine[row] += k + 1; /* the last of them */
       wave_lds_sync();
     };
-    if (found <= LIST) {
-      for (int e = 0; e < found; e += WAVE) {
-        const bool hit = e + lane < found;
-        const int at = hit ? list_pos[wid][e + lane] : 0, row = hit ? list_row[wid][e + lane] : 0;
-        place(at, row, hit, __ballot(hit));
-      }
-    } else {
-      look(place);
-    }
+    each_hit(place);
     __syncthreads();
   }
 }
@@ -283,20 +294,16 @@ __device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t
   store_row<GB, E>(out, j, left, v);
 }
 
-#ifndef SRB
-#define SRB 4
-#define SRF 4
-#endif
-#ifndef LMAX
-#define LMAX 256
-#endif
-template <bool GB>
-constexpr int sum_rows() { return GB ? SRB : SRF; }
+/* Rows that a thread takes one after the other: a workgroup writes 16 KiB.  (40970 rows of 2048 fp32, the whole
+ * gradient: 82 us; two rows 88, one 104.  151936 of 1024 bf16: 79; two rows 81, eight 80.  Through the caches 100 and
+ * 144.  A strip of columns for each XCD, so that dy stays in its L2: 84 and more.  Rows without ids filled
+ * by k_embed_group instead: 105 and 101.) */
+constexpr int SUM_ROWS = 4;
 
 template <bool DB, bool GB>
 __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
                                                   int hot_groups) {
-  constexpr int SUM_ROWS = sum_rows<GB>(), E = GB ? 8 : 4;
+  constexpr int E = GB ? 8 : 4;
   const int tid = (int)threadIdx.x;
   if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut */
     __shared__ uint32_t last;
@@ -425,10 +432,10 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   }
   GradRoom w;
   grad_layout(p, a.width, (char *)ws, &w);
-  k_embed_group<<<grid(p.slots * p.ranges), ET, GW * p.range * sizeof(int), s>>>(a, p, w);
+  k_embed_group<<<grid(p.slots * p.ranges), GT, GW * p.range * sizeof(int), s>>>(a, p, w);
   int lanes = 1;
-  while (lanes < LMAX && (int64_t)lanes * E < a.width) lanes *= 2;
-  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * (out == DT_BF16 ? sum_rows<true>() : sum_rows<false>());
+  while (lanes < ET && (int64_t)lanes * E < a.width) lanes *= 2;
+  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * SUM_ROWS;
   const int64_t blocks = strips * ((p.rows + rows - 1) / rows);
   const int64_t most = chunks_most(p);
   const int hot_groups = (int)(most < HOT_GROUPS ? most : HOT_GROUPS);
