@@ -308,7 +308,7 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
   if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut */
     __shared__ uint32_t last;
     const int64_t stride = (a.width + 7) / 8 * 8;
-    const int chunks = (int)w.counters[CNT_CHUNKS];
+    const int chunks = (int)__hip_atomic_load(w.counters + CNT_CHUNKS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int c = (int)blockIdx.x; c < chunks; c += hot_groups) {
       const Chunk k = w.chunks[c];
       for (int64_t j = tid * E; j < a.width; j += ET * E) {

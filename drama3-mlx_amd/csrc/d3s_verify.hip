@@ -62,13 +62,11 @@ __device__ __forceinline__ Outcome decide(int L, float u, float p, float q, bool
   return o;
 }
 
-__device__ __forceinline__ void write_tokens(int b, int n_draft, Outcome o, int token, const int32_t *drafted,
-                                             int32_t *tokens, int32_t *n_accepted) {
-  for (int i = (int)threadIdx.x; i <= n_draft; i += (int)blockDim.x) {
-    const size_t at = (size_t)b * (n_draft + 1) + i;
-    tokens[at] = i < o.accepted ? drafted[(size_t)b * n_draft + i] : i == o.accepted ? token : -1;
-  }
-  if (threadIdx.x == 0) n_accepted[b] = o.accepted;
+/* x: lane i's draft i (a place behind 64 drafts holds none) */
+__device__ __forceinline__ void write_tokens(int b, int n_draft, Outcome o, int token, int x, int32_t *tokens, int32_t *n_accepted) {
+  const int i = (int)threadIdx.x;
+  if (i <= n_draft) tokens[(size_t)b * (n_draft + 1) + i] = i < o.accepted ? x : i == o.accepted ? token : -1;
+  if (i == 0) n_accepted[b] = o.accepted;
 }
 
 /* A sequence: its length and temperatures, its rows (0 .. n_draft the target's, then the
@@ -96,9 +94,9 @@ struct Seq {
 };
 
 /* A lane's share of a row's chunks, every `step`-th from `ch` on, up to `hi`; a batch
- * is loaded while the one before it is added. */
-template <bool BF16>
-__device__ __forceinline__ void lane_sums(Sums &s, const Row<BF16> &R, int ch, int hi, int step, float c) {
+ * is loaded while the one before it is added, and beside() runs behind the first loads. */
+template <bool BF16, class F>
+__device__ __forceinline__ void lane_sums(Sums &s, const Row<BF16> &R, int ch, int hi, int step, float c, F beside) {
   constexpr int EPC = Row<BF16>::EPC;
   uint4 q[SU], next[SU];
   bool whole = ch + (SU - 1) * step < hi;
@@ -106,6 +104,7 @@ __device__ __forceinline__ void lane_sums(Sums &s, const Row<BF16> &R, int ch, i
 #pragma unroll
     for (int u = 0; u < SU; u++) q[u] = R.base[ch + u * step];
   }
+  beside();
   while (whole) {
     const int after = ch + SU * step;
     whole = after + (SU - 1) * step < hi;
@@ -120,6 +119,13 @@ __device__ __forceinline__ void lane_sums(Sums &s, const Row<BF16> &R, int ch, i
 #pragma unroll
     for (int u = 0; u < SU; u++) q[u] = next[u];
     ch = after;
+  }
+  if (__ballot(ch + step < hi) == 0ull) { /* (4097 bf16 over 64 lanes: two batches and a chunk) */
+    if (ch >= hi) return;
+    float v[EPC];
+    R.values(R.base[ch], ch, v);
+    add_batch<EPC, false>(s, v, c);
+    return;
   }
   if (ch >= hi) return;
   /* the rest, less than a batch: a place past the end is the last chunk again, masked */
@@ -163,8 +169,12 @@ __device__ __forceinline__ void settle_row(const d3s_verify_params &a, const Seq
   L.prob[r] = refused(st) ? __builtin_nanf("") : st.S > 0.0f ? d3s_expf_nonpos((l - st.m) / T) / st.S : 0.0f;
 }
 
+/* lane i's uniform and draft */
 __device__ __forceinline__ float lane_u(const d3s_verify_params &a, const Seq &s) {
   return lane_id() < s.len ? a.u_accept[(size_t)s.b * a.n_draft + lane_id()] : 0.0f;
+}
+__device__ __forceinline__ int lane_draft(const d3s_verify_params &a, const Seq &s) {
+  return lane_id() < s.len ? a.drafted[(size_t)s.b * a.n_draft + lane_id()] : -1;
 }
 
 /* the whole workgroup, the rows settled; u: lane_u */
@@ -182,17 +192,18 @@ template <bool TB, bool DB>
 struct Weights {
   const char *tp, *dp; /* the rows (dp null: none, or a certain draft) */
   int V, gone;         /* the certain draft's token, or -1 */
-  double mp, mq, cp, cq, ip, iq; /* greatest logits, log2(e) / T, the sums' reciprocals */
+  double mp, mq, cp, cq;       /* greatest logits, log2(e) / T */
+  double ip, iq, whole;        /* what the terms are multiplied by, and what p's then sum to */
 
   /* sp, sq: what the sequence's rows hold */
-  __device__ __forceinline__ Weights(const d3s_verify_params &a, const Seq &s, int accepted, bool rejected, float m_p, float m_q) {
+  __device__ __forceinline__ Weights(const d3s_verify_params &a, const Seq &s, int accepted, bool rejected, float m_p, float m_q, int x) {
     tp = (const char *)a.target + ((int64_t)s.b * (a.n_draft + 1) + accepted) * a.target_stride * (TB ? 2 : 4);
     dp = rejected && a.draft ? (const char *)a.draft + ((int64_t)s.b * a.n_draft + accepted) * a.draft_stride * (DB ? 2 : 4) : nullptr;
     V = (int)a.vocab;
-    gone = rejected && !a.draft ? a.drafted[(size_t)s.b * a.n_draft + accepted] : -1;
+    gone = rejected && !a.draft ? __builtin_amdgcn_readlane(x, accepted & (WAVE - 1)) : -1;
     mp = m_p, mq = m_q;
     cp = LOG2E_64 / s.T, cq = LOG2E_64 / s.Td;
-    ip = iq = 1.0;
+    ip = iq = whole = 1.0;
   }
   __device__ __forceinline__ int left(int j) const { return min(8, V - j); }
   /* eight terms of each sum from j on (0 past the end), j < V */
@@ -226,7 +237,7 @@ struct Weights {
       if (dp)
         r[e] = fmax(r[e] - q[e] * iq, 0.0);
       else if (j + e == gone)
-        r[e] = fmax(r[e] - 1.0, 0.0);
+        r[e] = fmax(r[e] - whole, 0.0);
     }
   }
 };
@@ -286,23 +297,26 @@ __device__ __forceinline__ double block_scan64(double v, DrawLds<NT> &L, double 
  * every thread: a thread's eight weights r follow each other from j on, `before` is the sum of
  * those before them. */
 template <int NT>
-__device__ __forceinline__ int first_past(const double *r, int j, double before, double bar, bool last_too, DrawLds<NT> &L) {
+__device__ __forceinline__ int first_past(const double *r, int j, double before, double bar, bool last_too, DrawLds<NT> &L,
+                                          bool ready = false) {
   int over = 0x7fffffff, last = -1;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     before += r[e];
-    if (r[e] > 0.0) {
-      last = j + e;
-      if (before > bar) over = min(over, j + e);
-    }
+    last = r[e] > 0.0 ? j + e : last;
+    over = min(over, r[e] > 0.0 && before > bar ? j + e : 0x7fffffff);
   }
-  if (threadIdx.x == 0) L.at = 0x7fffffff;
-  __syncthreads();
-  if (over != 0x7fffffff) atomicMin(&L.at, over);
+  if (!ready) { /* (L.at holds it) */
+    if (threadIdx.x == 0) L.at = 0x7fffffff;
+    __syncthreads();
+  }
+  /* (places rise with the lanes: the first that has one speaks for its wave) */
+  const uint64_t has = __ballot(over != 0x7fffffff);
+  if (has && lane_id() == (int)__builtin_ctzll(has)) atomicMin(&L.at, over);
   __syncthreads();
   int at = L.at;
   if (at != 0x7fffffff || !last_too) {
-    __syncthreads();
+    if (!ready) __syncthreads();
     return at != 0x7fffffff ? at : -1;
   }
   __syncthreads();
@@ -340,25 +354,29 @@ __device__ __forceinline__ int pick(const Weights<TB, DB> &W, int lo, int hi, do
 
 /* A workgroup a sequence: a wave a row of logits, then the draw.  HELD: rows of which a
  * thread's eight elements are all (VT * 8): their terms stay in registers from the sums to the
- * token; else three passes. */
+ * token; else three passes.  One row of 4097 of four drafts: a chain of dependent steps (loads, sums,
+ * decision, loads, 64-bit terms, two sums over the workgroup, the place). */
 template <bool TB, bool DB, bool HELD>
-__global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
+__global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a, int b0) {
   __shared__ Settled S;
   __shared__ DrawLds<VT> L;
+  __shared__ double pair[VT / WAVE][2];
   const int tid = (int)threadIdx.x, V = (int)a.vocab;
-  const Seq q(a, (int)blockIdx.x);
+  const Seq q(a, b0 + (int)blockIdx.x);
   const float u = lane_u(a, q), ud = a.u_draw[q.b];
+  const int x = lane_draft(a, q);
   for (int r = tid / WAVE; r < q.rows; r += VT / WAVE) {
     if (!q.there(a, r)) continue;
-    const float l = draft_logit<TB, DB>(a, q, r);
+    float l;
     Sums s{-FLT_MAX, 0.0f, 0.0f};
     const float c = LOG2E / q.temperature(a, r);
+    auto beside = [&] { l = draft_logit<TB, DB>(a, q, r); };
     if (q.target(a, r)) {
       const Row<TB> R(a.target, a.target_stride, q.row(a, r), V, -1);
-      lane_sums(s, R, lane_id(), R.chunks, WAVE, c);
+      lane_sums(s, R, lane_id(), R.chunks, WAVE, c, beside);
     } else {
       const Row<DB> R(a.draft, a.draft_stride, q.row(a, r), V, -1);
-      lane_sums(s, R, lane_id(), R.chunks, WAVE, c);
+      lane_sums(s, R, lane_id(), R.chunks, WAVE, c, beside);
     }
     join_wave(s, c);
     if (lane_id() == 0) settle_row(a, q, r, RowStat{s.m, s.S}, l, S);
@@ -371,7 +389,7 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
   if (o.refuse || masked) {
     if (tid == 0 && a.counters) atomicAdd(&a.counters[masked ? CNT_ALL_MASKED : CNT_REFUSED], 1u);
   } else {
-    Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, S.stat[o.rejected && a.draft ? a.n_draft + 1 + o.accepted : 0].m);
+    Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, S.stat[o.rejected && a.draft ? a.n_draft + 1 + o.accepted : 0].m, x);
     double sp = 0.0, sq = 0.0, p[8], t[8];
     if (HELD) {
 #pragma unroll
@@ -387,11 +405,18 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
       }
       if (HELD) break;
     }
-    W.ip = 1.0 / block_sum64(sp, L);
-    if (W.dp) {
-      sq = block_sum64(sq, L);
-      W.iq = sq > 0.0 ? 1.0 / sq : 0.0;
-    }
+    /* weights p_j - rho q_j: the draw needs no quotient by their sum */
+    sp = wave_scan64(sp);
+    sq = W.dp ? wave_scan64(sq) : 0.0;
+    if (lane_id() == WAVE - 1) pair[tid / WAVE][0] = sp, pair[tid / WAVE][1] = sq;
+    if (tid == 0) L.at = 0x7fffffff;
+    __syncthreads();
+    sp = sq = 0.0;
+#pragma unroll
+    for (int w = 0; w < VT / WAVE; w++) sp += pair[w][0], sq += pair[w][1];
+    W.iq = sq > 0.0 ? sp / sq : 0.0;
+    W.ip = 1.0;
+    W.whole = sp;
     bool plain = !o.rejected;
     double r[8], Z;
     for (;;) {
@@ -402,7 +427,7 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
         for (int e = 0; e < 8; e++) mine += r[e];
         const double before = block_scan64(mine, L, &Z);
         if (Z > 0.0 || plain) {
-          token = first_past(r, tid * 8, before, (double)ud * Z, true, L);
+          token = first_past(r, tid * 8, before, (double)ud * Z, true, L, true);
           break;
         }
       } else {
@@ -421,7 +446,7 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a) {
       plain = true; /* (p <= q everywhere: by rounding alone) */
     }
   }
-  write_tokens(q.b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
+  write_tokens(q.b, a.n_draft, o, token, x, a.tokens, a.n_accepted);
 }
 
 /* ---- long rows: two launches ---- */
@@ -454,7 +479,7 @@ __global__ __launch_bounds__(ST) void k_verify_rows(d3s_verify_params a, VerifyS
   const float c = LOG2E / q.temperature(a, r);
   auto go = [&](const auto &R) {
     const int per = (R.chunks + sp.nseg - 1) / sp.nseg;
-    lane_sums(s, R, seg * per + (int)threadIdx.x, min(R.chunks, (seg + 1) * per), ST, c);
+    lane_sums(s, R, seg * per + (int)threadIdx.x, min(R.chunks, (seg + 1) * per), ST, c, [] {});
   };
   if (q.target(a, r))
     go(Row<TB>(a.target, a.target_stride, q.row(a, r), (int)a.vocab, -1));
@@ -488,6 +513,7 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   const int blk = (int)(blockIdx.x % (unsigned)sp.nblk);
   const Seq q(a, (int)(blockIdx.x / (unsigned)sp.nblk));
   const float u = lane_u(a, q), ud = a.u_draw[q.b];
+  const int x = lane_draft(a, q);
   if (tid < q.rows && q.there(a, tid)) {
     const float l = draft_logit<TB, DB>(a, q, tid);
     const float c = LOG2E / q.temperature(a, tid);
@@ -503,33 +529,33 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   const bool masked = !o.refuse && P.S == 0.0f;
   if (o.refuse || masked) {
     if (blk != 0) return;
-    write_tokens(q.b, a.n_draft, o, masked ? 0 : -1, a.drafted, a.tokens, a.n_accepted);
+    write_tokens(q.b, a.n_draft, o, masked ? 0 : -1, x, a.tokens, a.n_accepted);
     if (tid == 0 && a.counters) atomicAdd(&a.counters[masked ? CNT_ALL_MASKED : CNT_REFUSED], 1u);
     return;
   }
-  Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, Q.m);
+  Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, Q.m, x);
   const double rho0 = W.dp && Q.S > 0.0f ? (double)P.S / Q.S : 0.0;
   const int part = sp.block / SWV;
   {
     const int lo = blk * sp.block + tid / WAVE * part, hi = (int)min((int64_t)a.vocab, (int64_t)lo + part);
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
     for (int j = lo + lane_id() * 8; j < hi; j += WAVE * 8) {
-      double x[8], y[8];
-      W.terms(j, x, y);
+      double p[8], t[8];
+      W.terms(j, p, t);
       if (W.dp) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          const double d = fma(-rho0, y[e], x[e]);
-          sum[0] += x[e];
-          sum[1] += y[e];
+          const double d = fma(-rho0, t[e], p[e]);
+          sum[0] += p[e];
+          sum[1] += t[e];
           sum[2] += d > 0.0 ? d : 0.0;
-          sum[3] += d > 0.0 ? y[e] : 0.0;
+          sum[3] += d > 0.0 ? t[e] : 0.0;
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          sum[0] += x[e];
-          sum[2] += j + e == W.gone ? 0.0 : x[e];
+          sum[0] += p[e];
+          sum[2] += j + e == W.gone ? 0.0 : p[e];
         }
       }
     }
@@ -605,7 +631,7 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     token = pick<ST>(W, which * part, (int)min((int64_t)a.vocab, (int64_t)(which + 1) * part), base, bar, plain, L);
     if (plain) break;
   }
-  write_tokens(q.b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
+  write_tokens(q.b, a.n_draft, o, token, x, a.tokens, a.n_accepted);
 }
 
 /* ------------------------------------------------------------------------ */
@@ -709,7 +735,7 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
       plain = true;
     }
   }
-  write_tokens(b, a.n_draft, o, token, a.drafted, a.tokens, a.n_accepted);
+  write_tokens(b, a.n_draft, o, token, mine, a.tokens, a.n_accepted);
 }
 
 }  // namespace
@@ -755,11 +781,14 @@ template <bool TB, bool DB>
 static void verify_launch(const d3s_verify_params &a, void *ws, hipStream_t s) {
   VerifySplit sp;
   if (!verify_split(a, &sp)) {
-    const dim3 grid((unsigned)a.n_seqs);
-    if (a.vocab <= VT * 8)
-      k_verify_one<TB, DB, true><<<grid, VT, 0, s>>>(a);
-    else
-      k_verify_one<TB, DB, false><<<grid, VT, 0, s>>>(a);
+    constexpr int64_t MOST = 1 << 21; /* workgroups a launch: their threads are counted in 32 bits */
+    for (int64_t b = 0; b < a.n_seqs; b += MOST) {
+      const dim3 grid((unsigned)(a.n_seqs - b < MOST ? a.n_seqs - b : MOST));
+      if (a.vocab <= VT * 8)
+        k_verify_one<TB, DB, true><<<grid, VT, 0, s>>>(a, (int)b);
+      else
+        k_verify_one<TB, DB, false><<<grid, VT, 0, s>>>(a, (int)b);
+    }
     return;
   }
   VerifyRoom w;
