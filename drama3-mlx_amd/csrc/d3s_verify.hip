@@ -652,6 +652,7 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
   const int i = lane_id();
   const int mine = i < a.n_draft ? a.drafted[(size_t)b * a.n_draft + i] : -1; /* lane i: draft i */
   const float u = i < a.n_draft ? a.u_accept[(size_t)b * a.n_draft + i] : 0.0f;
+  const float ud = tid < a.target_k ? a.u_draw[(size_t)b * a.target_k + tid] : 0.0f; /* rank tid's */
   const size_t t0 = (size_t)b * (a.n_draft + 1) * a.target_k, d0 = (size_t)b * a.n_draft * a.draft_k;
   const int nt = (len + 1) * a.target_k, nd = a.draft_cand ? len * a.draft_k : 0;
   const bool held = nt + nd <= HELD;
@@ -678,8 +679,8 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
   };
   look(a.target_cand + t0, a.target_probs + t0, a.target_k, nt, prob, 0);
   if (a.draft_cand) look(a.draft_cand + d0, a.draft_probs + d0, a.draft_k, nd, prob + D3S_MAX_DRAFT, nt);
-  const bool last_refused = a.target_cand[t0 + (size_t)len * a.target_k] < 0;
   __syncthreads();
+  const bool last_refused = (held ? cand[len * a.target_k] : a.target_cand[t0 + (size_t)len * a.target_k]) < 0;
   const float p = i < len ? prob[i] : 0.0f, q = i < len ? prob[D3S_MAX_DRAFT + i] : 0.0f;
   const Outcome o = decide(len, u, p, q, last_refused);
   if (a.accept && tid < a.n_draft) a.accept[(size_t)b * a.n_draft + i] = i < len ? accept_of(p, q) : 0.0f;
@@ -707,13 +708,15 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
         const int id = held ? cand[o.accepted * a.target_k + r] : tc[r];
         float w = held ? qs[o.accepted * a.target_k + r] : tp[r];
         if (!plain && pair) {
-          for (int e = 0; e < a.draft_k; e++)
-            if (cand[qa + e] == id && qs[qa + e] > 0.0f) w -= qs[qa + e];
+          float gone = 0.0f; /* (one candidate at most is this one) */
+#pragma unroll 8
+          for (int e = 0; e < a.draft_k; e++) gone = cand[qa + e] == id ? qs[qa + e] : gone;
+          if (gone > 0.0f) w -= gone;
         } else if (!plain && id == x) {
           w -= 1.0f;
         }
         if (!(w > 0.0f)) continue;
-        float score = w / -d3s_logf(1.0f - a.u_draw[(size_t)b * a.target_k + r]);
+        float score = w / -d3s_logf(1.0f - (r < RT ? ud : a.u_draw[(size_t)b * a.target_k + r]));
         score = score > -1.0f ? score : -1.0f; /* (u = 0 gives -inf, as the sampler's race: the last choice) */
         if (score > sc) sc = score, at = r;    /* (a thread's ranks rise) */
       }
@@ -724,7 +727,7 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
       for (int w = 0; w < RT / WAVE; w++)
         if (best[w] > sc || (best[w] == sc && best_at[w] < at)) sc = best[w], at = best_at[w];
       if (at != 0x7fffffff) {
-        token = tc[at];
+        token = held ? cand[o.accepted * a.target_k + at] : tc[at];
         break;
       }
       if (plain) { /* no rank has a probability: a masked row */
