@@ -11,7 +11,8 @@ constexpr int NT = 256;
 constexpr int NW = NT / WAVE;
 constexpr float E4M3_MOST = 448.0f;
 
-/* the sum (or greatest) over the workgroup, in every thread, added in one order */
+/* the sum (or greatest) over a workgroup of T threads, in every thread, added in one order */
+template <int T>
 __device__ __forceinline__ float block_sum(float v, float *part) {
   v = readlane_f(wave_scan_add_f32(v), 63);
   __syncthreads();
@@ -19,9 +20,10 @@ __device__ __forceinline__ float block_sum(float v, float *part) {
   __syncthreads();
   float t = 0.0f;
 #pragma unroll
-  for (int w = 0; w < NW; w++) t += part[w];
+  for (int w = 0; w < T / WAVE; w++) t += part[w];
   return t;
 }
+template <int T>
 __device__ __forceinline__ float block_max(float v, float *part) {
   v = wave_max_f(v);
   __syncthreads();
@@ -29,7 +31,7 @@ __device__ __forceinline__ float block_max(float v, float *part) {
   __syncthreads();
   float t = part[0];
 #pragma unroll
-  for (int w = 1; w < NW; w++) t = __builtin_elementwise_maximum(t, part[w]);
+  for (int w = 1; w < T / WAVE; w++) t = __builtin_elementwise_maximum(t, part[w]);
   return t;
 }
 
@@ -64,7 +66,7 @@ __device__ __forceinline__ float e4m3_scale(float most) {
 /* the sum (or greatest) over the G threads of a row, in each of them, added in one order */
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float *part) {
-  if constexpr (G == NT) return block_sum(v, part);
+  if constexpr (G >= NT) return block_sum<G>(v, part);
   if constexpr (G == WAVE) return readlane_f(wave_scan_add_f32(v), 63);
 #pragma unroll
   for (int d = 1; d < G; d *= 2) v += __shfl_xor(v, d);
@@ -72,7 +74,7 @@ __device__ __forceinline__ float row_sum(float v, float *part) {
 }
 template <int G>
 __device__ __forceinline__ float row_max(float v, float *part) {
-  if constexpr (G == NT) return block_max(v, part);
+  if constexpr (G >= NT) return block_max<G>(v, part);
   if constexpr (G == WAVE) return wave_max_f(v);
 #pragma unroll
   for (int d = 1; d < G; d *= 2) v = __builtin_elementwise_maximum(v, __shfl_xor(v, d));
@@ -188,9 +190,9 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
 /* The gradient, rows held the same way; a workgroup takes every gridDim.x-th set of
  * rows and keeps their columns' sums of dy xhat in registers. */
 template <bool BF16, int G, int U, bool SUM>
-__global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) {
-  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G, E = BF16 ? 8 : 4;
-  __shared__ float part[NW];
+__global__ __launch_bounds__(G > NT ? G : NT) void k_norm_grad(NormGradArgs a, float *parts) {
+  constexpr int ES = BF16 ? 2 : 4, ROWS = G > NT ? 1 : NT / G, E = BF16 ? 8 : 4;
+  __shared__ float part[G > NT ? G / WAVE : NW];
   __shared__ float sums[SUM && ROWS > 1 ? NT * U * E : 1];
   const int g = (int)threadIdx.x % G, width = (int)a.width;
   Vec<BF16, E> w[U];
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(NT) void k_norm_grad(NormGradArgs a, float *parts) 
 #pragma unroll
     for (int e = 0; e < E; e++) acc[u][e] = 0.0f;
   /* a row's inputs; the next row's are loaded while this one is worked on, where registers allow */
-  constexpr bool AHEAD = U * E <= 16;
+  constexpr bool AHEAD = U * E <= 8 || (G <= WAVE && U * E <= 16);
   struct In {
     Vec<BF16, E> d[U], h[U], r[U];
     float rstd;
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(NT) void k_norm_rows(NormArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; e++) s = fmaf(h[e], h[e], s);
     }
-    s = block_sum(s, part);
+    s = block_sum<NT>(s, part);
     const float rstd = 1.0f / sqrtf(s / (float)a.width + a.eps);
     if (tid == 0 && a.rstd) a.rstd[row] = rstd;
     auto scaled = [&](int64_t j, int left, float *h) {
@@ -341,7 +343,7 @@ __global__ __launch_bounds__(NT) void k_norm_rows(NormArgs a) {
         scaled(j, left_at(j), h);
         most = __builtin_elementwise_maximum(most, greatest(h, left_at(j)));
       }
-      row_scale = e4m3_scale(block_max(most, part));
+      row_scale = e4m3_scale(block_max<NT>(most, part));
       if (tid == 0) a.scales[row] = row_scale;
     }
     for (int64_t base = 0; base < a.width; base += NT * 8) {
@@ -398,7 +400,7 @@ __global__ __launch_bounds__(NT) void k_norm_grad_rows(NormGradArgs a) {
 #pragma unroll
       for (int e = 0; e < 8; e++) s = fmaf(p[e], xhat[e], s);
     }
-    const float mean = block_sum(s, part) / (float)a.width;
+    const float mean = block_sum<NT>(s, part) / (float)a.width;
     for (int64_t j = tid * 8; j < a.width; j += NT * 8) {
       const int left = (int)min((int64_t)8, a.width - j);
       float p[8], xhat[8], d[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -442,28 +444,38 @@ bool in_registers(int64_t width, F f) {
   return false;
 }
 
-/* The same for the gradient, whose inputs are three rows and whose sums stay: a workgroup a row
- * beyond 1024, so that the next row's loads fit beside them (8192 x 2048 bf16: 32 us; a wave a row,
- * without loads ahead, 43). */
+/* The same for the gradient, whose inputs are three rows and whose sums stay: beyond 1024 columns a
+ * workgroup a row, of as many threads as leave 8 elements each, so that the next row's loads fit beside them
+ * (8192 x 2048 bf16: 32 us; a wave a row, without loads ahead, 43.  4096 x 5000 fp32: 80 us; 256 threads
+ * 114).  32 beyond 8192 (1024 x 16384 fp32: 68 us; 1024 threads, whose registers spill, 77). */
 template <int E, class F>
 bool grad_in_registers(int64_t width, F f) {
-  if (width > 1024 && width <= 2048) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8 / E>{}), true;
-  return in_registers<E>(width, f);
+  constexpr int M = 8 / E;
+  auto go = [&](auto g, auto u) { return f(g, u), true; };
+  using std::integral_constant;
+  if (width <= 1024) return in_registers<E>(width, f);
+  if (width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, M>{});
+  if (width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, M>{});
+  if (width <= 8192) return go(integral_constant<int, 1024>{}, integral_constant<int, M>{});
+  if (width <= 16384) return go(integral_constant<int, 512>{}, integral_constant<int, 4 * M>{});
+  return false;
 }
 
 /* Workgroups of the gradient: the runs of its column sums.  As many as are resident (512: 36 us for
- * 8192 x 2048, 768 and 1024: 32, 1280 and 2048: 38). */
-constexpr int GRAD_RUNS = 1024;
+ * 8192 x 2048, 768 and 1024: 32, 1280 and 2048: 38); of wide rows fewer, since each leaves a row of
+ * sums (4096 x 4096 bf16 with 512, 768 and 1024: 31, 37 and 37; 2048 x 8192 with 256, 384 and 512: 33, 41 and
+ * 38). */
+int64_t grad_runs(int64_t width) { return width <= 2048 ? 1024 : width <= 4096 ? 512 : 256; }
 struct GradSplit {
   int64_t strips;
   int rows, runs;
 };
 GradSplit grad_split(int64_t n_rows, int64_t width) {
   GradSplit p{1, 0, 0};
-  const bool held = grad_in_registers<8>(width, [&](auto g, auto) { p.rows = NT / decltype(g)::value; });
+  const bool held = grad_in_registers<8>(width, [&](auto g, auto) { p.rows = decltype(g)::value > NT ? 1 : NT / decltype(g)::value; });
   if (held) {
     const int64_t sets = (n_rows + p.rows - 1) / p.rows;
-    p.runs = (int)(sets < GRAD_RUNS ? sets : GRAD_RUNS);
+    p.runs = (int)(sets < grad_runs(width) ? sets : grad_runs(width));
   } else {
     p.strips = (width + NT - 1) / NT;
     int64_t runs = 1024 / p.strips;
@@ -504,21 +516,24 @@ void launch_norm(const NormArgs &args, Dtype dt, hipStream_t s) {
 
 size_t norm_grad_workspace_bytes(int64_t n_rows, int64_t width, bool dgain) {
   if (!dgain || n_rows == 0 || width == 0) return 0;
-  return split_counter_bytes() + (size_t)grad_split(n_rows, width).runs * (size_t)width * sizeof(float);
+  const int runs = grad_split(n_rows, width).runs;
+  return runs == 1 ? 0 : split_counter_bytes() + (size_t)runs * (size_t)width * sizeof(float);
 }
 
 void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t s) {
   const NormGradArgs a = args;
   const GradSplit p = grad_split(a.n_rows, a.width);
-  float *parts = ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
+  /* (one run's sums are dgain) */
+  float *parts = p.runs == 1 ? a.dgain : ws ? (float *)((char *)ws + split_counter_bytes()) : nullptr;
   auto rows_held = [&](auto bf16) {
     constexpr bool B = decltype(bf16)::value;
     return grad_in_registers<B ? 8 : 4>(a.width, [&](auto g, auto u) {
       constexpr int G = decltype(g)::value, U = decltype(u)::value;
+      constexpr int T = G > NT ? G : NT;
       if (a.dgain)
-        k_norm_grad<B, G, U, true><<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts);
+        k_norm_grad<B, G, U, true><<<dim3((unsigned)p.runs), T, 0, s>>>(a, parts);
       else
-        k_norm_grad<B, G, U, false><<<dim3((unsigned)p.runs), NT, 0, s>>>(a, parts);
+        k_norm_grad<B, G, U, false><<<dim3((unsigned)p.runs), T, 0, s>>>(a, parts);
     });
   };
   const bool held = p.runs && (dt == DT_BF16 ? rows_held(std::true_type{}) : rows_held(std::false_type{}));
@@ -532,7 +547,7 @@ void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t 
     }
     if (a.dx) dt == DT_BF16 ? k_norm_grad_rows<true><<<rows, NT, 0, s>>>(a) : k_norm_grad_rows<false><<<rows, NT, 0, s>>>(a);
   }
-  if (a.dgain) launch_column_sums(parts, p.runs, (int)a.width, a.dgain, s);
+  if (a.dgain && p.runs != 1) launch_column_sums(parts, p.runs, (int)a.width, a.dgain, s);
 }
 
 }  // namespace d3s
