@@ -743,10 +743,11 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
 
 }  // namespace
 
-/* Long rows of not too many sequences are split over the chip (beyond, a workgroup a
- * sequence fills it). */
+/* Rows longer than a workgroup holds are split over the chip, unless there are so many sequences that
+ * a workgroup for each fills it (16 sequences of 4 drafts over 16384: 14 us, by a workgroup each 38; 300 of
+ * 3 over 16000: 39, 68). */
 static bool verify_split(const d3s_verify_params &a, VerifySplit *sp) {
-  if (a.vocab <= 16384 || a.n_seqs > 2048) return false;
+  if (a.vocab <= VT * 8 || a.n_seqs > 2048) return false;
   const int64_t rows = a.n_seqs * (2 * a.n_draft + 1);
   /* segments of two batches of bf16 chunks a lane, one where there are few */
   const int64_t batches = ((a.vocab + 7) / 8 + SU * ST - 1) / (SU * ST);
