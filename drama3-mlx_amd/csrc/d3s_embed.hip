@@ -53,6 +53,8 @@ __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, int lanes, int64_t st
  * the positions follow each other in `order` behind those of lower rows, which it counts
  * as it goes (a counter that each workgroup raises takes 23 ns a workgroup: 26 us for 1187), and seg
  * says for each row where and how many.
+ * Many ids are parted first, by range, so that no workgroup looks through all of them (k_part_count,
+ * k_part_scan, k_part_move: counts for each block of ids, their sums, the ids' places).
  * k_embed_sum: a row's positions are summed in that order, by lanes across its columns;
  * rows that no id names are filled with zeros.  A row of more than `hot` positions is cut into chunks
  * of as many, filed in a list; workgroups of their own sum the chunks in fp32, and the last
@@ -67,8 +69,19 @@ constexpr int HOT_GROUPS = 512;   /* workgroups for the chunks */
 constexpr int HOT_MOST = 4096;    /* rows that are cut, at most: a counter of arrivals each */
 constexpr int HOT_COUNTERS = 64;  /* words before them */
 
+
+constexpr int PT = 1024;          /* threads of the parting kernels */
+constexpr int PW = PT / WAVE;
+constexpr int PART_IDS = 8;       /* ids a thread */
+constexpr int PART_BLOCK = PT * PART_IDS;
+constexpr int PARTS = 1024;       /* ranges that ids are parted into, at most */
+constexpr int PART_LEAST = 65536; /* fewer ids are not parted (16384: 76 us, so 96) */
+
 struct Seg {
   int start, count; /* count < 0: cut into chunks */
+};
+struct Entry {
+  int pos, row; /* the row of dy, the row within its range */
 };
 struct Chunk {
   int64_t row;
@@ -81,6 +94,9 @@ struct GradPlan {
   int64_t slots, part, rows, n; /* parts of the table, rows of each and in all, ids of each */
   int range, hot;               /* rows of a range; a row of more positions is cut */
   int64_t ranges;               /* of each part */
+  bool parted;
+  int bits;                     /* range = 1 << bits */
+  int blocks;                   /* of ids to part */
 };
 struct GradRoom {
   uint32_t *counters;
@@ -88,6 +104,9 @@ struct GradRoom {
   int *order;
   Chunk *chunks;
   float *sums; /* a chunk's, [.., width] */
+  int *table;  /* [blocks, PARTS]: a block's ids of a range, then those of the blocks before */
+  int *begin;  /* [PARTS + 1]: the ranges' first entries */
+  Entry *entries;
 };
 
 GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) {
@@ -101,6 +120,13 @@ GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) 
   p.range = 256;
   auto count = [&](int64_t r) { return (vocab + r - 1) / r; };
   while (p.range < RANGE_MOST && p.slots * count(p.range) > 512 && p.slots * count(p.range) * p.n > (int64_t)32 << 20) p.range *= 2;
+  /* (ids that do not fit the parts' number are looked through) */
+  p.parted = p.n * p.slots >= PART_LEAST && p.slots * count(RANGE_MOST) <= PARTS;
+  if (p.parted)
+    for (p.range = 64; p.slots * count(p.range) > PARTS;) p.range *= 2;
+  p.bits = 0;
+  while ((1 << p.bits) < p.range) p.bits++;
+  p.blocks = p.parted ? (int)((p.n * p.slots + PART_BLOCK - 1) / PART_BLOCK) : 0;
   p.ranges = count(p.range);
   p.hot = 64;
   while ((int64_t)p.hot * HOT_MOST < p.n * p.slots) p.hot *= 2;
@@ -121,30 +147,140 @@ size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
   w->order = (int *)take((size_t)(p.n * p.slots) * sizeof(int));
   w->chunks = (Chunk *)take((size_t)chunks_most(p) * sizeof(Chunk));
   w->sums = (float *)take((size_t)chunks_most(p) * (size_t)((width + 7) / 8 * 8) * sizeof(float));
+  w->table = (int *)take((size_t)p.blocks * PARTS * sizeof(int));
+  w->begin = (int *)take(p.parted ? (PARTS + 1) * sizeof(int) : 0);
+  w->entries = (Entry *)take(p.parted ? (size_t)(p.n * p.slots) * sizeof(Entry) : 0);
   return at;
 }
 
+/* the range of id number `at`, or -1 */
+__device__ __forceinline__ int part_of(const EmbedArgs &a, const GradPlan &p, int at, int id) {
+  if ((uint32_t)id >= (uint64_t)a.vocab) return -1;
+  return (p.slots > 1 ? at % a.n_ids * (int)p.ranges : 0) + (id >> p.bits);
+}
+
+__global__ __launch_bounds__(PT) void k_part_count(EmbedArgs a, GradPlan p, GradRoom w) {
+  __shared__ int hist[PARTS];
+  const int tid = (int)threadIdx.x, n = (int)(p.n * p.slots);
+  if (tid < PARTS) hist[tid] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * PART_BLOCK;
+  for (int u = 0; u < PART_IDS; u++) {
+    const int64_t at = first + u * PT + tid;
+    const int r = at < n ? part_of(a, p, (int)at, a.ids[at]) : -1;
+    if (r >= 0) atomicAdd(&hist[r], 1);
+  }
+  __syncthreads();
+  if (tid < PARTS) w.table[(int64_t)blockIdx.x * PARTS + tid] = hist[tid];
+}
+
+/* a thread a range: its ids in the blocks before each, and the ranges' first places */
+__global__ __launch_bounds__(PARTS) void k_part_scan(GradPlan p, GradRoom w) {
+  __shared__ int wave_sum[PARTS / WAVE];
+  const int r = (int)threadIdx.x;
+  int sum = 0, b = 0;
+  constexpr int UN = 8;
+  for (; b + UN <= p.blocks; b += UN) {
+    int c[UN];
+#pragma unroll
+    for (int u = 0; u < UN; u++) c[u] = w.table[(int64_t)(b + u) * PARTS + r];
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+      w.table[(int64_t)(b + u) * PARTS + r] = sum;
+      sum += c[u];
+    }
+  }
+  for (; b < p.blocks; b++) {
+    const int c = w.table[(int64_t)b * PARTS + r];
+    w.table[(int64_t)b * PARTS + r] = sum;
+    sum += c;
+  }
+  const int incl = (int)wave_scan_add_u32((uint32_t)sum);
+  if (lane_id() == WAVE - 1) wave_sum[r / WAVE] = incl;
+  __syncthreads();
+  int before = 0;
+  for (int g = 0; g < r / WAVE; g++) before += wave_sum[g];
+  w.begin[r] = before + incl - sum;
+  if (r == PARTS - 1) w.begin[PARTS] = before + incl;
+}
+
+/* lanes of one key (`bits` wide) among those of `hits` */
+__device__ __forceinline__ uint64_t peers_of(int key, bool hit, uint64_t hits, int bits) {
+  uint64_t peers = hits;
+  for (int b = 0; b < bits; b++) {
+    const uint64_t m = __ballot(hit && (key >> b & 1));
+    peers &= key >> b & 1 ? m : ~m;
+  }
+  return peers;
+}
+__device__ __forceinline__ int lanes_below(uint64_t m) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+}
+
+/* a block's ids to their ranges' places, in their order */
+__global__ __launch_bounds__(PT) void k_part_move(EmbedArgs a, GradPlan p, GradRoom w) {
+  __shared__ uint16_t cnt[PW][PARTS]; /* a wave's ids of a range, then those of the waves before (at most 8192) */
+  __shared__ int base[PARTS];
+  const int tid = (int)threadIdx.x, wid = tid / WAVE, n = (int)(p.n * p.slots);
+  for (int i = tid; i < PW * PARTS / 2; i += PT) ((uint32_t *)cnt)[i] = 0u;
+  if (tid < PARTS) base[tid] = w.begin[tid] + w.table[(int64_t)blockIdx.x * PARTS + tid];
+  const int64_t first = (int64_t)blockIdx.x * PART_BLOCK + wid * (PART_IDS * WAVE) + lane_id();
+  int id[PART_IDS], key[PART_IDS];
+#pragma unroll
+  for (int u = 0; u < PART_IDS; u++) {
+    const int64_t at = first + u * WAVE;
+    id[u] = at < n ? a.ids[at] : -1;
+    key[u] = part_of(a, p, (int)at, id[u]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < PART_IDS; u++)
+    if (key[u] >= 0) atomicAdd((uint32_t *)&cnt[wid][key[u] & ~1], 1u << 16 * (key[u] & 1));
+  __syncthreads();
+  if (tid < PARTS) {
+    int sum = 0;
+    for (int g = 0; g < PW; g++) {
+      const int c = cnt[g][tid];
+      cnt[g][tid] = (uint16_t)sum;
+      sum += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < PART_IDS; u++) {
+    const bool hit = key[u] >= 0;
+    const uint64_t hits = __ballot(hit), peers = peers_of(key[u], hit, hits, 10);
+    const int k = lanes_below(peers);
+    int place = 0;
+    if (hit) {
+      place = cnt[wid][key[u]];
+      w.entries[base[key[u]] + place + k] = Entry{(int)((uint32_t)(first + u * WAVE) / (uint32_t)a.n_ids), id[u] & (p.range - 1)};
+    }
+    wave_lds_sync();
+    if (hit && (peers >> lane_id()) >> 1 == 0ull) cnt[wid][key[u]] = (uint16_t)(place + k + 1); /* the last of them */
+    wave_lds_sync();
+  }
+}
+
+template <bool PARTED>
 __global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
   extern __shared__ int cnt[]; /* [GW][range]: a wave's count of a row, then its place */
-  __shared__ int list_pos[GW][LIST];
-  __shared__ uint16_t list_row[GW][LIST];
+  __shared__ int list_pos[GW][PARTED ? 1 : LIST];
+  __shared__ uint16_t list_row[GW][PARTED ? 1 : LIST];
   __shared__ int wave_sum[GW], wave_less[GW];
   const int tid = (int)threadIdx.x, wid = tid / WAVE, lane = lane_id();
-  int bits = 0;
-  while ((1 << bits) < p.range) bits++;
-  const int n = (int)p.n, each = (n / GW + WAVE) / WAVE * WAVE; /* ids of a wave */
   const int step = a.slot_rows ? a.n_ids : 1;                   /* (the last is below 2^31) */
   for (int64_t blk = blockIdx.x; blk < p.slots * p.ranges; blk += gridDim.x) {
     const int64_t slot = blk / p.ranges, v0 = blk % p.ranges * p.range;
     const uint32_t rows = (uint32_t)min((int64_t)p.range, a.vocab - v0);
-    const int i0 = (int)min((int64_t)n, (int64_t)wid * each), i1 = (int)min((int64_t)n, (int64_t)i0 + each);
+    /* the wave's ids, of its slot's or of its range's entries */
+    const int from = PARTED ? w.begin[blk] : 0, n = PARTED ? w.begin[blk + 1] - from : (int)p.n;
+    const int each = (n / GW + WAVE) / WAVE * WAVE;
+    const int i0 = min(n, wid * each), i1 = min(n, i0 + each);
     const int32_t *ids = a.slot_rows ? a.ids + slot : a.ids;
     for (int i = tid; i < GW * p.range; i += GT) cnt[i] = 0;
     __syncthreads();
     int *mine = cnt + wid * p.range;
-    auto below = [&](uint64_t m) {
-      return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
-    };
     /* The wave's ids, AHEAD in a row for each lane: those of this range's rows go to its list, those of
      * lower rows are counted (an id below 0 is a row past 2^31 - v0 here).  Most of the kernel's time is this
      * chain; the code has to be short, since it is fetched while it runs (64 ids at a time by ballots,
@@ -161,8 +297,8 @@ __global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, Gra
         for (int e = 0; e < AHEAD; e++, q += step) next[e] = at + e < i1 ? *q : -1;
       }
     };
-    load(i0);
-    for (int i = i0; i < i1; i += AHEAD * WAVE) {
+    if (!PARTED) load(i0);
+    for (int i = i0; !PARTED && i < i1; i += AHEAD * WAVE) {
       const int at = i + lane * AHEAD;
       int id[AHEAD];
 #pragma unroll
@@ -184,21 +320,42 @@ __global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, Gra
       }
     }
     less = (int)wave_sum_u32((uint32_t)less);
-    /* f(position, row, whether it is this range's, which lanes' are) for them in their order: from the list, or
-     * where it does not hold them from the ids again */
+    /* f(row of dy, row, whether it is this range's, which lanes' are) for them in their order: from the entries, from
+     * the list, or where it does not hold them from the ids again; loads ahead */
     auto each_hit = [&](auto f) {
-      if (found <= LIST) {
-        for (int e = 0; e < found; e += WAVE) {
-          const bool hit = e + lane < found;
-          f(hit ? list_pos[wid][e + lane] : 0, hit ? (int)list_row[wid][e + lane] : 0, hit, __ballot(hit));
+      if constexpr (PARTED) {
+        const Entry *in = w.entries + from;
+        Entry now = {0, 0}, next;
+        if (i0 < i1) now = in[min(i0 + lane, i1 - 1)];
+        for (int e = i0; e < i1; e += WAVE) {
+          next = in[min(e + WAVE + lane, i1 - 1)];
+          const bool hit = e + lane < i1;
+          f(now.pos, now.row, hit, __ballot(hit));
+          now = next;
         }
         return;
       }
-#pragma nounroll
-      for (int at = i0 + lane; at - lane < i1; at += WAVE) {
-        const uint32_t row = at < i1 ? (uint32_t)ids[(uint32_t)at * (uint32_t)step] - (uint32_t)v0 : rows;
-        const uint64_t hits = __ballot(row < rows);
-        if (hits) f(at, (int)row, row < rows, hits);
+      auto row_of = [&](int at) { return a.slot_rows ? at : at / a.n_ids; };
+      if (found <= LIST) {
+        for (int e = 0; e < found; e += WAVE) {
+          const bool hit = e + lane < found;
+          f(hit ? row_of(list_pos[wid][e + lane]) : 0, hit ? (int)list_row[wid][e + lane] : 0, hit, __ballot(hit));
+        }
+        return;
+      }
+      constexpr int UN = 4;
+      for (int i = i0; i < i1; i += UN * WAVE) {
+        uint32_t row[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+          const int at = i + u * WAVE + lane;
+          row[u] = at < i1 ? (uint32_t)ids[(uint32_t)at * (uint32_t)step] - (uint32_t)v0 : rows;
+        }
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+          const uint64_t hits = __ballot(row[u] < rows);
+          if (hits) f(row_of(i + u * WAVE + lane), (int)row[u], row[u] < rows, hits);
+        }
       }
     };
     each_hit([&](int, int row, bool hit, uint64_t) {
@@ -213,51 +370,46 @@ __global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, Gra
     const int incl = (int)wave_scan_add_u32((uint32_t)total);
     if (lane == WAVE - 1) wave_sum[wid] = incl, wave_less[wid] = less;
     __syncthreads();
-    int start = (int)(slot * p.n) + incl - total;
-    for (int g = 0; g < GW; g++) start += wave_less[g] + (g < wid ? wave_sum[g] : 0);
+    int start = (PARTED ? from : (int)(slot * p.n)) + incl - total;
+    for (int g = 0; g < GW; g++) start += (PARTED ? 0 : wave_less[g]) + (g < wid ? wave_sum[g] : 0);
     for (int r = r0; r < r1 && (uint32_t)r < rows; r++) {
-      const int from = start;
+      const int at = start;
       for (int g = 0; g < GW; g++) {
         const int c = cnt[g * p.range + r];
         cnt[g * p.range + r] = start;
         start += c;
       }
-      const int n = start - from;
+      const int here = start - at;
       const int64_t row = slot * a.slot_rows + v0 + r;
-      w.seg[row] = Seg{from, n > p.hot ? -n : n};
-      if (n > p.hot) {
-        const int chunks = (n + p.hot - 1) / p.hot;
+      w.seg[row] = Seg{at, here > p.hot ? -here : here};
+      if (here > p.hot) {
+        const int chunks = (here + p.hot - 1) / p.hot;
         const int hot = (int)atomicAdd(&w.counters[CNT_HOT], 1u), first = (int)atomicAdd(&w.counters[CNT_CHUNKS], (uint32_t)chunks);
         for (int c = 0; c < chunks; c++)
-          w.chunks[first + c] = Chunk{row, from + c * p.hot, min(p.hot, n - c * p.hot), first, chunks, hot, 0};
+          w.chunks[first + c] = Chunk{row, at + c * p.hot, min(p.hot, here - c * p.hot), first, chunks, hot, 0};
       }
     }
     __syncthreads();
     /* the positions: lanes of one row find each other by ballots of its bits */
-    auto place = [&](int at, int row, bool hit, uint64_t hits) {
-      uint64_t peers = hits;
-      for (int b = 0; b < bits; b++) {
-        const uint64_t m = __ballot(hit && (row >> b & 1));
-        peers &= row >> b & 1 ? m : ~m;
-      }
-      const int k = below(peers);
+    each_hit([&](int at, int row, bool hit, uint64_t hits) {
+      const uint64_t peers = peers_of(row, hit, hits, p.bits);
+      const int k = lanes_below(peers);
+      int to = 0;
       if (hit) {
-        const int to = mine[row] + k;
-        w.order[to] = a.slot_rows ? at : at / a.n_ids;
+        to = mine[row] + k;
+        w.order[to] = at;
       }
       wave_lds_sync();
-      if (hit && (peers >> lane) >> 1 == 0ull) mine[row] += k + 1; /* the last of them */
+      if (hit && (peers >> lane) >> 1 == 0ull) mine[row] = to + 1; /* the last of them */
       wave_lds_sync();
-    };
-    each_hit(place);
+    });
     __syncthreads();
   }
 }
 
 /* the sum of n rows of dy, at the positions `at`, E columns from j on */
-template <bool DB, int E>
+template <bool DB, int E, int UN>
 __device__ __forceinline__ void add_rows(const EmbedArgs &a, const int *at, int n, int64_t j, int64_t left, float *v) {
-  constexpr int UN = 4;
   int k = 0;
   auto row = [&](int i) { return (const char *)a.in + (int64_t)at[i] * a.in_stride * (DB ? 2 : 4); };
   for (; k + UN <= n; k += UN) {
@@ -299,24 +451,40 @@ __device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t
  * 144.  A strip of columns for each XCD, so that dy stays in its L2: 84 and more.  Rows without ids filled
  * by k_embed_group instead: 105 and 101.) */
 constexpr int SUM_ROWS = 4;
+/* (six and eight waves a SIMD: with the registers that the chunks would take, 88 and 84 us, so 78 and 76) */
 
 template <bool DB, bool GB>
-__global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
+__global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
                                                   int hot_groups) {
   constexpr int E = GB ? 8 : 4;
   const int tid = (int)threadIdx.x;
-  if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut */
+  const int across = tid % lanes, down = tid / lanes, at_once = ET / lanes;
+  if ((int)blockIdx.x < hot_groups) { /* chunks of rows that are cut, a strip of columns at a time */
     __shared__ uint32_t last;
+    __shared__ float part[ET * E];
     const int64_t stride = (a.width + 7) / 8 * 8;
-    const int chunks = (int)__hip_atomic_load(w.counters + CNT_CHUNKS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int c = (int)blockIdx.x; c < chunks; c += hot_groups) {
-      const Chunk k = w.chunks[c];
-      for (int64_t j = tid * E; j < a.width; j += ET * E) {
-        float v[E];
+    const int64_t chunks = (int64_t)__hip_atomic_load(w.counters + CNT_CHUNKS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int64_t c = blockIdx.x; c < chunks * strips; c += hot_groups) {
+      const Chunk k = w.chunks[c / strips];
+      const int64_t j = (c % strips * lanes + across) * E;
+      /* each group of lanes a run of the positions, then the groups in order */
+      const int run = (k.count + at_once - 1) / at_once, e0 = min(k.count, down * run), e1 = min(k.count, e0 + run);
+      float v[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = 0.0f;
-        add_rows<DB, E>(a, w.order + k.start, k.count, j, a.width - j, v);
-        uint64_t *out = (uint64_t *)(w.sums + c * stride + j);
+      for (int e = 0; e < E; e++) v[e] = 0.0f;
+      if (j < a.width) add_rows<DB, E, DB ? 8 : 4>(a, w.order + k.start + e0, e1 - e0, j, a.width - j, v);
+      if (at_once > 1) {
+#pragma unroll
+        for (int e = 0; e < E; e++) part[tid * E + e] = v[e];
+        __syncthreads();
+        if (down == 0) {
+          for (int g = 1; g < at_once; g++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] += part[(g * lanes + across) * E + e];
+        }
+      }
+      if (down == 0 && j < a.width) {
+        uint64_t *out = (uint64_t *)(w.sums + c / strips * stride + j);
 #pragma unroll
         for (int e = 0; e < E / 2; e++) st_agent(out + e, (uint64_t)d3s_f2u(v[2 * e]) | (uint64_t)d3s_f2u(v[2 * e + 1]) << 32);
       }
@@ -324,26 +492,26 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
       __syncthreads();
       if (tid == 0) {
         uint32_t *cnt = w.counters + HOT_COUNTERS + k.hot;
-        last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.chunks - 1);
+        last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(k.chunks * strips - 1);
         if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
       if (last)
-        for (int64_t j = tid * E; j < a.width; j += ET * E) {
-          float v[E];
+        for (int64_t i = tid * E; i < a.width; i += ET * E) {
+          float t[E];
 #pragma unroll
-          for (int e = 0; e < E; e++) v[e] = 0.0f;
-#pragma unroll 4
-          for (int i = 0; i < k.chunks; i++) {
-            const uint64_t *in = (const uint64_t *)(w.sums + (k.first + i) * stride + j);
+          for (int e = 0; e < E; e++) t[e] = 0.0f;
+#pragma unroll 8
+          for (int g = 0; g < k.chunks; g++) {
+            const uint64_t *in = (const uint64_t *)(w.sums + (k.first + g) * stride + i);
 #pragma unroll
             for (int e = 0; e < E / 2; e++) {
               const uint64_t q = ld_agent(in + e);
-              v[2 * e] += d3s_u2f((uint32_t)q);
-              v[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
+              t[2 * e] += d3s_u2f((uint32_t)q);
+              t[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
             }
           }
-          put_row<GB, E>(a, k.row, j, a.width - j, v);
+          put_row<GB, E>(a, k.row, i, a.width - i, t);
         }
       __syncthreads();
     }
@@ -354,7 +522,6 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
     }
     return;
   }
-  const int across = tid % lanes, down = tid / lanes, at_once = ET / lanes;
   for (int64_t blk = blockIdx.x - hot_groups; blk < blocks; blk += gridDim.x - hot_groups) {
     const int64_t row0 = blk / strips * (at_once * SUM_ROWS) + down;
     const int64_t j = (blk % strips * lanes + across) * E;
@@ -373,7 +540,7 @@ __global__ __launch_bounds__(ET) void k_embed_sum(EmbedArgs a, GradPlan p, GradR
       float v[E];
 #pragma unroll
       for (int e = 0; e < E; e++) v[e] = 0.0f;
-      add_rows<DB, E>(a, w.order + seg[i].start, seg[i].count, j, a.width - j, v);
+      add_rows<DB, E, 4>(a, w.order + seg[i].start, seg[i].count, j, a.width - j, v);
       put_row<GB, E>(a, row, j, a.width - j, v);
     }
   }
@@ -432,7 +599,15 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   }
   GradRoom w;
   grad_layout(p, a.width, (char *)ws, &w);
-  k_embed_group<<<grid(p.slots * p.ranges), GT, GW * p.range * sizeof(int), s>>>(a, p, w);
+  const size_t counts = GW * p.range * sizeof(int);
+  if (p.parted) {
+    k_part_count<<<dim3((unsigned)p.blocks), PT, 0, s>>>(a, p, w);
+    k_part_scan<<<1, PARTS, 0, s>>>(p, w);
+    k_part_move<<<dim3((unsigned)p.blocks), PT, 0, s>>>(a, p, w);
+    k_embed_group<true><<<grid(p.slots * p.ranges), GT, counts, s>>>(a, p, w);
+  } else {
+    k_embed_group<false><<<grid(p.slots * p.ranges), GT, counts, s>>>(a, p, w);
+  }
   int lanes = 1;
   while (lanes < ET && (int64_t)lanes * E < a.width) lanes *= 2;
   const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * SUM_ROWS;

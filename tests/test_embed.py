@@ -90,7 +90,10 @@ GRADS = [
     (2000, 1, 5000, 0, 16, "f32", "bf16", "zipf", 0, 0), (1500, 2, 100, 100, 24, "bf16", "f32", "same", 0, 0),
     (5000, 1, 30, 0, 8, "bf16", "bf16", "same", 0, 0), (9000, 1, 20011, 0, 33, "bf16", "f32", "zipf", 0, 0),
     (300, 1, 70000, 0, 9, "bf16", "f32", "even", 0, 0), (20000, 3, 513, 600, 8, "f32", "f32", "zipf", 0, 0),
-    (70000, 1, 300000, 0, 8, "bf16", "f32", "zipf", 0, 0), (64, 64, 33, 40, 56, "bf16", "bf16", "zipf", 0, 0)]
+    (70000, 1, 300000, 0, 8, "bf16", "f32", "zipf", 0, 0), (66000, 1, 50, 0, 12, "bf16", "f32", "zipf", 0, 0),
+    (7001, 10, 333, 350, 16, "f32", "bf16", "zipf", 1, 0), (70003, 1, 3, 0, 5, "bf16", "f32", "same", 0, 0),
+    (140001, 1, 1000000, 0, 4, "f32", "f32", "even", 0, 0), (33333, 3, 4097, 0, 40, "bf16", "f32", "zipf", 0, 0),
+    (1100, 64, 2000, 2048, 8, "bf16", "f32", "even", 0, 0), (3000, 1, 9, 0, 3000, "bf16", "bf16", "same", 0, 0), (64, 64, 33, 40, 56, "bf16", "bf16", "zipf", 0, 0)]
 
 
 @pytest.mark.parametrize("n,t,vocab,slot_rows,width,dtype,out,how,dy_pad,pad", GRADS)
