@@ -60,11 +60,12 @@ __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, int lanes, int64_t st
  * of as many, filed in a list; workgroups of their own sum the chunks in fp32, and the last
  * of a row to arrive adds its chunks in order.  No atomics on floating-point values. */
 
-constexpr int GT = 512; /* threads of k_embed_group */
-constexpr int GW = GT / WAVE;
+/* threads of k_embed_group: of parted ids more, for the range of the most frequent ones */
+template <bool PARTED>
+constexpr int group_threads() { return PARTED ? 1024 : 512; }
 constexpr int LIST = 512;         /* positions that a wave keeps in LDS (more: the ids are looked through again) */
 constexpr int AHEAD = 8;          /* ids that a lane looks at at a time */
-constexpr int RANGE_MOST = 1024;  /* rows of the table that a workgroup takes: 32 KiB of counts */
+constexpr int RANGE_MOST = 1024;  /* rows of the table that a workgroup takes: 32 or 64 KiB of counts */
 constexpr int HOT_GROUPS = 512;   /* workgroups for the chunks */
 constexpr int HOT_MOST = 4096;    /* rows that are cut, at most: a counter of arrivals each */
 constexpr int HOT_COUNTERS = 64;  /* words before them */
@@ -128,11 +129,11 @@ GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) 
   while ((1 << p.bits) < p.range) p.bits++;
   p.blocks = p.parted ? (int)((p.n * p.slots + PART_BLOCK - 1) / PART_BLOCK) : 0;
   p.ranges = count(p.range);
-  p.hot = 64;
+  p.hot = 32;
   while ((int64_t)p.hot * HOT_MOST < p.n * p.slots) p.hot *= 2;
   return p;
 }
-/* chunks at most: each full, but the last of a row that is cut */
+/* chunks at most: of 2 hot positions, or one for a row of more than hot */
 int64_t chunks_most(const GradPlan &p) { return 2 * (p.n * p.slots / p.hot) + 1; }
 
 size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
@@ -263,7 +264,8 @@ __global__ __launch_bounds__(PT) void k_part_move(EmbedArgs a, GradPlan p, GradR
 }
 
 template <bool PARTED>
-__global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
+__global__ __launch_bounds__(group_threads<PARTED>()) void k_embed_group(EmbedArgs a, GradPlan p, GradRoom w) {
+  constexpr int GT = group_threads<PARTED>(), GW = GT / WAVE;
   extern __shared__ int cnt[]; /* [GW][range]: a wave's count of a row, then its place */
   __shared__ int list_pos[GW][PARTED ? 1 : LIST];
   __shared__ uint16_t list_row[GW][PARTED ? 1 : LIST];
@@ -382,11 +384,11 @@ __global__ __launch_bounds__(GT) void k_embed_group(EmbedArgs a, GradPlan p, Gra
       const int here = start - at;
       const int64_t row = slot * a.slot_rows + v0 + r;
       w.seg[row] = Seg{at, here > p.hot ? -here : here};
-      if (here > p.hot) {
-        const int chunks = (here + p.hot - 1) / p.hot;
+      if (here > p.hot) { /* chunks of 2 hot positions, or 64 of them */
+        const int size = max(2 * p.hot, (here + 63) / 64), chunks = (here + size - 1) / size;
         const int hot = (int)atomicAdd(&w.counters[CNT_HOT], 1u), first = (int)atomicAdd(&w.counters[CNT_CHUNKS], (uint32_t)chunks);
         for (int c = 0; c < chunks; c++)
-          w.chunks[first + c] = Chunk{row, at + c * p.hot, min(p.hot, here - c * p.hot), first, chunks, hot, 0};
+          w.chunks[first + c] = Chunk{row, at + c * size, min(size, here - c * size), first, chunks, hot, 0};
       }
     }
     __syncthreads();
@@ -464,6 +466,18 @@ __global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradP
     __shared__ float part[ET * E];
     const int64_t stride = (a.width + 7) / 8 * 8;
     const int64_t chunks = (int64_t)__hip_atomic_load(w.counters + CNT_CHUNKS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    /* the groups' values added in their order, in the first */
+    auto add_groups = [&](float *v) {
+      if (at_once == 1) return;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; e++) part[tid * E + e] = v[e];
+      __syncthreads();
+      if (down != 0) return;
+      for (int g = 1; g < at_once; g++)
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] += part[(g * lanes + across) * E + e];
+    };
     for (int64_t c = blockIdx.x; c < chunks * strips; c += hot_groups) {
       const Chunk k = w.chunks[c / strips];
       const int64_t j = (c % strips * lanes + across) * E;
@@ -473,16 +487,7 @@ __global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradP
 #pragma unroll
       for (int e = 0; e < E; e++) v[e] = 0.0f;
       if (j < a.width) add_rows<DB, E, DB ? 8 : 4>(a, w.order + k.start + e0, e1 - e0, j, a.width - j, v);
-      if (at_once > 1) {
-#pragma unroll
-        for (int e = 0; e < E; e++) part[tid * E + e] = v[e];
-        __syncthreads();
-        if (down == 0) {
-          for (int g = 1; g < at_once; g++)
-#pragma unroll
-            for (int e = 0; e < E; e++) v[e] += part[(g * lanes + across) * E + e];
-        }
-      }
+      add_groups(v);
       if (down == 0 && j < a.width) {
         uint64_t *out = (uint64_t *)(w.sums + c / strips * stride + j);
 #pragma unroll
@@ -496,23 +501,29 @@ __global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradP
         if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
-      if (last)
-        for (int64_t i = tid * E; i < a.width; i += ET * E) {
-          float t[E];
+      if (last) {
+        /* the same for the chunks' sums */
+        const int each = (k.chunks + at_once - 1) / at_once, g0 = min(k.chunks, down * each), g1 = min(k.chunks, g0 + each);
+        for (int64_t t = 0; t < strips; t++) {
+          const int64_t i = (t * lanes + across) * E;
 #pragma unroll
-          for (int e = 0; e < E; e++) t[e] = 0.0f;
-#pragma unroll 8
-          for (int g = 0; g < k.chunks; g++) {
-            const uint64_t *in = (const uint64_t *)(w.sums + (k.first + g) * stride + i);
+          for (int e = 0; e < E; e++) v[e] = 0.0f;
+          if (i < a.width) {
+#pragma unroll 4
+            for (int g = g0; g < g1; g++) {
+              const uint64_t *in = (const uint64_t *)(w.sums + (k.first + g) * stride + i);
 #pragma unroll
-            for (int e = 0; e < E / 2; e++) {
-              const uint64_t q = ld_agent(in + e);
-              t[2 * e] += d3s_u2f((uint32_t)q);
-              t[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
+              for (int e = 0; e < E / 2; e++) {
+                const uint64_t q = ld_agent(in + e);
+                v[2 * e] += d3s_u2f((uint32_t)q);
+                v[2 * e + 1] += d3s_u2f((uint32_t)(q >> 32));
+              }
             }
           }
-          put_row<GB, E>(a, k.row, i, a.width - i, t);
+          add_groups(v);
+          if (down == 0 && i < a.width) put_row<GB, E>(a, k.row, i, a.width - i, v);
         }
+      }
       __syncthreads();
     }
     /* the last to end clears what k_embed_group counted */
@@ -599,14 +610,14 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   }
   GradRoom w;
   grad_layout(p, a.width, (char *)ws, &w);
-  const size_t counts = GW * p.range * sizeof(int);
+  auto counts = [&](int threads) { return threads / WAVE * p.range * sizeof(int); };
   if (p.parted) {
     k_part_count<<<dim3((unsigned)p.blocks), PT, 0, s>>>(a, p, w);
     k_part_scan<<<1, PARTS, 0, s>>>(p, w);
     k_part_move<<<dim3((unsigned)p.blocks), PT, 0, s>>>(a, p, w);
-    k_embed_group<true><<<grid(p.slots * p.ranges), GT, counts, s>>>(a, p, w);
+    k_embed_group<true><<<grid(p.slots * p.ranges), group_threads<true>(), counts(group_threads<true>()), s>>>(a, p, w);
   } else {
-    k_embed_group<false><<<grid(p.slots * p.ranges), GT, counts, s>>>(a, p, w);
+    k_embed_group<false><<<grid(p.slots * p.ranges), group_threads<false>(), counts(group_threads<false>()), s>>>(a, p, w);
   }
   int lanes = 1;
   while (lanes < ET && (int64_t)lanes * E < a.width) lanes *= 2;
