@@ -1,5 +1,13 @@
 /* k_dropout: y = residual + kept x / (1 - p), the mask drawn from Philox as it is
- * used (gfx950, wave64; include/d3s_step.h). */
+ * used (gfx950, wave64; include/d3s_step.h).
+ *
+ * An element is kept iff the upper 24 bits of its word are at least p 2^24: the same as u >= p, since
+ * u is those bits times 2^-24, without forming it.  1 / (1 - p) is rounded to fp32 once, the product and
+ * the sum once each.  A lane takes one or two whole blocks of the generator (20 multiplies of 32 x 32 bits
+ * each, about as long as its share of the memory traffic in bf16).
+ *
+ * Bound: HBM, the multiplies close behind.  bf16 8192 x 2048 with a residual 19 us (5.3 TB/s; a block
+ * for each element 35); fp32 without 22 us (6.0 TB/s). */
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
 

@@ -1,5 +1,12 @@
-/* k_embed, k_embed_grad: the rows that ids stand for, and their gradient in the
- * table (gfx950, wave64; include/d3s_step.h). */
+/* k_embed, k_embed_group, k_embed_sum: the rows that ids stand for, and their
+ * gradient in the table (gfx950, wave64; include/d3s_step.h).
+ *
+ * The lookup is bound by HBM, or by what the caches give where rows come again: 8192 tokens of 2048
+ * bf16 10.2 us; 4096 frames of ten codes 28 us (6.7 TB/s of the ten rows each); one frame 4.1 us, a launch
+ * and two dependent loads.
+ * The gradient is bound by the table's writes: 40970 x 2048 fp32 from 40960 codes 79 us (9 of them
+ * grouping), 151936 x 1024 bf16 from 16384 tokens 69 us (12 grouping); many ids of few rows by
+ * the chains of the frequent rows (200000 of 512 bf16 130 us). */
 #include "d3s_rowcore.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
