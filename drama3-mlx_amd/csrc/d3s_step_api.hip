@@ -10,6 +10,8 @@ namespace {
 
 /* rows by a stride stay inside 63 bits of bytes */
 constexpr int64_t STRIDE_MOST = (int64_t)1 << 40;
+/* ids of a gradient: their places, and those that lanes look ahead to, are counted in 32 bits */
+constexpr int64_t IDS_MOST = ((int64_t)1 << 31) - 65536;
 bool stride_ok(int64_t stride, int64_t width) { return stride >= width && stride <= STRIDE_MOST; }
 
 int check_verify(const d3s_verify_params *p) {
@@ -30,6 +32,10 @@ int verify_call(const d3s_verify_params *params, Room room, void *stream) {
   if (!p.target || off(p.target, size_of(p.target_dtype)) || (p.draft && off(p.draft, size_of(p.draft_dtype))))
     return D3S_ERR_ARG;
   if (!p.u_draw || !p.tokens || !p.n_accepted || (p.n_draft > 0 && (!p.drafted || !p.u_accept))) return D3S_ERR_ARG;
+  for (const void *q : {(const void *)p.drafted, (const void *)p.lengths, (const void *)p.temperature,
+                        (const void *)p.draft_temperature, (const void *)p.u_accept, (const void *)p.u_draw,
+                        (const void *)p.tokens, (const void *)p.n_accepted, (const void *)p.accept, (const void *)p.counters})
+    if (off(q, 4)) return D3S_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   void *ws = nullptr;
   if (const int rc = take_room(room, verify_workspace_bytes(p), s, &ws)) return rc;
@@ -37,10 +43,10 @@ int verify_call(const d3s_verify_params *params, Room room, void *stream) {
   return done();
 }
 
-/* the rows of the table that ids can name (0: the arguments are out of range) */
+/* the rows of the table, parts and what lies between them (0: the arguments are out of range) */
 int64_t table_rows(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, int64_t width) {
   if (n_rows < 0 || n_rows > INT_MOST || n_ids < 1 || n_ids > D3S_MAX_IDS || vocab < 1 || vocab > INT_MOST || width < 0 ||
-      width > INT_MOST || slot_rows < 0 || slot_rows > INT_MOST)
+      width > INT_MOST || slot_rows < 0 || slot_rows > INT_MOST || (slot_rows != 0 && slot_rows < vocab))
     return 0;
   return vocab + (n_ids - 1) * slot_rows;
 }
@@ -49,8 +55,7 @@ int embed_grad_check(const int32_t *ids, int64_t n_rows, int n_ids, const void *
                      int64_t vocab, int64_t slot_rows, int64_t width, float scale, void *grad, int grad_dtype,
                      int64_t grad_stride) {
   if (!known(dtype) || !known(grad_dtype)) return D3S_ERR_DTYPE;
-  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || (slot_rows != 0 && slot_rows < vocab) ||
-      n_rows > INT_MOST / n_ids || !stride_ok(dy_stride, width) || !stride_ok(grad_stride, width))
+  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || n_rows > IDS_MOST / n_ids || !stride_ok(dy_stride, width) || !stride_ok(grad_stride, width))
     return D3S_ERR_ARG;
   if (width == 0) return D3S_OK;
   if (!grad || off(grad, size_of(grad_dtype))) return D3S_ERR_ARG;
@@ -131,6 +136,11 @@ int d3s_verify_ranked(const int32_t *target_cand, const float *target_probs, int
   if (!target_cand || !target_probs || (drafts && (!draft_cand || !draft_probs)) || !u_draw || !tokens || !n_accepted ||
       (n_draft > 0 && (!drafted || !u_accept)))
     return D3S_ERR_ARG;
+  for (const void *q : {(const void *)target_cand, (const void *)target_probs, (const void *)draft_cand,
+                        (const void *)draft_probs, (const void *)drafted, (const void *)lengths, (const void *)u_accept,
+                        (const void *)u_draw, (const void *)tokens, (const void *)n_accepted, (const void *)accept,
+                        (const void *)counters})
+    if (off(q, 4)) return D3S_ERR_ARG;
   launch_verify_ranked({target_cand, target_probs, target_k, draft_cand, draft_probs, drafts ? draft_k : 0, (int)n_seqs,
                         n_draft, drafted, lengths, u_accept, u_draw, tokens, n_accepted, accept, counters},
                        (hipStream_t)stream);
@@ -160,9 +170,7 @@ int d3s_embed_backward(const int32_t *ids, int64_t n_rows, int n_ids, const void
 }
 
 int64_t d3s_embed_backward_workspace_bytes(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, int64_t width) {
-  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || (slot_rows != 0 && slot_rows < vocab) ||
-      n_rows > INT_MOST / n_ids)
-    return D3S_ERR_ARG;
+  if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || n_rows > IDS_MOST / n_ids) return D3S_ERR_ARG;
   return (int64_t)embed_grad_workspace_bytes(n_rows, n_ids, vocab, slot_rows, width);
 }
 

@@ -203,7 +203,7 @@ struct Weights {
   const char *tp, *dp; /* the rows (dp null: none, or a certain draft) */
   int V, gone;         /* the certain draft's token, or -1 */
   double mp, mq, cp, cq;       /* greatest logits, log2(e) / T */
-  double ip, iq, whole;        /* what the terms are multiplied by, and what p's then sum to */
+  double ip, iq;               /* what the terms are multiplied by */
 
   /* sp, sq: what the sequence's rows hold */
   __device__ __forceinline__ Weights(const d3s_verify_params &a, const Seq &s, int accepted, bool rejected, float m_p, float m_q, int x) {
@@ -213,7 +213,7 @@ struct Weights {
     gone = rejected && !a.draft ? __builtin_amdgcn_readlane(x, accepted & (WAVE - 1)) : -1;
     mp = m_p, mq = m_q;
     cp = LOG2E_64 / s.T, cq = LOG2E_64 / s.Td;
-    ip = iq = whole = 1.0;
+    ip = iq = 1.0;
   }
   __device__ __forceinline__ int left(int j) const { return min(8, V - j); }
   /* eight terms of each sum from j on (0 past the end), j < V */
@@ -246,8 +246,8 @@ struct Weights {
       if (plain) continue;
       if (dp)
         r[e] = fmax(r[e] - q[e] * iq, 0.0);
-      else if (j + e == gone)
-        r[e] = fmax(r[e] - whole, 0.0);
+      else if (j + e == gone) /* (p <= 1) */
+        r[e] = 0.0;
     }
   }
 };
@@ -426,7 +426,6 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a, int b0) 
     for (int w = 0; w < VT / WAVE; w++) sp += pair[w][0], sq += pair[w][1];
     W.iq = sq > 0.0 ? sp / sq : 0.0;
     W.ip = 1.0;
-    W.whole = sp;
     bool plain = !o.rejected;
     double r[8], Z;
     for (;;) {

@@ -106,8 +106,8 @@ int d3s_verify_ranked(const int32_t *target_cand, const float *target_probs, int
 /* The rows that ids stand for: y[r] = scale * sum_t table[t slot_rows + ids[r, t]],
  * summed in fp32 in the order of t, rounded once.
  * ids [n_rows, n_ids], n_ids 1 .. D3S_MAX_IDS; an id outside [0, vocab) is none
- * and adds nothing.  slot_rows 0: one table of vocab rows for all; vocab (or
- * more): the t-th id has a part of the table of its own.  table [.., width] and
+ * and adds nothing.  slot_rows 0: one table of vocab rows for all; vocab or
+ * more (less is D3S_ERR_ARG): the t-th id has a part of the table of its own.  table [.., width] and
  * y [n_rows, width] fp32 or bf16 each. */
 int d3s_embed(const int32_t *ids, int64_t n_rows, int n_ids, const void *table, int dtype, int64_t table_stride,
               int64_t vocab, int64_t slot_rows, int64_t width, float scale, void *y, int y_dtype, int64_t y_stride,
@@ -118,7 +118,7 @@ int d3s_embed(const int32_t *ids, int64_t n_rows, int n_ids, const void *table, 
  * accumulate not 0, added to what is there before the rounding, else rows that no id
  * names are zeros (those between two slots' parts too).  dy [n_rows, width], grad
  * [vocab (+ (n_ids - 1) slot_rows), width]; fp32 or bf16 each.  slot_rows is 0
- * or at least vocab; n_rows * n_ids is below 2^31. */
+ * or at least vocab; n_rows * n_ids at most 2^31 - 65536. */
 int d3s_embed_backward(const int32_t *ids, int64_t n_rows, int n_ids, const void *dy, int dtype, int64_t dy_stride,
                        int64_t vocab, int64_t slot_rows, int64_t width, float scale, int accumulate, void *grad,
                        int grad_dtype, int64_t grad_stride, void *stream);

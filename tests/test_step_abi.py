@@ -161,3 +161,32 @@ DROP = dict(x=P, dtype=1, x_stride=64, residual=Q, residual_stride=64, n_rows=5,
     (dict(width=0), 0)])
 def test_dropout(d3s, change, status):
     assert d3s.dropout_raw(**{**DROP, **change}) == status
+
+
+@pytest.mark.parametrize("slot_rows,status", [(0, 0), (9, -1), (10, 0), (25, 0)])
+def test_parts_overlap_nowhere(d3s, slot_rows, status):
+    """the lookup and its gradient take the same parts of a table (n_rows 0: nothing is launched)"""
+    assert d3s.embed_raw(**{**EMBED, "n_rows": 0, "slot_rows": slot_rows}) == status
+    need = d3s.lib().d3s_embed_backward_workspace_bytes(5, 2, 10, slot_rows, 64)
+    assert need == -1 if status else need > 0
+
+
+@pytest.mark.parametrize("n_rows,n_ids,fits", [((1 << 31) - 65536, 1, True), ((1 << 31) - 65535, 1, False),
+                                               ((1 << 25) - 1024, 64, True), ((1 << 25) - 1023, 64, False)])
+def test_ids_of_a_gradient(d3s, n_rows, n_ids, fits):
+    need = d3s.lib().d3s_embed_backward_workspace_bytes(n_rows, n_ids, 10, 0, 8)
+    assert need > 4 * n_rows * n_ids if fits else need == -1
+    if not fits:
+        assert d3s.embed_backward_raw(**{**GRAD, "n_rows": n_rows, "n_ids": n_ids, "slot_rows": 0}) == -1
+
+
+@pytest.mark.parametrize("name", ["drafted", "lengths", "u_accept", "u_draw", "tokens", "n_accepted", "accept", "counters"])
+def test_verification_between_words(d3s, name):
+    """arrays of 32-bit words that begin between two"""
+    assert d3s.verify_raw(**{**VERIFY, name: P + 2}) == -1
+    assert d3s.verify_ranked_raw(**{**RANKED, name: P + 2}) == -1
+
+
+@pytest.mark.parametrize("name", ["target_cand", "target_probs", "draft_cand", "draft_probs"])
+def test_candidates_between_words(d3s, name):
+    assert d3s.verify_ranked_raw(**{**RANKED, name: P + 2}) == -1
