@@ -16,34 +16,20 @@ namespace {
 
 constexpr int DT_ = 256;
 
-/* a workgroup takes DT_ / lanes rows by E * lanes columns */
-struct DropSplit {
-  int lanes;
-  int64_t strips, blocks;
-};
-
-DropSplit drop_split(int64_t rows, int64_t places, int E) {
-  DropSplit s;
-  s.lanes = 1;
-  while (s.lanes < DT_ && (int64_t)s.lanes * E < places) s.lanes *= 2;
-  s.strips = (places + s.lanes * E - 1) / (s.lanes * E);
-  s.blocks = s.strips * ((rows + DT_ / s.lanes - 1) / (DT_ / s.lanes));
-  return s;
-}
-
 /* A lane's E elements begin at a multiple of four in the generator's count, so that its words are
  * whole blocks of Philox: in a row that does not (EVEN: none), the first lane's begin up to three
  * places before it.  (With lanes that begin with the row, a block more each and its words
- * picked: 8192 x 2049 bf16 at a stride of 2052 48 us, so 36.) */
+ * picked, 8192 x 2049 bf16 with a residual at a stride of 2052 takes a third more.)  Rows' chunks are counted
+ * through: these 22 us, a power of two of lanes for each row 36. */
 template <bool BF16, bool EVEN>
-__global__ __launch_bounds__(DT_) void k_dropout(DropoutArgs a, DropSplit sp) {
+__global__ __launch_bounds__(DT_) void k_dropout(DropoutArgs a, Spread c) {
   constexpr int E = BF16 ? 8 : 4, ES = BF16 ? 2 : 4;
-  const int across = (int)threadIdx.x % sp.lanes, down = (int)threadIdx.x / sp.lanes;
   const uint64_t draw = a.draw + (a.draw_add ? *a.draw_add : 0u);
-  for (int64_t blk = blockIdx.x; blk < sp.blocks; blk += gridDim.x) {
-    const int64_t row = blk / sp.strips * (DT_ / sp.lanes) + down;
+  for (int64_t blk = blockIdx.x; blk < c.blocks; blk += gridDim.x) {
+    int64_t row, chunk;
+    c.find<DT_>(blk, &row, &chunk);
     const uint64_t first = (uint64_t)row * (uint64_t)a.width;
-    const int64_t j = (blk % sp.strips * sp.lanes + across) * E - (EVEN ? 0 : (int64_t)(first & 3u)), left = a.width - j;
+    const int64_t j = chunk * E - (EVEN ? 0 : (int64_t)(first & 3u)), left = a.width - j;
     if (row >= a.n_rows || left <= 0) continue;
     const char *x = (const char *)a.x + row * a.x_stride * ES, *res = (const char *)a.residual + row * a.residual_stride * ES;
     char *y = (char *)a.y + row * a.y_stride * ES;
@@ -94,9 +80,9 @@ void launch_dropout(const DropoutArgs &args, Dtype dt, hipStream_t s) {
     a.n_rows = 1;
   }
   const bool even = a.n_rows == 1 || a.width % 4 == 0;
-  const DropSplit sp = drop_split(a.n_rows, a.width + (even ? 0 : 3), dt == DT_BF16 ? 8 : 4);
-  const dim3 grid((unsigned)(sp.blocks < STEP_GRID ? sp.blocks : STEP_GRID));
-  auto go = [&](auto kernel) { kernel<<<grid, DT_, 0, s>>>(a, sp); };
+  const Spread c = Spread::of<DT_>(a.n_rows, a.width + (even ? 0 : 3), dt == DT_BF16 ? 8 : 4);
+  const dim3 grid((unsigned)(c.blocks < STEP_GRID ? c.blocks : STEP_GRID));
+  auto go = [&](auto kernel) { kernel<<<grid, DT_, 0, s>>>(a, c); };
   if (dt == DT_BF16)
     even ? go(k_dropout<true, true>) : go(k_dropout<true, false>);
   else

@@ -101,6 +101,38 @@ __device__ __forceinline__ void store_row(void *row, int64_t j, int64_t left, co
   }
 }
 
+/* Rows of chunks, the chunks of all rows counted through, so that no lane is idle behind a row's
+ * end.  A thread finds its row from its workgroup's first chunk: one division for the workgroup, and
+ * a comparison (or, in short rows, a product by `over`, 2^20 / chunks rounded up: exact below
+ * 512) for the thread. */
+struct Spread {
+  int64_t chunks; /* of a row */
+  uint32_t over;
+  int64_t blocks; /* of T threads */
+
+  template <int T>
+  static Spread of(int64_t rows, int64_t width, int elements) {
+    static_assert(T <= 256, "");
+    Spread c;
+    c.chunks = (width + elements - 1) / elements;
+    c.over = c.chunks < T ? (uint32_t)(((1 << 20) + c.chunks - 1) / c.chunks) : 0u;
+    c.blocks = (rows * c.chunks + T - 1) / T;
+    return c;
+  }
+  template <int T>
+  __device__ __forceinline__ void find(int64_t blk, int64_t *row, int64_t *chunk) const {
+    const int64_t first = blk * T, r0 = first / chunks, c0 = first - r0 * chunks;
+    if (chunks < T) { /* c0 + threadIdx.x < 2 T */
+      const uint32_t t = (uint32_t)c0 + threadIdx.x, r = t * over >> 20;
+      *row = r0 + r, *chunk = t - r * (uint32_t)chunks;
+    } else {
+      const int64_t t = c0 + threadIdx.x;
+      const bool next = t >= chunks;
+      *row = r0 + next, *chunk = next ? t - chunks : t;
+    }
+  }
+};
+
 }  // namespace
 }  // namespace d3s
 
