@@ -6,7 +6,7 @@
  * and two dependent loads.
  * The gradient is bound by the table's writes: 40970 x 2048 fp32 from 40960 codes 79 us (9 of them
  * grouping), 151936 x 1024 bf16 from 16384 tokens 69 us (12 grouping); many ids of few rows by
- * the chains of the frequent rows (200000 of 512 bf16 130 us). */
+ * the chains of the frequent rows and their range's grouping (200000 of 512 bf16 119 us). */
 #include "d3s_rowcore.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(ET) void k_embed(EmbedArgs a, Spread c) {
  * k_part_scan, k_part_move: counts for each block of ids, their sums, the ids' places).
  * k_embed_sum: a row's positions are summed in that order, by lanes across its columns;
  * rows that no id names are filled with zeros.  A row of more than `hot` positions is cut into chunks
- * of as many, filed in a list; workgroups of their own sum the chunks in fp32, and the last
+ * of twice as many or more, filed in a list; workgroups of their own sum the chunks in fp32, and the last
  * of a row to arrive adds its chunks in order.  No atomics on floating-point values. */
 
 /* threads of k_embed_group: of parted ids more, for the range of the most frequent ones */
@@ -75,17 +75,25 @@ constexpr int group_threads() { return PARTED ? 1024 : 512; }
 constexpr int LIST = 512;         /* positions that a wave keeps in LDS (more: the ids are looked through again) */
 constexpr int AHEAD = 8;          /* ids that a lane looks at at a time */
 constexpr int RANGE_MOST = 1024;  /* rows of the table that a workgroup takes: 32 or 64 KiB of counts */
-constexpr int HOT_GROUPS = 512;   /* workgroups for the chunks */
-constexpr int HOT_MOST = 4096;    /* rows that are cut, at most: a counter of arrivals each */
+constexpr int RANGE_LEAST = 4;    /* ... and at least, of parted ids (400000 ids of 300 rows: 222 us; 16 rows 298) */
+/* workgroups for the chunks; of parted ids more (100000 ids of 1000 rows, 2048 columns: 146 us, with 512 320), since
+ * they are not counted as they end, 23 ns each */
+constexpr int HOT_GROUPS = 512;
+constexpr int HOT_GROUPS_PARTED = 2048;
+/* rows that are cut, at most: a counter of arrivals each (300000 ids of 5000 rows, 64 columns: 126 us; with 4096,
+ * which leave rows of 128 ids whole, 226) */
+constexpr int HOT_MOST = 32768;
 constexpr int HOT_COUNTERS = 64;  /* words before them */
-
 
 constexpr int PT = 1024;          /* threads of the parting kernels */
 constexpr int PW = PT / WAVE;
 constexpr int PART_IDS = 8;       /* ids a thread */
 constexpr int PART_BLOCK = PT * PART_IDS;
 constexpr int PARTS = 1024;       /* ranges that ids are parted into, at most */
-constexpr int PART_LEAST = 65536; /* fewer ids are not parted (16384: 76 us, so 96) */
+/* fewer ids are not parted (40960 ids of 40970 rows: 79 us, parted 98; 20000 of 5000 32 and 42), but half as
+ * many are where there are four or more a row, some of them perhaps most of all (50000 of 5000 rows, as often as
+ * words in text: 43 us, not parted 116; evenly 38 and 34) */
+constexpr int PART_LEAST = 65536;
 
 struct Seg {
   int start, count; /* count < 0: cut into chunks */
@@ -97,7 +105,8 @@ struct Chunk {
   int64_t row;
   int start, count, first, chunks, hot, pad; /* first: the row's first chunk */
 };
-/* the counters that the calls leave at zero: chunks, rows cut, arrivals */
+/* chunks, rows cut, workgroups that have ended, and then the rows' arrivals: among the counters that the calls
+ * leave at zero; of parted ids, whose first kernel clears them, behind those (no count of workgroups then) */
 enum { CNT_CHUNKS = 0, CNT_HOT = 16, CNT_DONE = 32 };
 
 struct GradPlan {
@@ -131,9 +140,10 @@ GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) 
   auto count = [&](int64_t r) { return (vocab + r - 1) / r; };
   while (p.range < RANGE_MOST && p.slots * count(p.range) > 512 && p.slots * count(p.range) * p.n > (int64_t)32 << 20) p.range *= 2;
   /* (ids that do not fit the parts' number are looked through) */
-  p.parted = p.n * p.slots >= PART_LEAST && p.slots * count(RANGE_MOST) <= PARTS;
+  const int64_t ids = p.n * p.slots;
+  p.parted = (ids >= PART_LEAST || (ids >= PART_LEAST / 2 && ids >= 4 * p.rows)) && p.slots * count(RANGE_MOST) <= PARTS;
   if (p.parted)
-    for (p.range = 64; p.slots * count(p.range) > PARTS;) p.range *= 2;
+    for (p.range = RANGE_LEAST; p.slots * count(p.range) > PARTS;) p.range *= 2;
   p.bits = 0;
   while ((1 << p.bits) < p.range) p.bits++;
   p.blocks = p.parted ? (int)((p.n * p.slots + PART_BLOCK - 1) / PART_BLOCK) : 0;
@@ -159,6 +169,7 @@ size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
   w->sums = (float *)take((size_t)chunks_most(p) * (size_t)((width + 7) / 8 * 8) * sizeof(float));
   w->table = (int *)take((size_t)p.blocks * PARTS * sizeof(int));
   w->begin = (int *)take(p.parted ? (PARTS + 1) * sizeof(int) : 0);
+  if (p.parted) w->counters = (uint32_t *)take((HOT_COUNTERS + HOT_MOST) * sizeof(uint32_t));
   w->entries = (Entry *)take(p.parted ? (size_t)(p.n * p.slots) * sizeof(Entry) : 0);
   return at;
 }
@@ -173,6 +184,7 @@ __global__ __launch_bounds__(PT) void k_part_count(EmbedArgs a, GradPlan p, Grad
   __shared__ int hist[PARTS];
   const int tid = (int)threadIdx.x, n = (int)(p.n * p.slots);
   if (tid < PARTS) hist[tid] = 0;
+  for (int i = (int)blockIdx.x * PT + tid; i < HOT_COUNTERS + HOT_MOST; i += (int)gridDim.x * PT) w.counters[i] = 0u;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * PART_BLOCK;
   for (int u = 0; u < PART_IDS; u++) {
@@ -336,13 +348,23 @@ __global__ __launch_bounds__(group_threads<PARTED>()) void k_embed_group(EmbedAr
     auto each_hit = [&](auto f) {
       if constexpr (PARTED) {
         const Entry *in = w.entries + from;
-        Entry now = {0, 0}, next;
-        if (i0 < i1) now = in[min(i0 + lane, i1 - 1)];
-        for (int e = i0; e < i1; e += WAVE) {
-          next = in[min(e + WAVE + lane, i1 - 1)];
-          const bool hit = e + lane < i1;
-          f(now.pos, now.row, hit, __ballot(hit));
-          now = next;
+        constexpr int UN = 4;
+        Entry now[UN], next[UN];
+        auto get = [&](int e, Entry *q) {
+#pragma unroll
+          for (int u = 0; u < UN; u++) q[u] = in[min(e + u * WAVE + lane, i1 - 1)];
+        };
+        if (i0 < i1) get(i0, now);
+        for (int e = i0; e < i1; e += UN * WAVE) {
+          if (e + UN * WAVE < i1) get(e + UN * WAVE, next);
+#pragma unroll
+          for (int u = 0; u < UN; u++) {
+            const bool hit = e + u * WAVE + lane < i1;
+            const uint64_t hits = __ballot(hit);
+            if (hits) f(now[u].pos, now[u].row, hit, hits);
+          }
+#pragma unroll
+          for (int u = 0; u < UN; u++) now[u] = next[u];
         }
         return;
       }
@@ -369,8 +391,13 @@ __global__ __launch_bounds__(group_threads<PARTED>()) void k_embed_group(EmbedAr
         }
       }
     };
-    each_hit([&](int, int row, bool hit, uint64_t) {
-      if (hit) atomicAdd(&mine[row], 1);
+    each_hit([&](int, int row, bool hit, uint64_t hits) {
+      if constexpr (PARTED) { /* (a frequent row's lanes would all add to one place) */
+        const uint64_t peers = peers_of(row, hit, hits, p.bits);
+        if (hit && lanes_below(peers) == 0) atomicAdd(&mine[row], __popcll(peers));
+      } else if (hit) {
+        atomicAdd(&mine[row], 1);
+      }
     });
     __syncthreads();
     /* the rows' places: a thread `per` rows in a row */
@@ -457,14 +484,17 @@ __device__ __forceinline__ void put_row(const EmbedArgs &a, int64_t row, int64_t
   store_row<GB, E>(out, j, left, v);
 }
 
-/* Rows that a thread takes one after the other: a workgroup writes 16 KiB.  (40970 rows of 2048 fp32, the whole
+/* SUM_ROWS rows that a thread takes one after the other: a workgroup writes 16 KiB.  (40970 rows of 2048 fp32, the whole
  * gradient: 82 us; two rows 88, one 104.  151936 of 1024 bf16: 79; two rows 81, eight 80.  Through the caches 100 and
  * 144.  A strip of columns for each XCD, so that dy stays in its L2: 84 and more.  Rows without ids filled
  * by k_embed_group instead: 105 and 101.) */
-constexpr int SUM_ROWS = 4;
+constexpr int FEW_IDS = 4;
+/* One row where there are two ids or more a row (300000 ids of 5000 rows: 90 us, four rows 126; of
+ * fewer, 200000 for 151936, 165 and 150). */
+constexpr int MANY_IDS = 1;
 /* (six and eight waves a SIMD: with the registers that the chunks would take, 88 and 84 us, so 78 and 76) */
 
-template <bool DB, bool GB>
+template <bool DB, bool GB, int SUM_ROWS>
 __global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradPlan p, GradRoom w, int lanes, int64_t strips, int64_t blocks,
                                                   int hot_groups) {
   constexpr int E = GB ? 8 : 4;
@@ -536,7 +566,7 @@ __global__ __launch_bounds__(ET, GB ? 6 : 8) void k_embed_sum(EmbedArgs a, GradP
       __syncthreads();
     }
     /* the last to end clears what k_embed_group counted */
-    if (tid == 0 && __hip_atomic_fetch_add(w.counters + CNT_DONE, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(hot_groups - 1)) {
+    if (!p.parted && tid == 0 && __hip_atomic_fetch_add(w.counters + CNT_DONE, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(hot_groups - 1)) {
       for (int c : {CNT_CHUNKS, CNT_HOT, CNT_DONE})
         __hip_atomic_store(w.counters + c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -626,17 +656,22 @@ void launch_embed_grad(const EmbedArgs &args, Dtype in, Dtype out, void *ws, hip
   }
   int lanes = 1;
   while (lanes < ET && (int64_t)lanes * E < a.width) lanes *= 2;
-  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * SUM_ROWS;
+  const int together = p.n * p.slots >= 2 * p.rows ? MANY_IDS : FEW_IDS;
+  const int64_t strips = (a.width + lanes * E - 1) / (lanes * E), rows = ET / lanes * together;
   const int64_t blocks = strips * ((p.rows + rows - 1) / rows);
   const int64_t most = chunks_most(p);
-  const int hot_groups = (int)(most < HOT_GROUPS ? most : HOT_GROUPS);
+  const int at_most = p.parted ? HOT_GROUPS_PARTED : HOT_GROUPS, hot_groups = (int)(most < at_most ? most : at_most);
   auto go = [&](auto kernel) {
     kernel<<<dim3((unsigned)(hot_groups + (blocks < STEP_GRID ? blocks : STEP_GRID))), ET, 0, s>>>(a, p, w, lanes, strips, blocks, hot_groups);
   };
+  auto typed = [&](auto db, auto gb) {
+    constexpr bool D = decltype(db)::value, G = decltype(gb)::value;
+    together == MANY_IDS ? go(k_embed_sum<D, G, MANY_IDS>) : go(k_embed_sum<D, G, FEW_IDS>);
+  };
   if (in == DT_BF16)
-    out == DT_BF16 ? go(k_embed_sum<true, true>) : go(k_embed_sum<true, false>);
+    out == DT_BF16 ? typed(std::true_type{}, std::true_type{}) : typed(std::true_type{}, std::false_type{});
   else
-    out == DT_BF16 ? go(k_embed_sum<false, true>) : go(k_embed_sum<false, false>);
+    out == DT_BF16 ? typed(std::false_type{}, std::true_type{}) : typed(std::false_type{}, std::false_type{});
 }
 
 }  // namespace d3s

@@ -93,6 +93,9 @@ GRADS = [
     (70000, 1, 300000, 0, 8, "bf16", "f32", "zipf", 0, 0), (66000, 1, 50, 0, 12, "bf16", "f32", "zipf", 0, 0),
     (7001, 10, 333, 350, 16, "f32", "bf16", "zipf", 1, 0), (70003, 1, 3, 0, 5, "bf16", "f32", "same", 0, 0),
     (140001, 1, 1000000, 0, 4, "f32", "f32", "even", 0, 0), (33333, 3, 4097, 0, 40, "bf16", "f32", "zipf", 0, 0),
+    (300000, 1, 8000, 0, 8, "bf16", "f32", "even", 0, 0), (40000, 1, 1000, 0, 17, "bf16", "bf16", "zipf", 0, 3),
+    (16384, 2, 4096, 0, 12, "f32", "bf16", "zipf", 1, 0), (16383, 2, 4096, 0, 12, "f32", "f32", "zipf", 0, 0),
+    (100000, 1, 1000, 0, 264, "bf16", "f32", "even", 0, 0),
     (1100, 64, 2000, 2048, 8, "bf16", "f32", "even", 0, 0), (3000, 1, 9, 0, 3000, "bf16", "bf16", "same", 0, 0), (64, 64, 33, 40, 56, "bf16", "bf16", "zipf", 0, 0)]
 
 
