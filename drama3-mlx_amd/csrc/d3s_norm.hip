@@ -2,7 +2,7 @@
  * output in 8 bits, and its gradient (gfx950, wave64; include/d3s_step.h).
  *
  * A row's inputs are read once, all in flight together, and stay in registers: up to 512
- * columns a part of a wave a row, up to 2048 a wave, up to 16384 a workgroup; longer rows are read once
+ * columns a part of a wave a row, up to 2048 a wave, up to 16384 a workgroup of 256 to 1024 threads; longer rows are read once
  * for each pass (k_norm_rows, k_norm_grad_rows, k_norm_dgain).  Squares are summed in fp32,
  * a lane's in order and then by a tree.  h stays in fp32 from the addition to y; rstd is
  * a correctly rounded root and quotient.  8 bits: a group's greatest |y| by exchanges among the lanes
@@ -94,6 +94,9 @@ __device__ __forceinline__ float row_max(float v, float *part) {
   return v;
 }
 
+/* threads of a workgroup whose rows are held by G each */
+constexpr int row_threads(int G) { return G > NT ? G : NT; }
+
 /* G threads hold a row, U chunks of eight elements each, in registers: one read of
  * everything, all of it in flight together. */
 /* elements that follow each other in a lane: as many as make a store of 16 bytes; eight for 8 bits */
@@ -101,9 +104,9 @@ template <bool BF16, int OUT>
 constexpr int norm_elements() { return OUT != D3S_DTYPE_E4M3 && (!BF16 || OUT == D3S_DTYPE_F32) ? 4 : 8; }
 
 template <bool BF16, int OUT, int G, int U>
-__global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
-  constexpr int ES = BF16 ? 2 : 4, ROWS = NT / G, E = norm_elements<BF16, OUT>();
-  __shared__ float part[NW];
+__global__ __launch_bounds__(row_threads(G)) void k_norm(NormArgs a) {
+  constexpr int ES = BF16 ? 2 : 4, ROWS = row_threads(G) / G, E = norm_elements<BF16, OUT>();
+  __shared__ float part[row_threads(G) / WAVE];
   const int g = (int)threadIdx.x % G;
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.n_rows; row0 += (int64_t)gridDim.x * ROWS) {
     const int64_t row = min(row0 + threadIdx.x / G, a.n_rows - 1);
@@ -203,9 +206,9 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs a) {
 /* The gradient, rows held the same way; a workgroup takes every gridDim.x-th set of
  * rows and keeps their columns' sums of dy xhat in registers. */
 template <bool BF16, int G, int U, bool SUM>
-__global__ __launch_bounds__(G > NT ? G : NT) void k_norm_grad(NormGradArgs a, float *parts) {
-  constexpr int ES = BF16 ? 2 : 4, ROWS = G > NT ? 1 : NT / G, E = BF16 ? 8 : 4;
-  __shared__ float part[G > NT ? G / WAVE : NW];
+__global__ __launch_bounds__(row_threads(G)) void k_norm_grad(NormGradArgs a, float *parts) {
+  constexpr int ES = BF16 ? 2 : 4, ROWS = row_threads(G) / G, E = BF16 ? 8 : 4;
+  __shared__ float part[row_threads(G) / WAVE];
   __shared__ float sums[SUM && ROWS > 1 ? NT * U * E : 1];
   const int g = (int)threadIdx.x % G, width = (int)a.width;
   Vec<BF16, E> w[U];
@@ -438,23 +441,30 @@ __global__ __launch_bounds__(NT) void k_norm_dgain(NormGradArgs a, int64_t strip
   parts[run * a.width + j] = s;
 }
 
-/* the threads and chunks of E elements that hold a row: f(G, U), or false for one that is streamed */
-template <int E, class F>
-bool in_registers(int64_t width, F f) {
+/* f(T) for a workgroup of T threads, as few as hold `chunks` of a row, or false */
+template <int... T, class F>
+bool of_threads(int64_t chunks, F f) {
+  return ((chunks <= T && (f(std::integral_constant<int, T>{}), true)) || ...);
+}
+
+/* The threads and chunks of E elements that hold a row: f(G, U), or false for one that is streamed.
+ * Beyond 2048 columns a workgroup of about as many threads as have eight elements each, or 16 (bf16 6553 x 2560
+ * 21 us, fp32 1524 x 11008 56; 256 threads that hold up to 64, 23.5 and 111); of 8 bits, whose groups' lanes wait for
+ * each other, 16 where they can (4096 x 4096 23 us, 8 elements 26.6). */
+template <int E, bool U1, class F>
+bool in_registers(int64_t width, F f) { /* (U1: eight may do) */
   constexpr int M = 8 / E;
-  auto c = [](auto v) { return v; };
-#define D3S_ROW(G, U) return f(c(std::integral_constant<int, G>{}), c(std::integral_constant<int, U * M>{})), true
-  if (width <= 64) D3S_ROW(8, 1);
-  if (width <= 128) D3S_ROW(16, 1);
-  if (width <= 256) D3S_ROW(32, 1);
-  if (width <= 512) D3S_ROW(64, 1);
-  if (width <= 1024) D3S_ROW(64, 2);
-  if (width <= 2048) D3S_ROW(64, 4);
-  if (width <= 4096) D3S_ROW(256, 2);
-  if (width <= 8192) D3S_ROW(256, 4);
-  if (width <= 16384) D3S_ROW(256, 8);
-#undef D3S_ROW
-  return false;
+  using std::integral_constant;
+  auto go = [&](auto g, auto u) { return f(g, u), true; };
+  if (width <= 64) return go(integral_constant<int, 8>{}, integral_constant<int, M>{});
+  if (width <= 128) return go(integral_constant<int, 16>{}, integral_constant<int, M>{});
+  if (width <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, M>{});
+  if (width <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, M>{});
+  if (width <= 1024) return go(integral_constant<int, 64>{}, integral_constant<int, 2 * M>{});
+  if (width <= 2048) return go(integral_constant<int, 64>{}, integral_constant<int, 4 * M>{});
+  const int64_t chunks = (width + 7) / 8;
+  return (U1 && of_threads<320, 384, 512, 640, 768, 1024>(chunks, [&](auto t) { go(t, integral_constant<int, M>{}); })) ||
+         of_threads<256, 320, 384, 512, 640, 768, 1024>((chunks + 1) / 2, [&](auto t) { go(t, integral_constant<int, 2 * M>{}); });
 }
 
 /* The same for the gradient, whose inputs are three rows and whose sums stay: beyond 1024 columns a
@@ -466,12 +476,10 @@ bool grad_in_registers(int64_t width, F f) {
   constexpr int M = 8 / E;
   auto go = [&](auto g, auto u) { return f(g, u), true; };
   using std::integral_constant;
-  if (width <= 1024) return in_registers<E>(width, f);
-  if (width <= 2048) return go(integral_constant<int, 256>{}, integral_constant<int, M>{});
-  if (width <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, M>{});
-  if (width <= 8192) return go(integral_constant<int, 1024>{}, integral_constant<int, M>{});
-  if (width <= 16384) return go(integral_constant<int, 512>{}, integral_constant<int, 4 * M>{});
-  return false;
+  if (width <= 1024) return in_registers<E, false>(width, f);
+  const int64_t chunks = (width + 7) / 8;
+  return of_threads<256, 512, 1024>(chunks, [&](auto t) { go(t, integral_constant<int, M>{}); }) ||
+         of_threads<512>((chunks + 3) / 4, [&](auto t) { go(t, integral_constant<int, 4 * M>{}); });
 }
 
 /* Workgroups of the gradient: the runs of its column sums.  As many as are resident (512: 36 us for
@@ -485,7 +493,7 @@ struct GradSplit {
 };
 GradSplit grad_split(int64_t n_rows, int64_t width) {
   GradSplit p{1, 0, 0};
-  const bool held = grad_in_registers<8>(width, [&](auto g, auto) { p.rows = decltype(g)::value > NT ? 1 : NT / decltype(g)::value; });
+  const bool held = grad_in_registers<8>(width, [&](auto g, auto) { p.rows = row_threads(decltype(g)::value) / decltype(g)::value; });
   if (held) {
     const int64_t sets = (n_rows + p.rows - 1) / p.rows;
     p.runs = (int)(sets < grad_runs(width) ? sets : grad_runs(width));
@@ -510,9 +518,9 @@ void launch_norm(const NormArgs &args, Dtype dt, hipStream_t s) {
   auto held = [&](auto bf16, auto type) {
     constexpr bool B = decltype(bf16)::value;
     constexpr int OUT = decltype(type)::value;
-    return in_registers<norm_elements<B, OUT>()>(a.width, [&](auto g, auto u) {
-      constexpr int G = decltype(g)::value;
-      k_norm<B, OUT, G, decltype(u)::value><<<grid(NT / G), NT, 0, s>>>(a);
+    return in_registers<norm_elements<B, OUT>(), OUT != D3S_DTYPE_E4M3>(a.width, [&](auto g, auto u) {
+      constexpr int G = decltype(g)::value, T = row_threads(G);
+      k_norm<B, OUT, G, decltype(u)::value><<<grid(T / G), T, 0, s>>>(a);
     });
   };
   auto of_type = [&](auto bf16) {
@@ -542,7 +550,7 @@ void launch_norm_grad(const NormGradArgs &args, Dtype dt, void *ws, hipStream_t 
     constexpr bool B = decltype(bf16)::value;
     return grad_in_registers<B ? 8 : 4>(a.width, [&](auto g, auto u) {
       constexpr int G = decltype(g)::value, U = decltype(u)::value;
-      constexpr int T = G > NT ? G : NT;
+      constexpr int T = row_threads(G);
       if (a.dgain)
         k_norm_grad<B, G, U, true><<<dim3((unsigned)p.runs), T, 0, s>>>(a, parts);
       else

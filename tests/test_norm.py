@@ -231,3 +231,20 @@ def test_no_rows(gpu):
         assert gpu.rms_norm_backward_raw(None, 1, 30, None, 30, None, None, None, 0, 0, 30, None, 0, g.ptr) == 0
         hiprt.synchronize()
         assert (g.download((30,), np.float32) == 0).all()
+
+
+WIDER = [(3, 2051), (5, 2560), (2, 3333), (3, 4100), (2, 5120), (2, 6001), (2, 7168), (2, 8191), (2, 8194), (2, 10240), (2, 12000),
+         (2, 14337), (600, 2600), (300, 9000)]
+
+
+@pytest.mark.parametrize("n,width", WIDER)
+@pytest.mark.parametrize("dtype,out", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+def test_norm_of_wider_rows(gpu, n, width, dtype, out):
+    """workgroups of every number of threads"""
+    test_norm(gpu, n, width, dtype, out)
+
+
+@pytest.mark.parametrize("n,width", WIDER)
+@pytest.mark.parametrize("group", [0, 64, 256])
+def test_8_bits_of_wider_rows(gpu, n, width, group):
+    test_8_bits(gpu, n, width, group)
