@@ -6,7 +6,7 @@
  * the sum once each.  A lane takes one or two whole blocks of the generator (20 multiplies of 32 x 32 bits
  * each, about as long as its share of the memory traffic in bf16).
  *
- * Bound: HBM, the multiplies close behind.  bf16 8192 x 2048 with a residual 19 us (5.3 TB/s; a block
+ * Bound: HBM, the multiplies close behind.  bf16 8192 x 2048 with a residual 18 us (5.6 TB/s; a block
  * for each element 35); fp32 without 22 us (6.0 TB/s). */
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"

@@ -462,15 +462,15 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a, int b0) 
 
 constexpr int SWV = ST / WAVE;
 
-/* how the rows are cut: nseg segments of 16-byte chunks for the statistics, nblk blocks of `block`
- * elements for the draw, SWV parts each */
+/* how the rows are cut: nseg segments of 16-byte chunks for the statistics, nblk blocks for the draw,
+ * a part for each of a block's waves, `subs` runs of `sub` elements a part */
 struct VerifySplit {
-  int nseg, nblk, block;
+  int nseg, nblk, subs, sub;
 };
 
 struct VerifyRoom {
   RowStat *stats; /* [n_seqs, rows, nseg] */
-  uint64_t *parts; /* [n_seqs, nblk, SWV, 4]: doubles */
+  uint64_t *parts; /* [n_seqs, nblk, SWV, subs, 4]: doubles */
   uint32_t *arrivals;
   int spacing; /* words between two sequences' counters */
 };
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(ST) void k_verify_rows(d3s_verify_params a, VerifyS
  * but the 32-bit sums give rho0, 1e-6 off at most, and with z = sum max(p_j - rho0 q_j, 0) and
  * B = sum of q_j over the same places, z - (rho - rho0) B is the sum at rho, but for places where
  * p_j - rho q_j changes its sign in between: those are 1e-6 q_j off at most and few.  Each wave leaves
- * P, Q, z and B of its part; the last block of a sequence to arrive finds the part
+ * P, Q, z and B of its runs; the last block of a sequence to arrive finds the run
  * that passes u Z, and the place in it by the weights themselves.  (A pass for P and Q and another
  * for the weights: 64 sequences of 151936, 49 us where this takes 32.) */
 template <bool TB, bool DB>
@@ -544,11 +544,15 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   }
   Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, Q.m, x);
   const double rho0 = W.dp && Q.S > 0.0f ? (double)P.S / Q.S : 0.0;
-  const int part = sp.block / SWV;
-  {
-    const int lo = blk * sp.block + tid / WAVE * part, hi = (int)min((int64_t)a.vocab, (int64_t)lo + part);
+  const int runs = sp.nblk * SWV * sp.subs; /* of the row, in its order */
+  uint64_t *parts = w.parts + (int64_t)q.b * runs * 4;
+  for (int r = 0; r < sp.subs; r++) {
+    const int run = (blk * SWV + tid / WAVE) * sp.subs + r;
+    const int64_t lo = (int64_t)run * sp.sub;
+    const int hi = (int)min((int64_t)a.vocab, lo + sp.sub);
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int j = lo + lane_id() * 8; j < hi; j += WAVE * 8) {
+    for (int64_t at = lo + lane_id() * 8; at < hi; at += WAVE * 8) {
+      const int j = (int)at;
       double p[8], t[8];
       W.terms(j, p, t);
       if (W.dp) {
@@ -570,10 +574,9 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) sum[i] = wave_scan64(sum[i]);
-    uint64_t *out = w.parts + (((int64_t)q.b * sp.nblk + blk) * SWV + tid / WAVE) * 4;
     if (lane_id() == WAVE - 1) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) st_agent(out + i, __builtin_bit_cast(uint64_t, sum[i]));
+      for (int i = 0; i < 4; i++) st_agent(parts + run * 4 + i, __builtin_bit_cast(uint64_t, sum[i]));
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -585,13 +588,13 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   }
   __syncthreads();
   if (!last) return;
-  /* a thread the parts of a block (nblk <= ST) */
+  /* a thread SWV runs (runs <= ST SWV, a multiple of SWV) */
   double at[SWV][4];
 #pragma unroll
   for (int i = 0; i < SWV; i++)
 #pragma unroll
     for (int k = 0; k < 4; k++)
-      at[i][k] = tid < sp.nblk ? __builtin_bit_cast(double, ld_agent(w.parts + (((int64_t)q.b * sp.nblk + tid) * SWV + i) * 4 + k)) : 0.0;
+      at[i][k] = tid * SWV < runs ? __builtin_bit_cast(double, ld_agent(parts + (tid * SWV + i) * 4 + k)) : 0.0;
   double p = 0.0, t = 0.0;
 #pragma unroll
   for (int i = 0; i < SWV; i++) p += at[i][0], t += at[i][1];
@@ -637,7 +640,8 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     if (over == which) L.from = over_from;
     __syncthreads();
     const double base = L.from;
-    token = pick<ST>(W, which * part, (int)min((int64_t)a.vocab, (int64_t)(which + 1) * part), base, bar, plain, L);
+    token = pick<ST>(W, (int)min((int64_t)a.vocab, (int64_t)which * sp.sub), (int)min((int64_t)a.vocab, (int64_t)(which + 1) * sp.sub),
+                     base, bar, plain, L);
     if (plain) break;
   }
   write_tokens(q.b, a.n_draft, o, token, x, a.tokens, a.n_accepted);
@@ -755,17 +759,22 @@ __global__ __launch_bounds__(RT) void k_verify_ranked(RankedArgs a) {
 /* Rows longer than a workgroup holds are split over the chip, unless there are so many sequences that
  * a workgroup for each fills it (16 sequences of 4 drafts over 16384: 14 us, by a workgroup each 38; 300 of
  * 3 over 16000: 39, 68). */
-static bool verify_split(const d3s_verify_params &a, VerifySplit *sp) {
+static bool verify_split(const d3s_verify_params &a, bool draft, VerifySplit *sp) {
   if (a.vocab <= VT * 8 || a.n_seqs > 2048) return false;
   const int64_t rows = a.n_seqs * (2 * a.n_draft + 1);
   /* segments of two batches of bf16 chunks a lane, one where there are few */
   const int64_t batches = ((a.vocab + 7) / 8 + SU * ST - 1) / (SU * ST);
   sp->nseg = (int)(rows * batches <= 2048 ? batches : (batches + 1) / 2);
-  /* blocks of whole rounds of eight elements a thread: at most ST of them a row, about 1024 or more in all */
-  int64_t block = ST * 8;
-  while ((a.vocab + block - 1) / block > ST || (block < 16384 && a.n_seqs * ((a.vocab + block - 1) / block) > 2048)) block *= 2;
-  sp->block = (int)block;
+  /* Few enough blocks that the decision, which each makes, is waited for once or little more (256 sequences of one
+   * certain draft over 151936: 1024 blocks 79 us, 1280 84, 2560 90; two rows a place, 64 sequences: 1216 blocks 56.6,
+   * 960 59.3).  Each run is summed for itself, so that the place is looked for in one of them. */
+  const int64_t most = (draft ? 1280 : 1024) / a.n_seqs, blocks = most < 1 ? 1 : most > ST ? ST : most;
+  auto up = [](int64_t n, int64_t of, int64_t to) { return ((n + of - 1) / of + to - 1) / to * to; };
+  const int64_t part = up(a.vocab, blocks * SWV, WAVE * 8), block = part * SWV;
   sp->nblk = (int)((a.vocab + block - 1) / block);
+  const int64_t subs = (part + ST * 8 - 1) / (ST * 8), room = ST / sp->nblk;
+  sp->subs = (int)(subs < room ? subs : room);
+  sp->sub = (int)up(part, sp->subs, WAVE * 8);
   return true;
 }
 
@@ -780,20 +789,25 @@ static size_t verify_layout(const d3s_verify_params &a, const VerifySplit &sp, c
   w->arrivals = (uint32_t *)base;
   w->spacing = 32;
   w->stats = (RowStat *)take(n * (2 * (size_t)a.n_draft + 1) * sp.nseg * sizeof(RowStat));
-  w->parts = (uint64_t *)take(n * sp.nblk * SWV * 4 * sizeof(uint64_t));
+  w->parts = (uint64_t *)take(n * sp.nblk * SWV * sp.subs * 4 * sizeof(uint64_t));
   return at;
 }
 
 size_t verify_workspace_bytes(const d3s_verify_params &a) {
-  VerifySplit sp;
-  VerifyRoom w;
-  return verify_split(a, &sp) ? verify_layout(a, sp, nullptr, &w) : 0;
+  size_t most = 0; /* with drafts that are certain and without */
+  for (const bool draft : {false, true}) {
+    VerifySplit sp;
+    VerifyRoom w;
+    const size_t need = verify_split(a, draft, &sp) ? verify_layout(a, sp, nullptr, &w) : 0;
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 template <bool TB, bool DB>
 static void verify_launch(const d3s_verify_params &a, void *ws, hipStream_t s) {
   VerifySplit sp;
-  if (!verify_split(a, &sp)) {
+  if (!verify_split(a, a.draft != nullptr, &sp)) {
     constexpr int64_t MOST = 1 << 21; /* workgroups a launch: their threads are counted in 32 bits */
     for (int64_t b = 0; b < a.n_seqs; b += MOST) {
       const dim3 grid((unsigned)(a.n_seqs - b < MOST ? a.n_seqs - b : MOST));

@@ -340,3 +340,11 @@ def test_many_sequences_of_long_rows(gpu, n, L, V):
     target, draft, drafted, ua, ud, _ = TV.inputs(n, L, V, 11) if L else (np.random.default_rng(1).standard_normal((n, 1, V)).astype(np.float32) * 2, np.zeros((n, 0, V), np.float32),
                                                                          np.zeros((n, 0), int), np.zeros((n, 0), np.float32), (np.arange(n) / n).astype(np.float32), None)
     TV.both(gpu, target, draft if L else None, drafted, None, 1.0, 1.0, ua, ud, "bf16", "bf16")
+
+
+@pytest.mark.parametrize("n,L,V,certain", [(200, 2, 30011, False), (300, 1, 40001, True), (1030, 1, 9001, True), (1, 1, 3000017, False),
+                                           (20, 2, 70007, True)])
+def test_runs_of_a_block(gpu, n, L, V, certain):
+    """blocks of one run and of several, the last ones past the row's end"""
+    target, draft, drafted, ua, ud, _ = TV.inputs(n, L, V, 12)
+    TV.both(gpu, target, None if certain else draft, drafted, None, 1.0, 1.0, ua, ud, "f32", "bf16")
