@@ -348,3 +348,23 @@ def test_runs_of_a_block(gpu, n, L, V, certain):
     """blocks of one run and of several, the last ones past the row's end"""
     target, draft, drafted, ua, ud, _ = TV.inputs(n, L, V, 12)
     TV.both(gpu, target, None if certain else draft, drafted, None, 1.0, 1.0, ua, ud, "f32", "bf16")
+
+
+@pytest.mark.parametrize("vocab,rows", [(2000003, 8000), (9000, 8000)])
+def test_many_rows_that_are_cut(gpu, vocab, rows):
+    """thousands of rows of fifty ids each, over a long table and over a short one: every call leaves
+    the workspace's counters at zero"""
+    import hiprt
+    rng = np.random.default_rng([vocab, rows])
+    n, width = 50 * rows, 4
+    names = rng.permutation(vocab)[:rows]
+    ids = names[rng.permutation(np.repeat(np.arange(rows), 50))].astype(np.int32).reshape(n, 1)
+    bits, dy = R.to_bits(rng.standard_normal((n, width)), "f32")
+    ref, size, count = SR.embed_grad(ids, dy, vocab, 0, 1.0)
+    W = gpu.Workspace(gpu.lib().d3s_embed_backward_workspace_bytes(n, 1, vocab, 0, width))
+    for _ in range(2):
+        got = TE.grad(gpu, ids, bits, "f32", vocab, 0, width, 1.0, "f32", workspace=W.arg())
+        R.assert_near(got, ref, SR.U * (count[:, None] + 3) * size)
+        hiprt.synchronize()
+        assert not W.buf.download((1 << 16,), np.uint32).any()
+    W.buf.free()
