@@ -48,18 +48,17 @@ __device__ __forceinline__ float block_max(float v, float *part) {
   return t;
 }
 
-/* eight values over their group's scale, as 8 bits.  By the scale's reciprocal, whose
- * rounding moves a quotient by 2^-23 of itself where a step is 2^-3, except where it
- * would overflow; saturating: the greatest quotient is 448 and a rounding. */
+/* eight values over their group's scale, as 8 bits; saturating: the greatest quotient is
+ * 448 and a rounding.  The quotient is the correctly rounded one of fp32, by the scale's reciprocal in 64 bits: the
+ * product is within 2^-52 of it, and no quotient of two 24-bit numbers is nearer than 2^-49 (both relative) to
+ * the middle of two fp32 numbers, which has 25. */
 __device__ __forceinline__ uint64_t pack_e4m3(const float *v, float scale) {
   uint32_t w[2] = {0u, 0u};
   float q[8];
-  const float inv = 1.0f / scale;
-  const bool tiny = !(scale >= 0x1p-100f); /* (zero and NaN too) */
+  const double inv = scale == 0.0f ? 0.0 : 1.0 / (double)scale;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    q[e] = v[e] * inv;
-    if (tiny) q[e] = scale > 0.0f ? v[e] / scale : scale == 0.0f ? 0.0f : __builtin_nanf("");
+    q[e] = (float)((double)v[e] * inv);
     q[e] = __builtin_elementwise_minimum(__builtin_elementwise_maximum(q[e], -E4M3_MOST), E4M3_MOST); /* (NaN stays) */
   }
 #pragma unroll

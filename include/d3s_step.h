@@ -137,8 +137,8 @@ int d3s_embed_backward_ws(const int32_t *ids, int64_t n_rows, int n_ids, const v
  * y_dtype D3S_DTYPE_F32 or _BF16 (y may be x or residual itself where types and
  * strides agree and sum is elsewhere), or D3S_DTYPE_E4M3: each `group`
  * elements of a row (32, 64, 128 or 256; 0: the whole row; the last group may be
- * shorter) share scales[r, g] = greatest |y| / 448, and y holds y / scale rounded to the
- * nearest 8 bits, so that q times scale stands for y.  A group of zeros has scale
+ * shorter) share scales[r, g] = greatest |y| / 448, and y holds the fp32 quotient y / scale rounded to
+ * the nearest 8 bits, so that q times scale stands for y.  A group of zeros has scale
  * 0 and zeros; one that holds a NaN or an infinity has scale NaN and NaNs. scales
  * [n_rows, ceil(width / group)] fp32 is needed then, and else not looked at.
  * eps >= 0; a row of zeros with eps 0 gives rstd +inf and NaN, as the formula does. */

@@ -248,3 +248,26 @@ def test_norm_of_wider_rows(gpu, n, width, dtype, out):
 @pytest.mark.parametrize("group", [0, 64, 256])
 def test_8_bits_of_wider_rows(gpu, n, width, group):
     test_8_bits(gpu, n, width, group)
+
+
+@pytest.mark.parametrize("n,width,group", [(1500, 2048, 128), (3000, 1000, 0), (2000, 40, 32), (150, 16391, 0), (150, 16391, 64), (600, 4100, 256)])
+def test_8_bits_are_the_quotients(gpu, n, width, group):
+    """every y is the fp32 quotient by its group's scale, rounded to the nearest even: equal, from the same rstd (the
+    products are fp32's own, one after the other)"""
+    rng = np.random.default_rng([n, width, group, 9])
+    x = (rng.standard_normal((n, width)) * np.exp(rng.uniform(-3, 3, (n, 1)))).astype(np.float32)
+    g = (1 + 0.3 * rng.standard_normal(width)).astype(np.float32)
+    x[:2] *= np.array([[1e-33], [1e-41]], np.float32)  # scales below 2^-100, subnormal ones
+    got = forward(gpu, x, None, g, 1e-6, "f32", "e4m3", group=group)
+    y = x * got["rstd"][:, None] * g
+    size = group or width
+    most = np.stack([np.abs(y[:, c:c + size]).max(1) for c in range(0, width, size)], 1)
+    assert np.array_equal(got["scales"], most / np.float32(448))
+    q = y / np.repeat(got["scales"], size, 1)[:, :width]
+    assert q.dtype == np.float32
+    v = SR.e4m3_values()[:127]
+    middle = (v[1:] + v[:-1]) / 2  # exact in fp32
+    at = np.searchsorted(middle, np.abs(q).astype(np.float64))  # (a tie: the lower)
+    tie = (at < 126) & (np.abs(q) == middle[np.minimum(at, 125)])
+    at += tie & (at % 2 == 1)
+    assert np.array_equal(got["y"], (at | np.where(np.signbit(q), 128, 0)).astype(np.uint8)), (got["y"] != (at | np.where(np.signbit(q), 128, 0))).sum()
