@@ -602,17 +602,24 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   W.ip = 1.0 / sum_p;
   W.iq = sum_q > 0.0 ? 1.0 / sum_q : 0.0;
   const double shift = sum_q > 0.0 ? sum_p / sum_q - rho0 : 0.0;
-  int token = -1;
-  for (bool plain = !o.rejected; token < 0; plain = true) {
-    double mine[SWV], all = 0.0, Z;
+  bool plain = !o.rejected;
+  double mine[SWV];
 #pragma unroll
-    for (int i = 0; i < SWV; i++) {
-      mine[i] = W.ip * (plain ? at[i][0] : fmax(at[i][2] - shift * at[i][3], 0.0));
-      all += mine[i];
-    }
+  for (int i = 0; i < SWV; i++) mine[i] = W.ip * (plain ? at[i][0] : fmax(at[i][2] - shift * at[i][3], 0.0));
+  int token;
+  for (;;) {
+    double all = 0.0, Z;
+#pragma unroll
+    for (int i = 0; i < SWV; i++) all += mine[i];
     double from = block_scan64(all, L, &Z);
-    /* (p <= q everywhere, or by rounding alone not so: p's own draw) */
-    if (!(Z > 0.0) && !plain) continue;
+    if (!(Z > 0.0)) { /* p <= q everywhere: p's own draw */
+      token = -1;
+      if (plain) break; /* (never: the greatest logit has a weight) */
+      plain = true;
+#pragma unroll
+      for (int i = 0; i < SWV; i++) mine[i] = W.ip * at[i][0];
+      continue;
+    }
     const double bar = (double)ud * Z;
     int over = 0x7fffffff, some = -1;
     double over_from = 0.0, some_from = 0.0;
@@ -642,7 +649,11 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     const double base = L.from;
     token = pick<ST>(W, (int)min((int64_t)a.vocab, (int64_t)which * sp.sub), (int)min((int64_t)a.vocab, (int64_t)(which + 1) * sp.sub),
                      base, bar, plain, L);
-    if (plain) break;
+    if (token >= 0) break;
+    /* (a sum by rounding alone, or of terms below 2^-1022, whose weights are 0 where their sum is not: the next run) */
+#pragma unroll
+    for (int i = 0; i < SWV; i++)
+      if (tid * SWV + i == which) mine[i] = 0.0;
   }
   write_tokens(q.b, a.n_draft, o, token, x, a.tokens, a.n_accepted);
 }

@@ -348,3 +348,55 @@ def test_ranked_without_drafts_is_the_samplers_draw(gpu, k, top_p):
 
 def test_nothing(gpu):
     assert gpu.verify_ranked_raw(4096, 4096, 3, None, None, 0, 0, 0, None, None, None, 4096, 4096, 4096) == 0
+
+
+def pairs(n, V, td, seed, k):
+    """rows of target [n, 2, V] and draft [n, 1, V] alike but for k pairs of places, one of each masked in the one
+    and the other in the other, at the same logit: p - q is above 0 at the first of each pair alone.  (Whatever
+    order the sums are added in, the pairs' places are beside each other, so that they are the same to the last bit.)"""
+    rng = np.random.default_rng([n, V, seed])
+    t = np.repeat(rng.standard_normal((n, 1, V)), 2, 1).astype(np.float32) * 2
+    d = t[:, :1].copy()
+    slots = (V // 2 - 4) // 4
+    at = V // 2 // 4 * 4 + 2 * np.sort(rng.permuted(np.tile(np.arange(slots), (n, 1)), axis=1)[:, :k], 1)
+    b = np.arange(n)[:, None]
+    l = R.to_bits((6 + rng.random((n, k))).astype(np.float32), td)[1]  # noqa: E741
+    t[b, 0, at], t[b, 0, at + 1], d[b, 0, at], d[b, 0, at + 1] = l, -np.inf, -np.inf, l
+    return t, d, at, np.exp(l), rng
+
+
+@pytest.mark.parametrize("V", [600, 8192, 9000, 20000, 151936])
+@pytest.mark.parametrize("td", ["f32", "bf16"])
+def test_rows_alike_but_for_pairs(gpu, V, td):
+    """weights that are 0 but at some places, far into the row: with u_draw = 0 the first of them is drawn"""
+    n = 48
+    for seed, k in enumerate((3, 50, 70)):
+        t, d, at, w, rng = pairs(n, V, td, seed, k)
+        drafted = at[:, rng.integers(0, k)][:, None] + 1  # p = 0: never accepted
+        ud = (rng.integers(0, 1 << 24, n) * 2.0 ** -24).astype(np.float32)
+        ud[:n // 2] = 0
+        c = w.cumsum(1) / w.sum(1, keepdims=True)
+        ud = np.where((np.abs(c - ud[:, None]) < 1e-6).any(1), np.float32(0.0), ud)
+        want = at[np.arange(n), (c <= ud[:, None].astype(np.float64)).sum(1)]
+        got, _ = run(gpu, t, d, drafted, None, 1.0, 1.0, np.zeros((n, 1)), ud, td, td)
+        assert (got[1] == 0).all()
+        assert np.array_equal(got[0][:, 0], want), (V, td, seed, got[0][:, 0][got[0][:, 0] != want], want[got[0][:, 0] != want])
+        assert (got[0][:, 1] == -1).all() and (got[3][:2] == 0).all()
+
+
+@pytest.mark.parametrize("V", [20000, 151936])
+@pytest.mark.parametrize("rejected", [False, True])
+def test_terms_below_the_least_normal_number(gpu, V, rejected):
+    """the first half's terms are 2^-1074, which no weight by the sum of twenty ones is: u_draw = 0 draws the first of these"""
+    n = 5
+    t = np.full((n, 2, V), -np.inf, np.float32)
+    t[:, :, :V // 2] = -744.6
+    d = np.full((n, 1, V), -np.inf, np.float32)
+    d[:, :, 1] = 0.0  # (a token that the target never draws)
+    t[:, :, 1] = -np.inf
+    ones = V - 20 - 7 * np.arange(n)
+    for b in range(n):
+        t[b, :, ones[b]:ones[b] + 20] = 0.0
+    drafted = np.full((n, 1), 1)
+    got, _ = run(gpu, t, d, drafted, None if rejected else np.zeros(n), 1.0, 1.0, np.zeros((n, 1)), np.zeros(n), "f32", "f32")
+    assert (got[1] == 0).all() and np.array_equal(got[0][:, 0], ones) and (got[3][:2] == 0).all()
