@@ -256,7 +256,7 @@ template <int NT>
 struct DrawLds {
   double wave[NT / WAVE];
   double from;
-  int at;
+  int at, close;
 };
 
 template <int CTRL, int ROWM>
@@ -305,14 +305,16 @@ __device__ __forceinline__ double block_scan64(double v, DrawLds<NT> &L, double 
 
 /* The first place whose sum passes bar, else (LAST) the last with a weight, else -1, in
  * every thread: a thread's eight weights r follow each other from j on, `before` is the sum of
- * those before them. */
+ * those before them.  L.close is set if a sum is within `doubt` of bar. */
 template <int NT>
 __device__ __forceinline__ int first_past(const double *r, int j, double before, double bar, bool last_too, DrawLds<NT> &L,
-                                          bool ready = false) {
+                                          bool ready = false, double doubt = -1.0) {
   int over = 0x7fffffff, last = -1;
+  bool close = fabs(before - bar) <= doubt;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     before += r[e];
+    close = close || fabs(before - bar) <= doubt;
     last = r[e] > 0.0 ? j + e : last;
     over = min(over, r[e] > 0.0 && before > bar ? j + e : 0x7fffffff);
   }
@@ -322,6 +324,7 @@ __device__ __forceinline__ int first_past(const double *r, int j, double before,
   }
   /* (places rise with the lanes: the first that has one speaks for its wave) */
   const uint64_t has = __ballot(over != 0x7fffffff);
+  if (close) L.close = 1;
   if (has && lane_id() == (int)__builtin_ctzll(has)) atomicMin(&L.at, over);
   __syncthreads();
   int at = L.at;
@@ -339,9 +342,10 @@ __device__ __forceinline__ int first_past(const double *r, int j, double before,
   return at;
 }
 
-/* the token among [lo, hi), `base` the weights before them */
+/* the token among [lo, hi), *sum the weights before them, and where there is none those up to hi */
 template <int NT, bool TB, bool DB>
-__device__ __forceinline__ int pick(const Weights<TB, DB> &W, int lo, int hi, double base, double bar, bool plain, DrawLds<NT> &L) {
+__device__ __forceinline__ int pick(const Weights<TB, DB> &W, int lo, int hi, double *sum, double bar, bool plain, DrawLds<NT> &L,
+                                    double doubt = -1.0) {
   int last = -1;
   for (int c = lo; c < hi; c += NT * 8) {
     const int j = c + (int)threadIdx.x * 8;
@@ -352,12 +356,12 @@ __device__ __forceinline__ int pick(const Weights<TB, DB> &W, int lo, int hi, do
       if (j + e >= hi) r[e] = 0.0;
       mine += r[e];
     }
-    const double before = base + block_scan64(mine, L, &total);
-    const int at = first_past(r, j, before, bar, false, L);
+    const double before = *sum + block_scan64(mine, L, &total);
+    const int at = first_past(r, j, before, bar, false, L, false, doubt);
     if (at >= 0) return at;
     const int end = first_past(r, j, before, __builtin_inf(), true, L);
     if (end >= 0) last = end;
-    base += total;
+    *sum += total;
   }
   return last;
 }
@@ -448,7 +452,8 @@ __global__ __launch_bounds__(VT) void k_verify_one(d3s_verify_params a, int b0) 
         }
         Z = block_sum64(Z, L);
         if (Z > 0.0 || plain) {
-          token = pick<VT>(W, 0, V, 0.0, (double)ud * Z, plain, L);
+          double sum = 0.0;
+          token = pick<VT>(W, 0, V, &sum, (double)ud * Z, plain, L);
           break;
         }
       }
@@ -468,9 +473,10 @@ struct VerifySplit {
   int nseg, nblk, subs, sub;
 };
 
+constexpr int PART = 5;
 struct VerifyRoom {
   RowStat *stats; /* [n_seqs, rows, nseg] */
-  uint64_t *parts; /* [n_seqs, nblk, SWV, subs, 4]: doubles */
+  uint64_t *parts; /* [n_seqs, nblk, SWV, subs, PART]: doubles */
   uint32_t *arrivals;
   int spacing; /* words between two sequences' counters */
 };
@@ -507,16 +513,21 @@ __global__ __launch_bounds__(ST) void k_verify_rows(d3s_verify_params a, VerifyS
 /* 2: the decision (by every block), and the sums of the rows that the token is drawn from, in 64
  * bits and in one pass.  With P and Q the rows' sums, the weights are p_j / P - q_j / Q =
  * (p_j - rho q_j) / P where that is positive, rho = P / Q.  P and Q are known only behind the pass,
- * but the 32-bit sums give rho0, 1e-6 off at most, and with z = sum max(p_j - rho0 q_j, 0) and
- * B = sum of q_j over the same places, z - (rho - rho0) B is the sum at rho, but for places where
- * p_j - rho q_j changes its sign in between: those are 1e-6 q_j off at most and few.  Each wave leaves
- * P, Q, z and B of its runs; the last block of a sequence to arrive finds the run
- * that passes u Z, and the place in it by the weights themselves.  (A pass for P and Q and another
- * for the weights: 64 sequences of 151936, 49 us where this takes 32.) */
+ * but the 32-bit sums give rho0 near it, and with z = sum max(p_j - rho0 q_j, 0) and
+ * B = sum of q_j over the same places, z - (rho - rho0) B is the sum at rho, unless p_j - rho q_j is of another sign
+ * than p_j - rho0 q_j somewhere: then it is below, by at most |rho - rho0| times these places' q_j.  A is the sum of q_j
+ * where that could be, p_j - rho0 q_j being nearer to 0 than BAND rho0 q_j (one place in two rows of 151936).  Each wave
+ * leaves P, Q, z, B and A of its runs; the last block of a sequence to arrive finds the run that passes u Z, and the place
+ * in it by the weights themselves.  Where what all A allow could decide, their runs are added again from their weights
+ * first, and all runs where rho is further than half of BAND from rho0, so that the token is the weights' own.  (A pass for P
+ * and Q and another for the weights: 64 sequences of 151936, 49 us where this takes 32.) */
+constexpr double BAND = 0x1p-18;
+
 template <bool TB, bool DB>
 __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifySplit sp, VerifyRoom w) {
   __shared__ Settled S;
   __shared__ DrawLds<ST> L;
+  __shared__ double three[3][SWV];
   __shared__ uint32_t last;
   const int tid = (int)threadIdx.x;
   const int blk = (int)(blockIdx.x % (unsigned)sp.nblk);
@@ -527,10 +538,22 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     const float l = draft_logit<TB, DB>(a, q, tid);
     const float c = LOG2E / q.temperature(a, tid);
     const RowStat *st = w.stats + ((int64_t)q.b * q.rows + tid) * sp.nseg;
-    Sums s{-FLT_MAX, 0.0f, 0.0f};
-#pragma unroll 8
-    for (int i = 0; i < sp.nseg; i++) join(s, st[i].m, st[i].S, 0.0f, c);
-    settle_row(a, q, tid, RowStat{s.m, s.S}, l, S);
+    float m = -FLT_MAX;
+    double sum = 0.0; /* (a thousand segments' in 32 bits would be 1e-5 off) */
+    constexpr int UN = 8;
+    for (int i = 0; i < sp.nseg; i += UN) {
+      RowStat part[UN];
+#pragma unroll
+      for (int u = 0; u < UN; u++) part[u] = st[min(i + u, sp.nseg - 1)];
+      float M = m, S = 0.0f;
+#pragma unroll
+      for (int u = 0; u < UN; u++) M = maximum(M, part[u].m);
+#pragma unroll
+      for (int u = 0; u < UN; u++) S += i + u < sp.nseg ? part[u].S * exp2_hw(drop(part[u].m, M, c)) : 0.0f;
+      sum = sum * (double)exp2_hw(drop(m, M, c)) + (double)S;
+      m = M;
+    }
+    settle_row(a, q, tid, RowStat{m, (float)sum}, l, S);
   }
   __syncthreads();
   const Outcome o = settle(a, q, S, u, blk == 0);
@@ -543,26 +566,32 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     return;
   }
   Weights<TB, DB> W(a, q, o.accepted, o.rejected, P.m, Q.m, x);
-  const double rho0 = W.dp && Q.S > 0.0f ? (double)P.S / Q.S : 0.0;
+  const double rho0 = W.dp && Q.S > 0.0f ? (double)P.S / Q.S : 0.0, band = rho0 * BAND;
   const int runs = sp.nblk * SWV * sp.subs; /* of the row, in its order */
-  uint64_t *parts = w.parts + (int64_t)q.b * runs * 4;
+  uint64_t *parts = w.parts + (int64_t)q.b * runs * PART;
   for (int r = 0; r < sp.subs; r++) {
     const int run = (blk * SWV + tid / WAVE) * sp.subs + r;
     const int64_t lo = (int64_t)run * sp.sub;
     const int hi = (int)min((int64_t)a.vocab, lo + sp.sub);
-    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    double sum[PART] = {0.0, 0.0, 0.0, 0.0, 0.0};
     for (int64_t at = lo + lane_id() * 8; at < hi; at += WAVE * 8) {
       const int j = (int)at;
       double p[8], t[8];
       W.terms(j, p, t);
       if (W.dp) {
+        double near = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const double d = fma(-rho0, t[e], p[e]);
+          near = fmin(near, fma(-band, t[e], fabs(d)));
           sum[0] += p[e];
           sum[1] += t[e];
-          sum[2] += d > 0.0 ? d : 0.0;
+          sum[2] += fmax(d, 0.0);
           sum[3] += d > 0.0 ? t[e] : 0.0;
+        }
+        if (__ballot(near < 0.0)) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) sum[4] += fabs(fma(-rho0, t[e], p[e])) < band * t[e] ? t[e] : 0.0;
         }
       } else {
 #pragma unroll
@@ -573,10 +602,10 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) sum[i] = wave_scan64(sum[i]);
+    for (int i = 0; i < PART; i++) sum[i] = wave_scan64(sum[i]);
     if (lane_id() == WAVE - 1) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) st_agent(parts + run * 4 + i, __builtin_bit_cast(uint64_t, sum[i]));
+      for (int i = 0; i < PART; i++) st_agent(parts + run * PART + i, __builtin_bit_cast(uint64_t, sum[i]));
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -589,30 +618,49 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
   __syncthreads();
   if (!last) return;
   /* a thread SWV runs (runs <= ST SWV, a multiple of SWV) */
-  double at[SWV][4];
+  double at[SWV][PART];
 #pragma unroll
   for (int i = 0; i < SWV; i++)
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-      at[i][k] = tid * SWV < runs ? __builtin_bit_cast(double, ld_agent(parts + (tid * SWV + i) * 4 + k)) : 0.0;
-  double p = 0.0, t = 0.0;
+    for (int k = 0; k < PART; k++)
+      at[i][k] = tid * SWV < runs ? __builtin_bit_cast(double, ld_agent(parts + (tid * SWV + i) * PART + k)) : 0.0;
+  /* P, Q and A of the row, by one exchange */
+  double row[3] = {0.0, 0.0, 0.0};
 #pragma unroll
-  for (int i = 0; i < SWV; i++) p += at[i][0], t += at[i][1];
-  const double sum_p = block_sum64(p, L), sum_q = W.dp ? block_sum64(t, L) : 0.0;
+  for (int i = 0; i < SWV; i++) row[0] += at[i][0], row[1] += at[i][1], row[2] += at[i][4];
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    row[k] = wave_scan64(row[k]);
+    if (lane_id() == WAVE - 1) three[k][tid / WAVE] = row[k];
+  }
+  __syncthreads();
+  row[0] = row[1] = row[2] = 0.0;
+#pragma unroll
+  for (int i = 0; i < SWV; i++)
+#pragma unroll
+    for (int k = 0; k < 3; k++) row[k] += three[k][i];
+  const double sum_p = row[0], sum_q = row[1];
   W.ip = 1.0 / sum_p;
   W.iq = sum_q > 0.0 ? 1.0 / sum_q : 0.0;
   const double shift = sum_q > 0.0 ? sum_p / sum_q - rho0 : 0.0;
-  bool plain = !o.rejected;
+  /* the runs' weights, the marked ones, and how much these may lack */
+  bool plain = !o.rejected, again = !plain && !(fabs(shift) <= 0.5 * band);
   double mine[SWV];
+  unsigned marked = 0u;
 #pragma unroll
-  for (int i = 0; i < SWV; i++) mine[i] = W.ip * (plain ? at[i][0] : fmax(at[i][2] - shift * at[i][3], 0.0));
+  for (int i = 0; i < SWV; i++) {
+    mine[i] = W.ip * (plain ? at[i][0] : fmax(at[i][2] - shift * at[i][3], 0.0));
+    if (tid * SWV < runs && (again || at[i][4] > 0.0)) marked |= 1u << i;
+  }
+  double doubt = plain ? 0.0 : (again ? sum_q : row[2]) * (fabs(shift) * W.ip * (1.0 + 0x1p-20));
   int token;
   for (;;) {
     double all = 0.0, Z;
 #pragma unroll
     for (int i = 0; i < SWV; i++) all += mine[i];
     double from = block_scan64(all, L, &Z);
-    if (!(Z > 0.0)) { /* p <= q everywhere: p's own draw */
+    again = again || (doubt > 0.0 && !(Z > 0.0));
+    if (!again && !(Z > 0.0)) { /* p <= q everywhere: p's own draw */
       token = -1;
       if (plain) break; /* (never: the greatest logit has a weight) */
       plain = true;
@@ -620,8 +668,9 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
       for (int i = 0; i < SWV; i++) mine[i] = W.ip * at[i][0];
       continue;
     }
-    const double bar = (double)ud * Z;
-    int over = 0x7fffffff, some = -1;
+    /* the run that passes bar, or the first that is to be added again */
+    const double bar = again ? __builtin_inf() : (double)ud * Z;
+    int over = again && marked ? tid * SWV + (int)__builtin_ctz(marked) : 0x7fffffff, some = -1;
     double over_from = 0.0, some_from = 0.0;
 #pragma unroll
     for (int i = 0; i < SWV; i++) {
@@ -631,12 +680,17 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
       }
       from += mine[i];
     }
-    if (tid == 0) L.at = 0x7fffffff;
+    if (tid == 0) L.at = 0x7fffffff, L.close = 0;
     __syncthreads();
     if (over != 0x7fffffff) atomicMin(&L.at, over);
     __syncthreads();
-    if (L.at == 0x7fffffff) { /* none by rounding: the last that has any */
+    if (L.at == 0x7fffffff) {
       __syncthreads();
+      if (again) { /* all are added */
+        again = false, doubt = 0.0;
+        continue;
+      }
+      /* none by rounding: the last that has any */
       if (tid == 0) L.at = -1;
       __syncthreads();
       if (some >= 0) atomicMax(&L.at, some);
@@ -646,14 +700,18 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
     const int which = L.at;
     if (over == which) L.from = over_from;
     __syncthreads();
-    const double base = L.from;
+    double sum = L.from;
     token = pick<ST>(W, (int)min((int64_t)a.vocab, (int64_t)which * sp.sub), (int)min((int64_t)a.vocab, (int64_t)(which + 1) * sp.sub),
-                     base, bar, plain, L);
-    if (token >= 0) break;
-    /* (a sum by rounding alone, or of terms below 2^-1022, whose weights are 0 where their sum is not: the next run) */
+                     &sum, bar, plain, L, again || !(doubt > 0.0) ? -1.0 : doubt);
+    const bool close = doubt > 0.0 && L.close; /* (read behind a barrier of pick's) */
+    if (!again && !close && token >= 0) break;
+    /* (no token: terms below 2^-1022 alone, whose weights are 0 where their sum is not) */
+    if (again || !close) {
 #pragma unroll
-    for (int i = 0; i < SWV; i++)
-      if (tid * SWV + i == which) mine[i] = 0.0;
+      for (int i = 0; i < SWV; i++)
+        if (tid * SWV + i == which) mine[i] = again ? sum : 0.0, marked &= ~(1u << i);
+    }
+    again = again || close;
   }
   write_tokens(q.b, a.n_draft, o, token, x, a.tokens, a.n_accepted);
 }
@@ -800,7 +858,7 @@ static size_t verify_layout(const d3s_verify_params &a, const VerifySplit &sp, c
   w->arrivals = (uint32_t *)base;
   w->spacing = 32;
   w->stats = (RowStat *)take(n * (2 * (size_t)a.n_draft + 1) * sp.nseg * sizeof(RowStat));
-  w->parts = (uint64_t *)take(n * sp.nblk * SWV * sp.subs * 4 * sizeof(uint64_t));
+  w->parts = (uint64_t *)take(n * sp.nblk * SWV * sp.subs * PART * sizeof(uint64_t));
   return at;
 }
 

@@ -400,3 +400,38 @@ def test_terms_below_the_least_normal_number(gpu, V, rejected):
     drafted = np.full((n, 1), 1)
     got, _ = run(gpu, t, d, drafted, None if rejected else np.zeros(n), 1.0, 1.0, np.zeros((n, 1)), np.zeros(n), "f32", "f32")
     assert (got[1] == 0).all() and np.array_equal(got[0][:, 0], ones) and (got[3][:2] == 0).all()
+
+
+@pytest.mark.parametrize("V", [600, 8192, 9000, 20000, 151936])
+def test_rows_alike_but_for_their_last_bits(gpu, V):
+    """pairs as above, and between them logits that differ by their last bits, one way or the other: weights
+    of 1e-8 of the terms, which sums in 32 bits do not see.  u_draw = 0 draws the first that is above 0 (the sums of both rows
+    agree to 1e-9)"""
+    n = 48
+    for seed, k in enumerate((30, 50, 70)):
+        t, d, at, w, rng = pairs(n, V, "f32", seed, k)
+        small = (0.25 + 0.25 * rng.random((n, V))).astype(np.float32)
+        alike = t[:, 0] == d[:, 0]
+        step = rng.choice([-1, 1], (n, V))
+        t[:, 0] = np.where(alike, small, t[:, 0])
+        d[:, 0] = np.where(alike, (small.view(np.int32) - step).astype(np.int32).view(np.float32), d[:, 0])
+        drafted = at[:, rng.integers(0, k)][:, None] + 1
+        want = (t[:, 0] > d[:, 0]).argmax(1)
+        got, _ = run(gpu, t, d, drafted, None, 1.0, 1.0, np.zeros((n, 1)), np.zeros(n), "f32", "f32")
+        assert (got[1] == 0).all() and np.array_equal(got[0][:, 0], want), (V, seed, got[0][:, 0], want)
+
+
+@pytest.mark.parametrize("u", [0.0, 0.37, 1 - 2.0 ** -24])
+def test_sums_that_32_bits_take_amiss(gpu, u):
+    """the longest rows of one logit or two, at temperatures whose quotients round apart: the 32-bit sums' quotient is
+    2.7e-6 off (each exponent of 13 is 1e-6 off), and the draw's are added again"""
+    V = (1 << 24) - 1
+    t, d = np.full((1, 2, V), -18.947877883911133, np.float32), np.full((1, 1, V), -18.965412139892578, np.float32)
+    t[:, :, :V // 2] = -18.878435134887695
+    t[:, :, 7] = d[:, :, 7] = 0.0
+    x = V - 9
+    t[:, 0, x] = -np.inf
+    T, Td, ud = np.float32(1.4257), np.float32(1.4274), np.float32(u)
+    got, _ = run(gpu, t, d, np.array([[x]]), None, float(T), float(Td), np.zeros((1, 1)), np.array([ud]), "f32", "f32")
+    w = np.maximum(SR.probs(t[0, 0].astype(np.float64), T) - SR.probs(d[0, 0].astype(np.float64), Td), 0)
+    assert got[1][0] == 0 and got[0][0, 0] == SR.draw(w, float(ud)) and (got[3][:2] == 0).all()
