@@ -157,3 +157,45 @@ def test_infinities_and_nan_stay_in_their_rows(gpu):
     hit = {(int(ids[5, 0]), 3), (int(ids[6, 0]), 4)} | {(int(ids[7, 0]), j) for j in range(width)}
     odd = {tuple(int(v) for v in i) for i in np.argwhere(~np.isfinite(got))}
     assert odd == hit
+
+
+def whole(rng, shape):
+    """whole numbers but 0, whose sums are exact in any order while they are below 2^24"""
+    return (rng.integers(1, 9, shape) * rng.choice([-1, 1], shape)).astype(np.float32)
+
+
+def check_whole(gpu, ids, vocab, slot_rows, width, dtype, out, rng, dy_pad=0, pad=0):
+    n, t = ids.shape
+    bits, dy = R.to_bits(whole(rng, (n, width)), dtype)
+    ref, size, count = SR.embed_grad(ids, dy, vocab, slot_rows, 0.25)
+    assert size.max() < 2 ** 22
+    for old in (None, R.to_bits(whole(rng, ref.shape), out)):
+        want = R.to_bits(ref if old is None else ref + old[1], out)[0]
+        got = grad(gpu, ids, bits, dtype, vocab, slot_rows, width, 0.25, out, dy_pad, pad, old=None if old is None else old[0])
+        assert np.array_equal(R.from_bits(np.ascontiguousarray(got)), R.from_bits(want))
+    return count
+
+
+@pytest.mark.parametrize("n,t,vocab,slot_rows,width,dtype,out,how,dy_pad,pad", GRADS)
+def test_gradient_of_whole_numbers(gpu, n, t, vocab, slot_rows, width, dtype, out, how, dy_pad, pad):
+    """equal, so that no position of a frequent row is lost or taken twice"""
+    rng = np.random.default_rng([n, t, vocab, width, 1])
+    check_whole(gpu, make_ids(rng, n, t, vocab, how), vocab, slot_rows, width, dtype, out, rng, dy_pad, pad)
+
+
+@pytest.mark.parametrize("counts,rows,vocab", [
+    ((65,), 500, 500), ((65,), 500, 40000), ((65,), 1000, 1000), ((65,), 1100, 2000003), ((33,), 900, 700000), ((65,), 16000, 16000),
+    ((1, 31, 32, 33, 63, 64, 65, 66, 127, 128, 129, 193, 4095, 4096, 4097, 8193), 1, 50),
+    ((1, 31, 32, 33, 63, 64, 65, 66, 127, 128, 129, 193, 4095, 4096, 4097, 8193), 4, 5000),
+    ((129, 65, 64, 2), 9000, 50000)])
+@pytest.mark.parametrize("width,out", [(4, "f32"), (41, "bf16")])
+def test_rows_of_so_many_ids(gpu, counts, rows, vocab, width, out):
+    """rows of exactly as many ids as one chunk, two or more begin at; all ids in cut rows"""
+    rng = np.random.default_rng([sum(counts), rows, vocab, width])
+    n = sum(counts) * rows
+    names = rng.permutation(vocab)[:rows * len(counts)]
+    ids = np.repeat(names, np.tile(counts, rows))
+    assert len(ids) == n
+    ids = ids[rng.permutation(n)].astype(np.int32)[:, None]
+    got = check_whole(gpu, ids, vocab, 0, width, "f32", out, rng)
+    assert set(got[got > 0]) == set(counts)

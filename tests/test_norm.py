@@ -271,3 +271,17 @@ def test_8_bits_are_the_quotients(gpu, n, width, group):
     tie = (at < 126) & (np.abs(q) == middle[np.minimum(at, 125)])
     at += tie & (at % 2 == 1)
     assert np.array_equal(got["y"], (at | np.where(np.signbit(q), 128, 0)).astype(np.uint8)), (got["y"] != (at | np.where(np.signbit(q), 128, 0))).sum()
+
+
+@pytest.mark.parametrize("n,width", WIDTHS + [(5000, 16), (20001, 100), (700, 513), (257, 8192), (1025, 1025), (3000, 3000), (40, 20000)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_column_sums_of_whole_numbers(gpu, n, width, dtype):
+    """dgain of whole dy and h and of rstd that are powers of two: equal, so that no row is lost or taken twice"""
+    rng = np.random.default_rng([n, width, 17])
+    whole = lambda: R.to_bits(rng.integers(1, 9, (n, width)) * rng.choice([-1, 1], (n, width)), dtype)  # noqa: E731
+    (db, dy), (hb, h) = whole(), whole()
+    rstd = rng.choice([0.25, 0.5, 1.0], n).astype(np.float32)
+    want = (dy * h * rstd[:, None]).sum(0)
+    assert (np.abs(dy * h).sum(0) < 2 ** 22).all()
+    for dx in (True, False):
+        assert np.array_equal(backward(gpu, db, hb, None, rstd, None, dtype, dx=dx)[1], want)
