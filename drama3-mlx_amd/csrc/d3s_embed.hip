@@ -152,8 +152,9 @@ GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) 
   while ((int64_t)p.hot * HOT_MOST < p.n * p.slots) p.hot *= 2;
   return p;
 }
-/* chunks at most: of 2 hot positions, or one for a row of more than hot */
-int64_t chunks_most(const GradPlan &p) { return 2 * (p.n * p.slots / p.hot) + 1; }
+/* chunks at most: a row's one has hot + 1 positions at least, c >= 2 of them 2 hot (c - 1) + 1, which is
+ * c (hot + 1 / 2) at least (rows of 2 hot + 1 have two) */
+int64_t chunks_most(const GradPlan &p) { return 2 * p.n * p.slots / (2 * p.hot + 1) + 1; }
 
 size_t grad_layout(const GradPlan &p, int64_t width, char *base, GradRoom *w) {
   size_t at = split_counter_bytes();

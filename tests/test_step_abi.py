@@ -190,3 +190,12 @@ def test_verification_between_words(d3s, name):
 @pytest.mark.parametrize("name", ["target_cand", "target_probs", "draft_cand", "draft_probs"])
 def test_candidates_between_words(d3s, name):
     assert d3s.verify_ranked_raw(**{**RANKED, name: P + 2}) == -1
+
+
+def test_room_for_the_chunks_of_a_gradient(d3s):
+    """a million ids: rows of more than 32 are cut into chunks of 64 or more positions, at most two for 65, each of which
+    has a row of sums"""
+    size = d3s.lib().d3s_embed_backward_workspace_bytes
+    n, chunks = 1000000, 2 * 1000000 // 65 + 1
+    narrow, wide = size(n, 1, 5000, 0, 8), size(n, 1, 5000, 0, 4096)
+    assert 0 < wide - narrow <= 4 * (4096 - 8) * chunks + 512
