@@ -2,7 +2,7 @@
  * gradient in the table (gfx950, wave64; include/d3s_step.h).
  *
  * The lookup is bound by HBM, or by what the caches give where rows come again: 8192 tokens of 2048
- * bf16 10.2 us; 4096 frames of ten codes 28 us (6.7 TB/s of the ten rows each); one frame 4.1 us, a launch
+ * bf16 10.2 us; 4096 frames of ten codes 28 us (6.7 TB/s of the ten rows each); one frame 3.7 us, a launch
  * and two dependent loads.
  * The gradient is bound by the table's writes: 40970 x 2048 fp32 from 40960 codes 79 us (9 of them
  * grouping), 151936 x 1024 bf16 from 16384 tokens 69 us (12 grouping); many ids of few rows by
@@ -110,7 +110,7 @@ struct Chunk {
 enum { CNT_CHUNKS = 0, CNT_HOT = 16, CNT_DONE = 32 };
 
 struct GradPlan {
-  int64_t slots, part, rows, n; /* parts of the table, rows of each and in all, ids of each */
+  int64_t slots, rows, n; /* parts of the table, rows in all, ids of each part */
   int range, hot;               /* rows of a range; a row of more positions is cut */
   int64_t ranges;               /* of each part */
   bool parted;
@@ -131,7 +131,6 @@ struct GradRoom {
 GradPlan grad_plan(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows) {
   GradPlan p;
   p.slots = slot_rows ? n_ids : 1;
-  p.part = slot_rows ? slot_rows : vocab;
   p.rows = vocab + (n_ids - 1) * slot_rows;
   p.n = slot_rows ? n_rows : n_rows * n_ids;
   /* Ranges of 256 rows (16384 ids for 151936 rows: 12 us; 64 and 128 rows 21), wider while looking through the ids

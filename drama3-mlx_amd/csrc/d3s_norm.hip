@@ -1,9 +1,9 @@
 /* k_norm, k_norm_grad: root-mean-square norm with the residual's addition and an
  * output in 8 bits, and its gradient (gfx950, wave64; include/d3s_step.h).
  *
- * A row's inputs are read once, all in flight together, and stay in registers: up to 512
- * columns a part of a wave a row, up to 2048 a wave, up to 16384 a workgroup of 256 to 1024 threads; longer rows are read once
- * for each pass (k_norm_rows, k_norm_grad_rows, k_norm_dgain).  Squares are summed in fp32,
+ * A row's inputs are read once, all in flight together, and stay in registers: up to 256
+ * columns a part of a wave a row, up to 2048 (the gradient's three rows: 1024) a wave, up to 16384 a workgroup of 256 to
+ * 1024 threads; longer rows are read once for each pass (k_norm_rows, k_norm_grad_rows, k_norm_dgain).  Squares are summed in fp32,
  * a lane's in order and then by a tree.  h stays in fp32 from the addition to y; rstd is
  * a correctly rounded root and quotient.  8 bits: a group's greatest |y| by exchanges among the lanes
  * that hold it, its scale an fp32 quotient, each y rounded once.
@@ -11,8 +11,8 @@
  * for each workgroup goes to the workspace, and a second launch adds them in order: no atomics.
  *
  * Bound: HBM.  bf16 8192 x 2048 with residual and kept sum, e4m3 by groups of 128: 25.7 us (4.6 TB/s);
- * its gradient with dsum and dgain 28 us (4.8 TB/s) and 4.6 of the second launch; 100000 x 64
- * 9.7 us (5.3 TB/s).  One row of 2048: 3.8 us, a launch and two dependent loads' latency. */
+ * its gradient with dsum and dgain 28 us (4.8 TB/s) and 4.4 of the second launch; 100000 x 64
+ * 9.7 us (5.3 TB/s).  One row of 2048: 3.5 us, a launch and two dependent loads' latency. */
 #include "d3s_colsums.h"
 #include "d3s_step_internal.h"
 #include "d3s_vec.h"

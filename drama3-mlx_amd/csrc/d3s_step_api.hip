@@ -52,8 +52,7 @@ int64_t table_rows(int64_t n_rows, int n_ids, int64_t vocab, int64_t slot_rows, 
 }
 
 int embed_grad_check(const int32_t *ids, int64_t n_rows, int n_ids, const void *dy, int dtype, int64_t dy_stride,
-                     int64_t vocab, int64_t slot_rows, int64_t width, float scale, void *grad, int grad_dtype,
-                     int64_t grad_stride) {
+                     int64_t vocab, int64_t slot_rows, int64_t width, void *grad, int grad_dtype, int64_t grad_stride) {
   if (!known(dtype) || !known(grad_dtype)) return D3S_ERR_DTYPE;
   if (!table_rows(n_rows, n_ids, vocab, slot_rows, width) || n_rows > IDS_MOST / n_ids || !stride_ok(dy_stride, width) || !stride_ok(grad_stride, width))
     return D3S_ERR_ARG;
@@ -66,8 +65,8 @@ int embed_grad_check(const int32_t *ids, int64_t n_rows, int n_ids, const void *
 int embed_grad_call(const int32_t *ids, int64_t n_rows, int n_ids, const void *dy, int dtype, int64_t dy_stride,
                     int64_t vocab, int64_t slot_rows, int64_t width, float scale, int accumulate, void *grad,
                     int grad_dtype, int64_t grad_stride, Room room, void *stream) {
-  if (const int rc = embed_grad_check(ids, n_rows, n_ids, dy, dtype, dy_stride, vocab, slot_rows, width, scale, grad,
-                                      grad_dtype, grad_stride))
+  if (const int rc = embed_grad_check(ids, n_rows, n_ids, dy, dtype, dy_stride, vocab, slot_rows, width, grad, grad_dtype,
+                                      grad_stride))
     return rc;
   if (width == 0 || (accumulate && n_rows == 0)) return D3S_OK;
   hipStream_t s = (hipStream_t)stream;

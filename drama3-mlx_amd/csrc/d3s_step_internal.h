@@ -59,7 +59,7 @@ struct NormArgs {
   void *y;
   int y_dtype;
   int64_t y_stride;
-  int group; /* of E4M3, the width for whole rows */
+  int group; /* of E4M3, 0 for whole rows */
   float *scales, *rstd;
 };
 void launch_norm(const NormArgs &a, Dtype dt, hipStream_t s);

@@ -205,7 +205,7 @@ struct Weights {
   double mp, mq, cp, cq;       /* greatest logits, log2(e) / T */
   double ip, iq;               /* what the terms are multiplied by */
 
-  /* sp, sq: what the sequence's rows hold */
+  /* m_p, m_q: the rows' greatest logits; x: lane i's draft i */
   __device__ __forceinline__ Weights(const d3s_verify_params &a, const Seq &s, int accepted, bool rejected, float m_p, float m_q, int x) {
     tp = (const char *)a.target + ((int64_t)s.b * (a.n_draft + 1) + accepted) * a.target_stride * (TB ? 2 : 4);
     dp = rejected && a.draft ? (const char *)a.draft + ((int64_t)s.b * a.n_draft + accepted) * a.draft_stride * (DB ? 2 : 4) : nullptr;
