@@ -589,7 +589,7 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
           sum[2] += fmax(d, 0.0);
           sum[3] += d > 0.0 ? t[e] : 0.0;
         }
-        if (__ballot(near < 0.0)) {
+        if (__builtin_expect(__ballot(near < 0.0) != 0ull, 0)) {
 #pragma unroll
           for (int e = 0; e < 8; e++) sum[4] += fabs(fma(-rho0, t[e], p[e])) < band * t[e] ? t[e] : 0.0;
         }
@@ -602,7 +602,11 @@ __global__ __launch_bounds__(ST) void k_verify_draw(d3s_verify_params a, VerifyS
       }
     }
 #pragma unroll
-    for (int i = 0; i < PART; i++) sum[i] = wave_scan64(sum[i]);
+    for (int i = 0; i < PART; i++) { /* (a certain draft's rows have P and z, few runs an A) */
+      if (i % 2 && !W.dp) continue;
+      if (i == 4 && __builtin_expect(!__ballot(sum[4] > 0.0), 1)) continue;
+      sum[i] = wave_scan64(sum[i]);
+    }
     if (lane_id() == WAVE - 1) {
 #pragma unroll
       for (int i = 0; i < PART; i++) st_agent(parts + run * PART + i, __builtin_bit_cast(uint64_t, sum[i]));
