@@ -8,8 +8,8 @@
  * the rate of 32-bit ones here).  All sums are added in an order that the sizes give.
  *
  * Bound: the rows' sums by HBM (64 sequences of 4 drafts over 151936 bf16: 29 us, 6.0 TB/s), the draw by
- * its 64-bit arithmetic (the same: 31 us, of which the decision is 5, the terms 19, the place 6); short rows
- * by the chain of dependent steps (4097: 9.9 us; 30 candidates 6.3). */
+ * its 64-bit arithmetic (the same: 33 us, of which the decision is 5, the terms 19); short rows
+ * by the chain of dependent steps (4097: 10 us; 30 candidates 6.3). */
 #include "d3s_rowcore.h"
 #include "d3s_rowsums.h"
 #include "d3s_step_internal.h"
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(ST) void k_verify_rows(d3s_verify_params a, VerifyS
  * leaves P, Q, z, B and A of its runs; the last block of a sequence to arrive finds the run that passes u Z, and the place
  * in it by the weights themselves.  Where what all A allow could decide, their runs are added again from their weights
  * first, and all runs where rho is further than half of BAND from rho0, so that the token is the weights' own.  (A pass for P
- * and Q and another for the weights: 64 sequences of 151936, 49 us where this takes 32.) */
+ * and Q and another for the weights: 64 sequences of 151936, 49 us where this takes 33.) */
 constexpr double BAND = 0x1p-18;
 
 template <bool TB, bool DB>
