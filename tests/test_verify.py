@@ -435,3 +435,15 @@ def test_sums_that_32_bits_take_amiss(gpu, u):
     got, _ = run(gpu, t, d, np.array([[x]]), None, float(T), float(Td), np.zeros((1, 1)), np.array([ud]), "f32", "f32")
     w = np.maximum(SR.probs(t[0, 0].astype(np.float64), T) - SR.probs(d[0, 0].astype(np.float64), Td), 0)
     assert got[1][0] == 0 and got[0][0, 0] == SR.draw(w, float(ud)) and (got[3][:2] == 0).all()
+
+
+def test_many_sequences_alike_but_for_pairs(gpu):
+    """more sequences of long rows than are split: a workgroup each"""
+    n, V, k = 2100, 8200, 40
+    t, d, at, w, rng = pairs(n, V, "f32", 1, k)
+    drafted = at[:, 5][:, None] + 1
+    ud = np.where(np.arange(n) % 2, (rng.integers(0, 1 << 24, n) * 2.0 ** -24), 0.0).astype(np.float32)
+    c = w.cumsum(1) / w.sum(1, keepdims=True)
+    ud = np.where((np.abs(c - ud[:, None]) < 1e-6).any(1), np.float32(0.0), ud)
+    got, _ = run(gpu, t, d, drafted, None, 1.0, 1.0, np.zeros((n, 1)), ud, "f32", "f32")
+    assert (got[1] == 0).all() and np.array_equal(got[0][:, 0], at[np.arange(n), (c <= ud[:, None].astype(np.float64)).sum(1)])
